@@ -73,7 +73,12 @@ int talm_set_wait_limit_ns(uint64_t limit_ns);
 #define TALM_KERNEL_PEER_REDUCE 9   /* reduce_gather_kernel (peer exchange, phase 2)      */
 #define TALM_KERNEL_PEER_FINISH 10  /* gather_finish_kernel (wait + copy out)             */
 #define TALM_KERNEL_NF4_GEMM 11     /* nf4_gemm_kernel (fused NF4 dequant + tcgen05 GEMM)  */
-#define TALM_KERNEL_KINDS 12
+#define TALM_KERNEL_NF4_MATVEC 12   /* few-row product with NF4 weights                   */
+#define TALM_KERNEL_ADAPTER_DOWN 13 /* adapter_down_kernel (the few-row product's adapter) */
+#define TALM_KERNEL_DROPOUT 14      /* dropout_kernel                                     */
+#define TALM_KERNEL_LORA_FORWARD 15 /* the launches of one talm_lora_forward              */
+#define TALM_KERNEL_LORA_BACKWARD 16 /* the launches of one talm_lora_backward            */
+#define TALM_KERNEL_KINDS 17
 int talm_profile_begin(void);
 int talm_profile_end(double* ms_out, int64_t* launches_out, int n_kinds);
 
@@ -130,6 +135,81 @@ int talm_nf4_linear(const uint16_t* a, int64_t ld_a, int64_t n_rows, const uint8
                     int64_t w_rows, int64_t w_cols, int64_t qblock, int64_t qblock2,
                     int transpose, const uint16_t* bias, uint16_t* y, int64_t ld_y,
                     void* stream);
+
+/* The product of a few rows with NF4 weights (1 to 32 rows: the single-token form of a 4-bit
+ * projection), the weights read packed and never written out, with an optional LoRA adapter:
+ *   y[n, o] = fp16( sum_k level[code(o, k)] * scale(o, k) * x[n, k] + bias[o]
+ *                   + scaling * sum_j (sum_k x[n, k] lora_a[j, k]) * lora_b[o, j] )
+ * with fp32 products and sums and one rounding (the weight itself is not rounded to fp16, as the
+ * dequantised copy is). Stands in for the dequantisation + product of solution/qgroup.py:346-355
+ * (GroupLinear) and the adapter of solution/lora.py:151-231 where there are few rows.
+ *   x        : fp16 [n_rows, w_cols], row stride ld_x elements
+ *   packed   : w_rows * w_cols / 2 bytes, row-major
+ *   scales   : either absmax8 != NULL: coded scales as in talm_nf4_group_dequant, one per
+ *              `blocksize` elements of the flattened weight, with code, absmax2, offset2 and levels,
+ *              the second level indexed by (absmax_row0 + block) / qblock2; or absmax8 == NULL and
+ *              absmax: one fp32 scale per `blocksize` elements (code .. qblock2 ignored)
+ *   levels   : 16 fp32; NULL = the NF4 table (fp32 absmax form only)
+ *   bias     : fp16 [w_rows] or NULL
+ *   lora_a, lora_b : fp32 [rank, w_cols], [w_rows, rank]; rank 0 = no adapter; `down`: a workspace
+ *              of n_rows * rank floats (overwritten)
+ *   y        : fp16 [n_rows, w_rows], row stride ld_y elements
+ * Preconditions: 0 <= n_rows <= 32, w_cols and blocksize even, 0 <= rank <= 64. Any alignment is
+ * accepted. */
+int talm_nf4_matvec(const uint16_t* x, int64_t ld_x, int64_t n_rows, const uint8_t* packed,
+                    const uint8_t* absmax8, const float* absmax, const float* code,
+                    const float* absmax2, const float* offset2, const float* levels,
+                    int64_t absmax_row0, int64_t w_rows, int64_t w_cols, int64_t blocksize,
+                    int64_t qblock2, const uint16_t* bias, const float* lora_a,
+                    const float* lora_b, int64_t rank, float scaling, float* down,
+                    uint16_t* y, int64_t ld_y, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Counter-based dropout and the LoRA branch (training form)
+ * ---------------------------------------------------------------------------------------- */
+
+/* Dropout whose mask is never stored: y[e] = keep(e) ? x[e] * 32768 / (32768 - drop) : 0 for
+ * element e in row-major order, in fp32 and rounded once to the type of x. keep(e) is u >= drop
+ * for the low 15 bits u of half e % 8 of the four words of Philox4x32 with 7 rounds, key *seed
+ * (device memory), counter e / 8. The backward pass is the same call on the gradient. A dropped
+ * element gives +0 whatever x holds.
+ *   x : [n_rows, n_cols] of `dtype` (TALM_DTYPE_*), row stride ld_x elements
+ *   drop : 0..32768 (round(p * 32768))      y : [n_rows, n_cols], contiguous
+ * Replaces the dropout of the reference's adapter (solution/lora.py:151-231). */
+int talm_dropout(const void* x, int64_t ld_x, int64_t n_rows, int64_t n_cols, int dtype,
+                 const int64_t* seed, int64_t drop, void* y, void* stream);
+
+/* Bytes that talm_lora_forward saves for talm_lora_backward, and of the backward's workspace. */
+int talm_lora_sizes(int64_t n_rows, int64_t n_in, int64_t n_out, int64_t rank, size_t* saved,
+                    size_t* backward_ws);
+
+/* The adapter's branch added to the frozen projection's product:
+ *   y = fp16(base + scaling * (dropout(x) lora_a^T) lora_b^T)
+ * with the dropout of talm_dropout over x (drop 0: none, seed may be NULL), fp32 sums and one
+ * rounding. Replaces solution/lora.py:151-231 (LoraProjectionTorch.forward).
+ *   x, base, y : fp16 [n_rows, n_in], [n_rows, n_out], [n_rows, n_out] (y contiguous), rows 16-byte
+ *                aligned with strides of a multiple of 8 elements
+ *   lora_a, lora_b : fp32 [rank, n_in], [n_out, rank], contiguous
+ *   saved : talm_lora_sizes bytes, 16-byte aligned, kept for the backward
+ * Preconditions: n_in and n_out multiples of 8, 1 <= rank <= 64. */
+int talm_lora_forward(const uint16_t* x, int64_t ld_x, const uint16_t* base, int64_t ld_base,
+                      const float* lora_a, const float* lora_b, int64_t n_rows, int64_t n_in,
+                      int64_t n_out, int64_t rank, float scaling, const int64_t* seed,
+                      int64_t drop, uint16_t* y, void* saved, size_t saved_bytes, void* stream);
+
+/* The gradients of talm_lora_forward for the output gradient g (fp16 [n_rows, n_out]):
+ *   dt = scaling g lora_b, grad_b = scaling g^T t, grad_a = dt^T dropout(x),
+ *   dx = fp16(mask * (dt lora_a))      (base's gradient is g itself)
+ * in fp32 sums taken in an order that does not depend on timing. dx (fp16 [n_rows, n_in],
+ * contiguous), grad_a and grad_b (fp32, overwritten) may each be NULL. `saved` is the forward's;
+ * x, seed and drop are the forward's arguments.
+ * Replaces solution/lora.py:151-231 (LoraProjectionTorch.backward). */
+int talm_lora_backward(const uint16_t* g, int64_t ld_g, const uint16_t* x, int64_t ld_x,
+                       const float* lora_a, const float* lora_b, const void* saved,
+                       size_t saved_bytes, int64_t n_rows, int64_t n_in, int64_t n_out,
+                       int64_t rank, float scaling, const int64_t* seed, int64_t drop,
+                       uint16_t* dx, float* grad_a, float* grad_b, void* workspace,
+                       size_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Fused LM head + cross-entropy (vocabulary-sliced, no materialised logits)

@@ -5,6 +5,7 @@ device pointers (`Tensor.data_ptr()`), the current CUDA stream as a raw handle. 
 a tensor that is not on a CUDA device or a non-zero status raises: there is no CPU path.
 """
 
+import contextlib
 import ctypes
 import os
 
@@ -19,6 +20,7 @@ _I64 = ctypes.c_int64
 _INT = ctypes.c_int
 _SZ = ctypes.c_size_t
 _U32 = ctypes.c_uint32
+_F32 = ctypes.c_float
 
 SIGNATURES = {
     "talm_abi_version": (_INT, []),
@@ -32,6 +34,15 @@ SIGNATURES = {
     "talm_nf4_group_dequant": (_INT, [_P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _P]),
     "talm_nf4_linear": (_INT, [_P, _I64, _I64, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
                                _I64, _INT, _P, _P, _I64, _P]),
+    "talm_nf4_matvec": (_INT, [_P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64,
+                               _I64, _P, _P, _P, _I64, _F32, _P, _P, _I64, _P]),
+    "talm_dropout": (_INT, [_P, _I64, _I64, _I64, _INT, _P, _I64, _P, _P]),
+    "talm_lora_sizes": (_INT, [_I64, _I64, _I64, _I64, ctypes.POINTER(_SZ),
+                               ctypes.POINTER(_SZ)]),
+    "talm_lora_forward": (_INT, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _F32, _P,
+                                 _I64, _P, _P, _SZ, _P]),
+    "talm_lora_backward": (_INT, [_P, _I64, _P, _I64, _P, _P, _P, _SZ, _I64, _I64, _I64, _I64,
+                                  _F32, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
     "talm_head_workspace_size": (_INT, [_I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
     "talm_head_shard": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P,
                                _P, _P, _SZ, _P]),
@@ -107,9 +118,25 @@ def stream_of(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(t):
+    """The raw handle of the current stream of a CUDA tensor's device."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+_HERE = contextlib.nullcontext()
+
+
+def device_of(t):
+    """A context in which the CUDA tensor's device is the current one (a launch takes the current
+    device's kernels); free where it already is."""
+    index = t.get_device()
+    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
 KERNEL_KINDS = ("head_slice", "head_combine", "head_reserved", "head_finalize", "head_merge",
                 "nf4", "nf4_tail", "head_scale", "peer_publish", "peer_reduce", "peer_finish",
-                "nf4_gemm")
+                "nf4_gemm", "nf4_matvec", "adapter_down", "dropout", "lora_forward",
+                "lora_backward")
 
 
 def profile_begin():

@@ -1,0 +1,199 @@
+"""The training form of a LoRA adapter, with counter-based dropout inside it.
+
+  dropout(x, p, seed)                               dropout whose mask is never stored
+  lora_branch(x, base, lora_A, lora_B, scaling, p, seed)
+                                                    base + scaling * (dropout(x) A^T) B^T
+  draw_seed(device)                                 the seed of one call, from torch's generator
+
+Both are autograd functions over the kernels of csrc/adapter.cu. The mask of a call is a function of
+its seed and of the element's place in row-major order (Philox4x32 with 7 rounds; element e of `x` is
+kept when the low 15 bits of half e % 8 of counter e / 8 reach round(p * 32768)), so the backward
+pass makes it again instead of reading it: the branch saves its input, the rank-wide product and the
+seed, no dropped copy of the input and no mask. The probability is thereby rounded to a multiple of
+1 / 32768; the factor 32768 / (32768 - drop) is that of the rounded one, which keeps the expectation.
+
+The seed is a one-element int64 tensor on the device. `draw_seed` fills it from torch's own CUDA
+generator: torch.manual_seed makes a run repeatable, a captured graph draws a new seed on every
+replay, and gradient checkpointing, which restores the generator, recomputes the same mask.
+
+The reference's adapter node (solution/lora.py:151-231) keeps the dropout's generator state and
+replays it in the backward; its products run in fp16. Here sums are fp32 and each fp16 result is
+rounded once. There is no CPU path.
+"""
+
+import math
+
+import torch
+
+from . import _lib
+from .engaged import RAN
+
+MAX_RANK = 64
+DROP_ALL = 32768
+_DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # TALM_DTYPE_*
+
+
+def draw_seed(device):
+    """A seed for one call: int64 [1] on `device`, drawn from torch's CUDA generator."""
+    return torch.empty(1, dtype=torch.int64, device=device).random_()
+
+
+def drop_threshold(p):
+    """round(p * 32768): the number of the 32768 values of a draw that drop an element."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout probability has to be between 0 and 1, got {p}")
+    return math.floor(p * DROP_ALL + 0.5)
+
+
+def _check_seed(seed, x):
+    if (not torch.is_tensor(seed) or seed.dtype != torch.int64 or seed.numel() != 1
+            or seed.get_device() != x.get_device()):
+        raise ValueError("seed must be an int64 tensor of one element on the input's device")
+
+
+def _rows(t, cols):
+    """`t` as [rows, cols] rows of unit stride that do not overlap (a view where its strides
+    allow it, else a copy)."""
+    t = t.reshape(-1, cols)
+    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t
+
+
+def _rows16(t, cols):
+    """`_rows` on 16-byte boundaries, as the branch's kernels read them."""
+    t = _rows(t, cols)
+    if t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % 8):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _stride(t):
+    """The row stride of a 2-D tensor (its width where a single row leaves it undefined)."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, seed, drop):
+        ctx.drop = drop
+        ctx.save_for_backward(seed)
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        if x.numel() == 0:
+            return y
+        cols = x.shape[-1] if x.dim() else 1
+        rows = _rows(x, cols)
+        with _lib.device_of(x):
+            _lib.check(_lib.load().talm_dropout(
+                _lib.ptr(rows), _stride(rows), rows.shape[0], cols, _DTYPES[x.dtype],
+                _lib.ptr(seed), drop, _lib.ptr(y), _lib.raw_stream(x)), "talm_dropout")
+        RAN["dropout"] += 1
+        return y
+
+    @staticmethod
+    def backward(ctx, grad):
+        (seed,) = ctx.saved_tensors
+        return _Dropout.apply(grad, seed, ctx.drop), None, None
+
+
+def dropout(x, p, seed):
+    """x * mask * 32768 / (32768 - drop), drop = round(p * 32768), the mask a function of `seed`
+    and the element's index. x: fp16, bf16 or fp32 of any shape and strides on a CUDA device; a
+    dropped element gives 0 whatever x holds. Differentiable (twice as well)."""
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"dropout takes fp16, bf16 or fp32, got {x.dtype}")
+    drop = drop_threshold(p)
+    _lib.ptr(x)
+    _check_seed(seed, x)
+    return _Dropout.apply(x, seed, drop)
+
+
+def branch_takes(x, base, rank):
+    """Whether `lora_branch` takes this call: fp16 on one CUDA device, widths of multiples of 8,
+    a rank of at most MAX_RANK."""
+    return (x.is_cuda and x.dtype == torch.float16 and base.dtype == torch.float16
+            and x.shape[-1] % 8 == 0 and base.shape[-1] % 8 == 0 and 1 <= rank <= MAX_RANK)
+
+
+def _sizes(n_rows, n_in, n_out, rank):
+    saved, work = _lib._SZ(0), _lib._SZ(0)
+    _lib.check(_lib.load().talm_lora_sizes(n_rows, n_in, n_out, rank, saved, work),
+               "talm_lora_sizes")
+    return saved.value, work.value
+
+
+class _LoraBranch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, base, lora_a, lora_b, scaling, seed, drop):
+        n_in, n_out, rank = x.shape[-1], base.shape[-1], lora_a.shape[0]
+        a, b = lora_a.contiguous(), lora_b.contiguous()
+        xr, br = _rows16(x, n_in), _rows16(base, n_out)
+        n_rows = xr.shape[0]
+        saved_bytes, ctx.work_bytes = _sizes(n_rows, n_in, n_out, rank)
+        y = torch.empty(base.shape, dtype=base.dtype, device=x.device)
+        saved = torch.empty(saved_bytes, dtype=torch.uint8, device=x.device)
+        with _lib.device_of(x):
+            _lib.check(_lib.load().talm_lora_forward(
+                _lib.ptr(xr), _stride(xr), _lib.ptr(br), _stride(br), _lib.ptr(a), _lib.ptr(b),
+                n_rows, n_in, n_out, rank, scaling, _lib.ptr(seed), drop, _lib.ptr(y),
+                _lib.ptr(saved), saved_bytes, _lib.raw_stream(x)), "talm_lora_forward")
+        ctx.scaling, ctx.drop = scaling, drop
+        ctx.save_for_backward(x, lora_a, lora_b, seed, saved)
+        RAN["lora"] += 1
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, lora_a, lora_b, seed, saved = ctx.saved_tensors
+        need_x, need_base, need_a, need_b = ctx.needs_input_grad[:4]
+        n_in, n_out, rank = x.shape[-1], grad.shape[-1], lora_a.shape[0]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        da = torch.empty(rank, n_in, dtype=torch.float32, device=x.device) if need_a else None
+        db = torch.empty(n_out, rank, dtype=torch.float32, device=x.device) if need_b else None
+        if need_x or need_a or need_b:
+            a, b = lora_a.contiguous(), lora_b.contiguous()
+            xr, gr = _rows16(x, n_in), _rows16(grad, n_out)
+            work = torch.empty(ctx.work_bytes, dtype=torch.uint8, device=x.device)
+            with _lib.device_of(x):
+                _lib.check(_lib.load().talm_lora_backward(
+                    _lib.ptr(gr), _stride(gr), _lib.ptr(xr), _stride(xr), _lib.ptr(a),
+                    _lib.ptr(b), _lib.ptr(saved), saved.numel(), xr.shape[0], n_in, n_out, rank,
+                    ctx.scaling, _lib.ptr(seed), ctx.drop, _lib.ptr(dx), _lib.ptr(da),
+                    _lib.ptr(db), _lib.ptr(work), work.numel(), _lib.raw_stream(x)),
+                    "talm_lora_backward")
+        return dx, grad if need_base else None, da, db, None, None, None
+
+
+def lora_branch(x, base, lora_A, lora_B, scaling, p=0.0, seed=None):
+    """base + scaling * (dropout(x) A^T) B^T, rounded to fp16 once, with gradients for x, base, A
+    and B. x [..., in] and base [..., out]: fp16 with the same leading sizes; lora_A [r, in] and
+    lora_B [out, r]: fp32, r in 1..64; `in` and `out` multiples of 8. p > 0 takes a `seed`
+    (`draw_seed`); the mask is that of `dropout(x, p, seed)`."""
+    n_in, n_out = x.shape[-1], base.shape[-1]
+    if x.dtype != torch.float16 or base.dtype != torch.float16:
+        raise TypeError(f"lora_branch takes fp16 x and base, got {x.dtype} and {base.dtype}")
+    if lora_A.dtype != torch.float32 or lora_B.dtype != torch.float32:
+        raise TypeError("lora_A and lora_B must be fp32")
+    if x.shape[:-1] != base.shape[:-1]:
+        raise ValueError(f"x {tuple(x.shape)} and base {tuple(base.shape)} differ in their rows")
+    rank = lora_A.shape[0]
+    if lora_A.shape != (rank, n_in) or lora_B.shape != (n_out, rank):
+        raise ValueError(f"adapter {tuple(lora_A.shape)}, {tuple(lora_B.shape)} does not map "
+                         f"{n_in} to {n_out}")
+    if not 1 <= rank <= MAX_RANK or n_in % 8 or n_out % 8:
+        raise ValueError(f"lora_branch needs a rank of 1..{MAX_RANK} and widths of multiples of "
+                         f"8, got rank {rank}, {n_in} -> {n_out}")
+    drop = drop_threshold(p)
+    for t in (x, base, lora_A, lora_B):
+        _lib.ptr(t)
+        if t.get_device() != x.get_device():
+            raise ValueError("x, base and the adapter must be on one device")
+    if drop == 0:
+        seed = None
+    else:
+        if seed is None:
+            raise ValueError("dropout needs a seed (adapter.draw_seed)")
+        _check_seed(seed, x)
+    return _LoraBranch.apply(x, base, lora_A, lora_B, float(scaling), seed, drop)

@@ -3,6 +3,8 @@
 #include "abi.cu"
 #include "nf4.cu"
 #include "nf4_gemm.cu"
+#include "nf4_matvec.cu"
+#include "adapter.cu"
 #include "peer.cu"
 #include "head.cu"
 #include "head_noalloc.cu"

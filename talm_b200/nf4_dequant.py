@@ -52,6 +52,33 @@ def nf4_dequantize(packed, absmax, blocksize, out):
     return out
 
 
+def nf4_matvec(x, packed, absmax, blocksize, out=None, bias=None, adapter=None):
+    """x W^T (+ bias) (+ the adapter's branch) for at most 32 rows x [..., in] fp16 and a packed
+    NF4 weight [out, in] (sizes from the packed bytes): the product that `nf4_dequantize` and a
+    GEMM would give, with the weight read packed, not rounded to fp16, and never written. packed:
+    uint8 of any shape, absmax: fp32 [ceil(n / blocksize)], bias: fp16 [out], adapter: (lora_A,
+    lora_B, scaling) as in `qgroup.matvec`; out: fp16 [rows, out] to write into."""
+    from . import qgroup
+
+    n_cols = x.shape[-1]
+    if absmax.dtype != torch.float32 or packed.dtype != torch.uint8:
+        raise ValueError("packed must be uint8 and absmax fp32")
+    packed = packed.contiguous().view(-1)
+    absmax = absmax.contiguous()
+    n = 2 * packed.numel()
+    if n_cols == 0 or n % n_cols:
+        raise ValueError(f"{n} packed weights are not rows of {n_cols}")
+    if blocksize < 1 or absmax.numel() < -(-n // blocksize):
+        raise ValueError(f"{absmax.numel()} scales for {n} weights in blocks of {blocksize}")
+    a = qgroup._few_rows(x, n_cols)
+    n_rows = n // n_cols
+    y = torch.empty(a.shape[0], n_rows, dtype=torch.float16, device=a.device) if out is None \
+        else out
+    qgroup.run_matvec(a, packed, None, absmax, None, None, None, None, 0, n_rows, n_cols,
+                      int(blocksize), 1, bias, adapter, y)
+    return y.view(*x.shape[:-1], n_rows) if out is None else out
+
+
 def _self_check(original_impl):
     """Before taking over, one comparison with bitsandbytes' own kernel: a 1 M-element NF4 buffer
     of random codes with random fp32 block scales (block size 64), dequantised by both; True

@@ -166,12 +166,23 @@ class NF4Linear(torch.nn.Module):
     def forward(self, x):
         if self._talm_group is None:
             raise RuntimeError("NF4Linear is not packed into a layer group (nf4_format.load_layer)")
+        if qgroup.takes_matvec(x):
+            return self.matvec(x)
         group, idx = self._talm_group
         in_dtype = x.dtype
         out = qgroup.GroupLinear.apply(x.to(torch.float16), group, idx)
         if torch.is_grad_enabled() and x.requires_grad:
             group.expected_bwd += 1
         return out.to(in_dtype)
+
+    def matvec(self, x, adapter=None):
+        """The product (with an adapter's branch in it) for a few rows, as `qgroup.serving` routes
+        it: the weight read packed, inputs cast to fp16 and the result back."""
+        if self._talm_group is None:
+            raise RuntimeError("NF4Linear is not packed into a layer group (nf4_format.load_layer)")
+        group, idx = self._talm_group
+        return qgroup.matvec(x.to(torch.float16), group, idx, bias=group.biases[idx],
+                             adapter=adapter).to(x.dtype)
 
     def extra_repr(self):
         return f"in_features={self.in_features}, out_features={self.out_features}, nf4"

@@ -21,6 +21,7 @@ patches follow that file statement for statement, because callers and tests depe
 exact behaviour; the CUDA kernels they call are this package's own.
 """
 
+import contextlib
 import os
 import weakref
 
@@ -322,6 +323,125 @@ def fused_linear(x, group, first, last=None, bias=None, transpose=False):
         _lib.ptr(group.levels), row0, rows, cols, group.qblock, group.qblock2, int(transpose),
         _lib.ptr(bias), _lib.ptr(y), y.stride(0), _lib.stream_of(a.device)), "talm_nf4_linear")
     return y.view(*x.shape[:-1], n_out)
+
+
+# Rows (tokens) that the few-row product takes in one call (csrc/nf4_matvec.cu).
+MATVEC_MAX_ROWS = 32
+
+
+def _few_rows(x, n_cols):
+    """`x` as [rows, n_cols] fp16 rows of unit stride, checked for the few-row product."""
+    if x.dtype != torch.float16:
+        raise TypeError(f"the few-row product takes fp16 rows, got {x.dtype}")
+    if x.shape[-1] != n_cols:
+        raise ValueError(f"last dimension {x.shape[-1]}, expected {n_cols}")
+    x = x.reshape(-1, n_cols)
+    if x.shape[0] > MATVEC_MAX_ROWS:
+        raise ValueError(f"the few-row product takes at most {MATVEC_MAX_ROWS} rows, got "
+                         f"{x.shape[0]}")
+    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < n_cols):
+        x = x.contiguous()
+    return x
+
+
+def run_matvec(x, packed, absmax8, absmax, code, absmax2, offset2, levels, row0, n_rows, n_cols,
+               blocksize, qblock2, bias, adapter, out):
+    """The checked call of talm_nf4_matvec behind `launch_matvec`, `matvec` and
+    `nf4_dequant.nf4_matvec`: x [rows, n_cols] from `_few_rows`, out [rows, n_rows]."""
+    device = x.get_device()
+    lora_a = lora_b = down = None
+    rank, scaling = 0, 0.0
+    if adapter is not None:
+        lora_a, lora_b, scaling = adapter
+        rank = lora_a.shape[0]
+        if lora_a.dtype != torch.float32 or lora_b.dtype != torch.float32:
+            raise TypeError("the adapter's A and B must be fp32")
+        if lora_a.shape != (rank, n_cols) or lora_b.shape != (n_rows, rank):
+            raise ValueError(f"adapter {tuple(lora_a.shape)}, {tuple(lora_b.shape)} does not map "
+                             f"{n_cols} to {n_rows}")
+        lora_a, lora_b = lora_a.contiguous(), lora_b.contiguous()
+        down = torch.empty(x.shape[0] * rank, dtype=torch.float32, device=x.device)
+    if bias is not None:
+        if bias.dtype != torch.float16 or bias.shape != (n_rows,):
+            raise ValueError(f"the bias must be fp16 [{n_rows}]")
+        bias = bias.contiguous()
+    if out.dtype != torch.float16 or out.shape != (x.shape[0], n_rows) or (
+            out.numel() and out.stride(1) != 1) or (x.shape[0] > 1 and out.stride(0) < n_rows):
+        raise ValueError(f"out must be fp16 [{x.shape[0]}, {n_rows}] with rows of unit stride")
+    pointers = []
+    for t in (x, packed, absmax8, absmax, code, absmax2, offset2, levels, bias, lora_a, lora_b,
+              down, out):
+        pointers.append(_lib.ptr(t))
+        if t is not None and t.get_device() != device:
+            raise ValueError("the operands of the few-row product must be on one device")
+    px, pp, p8, pm, pc, p2, po, pl, pb, pa, pB, pd, py = pointers
+    with _lib.device_of(x):
+        _lib.check(_lib.load().talm_nf4_matvec(
+            px, max(x.stride(0), n_cols), x.shape[0], pp, p8, pm, pc, p2, po, pl, row0, n_rows,
+            n_cols, blocksize, qblock2, pb, pa, pB, rank, scaling, pd, py,
+            max(out.stride(0), n_rows), _lib.raw_stream(x)), "talm_nf4_matvec")
+    RAN["matvec"] += 1
+    return out
+
+
+def launch_matvec(x, packed, absmax8, code, absmax2, offset2, levels, out, row0, n_rows, n_cols,
+                  qblock, qblock2, bias=None, adapter=None):
+    """x W^T (+ bias) (+ the adapter's branch) for at most 32 rows x [rows, n_cols] fp16 and the
+    n_rows x n_cols weight whose packed bytes and coded scales are given (`row0`: the group-wide
+    index of its first absmax row, which the second level is indexed by), into `out` [rows, n_rows]
+    fp16. The raw form of `matvec`, as `launch` is of `dequantize_all`; adapter = (lora_A [r,
+    n_cols], lora_B [n_rows, r], scaling), fp32."""
+    n = n_rows * n_cols
+    blocks = -(-n // qblock)
+    if 2 * packed.numel() < n or absmax8.numel() < blocks or code.numel() != 256 or (
+            min(absmax2.numel(), offset2.numel()) * qblock2 < row0 + blocks) or levels.numel() != 16:
+        raise ValueError("the packed weight or its scales are shorter than the weight")
+    for t, dtype in ((packed, torch.uint8), (absmax8, torch.uint8), (code, torch.float32),
+                     (absmax2, torch.float32), (offset2, torch.float32), (levels, torch.float32)):
+        if t.dtype != dtype or not t.is_contiguous():
+            raise ValueError(f"the packed weight's arrays must be contiguous, this one {dtype}")
+    return run_matvec(_few_rows(x, n_cols), packed, absmax8, None, code, absmax2, offset2, levels,
+                      row0, n_rows, n_cols, qblock, qblock2, bias, adapter, out)
+
+
+def matvec(x, group, first, last=None, bias=None, adapter=None):
+    """x W^T (+ bias) for a few rows, W projections first .. last - 1 of `group` (default: `first`
+    alone): x [..., in] fp16 of at most 32 rows -> [..., sum of out]. The weights are read packed
+    (a quarter of the fp16 bytes, none written) and not rounded to fp16 before the product; fp32
+    sums, one rounding. `adapter` = (lora_A [r, in], lora_B [sum of out, r], scaling) adds its
+    branch before the rounding. No gradient: the serving form of GroupLinear."""
+    last = first + 1 if last is None else last
+    packed, absmax8, row0, rows, cols = _span(group, first, last)
+    a = _few_rows(x, cols)
+    out = torch.empty(a.shape[0], rows, dtype=torch.float16, device=a.device)
+    run_matvec(a, packed, absmax8, None, group.code, group.absmax2, group.offset2, group.levels,
+               row0, rows, cols, group.qblock, group.qblock2, bias, adapter, out)
+    return out.view(*x.shape[:-1], rows)
+
+
+_SERVING = {"rows": 0}
+
+
+@contextlib.contextmanager
+def serving(rows=MATVEC_MAX_ROWS):
+    """Within it, 4-bit projections called without gradients on at most `rows` rows take `matvec`
+    instead of the layer's dequantised buffer (`NF4Linear`, and `LoraLinear` with its adapter in
+    the same call). For the whole process, as torch's global switches are."""
+    if not 0 <= rows <= MATVEC_MAX_ROWS:
+        raise ValueError(f"the few-row product takes 0..{MATVEC_MAX_ROWS} rows, got {rows}")
+    before = _SERVING["rows"]
+    _SERVING["rows"] = rows
+    try:
+        yield
+    finally:
+        _SERVING["rows"] = before
+
+
+def takes_matvec(x):
+    """Whether a projection of `x` is served by `matvec` now."""
+    limit = _SERVING["rows"]
+    return (limit > 0 and x.is_cuda and not torch.is_grad_enabled()
+            and 0 < x.numel() <= limit * x.shape[-1])
 
 
 class GroupLinear(torch.autograd.Function):

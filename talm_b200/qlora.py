@@ -27,7 +27,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from . import nf4_format, qgroup
+from . import adapter, nf4_format, qgroup
 
 LORA_TARGETS = ("self_attn.q_proj", "self_attn.v_proj")
 
@@ -51,12 +51,19 @@ class LoraLinear(torch.nn.Module):
     (solution/lora.py:151-231): dropout of the input, the fp32 adapter weights cast to fp16, two
     fp16 GEMMs ([T, in] x [in, r], then [T, r] x [r, out]), the product times scaling, added to
     the base output. A is Kaiming-uniform and B zero at initialisation, as PEFT does; autograd
-    derives the backward."""
+    derives the backward.
 
-    def __init__(self, base, r, alpha, dropout, generator=None, b_std=0.0):
+    With `fused` the branch runs through `adapter.lora_branch` (fp32 adapter weights and sums, one
+    rounding, dropout from a counter: other masks than torch's for the same torch seed, no mask
+    and no dropped copy kept); a branch that it does not take (another type, a rank over 64) through
+    `adapter.dropout` and the products above. Under `qgroup.serving`, a call without gradients and
+    without dropout on a few rows is one product with base, bias and adapter in it."""
+
+    def __init__(self, base, r, alpha, dropout, generator=None, b_std=0.0, fused=False):
         super().__init__()
         self.base = base
         self.r, self.scaling, self.dropout = r, alpha / r, dropout
+        self.fused = fused
         device = base.weight.device
         a = torch.empty(r, base.in_features, dtype=torch.float32, device=device)
         torch.nn.init.kaiming_uniform_(a, a=math.sqrt(5), generator=generator)
@@ -75,8 +82,18 @@ class LoraLinear(torch.nn.Module):
         return self.base.out_features
 
     def forward(self, x):
+        p = self.dropout if self.training else 0.0
+        if p == 0 and self.r <= adapter.MAX_RANK and isinstance(self.base, nf4_format.NF4Linear) \
+                and qgroup.takes_matvec(x):
+            return self.base.matvec(x, (self.lora_A, self.lora_B, self.scaling))
         out = self.base(x)
-        xd = F.dropout(x, self.dropout, self.training) if self.dropout > 0 else x
+        if self.fused:
+            seed = adapter.draw_seed(x.device) if p > 0 else None
+            if adapter.branch_takes(x, out, self.r):
+                return adapter.lora_branch(x, out, self.lora_A, self.lora_B, self.scaling, p, seed)
+            xd = adapter.dropout(x, p, seed) if p > 0 else x
+        else:
+            xd = F.dropout(x, self.dropout, self.training) if self.dropout > 0 else x
         t = torch.matmul(xd.to(torch.float16), self.lora_A.to(torch.float16).t())
         branch = torch.matmul(t, self.lora_B.to(torch.float16).t())
         return out + (branch * self.scaling).to(out.dtype)
@@ -143,13 +160,13 @@ def _replace(root, path, module):
 
 def build_model(config, device, seed=0, lora_r=16, lora_alpha=32, lora_dropout=0.05,
                 lora_targets=LORA_TARGETS, qblock=64, qblock2=256, weight_scale=0.035,
-                lora_b_std=0.0):
+                lora_b_std=0.0, lora_fused=False):
     """`Qwen2ForCausalLM(config)` in fp16 on `device` (random init from `seed`), its decoder
     projections 4-bit (`NF4Linear`, one `LayerGroup` per layer, loaded from a synthetic stored
     checkpoint) and LoRA on `lora_targets`; every parameter but the adapters frozen. The fp16
     projection weights the constructor made are freed layer by layer before the 4-bit ones are
     loaded. `lora_b_std` > 0 starts B at random instead of zero (tests use it to give A a
-    gradient on the first step)."""
+    gradient on the first step); `lora_fused` gives the adapters the fused branch."""
     from transformers import Qwen2ForCausalLM
 
     device = torch.device(device)
@@ -181,7 +198,7 @@ def build_model(config, device, seed=0, lora_r=16, lora_alpha=32, lora_dropout=0
         for path, module in modules.items():
             if path in lora_targets:
                 module = LoraLinear(module, lora_r, lora_alpha, lora_dropout, lora_generator,
-                                    lora_b_std)
+                                    lora_b_std, lora_fused)
             _replace(layer, path, module)
         layer._talm_layer_group = group
         layer._talm_group_done = True
@@ -229,6 +246,29 @@ def train_step(model, optimizer, batch):
     optimizer.step()
     optimizer.zero_grad(set_to_none=True)
     return out.loss.detach()
+
+
+@torch.no_grad()
+def generate(model, input_ids, new_tokens):
+    """Greedy decoding of `new_tokens` tokens after the prompts input_ids [B, S] (B at most 32 rows
+    of one length): one pass over the prompt, then one token of every row per pass with the
+    decoder's key-value cache. Passes of at most 32 tokens run under `qgroup.serving`: each 4-bit
+    projection is a few-row product with the packed weights, its adapter included. The model is
+    put into evaluation mode for the call. Returns [B, S + new_tokens]."""
+    was_training = model.training
+    model.eval()
+    try:
+        ids, step, cache = input_ids, input_ids, None
+        with qgroup.serving():
+            for _ in range(new_tokens):
+                out = model(input_ids=step, past_key_values=cache, use_cache=True,
+                            logits_to_keep=1)
+                cache = out.past_key_values
+                step = out.logits[:, -1].argmax(-1, keepdim=True)
+                ids = torch.cat([ids, step], dim=1)
+        return ids
+    finally:
+        model.train(was_training)
 
 
 def causal_padding_mask(attention_mask):
