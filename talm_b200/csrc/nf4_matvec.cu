@@ -132,10 +132,12 @@ constexpr int WARPS = 16;
 constexpr int STEP_BLOCKS = 4;  // blocks of 64 columns that a warp loads ahead
 constexpr float LEVEL_GAIN = 1.6776883602142334f;
 constexpr int LUT_BYTES = 256 * 32 * 4;
+constexpr int STAGES = 4;       // a warp's ring of steps
+constexpr int STAGE_BYTES = 16 * 32 * STEP_BLOCKS;
 
 template <int NT>
 constexpr int mma_smem() {
-  return LUT_BYTES + 256 * 4 + WARPS * 16 * 8 * NT * 4;
+  return LUT_BYTES + WARPS * STAGES * STAGE_BYTES + 256 * 4 + WARPS * 16 * 8 * NT * 4;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -155,45 +157,67 @@ struct Split {
   int shift2;          // log2(qblock2)
 };
 
-// What a lane has loaded of one step: the packed bytes of its two rows, and the scale inputs of
-// one block (block t of the step) of each row.
-struct Step {
-  uint2 w[2][STEP_BLOCKS];
+// The scale inputs that a lane has loaded for one step: those of block t of the step for its two
+// rows (the quad exchanges the finished scales).
+struct ScaleIn {
   float s[2], a2[2], o2[2];
   uint32_t a8[2];
 };
 
 template <bool GROUPED>
-__device__ __forceinline__ void load_step(Step& st, const Weight& w, const Split& sp,
-                                          const int64_t (&row)[2], int b0, int b1, int t) {
+__device__ __forceinline__ void load_scales(ScaleIn& in, const Weight& w, const Split& sp,
+                                            int64_t row0, int64_t row1, int b) {
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const uint8_t* p = w.packed + row[h] * (w.n_in >> 1) + t * 8;
-#pragma unroll
-    for (int i = 0; i < STEP_BLOCKS; ++i) {
-      const int b = b0 + i < b1 ? b0 + i : b1 - 1;
-      st.w[h][i] = __ldg(reinterpret_cast<const uint2*>(p + static_cast<int64_t>(b) * 32));
-    }
-    const int b = b0 + t < b1 ? b0 + t : b1 - 1;
-    const int64_t block = (row[h] * w.n_in + int64_t{b} * 64) >> sp.shift;
+    const int64_t block = ((h ? row1 : row0) * w.n_in + int64_t{b} * 64) >> sp.shift;
     if constexpr (GROUPED) {
       const int64_t second = (w.row0 + block) >> sp.shift2;
-      st.a8[h] = __ldg(w.absmax8 + block);
-      st.a2[h] = __ldg(w.absmax2 + second);
-      st.o2[h] = __ldg(w.offset2 + second);
+      in.a8[h] = __ldg(w.absmax8 + block);
+      in.a2[h] = __ldg(w.absmax2 + second);
+      in.o2[h] = __ldg(w.offset2 + second);
     } else {
-      st.s[h] = __ldg(w.absmax + block);
+      in.s[h] = __ldg(w.absmax + block);
     }
   }
+}
+
+// x of rows 8 q + g (zeros past n_rows), the 16 columns of lane t in block b
+template <int NT>
+__device__ __forceinline__ void load_x(uint32_t (&v)[NT][8], const __half* x, int64_t ld_x,
+                                       int n_rows, int g, int t, int b) {
+#pragma unroll
+  for (int q = 0; q < NT; ++q) {
+    const int n = q * 8 + g;
+    uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
+    if (n < n_rows) {
+      const uint4* p = reinterpret_cast<const uint4*>(x + n * ld_x + b * 64 + t * 16);
+      v0 = __ldg(p);
+      v1 = __ldg(p + 1);
+    }
+    v[q][0] = v0.x; v[q][1] = v0.y; v[q][2] = v0.z; v[q][3] = v0.w;
+    v[q][4] = v1.x; v[q][5] = v1.y; v[q][6] = v1.z; v[q][7] = v1.w;
+  }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 template <int NT, bool GROUPED>
 __global__ void __launch_bounds__(32 * WARPS, 1)
     nf4_mma_kernel(const __half* __restrict__ x, int64_t ld_x, int n_rows, Weight w, Split sp,
                    Epilogue ep, __half* __restrict__ y, int64_t ld_y) {
-  extern __shared__ __align__(16) uint32_t mv_smem[];
+  extern __shared__ __align__(128) uint32_t mv_smem[];
   uint32_t* lut = mv_smem;                                        // [256][32]
-  float* code_s = reinterpret_cast<float*>(lut + 256 * 32);       // [256]
+  uint8_t* rings = reinterpret_cast<uint8_t*>(lut + 256 * 32);    // [WARPS][STAGES][16][128]
+  float* code_s = reinterpret_cast<float*>(rings + WARPS * STAGES * STAGE_BYTES);  // [256]
   float* part = code_s + 256;                                     // [WARPS][8 NT rows of x][16]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -201,28 +225,59 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
   const int group = warp / W, share = warp % W;
   const int b_first = static_cast<int>(int64_t{sp.n_blocks} * share / W);
   const int b_last = static_cast<int>(int64_t{sp.n_blocks} * (share + 1) / W);
+  const int n_steps = (b_last - b_first + STEP_BLOCKS - 1) / STEP_BLOCKS;  // of one tile
   const int stride = gridDim.x * groups;
-  int tile = blockIdx.x * groups + group;
+  const int first_tile = blockIdx.x * groups + group;
 
-  auto rows_of = [&](int tl, int64_t (&row)[2]) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t r = int64_t{tl} * 16 + g + 8 * h;
-      row[h] = r < w.n_out ? r : w.n_out - 1;  // rows past the end read the last one's bytes
-    }
-  };
   auto sync_tile = [&] {  // the warps of this tile; W >= 2 leaves at most eight barriers
     if (W == 1)
       __syncwarp();
     else
       named_barrier(1 + group, 32 * W);
   };
-  int64_t row[2];
-  Step cur;
-  const bool any = b_first < b_last;
-  rows_of(tile < sp.n_tiles ? tile : sp.n_tiles - 1, row);
-  if (any) load_step<GROUPED>(cur, w, sp, row, b_first, b_last, t);
+  // rows past the end read the last one's bytes
+  auto row_of = [&](int tile, int r) {
+    const int64_t v = int64_t{tile} * 16 + r;
+    return v < w.n_out ? v : w.n_out - 1;
+  };
 
+  // This warp's ring of packed bytes: a stage holds four blocks (128 bytes) of the tile's 16 rows,
+  // the 16-byte chunk c of row r at chunk c ^ (r & 7) (the reads of eight rows then meet in no
+  // bank). The warp fills and reads it alone, STAGES - 1 steps ahead.
+  const uint32_t ring = smem_u32(rings) + warp * (STAGES * STAGE_BYTES);
+  int f_tile = first_tile, f_b = b_first, f_stage = 0;
+  auto fetch = [&] {
+    if (f_tile < sp.n_tiles && n_steps > 0) {
+      const int chunk = lane & 7;
+      if (f_b + (chunk >> 1) < b_last) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * i + (lane >> 3);
+          const uint8_t* src = w.packed + row_of(f_tile, r) * (w.n_in >> 1) +
+                               static_cast<int64_t>(f_b) * 32 + chunk * 16;
+          cp_async16(ring + f_stage * STAGE_BYTES + r * 128 + ((chunk ^ (r & 7)) << 4), src);
+        }
+      }
+      f_b += STEP_BLOCKS;
+      if (f_b >= b_last) {
+        f_b = b_first;
+        f_tile += stride;
+      }
+      f_stage = f_stage + 1 == STAGES ? 0 : f_stage + 1;
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) fetch();
+
+  const bool any = n_steps > 0 && first_tile < sp.n_tiles;
+  ScaleIn cur;
+  uint32_t xv[NT][8];
+  if (any) {
+    load_scales<GROUPED>(cur, w, sp, row_of(first_tile, g), row_of(first_tile, g + 8),
+                         min(b_first + t, b_last - 1));
+    load_x<NT>(xv, x, ld_x, n_rows, g, t, b_first);
+  }
   static_assert(32 * WARPS == 512, "two threads fill the 32 copies of a table entry");
   {
     const int i = threadIdx.x & 255, half = threadIdx.x >> 8;
@@ -237,18 +292,24 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
   }
   __syncthreads();
   const uint32_t* my_lut = lut + lane;
+  const uint8_t* my_ring = rings + warp * (STAGES * STAGE_BYTES) + g * 128 + (t & 1) * 8;
 
-  for (; tile < sp.n_tiles; tile += stride) {
+  int stage = 0;
+  for (int tile = first_tile; tile < sp.n_tiles; tile += stride) {
     float acc[NT][4] = {};
     for (int b = b_first; b < b_last; b += STEP_BLOCKS) {
-      Step next;
-      const bool more = b + STEP_BLOCKS < b_last;
-      if (more) {
-        load_step<GROUPED>(next, w, sp, row, b + STEP_BLOCKS, b_last, t);
-      } else if (tile + stride < sp.n_tiles) {
-        rows_of(tile + stride, row);
-        load_step<GROUPED>(next, w, sp, row, b_first, b_last, t);
-      }
+      fetch();
+      cp_async_wait<STAGES - 1>();
+      __syncwarp();  // every lane's copies of this stage have landed
+      // the step after this one (of the next tile behind the last): scales now, x block by block
+      const bool last = b + STEP_BLOCKS >= b_last;
+      const int n_tile = last ? tile + stride : tile;
+      const int n_b = last ? b_first : b + STEP_BLOCKS;
+      const bool more = n_tile < sp.n_tiles;
+      ScaleIn next = cur;
+      if (more)
+        load_scales<GROUPED>(next, w, sp, row_of(n_tile, g), row_of(n_tile, g + 8),
+                             min(n_b + t, b_last - 1));
       float mine[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -259,29 +320,23 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
           s = cur.s[h];
         mine[h] = s * (1.0f / LEVEL_GAIN);
       }
+      const uint8_t* st = my_ring + stage * STAGE_BYTES;
 #pragma unroll
       for (int i = 0; i < STEP_BLOCKS; ++i) {
+        if (b + i >= b_last) break;  // the same for the whole warp
         const float s0 = __shfl_sync(0xffffffffu, mine[0], (lane & 28) | i);
         const float s1 = __shfl_sync(0xffffffffu, mine[1], (lane & 28) | i);
-        if (b + i >= b_last) continue;  // the same for the whole warp
-        uint32_t xv[NT][8];
-#pragma unroll
-        for (int q = 0; q < NT; ++q) {
-          const int n = q * 8 + g;
-          uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
-          if (n < n_rows) {
-            const uint4* xp = reinterpret_cast<const uint4*>(x + n * ld_x + (b + i) * 64 + t * 16);
-            v0 = __ldg(xp);
-            v1 = __ldg(xp + 1);
-          }
-          xv[q][0] = v0.x; xv[q][1] = v0.y; xv[q][2] = v0.z; xv[q][3] = v0.w;
-          xv[q][4] = v1.x; xv[q][5] = v1.y; xv[q][6] = v1.z; xv[q][7] = v1.w;
-        }
+        uint32_t xn[NT][8];
+        const bool in_step = i + 1 < STEP_BLOCKS && b + i + 1 < b_last;
+        if (in_step || more)
+          load_x<NT>(xn, x, ld_x, n_rows, g, t, in_step ? b + i + 1 : n_b);
+        const int at = ((2 * i + (t >> 1)) ^ g) << 4;
+        const uint2 wa2 = *reinterpret_cast<const uint2*>(st + at);
+        const uint2 wb2 = *reinterpret_cast<const uint2*>(st + 8 * 128 + at);
         float c[NT][4] = {};
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const uint32_t wa = m < 2 ? cur.w[0][i].x : cur.w[0][i].y;
-          const uint32_t wb = m < 2 ? cur.w[1][i].x : cur.w[1][i].y;
+          const uint32_t wa = m < 2 ? wa2.x : wa2.y, wb = m < 2 ? wb2.x : wb2.y;
           const int sh = 16 * (m & 1);
           const uint32_t a[4] = {my_lut[((wa >> sh) & 0xFFu) * 32],
                                  my_lut[((wb >> sh) & 0xFFu) * 32],
@@ -296,8 +351,12 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
           acc[q][1] = fmaf(s0, c[q][1], acc[q][1]);
           acc[q][2] = fmaf(s1, c[q][2], acc[q][2]);
           acc[q][3] = fmaf(s1, c[q][3], acc[q][3]);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) xv[q][k] = xn[q][k];
         }
       }
+      __syncwarp();  // the stage has been read; the next fetch may fill it
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
       cur = next;
     }
     // the warps of a tile add their shares in share order
@@ -329,6 +388,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
     }
     sync_tile();
   }
+  cp_async_wait<0>();
 }
 
 // Launches the tensor-core kernel for NT groups of eight rows.
