@@ -130,7 +130,7 @@ def device_of(t):
     """A context in which the CUDA tensor's device is the current one (a launch takes the current
     device's kernels); free where it already is."""
     index = t.get_device()
-    return _HERE if index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
 
 
 KERNEL_KINDS = ("head_slice", "head_combine", "head_reserved", "head_finalize", "head_merge",

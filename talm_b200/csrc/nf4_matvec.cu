@@ -37,77 +37,111 @@ struct Weight {
 
 struct Epilogue {
   const __half* bias;   // null: none
-  const float* t;       // [n_rows, rank] or null
+  const float* t;       // [parts, n_rows, rank] (t is the sum over the parts) or null
   const float* lora_b;  // [n_out, rank]
-  int rank;
+  int rank, parts;
   float scaling;
 };
 
-// t = x A^T: a CTA takes eight rows of x and two of A, its warps share the reduction.
-constexpr int DOWN_WARPS = 8;
-constexpr int DOWN_ROWS = 8;
-constexpr int DOWN_RANKS = 2;
+// fp32 on the tensor cores: an operand is split into a tf32 part (11 significant bits, cut off) and
+// the exact rest, whose own tf32 part leaves 2^-21 of the operand. mma.sync m16n8k8.
+__device__ __forceinline__ void split_tf32(float v, uint32_t& hi, uint32_t& lo) {
+  hi = __float_as_uint(v) & 0xFFFFE000u;
+  lo = __float_as_uint(v - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
-template <bool VEC>
+// t = x A^T in DOWN_PARTS or fewer partial sums over the columns (the product that reads t adds
+// them up): CTA (j, p) takes 16 rows of A and part p of the columns, its warps share those. fp16
+// x is exact in tf32, A is split in two.
+constexpr int DOWN_WARPS = 16;
+constexpr int DOWN_PARTS = 8;
+
+template <int NT, bool VEC>
 __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
     const __half* __restrict__ x, int64_t ld_x, const float* __restrict__ a, int n_in, int n_rows,
-    int rank, float* __restrict__ t) {
-  __shared__ float part[DOWN_WARPS][DOWN_ROWS * DOWN_RANKS];
+    int rank, float* __restrict__ t_out) {
+  __shared__ float part[DOWN_WARPS][128 * NT];
   // the product that follows may start now: it reads t only after it has waited for this grid
   grid_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n0 = blockIdx.x * DOWN_ROWS, j0 = blockIdx.y * DOWN_RANKS;
-  const int nt = min(DOWN_ROWS, n_rows - n0);
-  const bool two = j0 + 1 < rank;
-  const float* a0 = a + int64_t{j0} * n_in;
-  const float* a1 = two ? a0 + n_in : a0;
-  float acc[DOWN_ROWS * DOWN_RANKS] = {};
-  constexpr int STEP = VEC ? 4 : 1;
-  for (int k = (warp * 32 + lane) * STEP; k < n_in; k += 32 * DOWN_WARPS * STEP) {
-    float v0[STEP], v1[STEP];
-    if constexpr (VEC) {
+  const int g = lane >> 2, t = lane & 3;
+  const int j0 = blockIdx.x * 16;
+  const float* a0 = a + int64_t{min(j0 + g, rank - 1)} * n_in;
+  const float* a1 = a + int64_t{min(j0 + g + 8, rank - 1)} * n_in;
+  const __half* xp[NT];
+#pragma unroll
+  for (int q = 0; q < NT; ++q) xp[q] = x + min(q * 8 + g, n_rows - 1) * ld_x;
+  float acc[NT][4] = {};
+  // steps of 16 columns, four consecutive ones per lane of a quad
+  const int steps = (n_in + 15) / 16;
+  const int shares = gridDim.y * DOWN_WARPS, share = blockIdx.y * DOWN_WARPS + warp;
+#pragma unroll 2
+  for (int s = share; s < steps; s += shares) {
+    const int k = s * 16 + t * 4;
+    float v0[4], v1[4];
+    uint32_t xv[NT][4];
+    if (VEC && k + 4 <= n_in) {
       const float4 f0 = __ldg(reinterpret_cast<const float4*>(a0 + k));
       const float4 f1 = __ldg(reinterpret_cast<const float4*>(a1 + k));
       v0[0] = f0.x; v0[1] = f0.y; v0[2] = f0.z; v0[3] = f0.w;
       v1[0] = f1.x; v1[1] = f1.y; v1[2] = f1.z; v1[3] = f1.w;
-    } else {
-      v0[0] = __ldg(a0 + k);
-      v1[0] = __ldg(a1 + k);
-    }
 #pragma unroll
-    for (int n = 0; n < DOWN_ROWS; ++n) {
-      if (n >= nt) break;
-      const __half* xr = x + (n0 + n) * ld_x + k;
-      float xv[STEP];
-      if constexpr (VEC) {
-        const uint2 h = __ldg(reinterpret_cast<const uint2*>(xr));
+      for (int q = 0; q < NT; ++q) {
+        const uint2 h = __ldg(reinterpret_cast<const uint2*>(xp[q] + k));
         const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&h.x));
         const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
-        xv[0] = lo.x; xv[1] = lo.y; xv[2] = hi.x; xv[3] = hi.y;
-      } else {
-        xv[0] = __half2float(xr[0]);
+        xv[q][0] = __float_as_uint(lo.x);
+        xv[q][1] = __float_as_uint(lo.y);
+        xv[q][2] = __float_as_uint(hi.x);
+        xv[q][3] = __float_as_uint(hi.y);
       }
+    } else {
 #pragma unroll
-      for (int i = 0; i < STEP; ++i) {
-        acc[2 * n] = fmaf(xv[i], v0[i], acc[2 * n]);
-        acc[2 * n + 1] = fmaf(xv[i], v1[i], acc[2 * n + 1]);
+      for (int i = 0; i < 4; ++i) {
+        const bool in = k + i < n_in;
+        v0[i] = in ? __ldg(a0 + k + i) : 0.0f;
+        v1[i] = in ? __ldg(a1 + k + i) : 0.0f;
+#pragma unroll
+        for (int q = 0; q < NT; ++q)
+          xv[q][i] = in ? __float_as_uint(__half2float(xp[q][k + i])) : 0u;
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t hi[4], lo[4];
+      split_tf32(v0[2 * h], hi[0], lo[0]);
+      split_tf32(v1[2 * h], hi[1], lo[1]);
+      split_tf32(v0[2 * h + 1], hi[2], lo[2]);
+      split_tf32(v1[2 * h + 1], hi[3], lo[3]);
+#pragma unroll
+      for (int q = 0; q < NT; ++q) {
+        mma_tf32(acc[q], lo, xv[q][2 * h], xv[q][2 * h + 1]);
+        mma_tf32(acc[q], hi, xv[q][2 * h], xv[q][2 * h + 1]);
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < DOWN_ROWS * DOWN_RANKS; ++i) {
-    if (i >= 2 * nt) break;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], d);
-    if (lane == 0) part[warp][i] = acc[i];
+  for (int q = 0; q < NT; ++q) {
+    part[warp][(q * 8 + 2 * t) * 16 + g] = acc[q][0];
+    part[warp][(q * 8 + 2 * t + 1) * 16 + g] = acc[q][1];
+    part[warp][(q * 8 + 2 * t) * 16 + g + 8] = acc[q][2];
+    part[warp][(q * 8 + 2 * t + 1) * 16 + g + 8] = acc[q][3];
   }
   __syncthreads();
-  const int n = threadIdx.x / DOWN_RANKS, j = threadIdx.x % DOWN_RANKS;
-  if (n < nt && j0 + j < rank) {
+  for (int i = threadIdx.x; i < 16 * n_rows; i += blockDim.x) {
+    const int n = i >> 4, j = j0 + (i & 15);
     float sum = 0.0f;
 #pragma unroll
-    for (int w = 0; w < DOWN_WARPS; ++w) sum += part[w][threadIdx.x];
-    t[(n0 + n) * rank + j0 + j] = sum;
+    for (int v = 0; v < DOWN_WARPS; ++v) sum += part[v][i];
+    if (j < rank) t_out[(int64_t{blockIdx.y} * n_rows + n) * rank + j] = sum;
   }
 }
 
@@ -118,7 +152,9 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 // A warp takes tiles of 16 weight rows; lane (g, t) = (lane / 4, lane % 4) reads 8 packed bytes of
 // rows g and g + 8 per block (a quad reads a row's 32 bytes) and turns each byte into the fp16
 // pair of its two levels by one shared-memory read: a table of 256 pairs, one copy per lane, so
-// that no two lanes meet in a bank. The reduction index may be permuted as long as both operands
+// that no two lanes meet in a bank. Entries lie 256 bytes apart (the second 128 are not used), so
+// that one byte permutation makes the address: the packed byte above the lane's own four-byte
+// offset. The reduction index may be permuted as long as both operands
 // agree, so a lane's 16 consecutive weights go into four mma's as they are and the matching
 // operand is 32 consecutive bytes of x. A block's 64 columns have one scale per row: its four
 // mma's start from zero and their result is added to the fp32 sum with one FMA per value, times
@@ -131,7 +167,7 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 constexpr int WARPS = 16;
 constexpr int STEP_BLOCKS = 4;  // blocks of 64 columns that a warp loads ahead
 constexpr float LEVEL_GAIN = 1.6776883602142334f;
-constexpr int LUT_BYTES = 256 * 32 * 4;
+constexpr int LUT_BYTES = 256 * 256;
 constexpr int STAGES = 4;       // a warp's ring of steps
 constexpr int STAGE_BYTES = 16 * 32 * STEP_BLOCKS;
 
@@ -149,8 +185,18 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4],
+                                              uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 struct Split {
-  int warps_per_tile;  // W: warps that share a tile's columns (a power of two up to WARPS)
+  int log_w;           // log2 of W, the warps of a CTA that share a tile's columns
+  int cluster;         // CTAs that share a tile's columns
   int n_tiles;         // 16-row tiles
   int n_blocks;        // 64-column blocks of a row
   int shift;           // log2(blocksize)
@@ -166,10 +212,10 @@ struct ScaleIn {
 
 template <bool GROUPED>
 __device__ __forceinline__ void load_scales(ScaleIn& in, const Weight& w, const Split& sp,
-                                            int64_t row0, int64_t row1, int b) {
+                                            const int64_t (&first)[2], int b) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int64_t block = ((h ? row1 : row0) * w.n_in + int64_t{b} * 64) >> sp.shift;
+  for (int h = 0; h < 2; ++h) {  // first[h]: the flattened index of the row's first weight
+    const int64_t block = (first[h] + b * 64) >> sp.shift;
     if constexpr (GROUPED) {
       const int64_t second = (w.row0 + block) >> sp.shift2;
       in.a8[h] = __ldg(w.absmax8 + block);
@@ -181,21 +227,14 @@ __device__ __forceinline__ void load_scales(ScaleIn& in, const Weight& w, const 
   }
 }
 
-// x of rows 8 q + g (zeros past n_rows), the 16 columns of lane t in block b
+// x of rows 8 q + g, the 16 columns of lane t in block b
 template <int NT>
-__device__ __forceinline__ void load_x(uint32_t (&v)[NT][8], const __half* x, int64_t ld_x,
-                                       int n_rows, int g, int t, int b) {
+__device__ __forceinline__ void load_x(uint4 (&v)[NT][2], const __half* const (&xp)[NT], int b) {
 #pragma unroll
   for (int q = 0; q < NT; ++q) {
-    const int n = q * 8 + g;
-    uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
-    if (n < n_rows) {
-      const uint4* p = reinterpret_cast<const uint4*>(x + n * ld_x + b * 64 + t * 16);
-      v0 = __ldg(p);
-      v1 = __ldg(p + 1);
-    }
-    v[q][0] = v0.x; v[q][1] = v0.y; v[q][2] = v0.z; v[q][3] = v0.w;
-    v[q][4] = v1.x; v[q][5] = v1.y; v[q][6] = v1.z; v[q][7] = v1.w;
+    const uint4* p = reinterpret_cast<const uint4*>(xp[q] + b * 64);
+    v[q][0] = __ldg(p);
+    v[q][1] = __ldg(p + 1);
   }
 }
 
@@ -215,19 +254,25 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
     nf4_mma_kernel(const __half* __restrict__ x, int64_t ld_x, int n_rows, Weight w, Split sp,
                    Epilogue ep, __half* __restrict__ y, int64_t ld_y) {
   extern __shared__ __align__(128) uint32_t mv_smem[];
-  uint32_t* lut = mv_smem;                                        // [256][32]
-  uint8_t* rings = reinterpret_cast<uint8_t*>(lut + 256 * 32);    // [WARPS][STAGES][16][128]
-  float* code_s = reinterpret_cast<float*>(rings + WARPS * STAGES * STAGE_BYTES);  // [256]
-  float* part = code_s + 256;                                     // [WARPS][8 NT rows of x][16]
+  uint8_t* lut = reinterpret_cast<uint8_t*>(mv_smem);             // [256][256]
+  uint8_t* rings = lut + LUT_BYTES;                               // [WARPS][STAGES][16][128]
+  float* part = reinterpret_cast<float*>(rings + WARPS * STAGES * STAGE_BYTES);
+  float* code_s = part + WARPS * 128 * NT;  // part: [WARPS][8 NT rows of x][16]; code: [256]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int W = sp.warps_per_tile, groups = WARPS / W;
-  const int group = warp / W, share = warp % W;
-  const int b_first = static_cast<int>(int64_t{sp.n_blocks} * share / W);
-  const int b_last = static_cast<int>(int64_t{sp.n_blocks} * (share + 1) / W);
+  // W warps of each of the cluster's CTAs share a tile's columns; a CTA works on WARPS / W tiles
+  const int W = 1 << sp.log_w, groups = WARPS >> sp.log_w;
+  const int group = warp >> sp.log_w, share = warp & (W - 1);
+  const int rank = NT == 1 ? 0 : static_cast<int>(cluster_ctarank());
+  const int shares = NT == 1 ? W : W * sp.cluster;
+  const int place = rank * W + share;
+  const int b_first = static_cast<int>(static_cast<unsigned>(sp.n_blocks) * place / shares);
+  const int b_last = static_cast<int>(static_cast<unsigned>(sp.n_blocks) * (place + 1) / shares);
   const int n_steps = (b_last - b_first + STEP_BLOCKS - 1) / STEP_BLOCKS;  // of one tile
-  const int stride = gridDim.x * groups;
-  const int first_tile = blockIdx.x * groups + group;
+  const int stride = (NT == 1 ? gridDim.x : gridDim.x / sp.cluster) * groups;
+  const int base_tile = (NT == 1 ? blockIdx.x : blockIdx.x / sp.cluster) * groups;
+  const int first_tile = base_tile + group;
+  const int n_out = static_cast<int>(w.n_out);
 
   auto sync_tile = [&] {  // the warps of this tile; W >= 2 leaves at most eight barriers
     if (W == 1)
@@ -236,34 +281,40 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
       named_barrier(1 + group, 32 * W);
   };
   // rows past the end read the last one's bytes
-  auto row_of = [&](int tile, int r) {
-    const int64_t v = int64_t{tile} * 16 + r;
-    return v < w.n_out ? v : w.n_out - 1;
-  };
+  auto row_of = [&](int tile, int r) { return static_cast<int64_t>(min(tile * 16 + r, n_out - 1)); };
 
   // This warp's ring of packed bytes: a stage holds four blocks (128 bytes) of the tile's 16 rows,
   // the 16-byte chunk c of row r at chunk c ^ (r & 7) (the reads of eight rows then meet in no
   // bank). The warp fills and reads it alone, STAGES - 1 steps ahead.
   const uint32_t ring = smem_u32(rings) + warp * (STAGES * STAGE_BYTES);
-  int f_tile = first_tile, f_b = b_first, f_stage = 0;
+  const int chunk = lane & 7, r8 = lane >> 3;  // this lane copies that chunk of rows r8 + 4 i
+  const uint32_t dst0 = ring + r8 * 128 + ((chunk ^ r8) << 4);
+  const uint32_t dst1 = ring + (r8 + 4) * 128 + ((chunk ^ (r8 + 4)) << 4);
+  const uint8_t* src[4];
+  auto aim = [&](int tile) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      src[i] = w.packed + row_of(tile, 4 * i + r8) * (w.n_in >> 1) + chunk * 16;
+  };
+  int f_tile = first_tile, f_b = b_first;
+  uint32_t f_at = 0;
+  if (n_steps > 0 && f_tile < sp.n_tiles) aim(f_tile);
   auto fetch = [&] {
     if (f_tile < sp.n_tiles && n_steps > 0) {
-      const int chunk = lane & 7;
       if (f_b + (chunk >> 1) < b_last) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = 4 * i + (lane >> 3);
-          const uint8_t* src = w.packed + row_of(f_tile, r) * (w.n_in >> 1) +
-                               static_cast<int64_t>(f_b) * 32 + chunk * 16;
-          cp_async16(ring + f_stage * STAGE_BYTES + r * 128 + ((chunk ^ (r & 7)) << 4), src);
-        }
+        const int off = f_b * 32;
+        cp_async16(dst0 + f_at, src[0] + off);
+        cp_async16(dst1 + f_at, src[1] + off);
+        cp_async16(dst0 + f_at + 1024, src[2] + off);
+        cp_async16(dst1 + f_at + 1024, src[3] + off);
       }
       f_b += STEP_BLOCKS;
       if (f_b >= b_last) {
         f_b = b_first;
         f_tile += stride;
+        if (f_tile < sp.n_tiles) aim(f_tile);
       }
-      f_stage = f_stage + 1 == STAGES ? 0 : f_stage + 1;
+      f_at = f_at + STAGE_BYTES == STAGES * STAGE_BYTES ? 0 : f_at + STAGE_BYTES;
     }
     cp_async_commit();
   };
@@ -271,12 +322,22 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
   for (int i = 0; i < STAGES - 1; ++i) fetch();
 
   const bool any = n_steps > 0 && first_tile < sp.n_tiles;
+  const __half* xp[NT];
+#pragma unroll
+  for (int q = 0; q < NT; ++q)
+    // rows past n_rows read the last one: their columns of the result are not stored
+    xp[q] = x + min(q * 8 + g, n_rows - 1) * ld_x + t * 16;
+  int64_t e[2];  // of the tile whose scales are loaded: the flattened index of rows g and g + 8
+  auto first_of = [&](int tile) {
+    e[0] = row_of(tile, g) * w.n_in;
+    e[1] = row_of(tile, g + 8) * w.n_in;
+  };
   ScaleIn cur;
-  uint32_t xv[NT][8];
+  uint4 xv[NT][2];
   if (any) {
-    load_scales<GROUPED>(cur, w, sp, row_of(first_tile, g), row_of(first_tile, g + 8),
-                         min(b_first + t, b_last - 1));
-    load_x<NT>(xv, x, ld_x, n_rows, g, t, b_first);
+    first_of(first_tile);
+    load_scales<GROUPED>(cur, w, sp, e, min(b_first + t, b_last - 1));
+    load_x<NT>(xv, xp, b_first);
   }
   static_assert(32 * WARPS == 512, "two threads fill the 32 copies of a table entry");
   {
@@ -287,17 +348,25 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
     const uint4 four = make_uint4(pair, pair, pair, pair);
 #pragma unroll
     for (int k = 0; k < 4; ++k)  // eight neighbours write eight different bank groups
-      reinterpret_cast<uint4*>(lut)[i * 8 + ((4 * half + k + i) & 7)] = four;
+      reinterpret_cast<uint4*>(lut)[i * 16 + ((4 * half + k + i) & 7)] = four;
     if (GROUPED && half == 0) code_s[i] = __ldg(w.code + i);
   }
   __syncthreads();
-  const uint32_t* my_lut = lut + lane;
+  // the pair of byte i of v: bytes (lane * 4, v.i, 0, 0) are the entry's offset
+  const char* const lut_bytes = reinterpret_cast<const char*>(mv_smem);
+  const uint32_t lane4 = lane * 4;
+  auto level_pair = [&](uint32_t v, int i) {
+    return *reinterpret_cast<const uint32_t*>(lut_bytes + __byte_perm(v, lane4, 0x5504 | (i << 4)));
+  };
   const uint8_t* my_ring = rings + warp * (STAGES * STAGE_BYTES) + g * 128 + (t & 1) * 8;
 
   int stage = 0;
-  for (int tile = first_tile; tile < sp.n_tiles; tile += stride) {
+  // every warp of a cluster makes the same rounds, those without a tile in the last one too
+  for (int base = base_tile; base < sp.n_tiles; base += stride) {
+    const int tile = base + group;
+    const bool has = tile < sp.n_tiles;
     float acc[NT][4] = {};
-    for (int b = b_first; b < b_last; b += STEP_BLOCKS) {
+    for (int b = has ? b_first : b_last; b < b_last; b += STEP_BLOCKS) {
       fetch();
       cp_async_wait<STAGES - 1>();
       __syncwarp();  // every lane's copies of this stage have landed
@@ -307,9 +376,10 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
       const int n_b = last ? b_first : b + STEP_BLOCKS;
       const bool more = n_tile < sp.n_tiles;
       ScaleIn next = cur;
-      if (more)
-        load_scales<GROUPED>(next, w, sp, row_of(n_tile, g), row_of(n_tile, g + 8),
-                             min(n_b + t, b_last - 1));
+      if (more) {
+        if (last) first_of(n_tile);
+        load_scales<GROUPED>(next, w, sp, e, min(n_b + t, b_last - 1));
+      }
       float mine[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -321,29 +391,27 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
         mine[h] = s * (1.0f / LEVEL_GAIN);
       }
       const uint8_t* st = my_ring + stage * STAGE_BYTES;
-#pragma unroll
-      for (int i = 0; i < STEP_BLOCKS; ++i) {
-        if (b + i >= b_last) break;  // the same for the whole warp
-        const float s0 = __shfl_sync(0xffffffffu, mine[0], (lane & 28) | i);
-        const float s1 = __shfl_sync(0xffffffffu, mine[1], (lane & 28) | i);
-        uint32_t xn[NT][8];
-        const bool in_step = i + 1 < STEP_BLOCKS && b + i + 1 < b_last;
-        if (in_step || more)
-          load_x<NT>(xn, x, ld_x, n_rows, g, t, in_step ? b + i + 1 : n_b);
+      // block b + i of this step with its x in xv
+      auto block = [&](int i, const uint4 (&xb)[NT][2]) {
+        const float s0 = __shfl_sync(0xffffffffu, mine[0], i, 4);
+        const float s1 = __shfl_sync(0xffffffffu, mine[1], i, 4);
         const int at = ((2 * i + (t >> 1)) ^ g) << 4;
         const uint2 wa2 = *reinterpret_cast<const uint2*>(st + at);
         const uint2 wb2 = *reinterpret_cast<const uint2*>(st + 8 * 128 + at);
-        float c[NT][4] = {};
+        float c[NT][4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
           const uint32_t wa = m < 2 ? wa2.x : wa2.y, wb = m < 2 ? wb2.x : wb2.y;
-          const int sh = 16 * (m & 1);
-          const uint32_t a[4] = {my_lut[((wa >> sh) & 0xFFu) * 32],
-                                 my_lut[((wb >> sh) & 0xFFu) * 32],
-                                 my_lut[((wa >> (sh + 8)) & 0xFFu) * 32],
-                                 my_lut[((wb >> (sh + 8)) & 0xFFu) * 32]};
+          const uint32_t a[4] = {level_pair(wa, 2 * (m & 1)), level_pair(wb, 2 * (m & 1)),
+                                 level_pair(wa, 2 * (m & 1) + 1), level_pair(wb, 2 * (m & 1) + 1)};
 #pragma unroll
-          for (int q = 0; q < NT; ++q) mma_f16(c[q], a, xv[q][2 * m], xv[q][2 * m + 1]);
+          for (int q = 0; q < NT; ++q) {
+            const uint4& h = xb[q][m >> 1];
+            if (m == 0)
+              mma_f16_first(c[q], a, h.x, h.y);
+            else
+              mma_f16(c[q], a, m & 1 ? h.z : h.x, m & 1 ? h.w : h.y);
+          }
         }
 #pragma unroll
         for (int q = 0; q < NT; ++q) {
@@ -351,15 +419,77 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
           acc[q][1] = fmaf(s0, c[q][1], acc[q][1]);
           acc[q][2] = fmaf(s1, c[q][2], acc[q][2]);
           acc[q][3] = fmaf(s1, c[q][3], acc[q][3]);
+        }
+      };
+      const int ahead = more ? n_b : b;  // whose x is loaded behind this step's
+      if (b + STEP_BLOCKS <= b_last) {
+        uint4 xw[NT][2];
+        load_x<NT>(xw, xp, b + 1);
+        block(0, xv);
+        load_x<NT>(xv, xp, b + 2);
+        block(1, xw);
+        load_x<NT>(xw, xp, b + 3);
+        block(2, xv);
+        load_x<NT>(xv, xp, ahead);
+        block(3, xw);
+      } else {  // the share's ragged end
+#pragma unroll 1
+        for (int i = 0; b + i < b_last; ++i) {
+          uint4 xw[NT][2];
+          load_x<NT>(xw, xp, b + i + 1 < b_last ? b + i + 1 : ahead);
+          block(i, xv);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) xv[q][k] = xn[q][k];
+          for (int q = 0; q < NT; ++q) {
+            xv[q][0] = xw[q][0];
+            xv[q][1] = xw[q][1];
+          }
         }
       }
       __syncwarp();  // the stage has been read; the next fetch may fill it
       stage = stage + 1 == STAGES ? 0 : stage + 1;
       cur = next;
     }
-    // the warps of a tile add their shares in share order
+    // the outputs that this thread finishes, bias first: i = (row of x) * 16 + (row of the tile)
+    const int i0 = (rank * W + share) * 32 + lane, i_step = 32 * shares;
+    const int o = tile * 16 + (lane & 15);  // i0 and i_step are multiples of 16 apart
+    const float bias = ep.bias != nullptr && has && o < n_out ? __half2float(ep.bias[o]) : 0.0f;
+    if (ep.t != nullptr && has) {
+      // scaling * t B^T, eight columns of the rank per share, as tf32 products of split operands
+      // (without the product of the two rests): lane columns j + 2 t and j + 2 t + 1
+      bool waited = false;
+      for (int j = 8 * place; j < ep.rank; j += 8 * shares) {
+        float bv[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float* br = ep.lora_b + row_of(tile, g + 8 * h) * ep.rank;
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            bv[h + 2 * u] = j + 2 * t + u < ep.rank ? __ldg(br + j + 2 * t + u) * ep.scaling : 0.0f;
+        }
+        uint32_t b_hi[4], b_lo[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) split_tf32(bv[u], b_hi[u], b_lo[u]);
+        if (!waited) grid_dependency_wait();  // t comes from the launch before this one
+        waited = true;
+#pragma unroll
+        for (int q = 0; q < NT; ++q) {
+          const int n = min(q * 8 + g, n_rows - 1);
+          float tv[2] = {};
+          for (int k = 0; k < ep.parts; ++k) {
+            const float* tp = ep.t + (static_cast<int64_t>(k) * n_rows + n) * ep.rank + j + 2 * t;
+            if (j + 2 * t < ep.rank) tv[0] += __ldcg(tp);
+            if (j + 2 * t + 1 < ep.rank) tv[1] += __ldcg(tp + 1);
+          }
+          uint32_t t_hi[2], t_lo[2];
+          split_tf32(tv[0], t_hi[0], t_lo[0]);
+          split_tf32(tv[1], t_hi[1], t_lo[1]);
+          mma_tf32(acc[q], b_lo, t_hi[0], t_hi[1]);
+          mma_tf32(acc[q], b_hi, t_lo[0], t_lo[1]);
+          mma_tf32(acc[q], b_hi, t_hi[0], t_hi[1]);
+        }
+      }
+    }
+    // the tile's warps add their shares in share order, then the cluster's CTAs in rank order
     float* mine = part + warp * (128 * NT);
 #pragma unroll
     for (int q = 0; q < NT; ++q) {
@@ -369,26 +499,40 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
       mine[(q * 8 + 2 * t + 1) * 16 + g + 8] = acc[q][3];
     }
     sync_tile();
-    if (ep.t != nullptr) grid_dependency_wait();  // t comes from the launch before this one
-    for (int i = share * 32 + lane; i < 16 * n_rows; i += 32 * W) {
-      const int n = i >> 4;
-      const int64_t o = int64_t{tile} * 16 + (i & 15);
-      if (o >= w.n_out) continue;
-      float v = 0.0f;
-      for (int k = 0; k < W; ++k) v += part[(group * W + k) * (128 * NT) + i];
-      if (ep.t != nullptr) {
-        float extra = 0.0f;
-#pragma unroll 8
-        for (int j = 0; j < ep.rank; ++j)
-          extra = fmaf(__ldcg(ep.t + n * ep.rank + j), __ldg(ep.lora_b + o * ep.rank + j), extra);
-        v = fmaf(ep.scaling, extra, v);
+    float* sums = part + (group << sp.log_w) * (128 * NT);
+    if constexpr (NT == 1) {
+      if (has && o < n_out)
+        for (int i = i0; i < 16 * n_rows; i += i_step) {
+          float v = sums[i];
+          for (int k = 1; k < W; ++k) v += sums[k * (128 * NT) + i];
+          y[(i >> 4) * ld_y + o] = __float2half_rn(v + bias);
+        }
+      sync_tile();
+    } else {
+      if (W > 1) {
+        for (int i = share * 32 + lane; i < 16 * n_rows; i += 32 * W) {
+          float v = sums[i];
+          for (int k = 1; k < W; ++k) v += sums[k * (128 * NT) + i];
+          sums[i] = v;
+        }
       }
-      if (ep.bias != nullptr) v += __half2float(ep.bias[o]);
-      y[n * ld_y + o] = __float2half_rn(v);
+      cluster_sync();
+      if (has && o < n_out)
+        for (int i = i0; i < 16 * n_rows; i += i_step) {
+          const uint32_t at = smem_u32(sums + i);
+          float v = 0.0f;
+          for (int c = 0; c < sp.cluster; ++c) {
+            float p;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p) : "r"(mapa_shared(at, c)));
+            v += p;
+          }
+          y[(i >> 4) * ld_y + o] = __float2half_rn(v + bias);
+        }
+      cluster_sync();  // the sums have been read by every CTA
     }
-    sync_tile();
   }
   cp_async_wait<0>();
+  if (ep.t != nullptr) grid_dependency_wait();  // no CTA completes before the launch it follows
 }
 
 // Launches the tensor-core kernel for NT groups of eight rows.
@@ -409,24 +553,55 @@ int run_mma(const __half* x, int64_t ld_x, int n_rows, const Weight& w, Split sp
   }
   const int sms = current_sm_count();
   if (sms <= 0) return set_error(TALM_ENODEV, "no CUDA device");
-  int W = 1;
-  while (W < WARPS && int64_t{sp.n_tiles} * W < int64_t{sms} * WARPS && W < sp.n_blocks) W *= 2;
-  sp.warps_per_tile = W;
-  const int groups = WARPS / W;
-  const int ctas = (sp.n_tiles + groups - 1) / groups;
-  const int cap = sms;
+  // How many warps (and CTAs) share a tile's columns: the least time by a model in units of one
+  // block of one warp, ~720 cycles at 16 warps per SM: the blocks a warp runs one after another in
+  // every round of tiles, three more for the epilogue, two for a cluster's barriers, and the rows of
+  // x that a CTA reads from L2 (64 bytes per cycle) for its share of the columns. (gate + up of
+  // one row, 1120 tiles of 24 blocks: W = 2 one round of 12 + 3, W = 4 two of 6 + 3; down_proj of
+  // 32 rows: a cluster of 4 reads a quarter of 573 KB per CTA.) Clusters of 4 find 33 places.
+  int64_t least = -1;
+  int groups = 1, clusters = 1;
+  for (int c = 1; c <= (NT == 1 ? 1 : 4); c *= 2) {
+    for (int lw = 0; (1 << lw) <= WARPS; ++lw) {
+      const int64_t places = c == 4 ? sms * 33 / 148 : sms / c;
+      const int64_t slots = (places > 0 ? places : 1) * (WARPS >> lw);
+      const int64_t rounds = (sp.n_tiles + slots - 1) / slots;
+      const int64_t blocks = (sp.n_blocks + (c << lw) - 1) / (c << lw);
+      const int64_t x_read = int64_t{n_rows} * sp.n_blocks * 128 / c / (64 * 720);
+      const int64_t cost = rounds * (blocks * (NT == 4 ? 2 : 1) + 3 + (c > 1 ? 2 : 0) + x_read);
+      if (least < 0 || cost < least) {
+        least = cost;
+        sp.log_w = lw;
+        sp.cluster = c;
+        groups = WARPS >> lw;
+        clusters = static_cast<int>(places);
+      }
+    }
+  }
+  const int wanted = (sp.n_tiles + groups - 1) / groups;
+  const int grid = (wanted < clusters ? wanted : clusters) * sp.cluster;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas < cap ? ctas : cap), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
   cfg.blockDim = dim3(32 * WARPS, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
-  // behind the adapter's down kernel only: it starts once everything before it has completed, and
-  // this kernel waits for it before it reads t
-  cfg.numAttrs = ep.t != nullptr ? 1 : 0;
+  cfg.numAttrs = 0;
+  if (NT > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(sp.cluster);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  if (ep.t != nullptr) {
+    // behind the adapter's down kernel only: that one starts once everything before it has
+    // completed, and this kernel waits for it before it reads t
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
   const cudaError_t e = cudaLaunchKernelEx(&cfg, nf4_mma_kernel<NT, GROUPED>, x, ld_x, n_rows, w,
                                            sp, ep, y, ld_y);
   if (e != cudaSuccess) return set_error(TALM_ECUDA, "nf4 matvec: %s", cudaGetErrorString(e));
@@ -474,8 +649,12 @@ __global__ void __launch_bounds__(256) nf4_matvec_any_kernel(const __half* __res
       if (n0 + n >= n_rows) break;
       float extra = 0.0f;
       if (ep.t != nullptr)
-        for (int j = lane; j < ep.rank; j += 32)
-          extra = fmaf(ep.t[(n0 + n) * ep.rank + j], ep.lora_b[o * ep.rank + j], extra);
+        for (int j = lane; j < ep.rank; j += 32) {
+          float t = 0.0f;
+          for (int k = 0; k < ep.parts; ++k)
+            t += ep.t[(static_cast<int64_t>(k) * n_rows + n0 + n) * ep.rank + j];
+          extra = fmaf(t, ep.lora_b[o * ep.rank + j], extra);
+        }
       float v = fmaf(ep.scaling, extra, acc[n]);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -516,7 +695,7 @@ int talm_nf4_matvec(const uint16_t* x, int64_t ld_x, int64_t n_rows, const uint8
     return set_error(TALM_EINVAL, "adapter rank %lld is not in 0..%d", (long long)rank, MAX_RANK);
   if (ld_x < w_cols || ld_y < w_rows)
     return set_error(TALM_EINVAL, "row strides must cover the rows");
-  if (w_cols >= (int64_t{1} << 31) || w_rows >= (int64_t{1} << 31) ||
+  if (w_cols >= (int64_t{1} << 30) || w_rows >= (int64_t{1} << 30) ||
       (w_rows > 0 && w_cols > (int64_t{1} << 40) / w_rows))
     return set_error(TALM_ERANGE, "weight of %lld x %lld is beyond the kernel's range",
                      (long long)w_rows, (long long)w_cols);
@@ -527,30 +706,34 @@ int talm_nf4_matvec(const uint16_t* x, int64_t ld_x, int64_t n_rows, const uint8
     return set_error(TALM_EINVAL, "null pointer");
   const Weight w{packed, absmax8, absmax,      code,      absmax2, offset2,
                  levels, absmax_row0, blocksize, qblock2, w_rows,  w_cols};
-  const Epilogue ep{reinterpret_cast<const __half*>(bias), rank > 0 ? down : nullptr, lora_b,
-                    static_cast<int>(rank), scaling};
   const __half* xh = reinterpret_cast<const __half*>(x);
+  int parts = 0;
   if (rank > 0) {
     LaunchTimer timer(TALM_KERNEL_ADAPTER_DOWN, stream);
-    const dim3 grid(static_cast<unsigned>((n_rows + DOWN_ROWS - 1) / DOWN_ROWS),
-                    static_cast<unsigned>((rank + DOWN_RANKS - 1) / DOWN_RANKS), 1);
+    // as many parts as leave each a thousand columns
+    parts = static_cast<int>(w_cols / 1024 < 1 ? 1 : w_cols / 1024);
+    parts = parts < DOWN_PARTS ? parts : DOWN_PARTS;
+    const dim3 grid(static_cast<unsigned>((rank + 15) / 16), static_cast<unsigned>(parts), 1);
     const bool vec = w_cols % 4 == 0 && ld_x % 4 == 0 &&
                      (reinterpret_cast<uintptr_t>(x) & 7) == 0 &&
                      (reinterpret_cast<uintptr_t>(lora_a) & 15) == 0;
-    auto kernel = vec ? adapter_down_kernel<true> : adapter_down_kernel<false>;
+    auto kernel = n_rows <= 8 ? (vec ? adapter_down_kernel<1, true> : adapter_down_kernel<1, false>)
+                              : (vec ? adapter_down_kernel<4, true> : adapter_down_kernel<4, false>);
     kernel<<<grid, 32 * DOWN_WARPS, 0, stream>>>(xh, ld_x, lora_a, static_cast<int>(w_cols),
                                                  static_cast<int>(n_rows),
                                                  static_cast<int>(rank), down);
     const int st = check_launch("adapter down kernel");
     if (st != TALM_OK) return st;
   }
+  const Epilogue ep{reinterpret_cast<const __half*>(bias), rank > 0 ? down : nullptr, lora_b,
+                    static_cast<int>(rank), parts, scaling};
   LaunchTimer timer(TALM_KERNEL_NF4_MATVEC, stream);
   // The tensor-core kernel takes whole 64-column blocks of one scale each, on the boundaries of its
   // wide loads; anything else the byte-wise kernel.
   const int shift = log2_exact(blocksize), shift2 = absmax8 ? log2_exact(qblock2) : 0;
   if (w_cols % 64 == 0 && shift >= 6 && shift2 >= 0 && ld_x % 8 == 0 &&
       (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(packed) & 7) == 0) {
-    const Split sp{1, static_cast<int>((w_rows + 15) / 16), static_cast<int>(w_cols / 64), shift,
+    const Split sp{0, 1, static_cast<int>((w_rows + 15) / 16), static_cast<int>(w_cols / 64), shift,
                    shift2};
     __half* yh = reinterpret_cast<__half*>(y);
     const int n = static_cast<int>(n_rows);

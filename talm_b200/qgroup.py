@@ -330,56 +330,71 @@ MATVEC_MAX_ROWS = 32
 
 
 def _few_rows(x, n_cols):
-    """`x` as [rows, n_cols] fp16 rows of unit stride, checked for the few-row product."""
-    if x.dtype != torch.float16:
+    """`x` as [rows, n_cols] fp16 rows of unit stride that the wide loads take (a view where they
+    lie that way, else a copy), checked for the few-row product."""
+    if x.dtype is not torch.float16:
         raise TypeError(f"the few-row product takes fp16 rows, got {x.dtype}")
     if x.shape[-1] != n_cols:
         raise ValueError(f"last dimension {x.shape[-1]}, expected {n_cols}")
-    x = x.reshape(-1, n_cols)
-    if x.shape[0] > MATVEC_MAX_ROWS:
-        raise ValueError(f"the few-row product takes at most {MATVEC_MAX_ROWS} rows, got "
-                         f"{x.shape[0]}")
-    if x.stride(1) != 1 or (x.shape[0] > 1 and x.stride(0) < n_cols):
-        x = x.contiguous()
+    if x.dim() != 2:
+        x = x.reshape(-1, n_cols)
+    n = x.shape[0]
+    if n > MATVEC_MAX_ROWS:
+        raise ValueError(f"the few-row product takes at most {MATVEC_MAX_ROWS} rows, got {n}")
+    if x.is_contiguous():
+        return x if x.data_ptr() % 16 == 0 else x.clone()
+    ld, unit = x.stride()
+    if unit != 1 or ld < n_cols or ld % 8 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
 def run_matvec(x, packed, absmax8, absmax, code, absmax2, offset2, levels, row0, n_rows, n_cols,
                blocksize, qblock2, bias, adapter, out):
-    """The checked call of talm_nf4_matvec behind `launch_matvec`, `matvec` and
-    `nf4_dequant.nf4_matvec`: x [rows, n_cols] from `_few_rows`, out [rows, n_rows]."""
-    device = x.get_device()
-    lora_a = lora_b = down = None
-    rank, scaling = 0, 0.0
+    """The call of talm_nf4_matvec behind `launch_matvec`, `matvec` and `nf4_dequant.nf4_matvec`:
+    x [rows, n_cols] from `_few_rows`, out [rows, n_rows], the weight's arrays checked by those."""
+    ptr = _lib.ptr
+    n, device = x.shape[0], x.get_device()
+    ld_y = n_rows
+    if out.dtype is not torch.float16 or out.shape != (n, n_rows):
+        raise ValueError(f"out must be fp16 [{n}, {n_rows}]")
+    if not out.is_contiguous():
+        ld_y = out.stride(0) if n > 1 else n_rows
+        if (n_rows > 1 and out.stride(1) != 1) or ld_y < n_rows:
+            raise ValueError("out must have rows of unit stride that do not overlap")
     if adapter is not None:
         lora_a, lora_b, scaling = adapter
         rank = lora_a.shape[0]
-        if lora_a.dtype != torch.float32 or lora_b.dtype != torch.float32:
+        if lora_a.dtype is not torch.float32 or lora_b.dtype is not torch.float32:
             raise TypeError("the adapter's A and B must be fp32")
         if lora_a.shape != (rank, n_cols) or lora_b.shape != (n_rows, rank):
             raise ValueError(f"adapter {tuple(lora_a.shape)}, {tuple(lora_b.shape)} does not map "
                              f"{n_cols} to {n_rows}")
+    if absmax8 is None:
+        scales = (None, ptr(absmax), None, None, None, None)
+        apart = absmax.get_device() != device
+    else:
+        scales = (ptr(absmax8), None, ptr(code), ptr(absmax2), ptr(offset2), ptr(levels))
+        apart = not (absmax8.get_device() == code.get_device() == absmax2.get_device()
+                     == offset2.get_device() == levels.get_device() == device)
+    extra = (None, None, 0, 0.0, None)
+    if adapter is not None:
         lora_a, lora_b = lora_a.contiguous(), lora_b.contiguous()
-        down = torch.empty(x.shape[0] * rank, dtype=torch.float32, device=x.device)
+        down = torch.empty(8 * n * rank, dtype=torch.float32, device=x.device)
+        extra = (ptr(lora_a), ptr(lora_b), rank, scaling, ptr(down))
+        apart = apart or not lora_a.get_device() == lora_b.get_device() == device
     if bias is not None:
-        if bias.dtype != torch.float16 or bias.shape != (n_rows,):
+        if bias.dtype is not torch.float16 or bias.shape != (n_rows,):
             raise ValueError(f"the bias must be fp16 [{n_rows}]")
         bias = bias.contiguous()
-    if out.dtype != torch.float16 or out.shape != (x.shape[0], n_rows) or (
-            out.numel() and out.stride(1) != 1) or (x.shape[0] > 1 and out.stride(0) < n_rows):
-        raise ValueError(f"out must be fp16 [{x.shape[0]}, {n_rows}] with rows of unit stride")
-    pointers = []
-    for t in (x, packed, absmax8, absmax, code, absmax2, offset2, levels, bias, lora_a, lora_b,
-              down, out):
-        pointers.append(_lib.ptr(t))
-        if t is not None and t.get_device() != device:
-            raise ValueError("the operands of the few-row product must be on one device")
-    px, pp, p8, pm, pc, p2, po, pl, pb, pa, pB, pd, py = pointers
+        apart = apart or bias.get_device() != device
+    if apart or not packed.get_device() == out.get_device() == device:
+        raise ValueError("the operands of the few-row product must be on one device")
     with _lib.device_of(x):
         _lib.check(_lib.load().talm_nf4_matvec(
-            px, max(x.stride(0), n_cols), x.shape[0], pp, p8, pm, pc, p2, po, pl, row0, n_rows,
-            n_cols, blocksize, qblock2, pb, pa, pB, rank, scaling, pd, py,
-            max(out.stride(0), n_rows), _lib.raw_stream(x)), "talm_nf4_matvec")
+            ptr(x), x.stride(0) if n > 1 else n_cols, n, ptr(packed), *scales, row0, n_rows,
+            n_cols, blocksize, qblock2, None if bias is None else ptr(bias), *extra, ptr(out),
+            ld_y, _lib.raw_stream(x)), "talm_nf4_matvec")
     RAN["matvec"] += 1
     return out
 
@@ -396,10 +411,13 @@ def launch_matvec(x, packed, absmax8, code, absmax2, offset2, levels, out, row0,
     if 2 * packed.numel() < n or absmax8.numel() < blocks or code.numel() != 256 or (
             min(absmax2.numel(), offset2.numel()) * qblock2 < row0 + blocks) or levels.numel() != 16:
         raise ValueError("the packed weight or its scales are shorter than the weight")
-    for t, dtype in ((packed, torch.uint8), (absmax8, torch.uint8), (code, torch.float32),
-                     (absmax2, torch.float32), (offset2, torch.float32), (levels, torch.float32)):
-        if t.dtype != dtype or not t.is_contiguous():
-            raise ValueError(f"the packed weight's arrays must be contiguous, this one {dtype}")
+    if not (packed.dtype is torch.uint8 is absmax8.dtype
+            and code.dtype is torch.float32 is absmax2.dtype
+            and offset2.dtype is torch.float32 is levels.dtype):
+        raise ValueError("packed and absmax8 must be uint8, the other arrays fp32")
+    if not (packed.is_contiguous() and absmax8.is_contiguous() and code.is_contiguous()
+            and absmax2.is_contiguous() and offset2.is_contiguous() and levels.is_contiguous()):
+        raise ValueError("the packed weight's arrays must be contiguous")
     return run_matvec(_few_rows(x, n_cols), packed, absmax8, None, code, absmax2, offset2, levels,
                       row0, n_rows, n_cols, qblock, qblock2, bias, adapter, out)
 
