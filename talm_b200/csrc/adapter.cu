@@ -75,25 +75,132 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
 }
 
-// One thread per group of eight elements of the flattened tensor.
+// All ones in each half of the result whose element is kept: the 15-bit draws of a word plus
+// 0x8000 - drop carry into bit 15 of their own half exactly when they reach the threshold, and the
+// permutation copies that bit over the half.
+__device__ __forceinline__ uint32_t keep_mask2(uint32_t word, uint32_t bias2) {
+  const uint32_t sum = (word & 0x7FFF7FFFu) + bias2;
+  uint32_t mask;
+  asm("prmt.b32 %0, %1, 0, 0xBB99;" : "=r"(mask) : "r"(sum));
+  return mask;
+}
+__device__ __forceinline__ uint32_t keep_bias2(uint32_t drop) {
+  return (0x8000u - drop) * 0x10001u;
+}
+
+__device__ __forceinline__ uint32_t scale2(uint32_t v, float f, __half) {
+  const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return pack_half2(p.x * f, p.y * f);
+}
+__device__ __forceinline__ uint32_t scale2(uint32_t v, float f, __nv_bfloat16) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(__uint_as_float(v << 16) * f,
+                                                 __uint_as_float(v & 0xFFFF0000u) * f);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// The flattened tensor on 16-byte boundaries: a thread takes UNROLL groups of eight elements, their
+// loads first.
+template <class T, int UNROLL>
+__global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, int64_t n,
+                                                      Dropout d, T* __restrict__ y) {
+  constexpr int V = sizeof(T) == 4 ? 2 : 1;  // 16-byte pieces of a group
+  const uint64_t key = static_cast<uint64_t>(__ldg(d.seed));
+  const uint32_t bias2 = keep_bias2(d.drop);
+  const int64_t n_groups = n >> 3;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * (256 * UNROLL);
+  for (int64_t q0 = static_cast<int64_t>(blockIdx.x) * (256 * UNROLL) + threadIdx.x;
+       q0 < n_groups; q0 += stride) {
+    uint4 v[UNROLL][V];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (q0 + u * 256 < n_groups)
+          v[u][i] = __ldg(reinterpret_cast<const uint4*>(x) + (q0 + u * 256) * V + i);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int64_t q = q0 + u * 256;
+      if (q >= n_groups) break;
+      uint32_t c[4];
+      philox(static_cast<uint64_t>(q), key, c);
+      uint4* out = reinterpret_cast<uint4*>(y) + q * V;
+      if constexpr (V == 1) {
+        const uint4 w = v[u][0];
+        out[0] = make_uint4(scale2(w.x, d.factor, T()) & keep_mask2(c[0], bias2),
+                            scale2(w.y, d.factor, T()) & keep_mask2(c[1], bias2),
+                            scale2(w.z, d.factor, T()) & keep_mask2(c[2], bias2),
+                            scale2(w.w, d.factor, T()) & keep_mask2(c[3], bias2));
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const uint32_t w[4] = {v[u][i].x, v[u][i].y, v[u][i].z, v[u][i].w};
+          uint32_t r[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            r[k] = kept(c, 4 * i + k, d.drop) ? __float_as_uint(__uint_as_float(w[k]) * d.factor)
+                                              : 0u;
+          out[i] = make_uint4(r[0], r[1], r[2], r[3]);
+        }
+      }
+    }
+  }
+  // the elements behind the last whole group
+  const int tail = static_cast<int>(n & 7);
+  if (tail != 0 && blockIdx.x == 0 && threadIdx.x < tail) {
+    uint32_t c[4];
+    philox(static_cast<uint64_t>(n_groups), key, c);
+    const int64_t e = 8 * n_groups + threadIdx.x;
+    y[e] = kept(c, threadIdx.x, d.drop) ? from_f32<T>(to_f32(x[e]) * d.factor) : from_f32<T>(0.0f);
+  }
+}
+
+// Any strides and alignment: one thread per group of eight elements in row-major order.
 template <class T>
-__global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, int64_t ld_x,
-                                                      int64_t n_cols, int64_t n, Dropout d,
-                                                      T* __restrict__ y) {
+__global__ void __launch_bounds__(256) dropout_rows_kernel(const T* __restrict__ x, int64_t ld_x,
+                                                           int64_t n_cols, int64_t n, Dropout d,
+                                                           T* __restrict__ y) {
   const uint64_t key = static_cast<uint64_t>(*d.seed);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
   for (int64_t q = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; 8 * q < n;
        q += stride) {
     uint32_t c[4];
     philox(static_cast<uint64_t>(q), key, c);
+    int64_t row = 8 * q / n_cols, col = 8 * q - row * n_cols;
     for (int i = 0; i < 8; ++i) {
       const int64_t e = 8 * q + i;
       if (e >= n) break;
-      const int64_t row = e / n_cols;
-      const float v = to_f32(x[row * ld_x + (e - row * n_cols)]);
+      const float v = to_f32(x[row * ld_x + col]);
       y[e] = kept(c, i, d.drop) ? from_f32<T>(v * d.factor) : from_f32<T>(0.0f);
+      if (++col == n_cols) {
+        col = 0;
+        ++row;
+      }
     }
   }
+}
+
+template <class T>
+int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, const Dropout& d,
+                void* y_, cudaStream_t stream) {
+  const T* x = static_cast<const T*>(x_);
+  T* y = static_cast<T*>(y_);
+  const int64_t n = n_rows * n_cols;
+  const int sms = current_sm_count();
+  if (sms <= 0) return set_error(TALM_ENODEV, "no CUDA device");
+  LaunchTimer timer(TALM_KERNEL_DROPOUT, stream);
+  const bool flat = ld_x == n_cols || n_rows == 1;
+  const int64_t cap = int64_t{sms} * 8;
+  if (flat && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0) {
+    constexpr int UNROLL = sizeof(T) == 4 ? 2 : 4;
+    const int64_t want = (n / 8 + 256 * UNROLL - 1) / (256 * UNROLL);
+    const int64_t grid = want < 1 ? 1 : want < cap ? want : cap;
+    dropout_kernel<T, UNROLL><<<static_cast<unsigned>(grid), 256, 0, stream>>>(x, n, d, y);
+  } else {
+    const int64_t want = (n + 2047) / 2048;
+    dropout_rows_kernel<<<static_cast<unsigned>(want < cap ? want : cap), 256, 0, stream>>>(
+        x, ld_x, n_cols, n, d, y);
+  }
+  return check_launch("dropout kernel");
 }
 
 // ------------------------------------------------------------------------------------------
@@ -301,22 +408,10 @@ int talm_dropout(const void* x, int64_t ld_x, int64_t n_rows, int64_t n_cols, in
   if (n_rows == 0 || n_cols == 0) return TALM_OK;
   if (n_cols > (int64_t{1} << 48) / n_rows) return set_error(TALM_ERANGE, "too many elements");
   if (!x || !y || !seed) return set_error(TALM_EINVAL, "null pointer");
-  const int64_t n = n_rows * n_cols;
-  const int sms = current_sm_count();
-  if (sms <= 0) return set_error(TALM_ENODEV, "no CUDA device");
-  const int64_t want = (n + 2047) / 2048;
-  const unsigned grid = static_cast<unsigned>(want < int64_t{sms} * 8 ? want : int64_t{sms} * 8);
-  LaunchTimer timer(TALM_KERNEL_DROPOUT, stream);
-  if (dtype == TALM_DTYPE_F16)
-    dropout_kernel<<<grid, 256, 0, stream>>>(static_cast<const __half*>(x), ld_x, n_cols, n, d,
-                                             static_cast<__half*>(y));
-  else if (dtype == TALM_DTYPE_BF16)
-    dropout_kernel<<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16*>(x), ld_x, n_cols,
-                                             n, d, static_cast<__nv_bfloat16*>(y));
-  else
-    dropout_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(x), ld_x, n_cols, n, d,
-                                             static_cast<float*>(y));
-  return check_launch("dropout kernel");
+  if (dtype == TALM_DTYPE_F16) return run_dropout<__half>(x, ld_x, n_rows, n_cols, d, y, stream);
+  if (dtype == TALM_DTYPE_BF16)
+    return run_dropout<__nv_bfloat16>(x, ld_x, n_rows, n_cols, d, y, stream);
+  return run_dropout<float>(x, ld_x, n_rows, n_cols, d, y, stream);
 }
 
 int talm_lora_sizes(int64_t n_rows, int64_t n_in, int64_t n_out, int64_t rank, size_t* saved,
