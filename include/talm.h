@@ -179,9 +179,9 @@ int talm_nf4_matvec(const uint16_t* x, int64_t ld_x, int64_t n_rows, const uint8
 int talm_dropout(const void* x, int64_t ld_x, int64_t n_rows, int64_t n_cols, int dtype,
                  const int64_t* seed, int64_t drop, void* y, void* stream);
 
-/* Bytes that talm_lora_forward saves for talm_lora_backward, and of the backward's workspace. */
+/* Bytes that talm_lora_forward saves for talm_lora_backward, and of the two workspaces. */
 int talm_lora_sizes(int64_t n_rows, int64_t n_in, int64_t n_out, int64_t rank, size_t* saved,
-                    size_t* backward_ws);
+                    size_t* forward_ws, size_t* backward_ws);
 
 /* The adapter's branch added to the frozen projection's product:
  *   y = fp16(base + scaling * (dropout(x) lora_a^T) lora_b^T)
@@ -190,12 +190,14 @@ int talm_lora_sizes(int64_t n_rows, int64_t n_in, int64_t n_out, int64_t rank, s
  *   x, base, y : fp16 [n_rows, n_in], [n_rows, n_out], [n_rows, n_out] (y contiguous), rows 16-byte
  *                aligned with strides of a multiple of 8 elements
  *   lora_a, lora_b : fp32 [rank, n_in], [n_out, rank], contiguous
- *   saved : talm_lora_sizes bytes, 16-byte aligned, kept for the backward
+ *   saved : talm_lora_sizes bytes, 16-byte aligned, kept for the backward; workspace likewise,
+ *           free again once the call's work is done
  * Preconditions: n_in and n_out multiples of 8, 1 <= rank <= 64. */
 int talm_lora_forward(const uint16_t* x, int64_t ld_x, const uint16_t* base, int64_t ld_base,
                       const float* lora_a, const float* lora_b, int64_t n_rows, int64_t n_in,
                       int64_t n_out, int64_t rank, float scaling, const int64_t* seed,
-                      int64_t drop, uint16_t* y, void* saved, size_t saved_bytes, void* stream);
+                      int64_t drop, uint16_t* y, void* saved, size_t saved_bytes,
+                      void* workspace, size_t ws_bytes, void* stream);
 
 /* The gradients of talm_lora_forward for the output gradient g (fp16 [n_rows, n_out]):
  *   dt = scaling g lora_b, grad_b = scaling g^T t, grad_a = dt^T dropout(x),

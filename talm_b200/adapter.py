@@ -117,10 +117,10 @@ def branch_takes(x, base, rank):
 
 
 def _sizes(n_rows, n_in, n_out, rank):
-    saved, work = _lib._SZ(0), _lib._SZ(0)
-    _lib.check(_lib.load().talm_lora_sizes(n_rows, n_in, n_out, rank, saved, work),
+    saved, forward, backward = _lib._SZ(0), _lib._SZ(0), _lib._SZ(0)
+    _lib.check(_lib.load().talm_lora_sizes(n_rows, n_in, n_out, rank, saved, forward, backward),
                "talm_lora_sizes")
-    return saved.value, work.value
+    return saved.value, forward.value, backward.value
 
 
 class _LoraBranch(torch.autograd.Function):
@@ -130,14 +130,16 @@ class _LoraBranch(torch.autograd.Function):
         a, b = lora_a.contiguous(), lora_b.contiguous()
         xr, br = _rows16(x, n_in), _rows16(base, n_out)
         n_rows = xr.shape[0]
-        saved_bytes, ctx.work_bytes = _sizes(n_rows, n_in, n_out, rank)
+        saved_bytes, work_bytes, ctx.work_bytes = _sizes(n_rows, n_in, n_out, rank)
         y = torch.empty(base.shape, dtype=base.dtype, device=x.device)
         saved = torch.empty(saved_bytes, dtype=torch.uint8, device=x.device)
+        work = torch.empty(work_bytes, dtype=torch.uint8, device=x.device)
         with _lib.device_of(x):
             _lib.check(_lib.load().talm_lora_forward(
                 _lib.ptr(xr), _stride(xr), _lib.ptr(br), _stride(br), _lib.ptr(a), _lib.ptr(b),
                 n_rows, n_in, n_out, rank, scaling, _lib.ptr(seed), drop, _lib.ptr(y),
-                _lib.ptr(saved), saved_bytes, _lib.raw_stream(x)), "talm_lora_forward")
+                _lib.ptr(saved), saved_bytes, _lib.ptr(work), work_bytes, _lib.raw_stream(x)),
+                "talm_lora_forward")
         ctx.scaling, ctx.drop = scaling, drop
         ctx.save_for_backward(x, lora_a, lora_b, seed, saved)
         RAN["lora"] += 1

@@ -205,157 +205,774 @@ int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, co
 
 // ------------------------------------------------------------------------------------------
 // the branch
+//
+// Six products, three of them along the wide dimensions:
+//   inner   t = keep x A^T and dt = g B      (sums over the columns of a wide activation)
+//   outer   dA = dt^T keep x, dB = g^T t     (sums over its rows), with dx in dA's pass
+//   up      y = base + s t B^T               (sums over the rank; dx = keep dt A likewise)
+// Every pass reads a wide activation once from HBM and keeps the rank-wide operand in registers
+// and caches; all of them run on mma.sync m16n8k16, whose fragments are loaded straight from global
+// memory (16 bytes per lane and load, no shared memory): the reduction index of an mma may be
+// permuted, so the eight consecutive columns that a lane loads are used as they lie.
+//
+// fp32 operands are split in two 16-bit parts. Where the other operand is an activation (t, dt,
+// dA, dB: fp32 results) they are fp16 parts of the operand scaled by a power of two that brings its
+// largest element to [2^14, 2^15): 2^-22 and better, at any size of the operand; the scale is one
+// per adapter row (A, B) or per 16 rows of the activation (t, dt). Where both operands are
+// fp32 and the result is fp16 (y, dx) they are bf16 parts without scale, and the product of the two
+// small parts is left out: 2^-16 of each term, under a sixteenth of the result's own rounding.
+// mma sums are moved into separate fp32 sums every 64 columns or 16 rows: the tensor core cuts its
+// sums off instead of rounding them, which would add up over a long chain.
 // ------------------------------------------------------------------------------------------
 struct Shape {
   int64_t n_rows, n_in, n_out;
   int rank;
 };
 
-// The eight dropped-out inputs of group (row n, columns k .. k + 7), without the factor.
-__device__ __forceinline__ void masked8(const __half* x, int64_t ld_x, int64_t n, int64_t k,
-                                        int64_t n_in, uint64_t key, const Dropout& d,
-                                        float (&v)[8]) {
-  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(x + n * ld_x + k));
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+// The two bf16 parts of a pair.
+__device__ __forceinline__ void split_bf16(float v0, float v1, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16(v0, v1);
+  lo = pack_bf16(v0 - __uint_as_float(hi << 16), v1 - __uint_as_float(hi & 0xFFFF0000u));
+}
+// The two fp16 parts of a pair that has been scaled.
+__device__ __forceinline__ void split_f16(float v0, float v1, uint32_t& hi, uint32_t& lo) {
+  hi = pack_half2(v0, v1);
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  lo = pack_half2(v0 - h.x, v1 - h.y);
+}
+// For a largest magnitude m: *up brings it to [2^14, 2^15), *down undoes that. Clamped so that both
+// are normal numbers; 1 for zero (and for what is not finite, which stays so).
+__device__ __forceinline__ void power_scale(float m, float* up, float* down) {
+  int e = static_cast<int>((__float_as_uint(m) >> 23) & 255) - 127 - 14;
+  if (m == 0.0f || !(m < __int_as_float(0x7F800000))) e = 0;
+  e = max(-112, min(112, e));
+  *up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  *down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+// ---- prepared operands -----------------------------------------------------------------------
+// RP: the rank rounded up to 16, 32 or 64, zeros behind it.
+//   Rows:  fp16 parts hi[RP][n], lo[RP][n] of an adapter matrix with the rank in the rows (A, B^T),
+//          each row scaled; down[RP] undoes the scale.
+//   Cols:  bf16 parts of the same matrix as 16 x 16 mma operands of 16 columns and 16 ranks:
+//          [n / 64][4][RP / 16][part][lane] uint4; tile i of a 64-column block holds, for m = g and
+//          g + 8, columns 8 g + 2 i and 8 g + 2 i + 1.
+//   T:     of t or dt: bf16 parts as the n operand of 16 rows, t_row [rows / 16][RP / 16][part]
+//          [lane] uint4, and fp16 parts of the rows scaled together as the m operand, t_col of the
+//          same size, with t_down[rows / 16].
+struct Rows {
+  __half *hi, *lo;
+  float* down;
+};
+struct TParts {
+  uint4 *row, *col;
+  float* down;
+};
+
+__host__ __device__ constexpr int padded_rank(int rank) {
+  return rank <= 16 ? 16 : rank <= 32 ? 32 : 64;
+}
+
+constexpr int PREP_THREADS = 256;
+
+// One CTA per padded rank builds its row of `rows` from m0 (element (j, c) at m0[j * j0 + c * c0]);
+// the others build `cols` from m1, a thread per lane of an operand.
+__global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(
+    const float* __restrict__ m0, int64_t j0, int64_t c0, int n0, Rows rows,
+    const float* __restrict__ m1, int64_t j1, int64_t c1, int n1, uint4* __restrict__ cols,
+    int rank, int rp) {
+  const int tid = threadIdx.x;
+  if (static_cast<int>(blockIdx.x) < rp) {
+    __shared__ float most[PREP_THREADS / 32];
+    const int j = blockIdx.x;
+    const float* src = m0 + j * j0;
+    float m = 0.0f;
+    if (j < rank)
+      for (int c = tid; c < n0; c += PREP_THREADS) m = fmaxf(m, fabsf(__ldg(src + c * c0)));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if ((tid & 31) == 0) most[tid >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PREP_THREADS / 32; ++i) m = fmaxf(m, most[i]);
+    float up, down;
+    power_scale(m, &up, &down);
+    uint32_t* hi = reinterpret_cast<uint32_t*>(rows.hi + static_cast<int64_t>(j) * n0);
+    uint32_t* lo = reinterpret_cast<uint32_t*>(rows.lo + static_cast<int64_t>(j) * n0);
+    for (int c = 2 * tid; c < n0; c += 2 * PREP_THREADS) {  // n0 is even
+      uint32_t h = 0, l = 0;
+      if (j < rank) split_f16(__ldg(src + c * c0) * up, __ldg(src + (c + 1) * c0) * up, h, l);
+      hi[c >> 1] = h;
+      lo[c >> 1] = l;
+    }
+    if (tid == 0) rows.down[j] = down;
+    return;
   }
-  if (d.drop == 0) return;
+  const int ks = rp / 16;
+  const int64_t e = static_cast<int64_t>(blockIdx.x - rp) * PREP_THREADS + tid;
+  const int64_t blocks = (n1 + 63) / 64;
+  if (e >= blocks * 4 * ks * 32) return;
+  const int lane = static_cast<int>(e & 31), g = lane >> 2, t = lane & 3;
+  const int64_t tile = e >> 5;  // (block * 4 + i) * ks + k
+  const int k = static_cast<int>(tile % ks), i = static_cast<int>(tile / ks % 4);
+  const int64_t c = tile / ks / 4 * 64 + 8 * g + 2 * i;
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {  // registers: (m = g, g + 8) x (k low, k high)
+    const int64_t col = c + (r & 1);
+    const int j = 16 * k + 2 * t + 8 * (r >> 1);
+    float v[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      v[u] = col < n1 && j + u < rank ? __ldg(m1 + (j + u) * j1 + col * c1) : 0.0f;
+    split_bf16(v[0], v[1], hi[r], lo[r]);
+  }
+  cols[tile * 64 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  cols[tile * 64 + 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
+// ---- inner: sums over the columns ------------------------------------------------------------
+constexpr int INNER_WARPS = 8;
+
+// The four keep masks of the group of eight at (row n, column k).
+__device__ __forceinline__ uint4 masked(uint4 v, int64_t n, int64_t n_in, int k, uint64_t key,
+                                        uint32_t bias2) {
   uint32_t c[4];
   philox(static_cast<uint64_t>((n * n_in + k) >> 3), key, c);
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (!kept(c, i, d.drop)) v[i] = 0.0f;
+  return make_uint4(v.x & keep_mask2(c[0], bias2), v.y & keep_mask2(c[1], bias2),
+                    v.z & keep_mask2(c[2], bias2), v.w & keep_mask2(c[3], bias2));
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  return v;
-}
+// part[split][n][j] = sum over the split's columns of (keep) x[n, c] w[j, c], w the scaled rows. A
+// warp takes 32 rows and every KG-th 64-column step of its CTA's columns: per step, lane (g, t)
+// loads the columns 8 t .. 8 t + 7 of both 32-column halves for rows g, g + 8, g + 16, g + 24.
+template <int NT, bool MASK>
+__global__ void __launch_bounds__(32 * INNER_WARPS, NT == 2 ? 2 : 1) inner_kernel(
+    const __half* __restrict__ x, int64_t ld_x, int64_t n_rows, int n_cols, Rows w, Dropout d,
+    int row_groups, int steps_per_split, float* __restrict__ part) {
+  extern __shared__ __align__(16) float inner_smem[];  // [INNER_WARPS][32][8 NT]
+  constexpr int RP = 8 * NT;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int kg = INNER_WARPS / row_groups;  // warps that share a row group's columns
+  const int rg = warp / kg, kw = warp % kg;
+  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * row_groups + rg) * 32;
+  const int steps = (n_cols + 63) / 64;
+  const int s0 = blockIdx.y * steps_per_split;
+  const int s1 = min(steps, s0 + steps_per_split);
+  const uint64_t key = MASK ? static_cast<uint64_t>(__ldg(d.seed)) : 0;
+  const uint32_t bias2 = keep_bias2(d.drop);
 
-// t[n, j] = f sum_k keep x[n, k] A[j, k]: one warp per row, 16 adapter rows per pass
-__global__ void __launch_bounds__(256) down_kernel(const __half* __restrict__ x, int64_t ld_x,
-                                                   const float* __restrict__ a, Shape s,
-                                                   Dropout d, float* __restrict__ t) {
-  const int lane = threadIdx.x & 31;
-  const int64_t n = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  if (n >= s.n_rows) return;
-  const uint64_t key = d.drop ? static_cast<uint64_t>(*d.seed) : 0;
-  for (int j0 = 0; j0 < s.rank; j0 += 16) {
-    float acc[16] = {};
-    for (int64_t k = 8 * lane; k < s.n_in; k += 256) {
-      float v[8];
-      masked8(x, ld_x, n, k, s.n_in, key, d, v);
+  const __half* xr[4];
+  int64_t row[4];
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j0 + j < s.rank)
-          for (int i = 0; i < 8; ++i) acc[j] = fmaf(v[i], a[(j0 + j) * s.n_in + k + i], acc[j]);
+  for (int i = 0; i < 4; ++i) {  // rows past the end read the last one; they are not stored
+    row[i] = min(r0 + g + 8 * i, n_rows - 1);
+    xr[i] = x + row[i] * ld_x + 8 * t;
+  }
+  auto load = [&](int s, uint4 (&v)[4][2]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        v[i][h] = s * 64 + h * 32 + 8 * t < n_cols
+                      ? __ldg(reinterpret_cast<const uint4*>(xr[i] + s * 64 + h * 32))
+                      : make_uint4(0, 0, 0, 0);
+  };
+  float acc[2][NT][4] = {};
+  uint4 cur[4][2];
+  if (s0 + kw < s1) load(s0 + kw, cur);
+  for (int s = s0 + kw; s < s1; s += kg) {
+    uint4 next[4][2];
+    const bool more = s + kg < s1;
+    if (more) load(s + kg, next);
+    if (MASK) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          cur[i][h] = masked(cur[i][h], row[i], n_cols, s * 64 + h * 32 + 8 * t, key, bias2);
     }
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float v = warp_sum(acc[j]);
-      if (lane == 0 && j0 + j < s.rank) t[n * s.rank + j0 + j] = v * d.factor;
+    for (int nt = 0; nt < NT; ++nt) {
+      float c[2][4] = {};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int col = s * 64 + h * 32 + 8 * t;
+        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+        if (col < n_cols) {
+          const int64_t at = static_cast<int64_t>(nt * 8 + g) * n_cols + col;
+          hi = __ldg(reinterpret_cast<const uint4*>(w.hi + at));
+          lo = __ldg(reinterpret_cast<const uint4*>(w.lo + at));
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const uint4 &a = cur[2 * m][h], &b = cur[2 * m + 1][h];
+          mma_f16(c[m], a.x, b.x, a.y, b.y, lo.x, lo.y);
+          mma_f16(c[m], a.z, b.z, a.w, b.w, lo.z, lo.w);
+          mma_f16(c[m], a.x, b.x, a.y, b.y, hi.x, hi.y);
+          mma_f16(c[m], a.z, b.z, a.w, b.w, hi.z, hi.w);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][nt][i] += c[m][i];
+    }
+    if (more) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cur[i][0] = next[i][0];
+        cur[i][1] = next[i][1];
+      }
+    }
+  }
+  // the warps of a row group add their sums in warp order
+  float* mine = inner_smem + warp * (32 * RP);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float* q = mine + (16 * m + g) * RP + nt * 8 + 2 * t;
+      *reinterpret_cast<float2*>(q) = make_float2(acc[m][nt][0], acc[m][nt][1]);
+      *reinterpret_cast<float2*>(q + 8 * RP) = make_float2(acc[m][nt][2], acc[m][nt][3]);
+    }
+  __syncthreads();
+  float* out = part + static_cast<int64_t>(blockIdx.y) * n_rows * RP;
+  for (int i = threadIdx.x; i < row_groups * 32 * RP; i += 32 * INNER_WARPS) {
+    const int grp = i / (32 * RP), in = i % (32 * RP);
+    const int64_t n = (static_cast<int64_t>(blockIdx.x) * row_groups + grp) * 32 + in / RP;
+    if (n >= n_rows) continue;
+    float v = 0.0f;
+    for (int k = 0; k < kg; ++k) v += inner_smem[(grp * kg + k) * (32 * RP) + in];
+    out[n * RP + in % RP] = v;
+  }
+}
+
+// ---- the operands made of t (or dt) ----------------------------------------------------------
+// t[n, j] = factor * down[j] * (sum of the parts), one warp per 16 rows.
+template <int KS>
+__global__ void __launch_bounds__(128) t_parts_kernel(const float* __restrict__ part, int splits,
+                                                      int64_t n_rows, const float* __restrict__ down,
+                                                      float factor, TParts out) {
+  constexpr int RP = 16 * KS;
+  __shared__ float sh[4][16][RP + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int64_t block = static_cast<int64_t>(blockIdx.x) * 4 + warp;
+  if (block * 16 >= n_rows) return;
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16 * RP / 32; ++i) {
+    const int e = i * 32 + lane, r = e / RP, j = e % RP;
+    const int64_t n = block * 16 + r;
+    float v = 0.0f;
+    if (n < n_rows) {
+      const float* p = part + n * RP + j;
+      for (int k = 0; k < splits; ++k) v += __ldg(p + static_cast<int64_t>(k) * n_rows * RP);
+      v *= __ldg(down + j) * factor;
+    }
+    sh[warp][r][j] = v;
+    most = fmaxf(most, fabsf(v));
+  }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+  float up, back;
+  power_scale(most, &up, &back);
+  __syncwarp();
+  const auto& m = sh[warp];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    const int64_t at = (block * KS + k) * 64 + lane;
+    uint32_t hi[4], lo[4];
+    // n operand: registers (rows g, rows 8 + g) x (ranks 2 t, 2 t + 8)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int n = g + 8 * (r >> 1), j = 16 * k + 2 * t + 8 * (r & 1);
+      split_bf16(m[n][j], m[n][j + 1], hi[r], lo[r]);
+    }
+    out.row[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    out.row[at + 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    // m operand of the transpose: registers (ranks g, g + 8) x (rows 2 t, 2 t + 8)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int j = 16 * k + g + 8 * (r & 1), n = 2 * t + 8 * (r >> 1);
+      split_f16(m[n][j] * up, m[n + 1][j] * up, hi[r], lo[r]);
+    }
+    out.col[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    out.col[at + 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+  if (lane == 0) out.down[block] = back;
+}
+
+// D tiles of rank-wide products: for 64 columns and 16 rows, c[i][h][..] = sum_j M[col, j] T[row, j]
+// with columns 8 g + 2 i, 8 g + 2 i + 1 and rows 8 h + 2 t, 8 h + 2 t + 1: lane (g, t) gets eight
+// consecutive columns of four rows.
+template <int KS>
+__device__ __forceinline__ void rank_product(float (&c)[4][2][4], const uint4* __restrict__ cols,
+                                             const uint4 (&t_hi)[KS], const uint4 (&t_lo)[KS],
+                                             int lane) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) c[i][h][u] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const uint4 hi = __ldg(cols + (i * KS + k) * 64 + lane);
+      const uint4 lo = __ldg(cols + (i * KS + k) * 64 + 32 + lane);
+      mma_bf16(c[i][0], lo, t_hi[k].x, t_hi[k].y);
+      mma_bf16(c[i][1], lo, t_hi[k].z, t_hi[k].w);
+      mma_bf16(c[i][0], hi, t_lo[k].x, t_lo[k].y);
+      mma_bf16(c[i][1], hi, t_lo[k].z, t_lo[k].w);
+      mma_bf16(c[i][0], hi, t_hi[k].x, t_hi[k].y);
+      mma_bf16(c[i][1], hi, t_hi[k].z, t_hi[k].w);
     }
   }
 }
 
-// y = fp16(base + s t B^T): one thread per output
+// Where the rows of lane t lie in a block of 16: 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
+__device__ __forceinline__ int row_of(int i, int t) { return 2 * t + (i & 1) + 8 * (i >> 1); }
+
+// ---- up: y = fp16(base + s t B^T) ------------------------------------------------------------
+// A warp takes 64 columns and every `stride`-th block of 16 rows.
+template <int KS>
 __global__ void __launch_bounds__(256) up_kernel(const __half* __restrict__ base, int64_t ld_base,
-                                                 const float* __restrict__ t,
-                                                 const float* __restrict__ b, Shape s,
-                                                 float scaling, __half* __restrict__ y) {
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (e >= s.n_rows * s.n_out) return;
-  const int64_t n = e / s.n_out, o = e % s.n_out;
-  float acc = 0.0f;
-  for (int j = 0; j < s.rank; ++j) acc = fmaf(t[n * s.rank + j], b[o * s.rank + j], acc);
-  y[e] = __float2half_rn(fmaf(scaling, acc, __half2float(base[n * ld_base + o])));
-}
-
-// dt[n, j] = s sum_o g[n, o] B[o, j]: one warp per row
-__global__ void __launch_bounds__(256) grad_t_kernel(const __half* __restrict__ g, int64_t ld_g,
-                                                     const float* __restrict__ b, Shape s,
-                                                     float scaling, float* __restrict__ dt) {
+                                                 const uint4* __restrict__ t_row,
+                                                 const uint4* __restrict__ cols, int64_t n_rows,
+                                                 int n_out, float scaling, int shares,
+                                                 __half* __restrict__ y) {
   const int lane = threadIdx.x & 31;
-  const int64_t n = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-  if (n >= s.n_rows) return;
-  for (int j0 = 0; j0 < s.rank; j0 += 16) {
-    float acc[16] = {};
-    for (int64_t o = lane; o < s.n_out; o += 32) {
-      const float v = __half2float(g[n * ld_g + o]);
+  const int g = lane >> 2, t = lane & 3;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int col_blocks = (n_out + 63) / 64;
+  const int cb = static_cast<int>(id % col_blocks);
+  const int64_t share = id / col_blocks;
+  const int64_t row_blocks = (n_rows + 15) / 16;
+  if (share >= shares) return;
+  const int col = cb * 64 + 8 * g;
+  const bool in = col < n_out;
+  const uint4* my_cols = cols + static_cast<int64_t>(cb) * (4 * KS * 64);
+  for (int64_t rb = share; rb < row_blocks; rb += shares) {
+    uint4 bv[4];
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j0 + j < s.rank) acc[j] = fmaf(v, b[o * s.rank + j0 + j], acc[j]);
+    for (int i = 0; i < 4; ++i) {
+      const int64_t n = rb * 16 + row_of(i, t);
+      bv[i] = in && n < n_rows ? __ldg(reinterpret_cast<const uint4*>(base + n * ld_base + col))
+                               : make_uint4(0, 0, 0, 0);
     }
+    uint4 t_hi[KS], t_lo[KS];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float v = warp_sum(acc[j]);
-      if (lane == 0 && j0 + j < s.rank) dt[n * s.rank + j0 + j] = v * scaling;
+    for (int k = 0; k < KS; ++k) {
+      t_hi[k] = __ldg(t_row + (rb * KS + k) * 64 + lane);
+      t_lo[k] = __ldg(t_row + (rb * KS + k) * 64 + 32 + lane);
+    }
+    float c[4][2][4];
+    rank_product<KS>(c, my_cols, t_hi, t_lo, lane);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t n = rb * 16 + row_of(i, t);
+      const uint32_t w[4] = {bv[i].x, bv[i].y, bv[i].z, bv[i].w};
+      uint32_t o[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+        o[k] = pack_half2(fmaf(scaling, c[k][i >> 1][i & 1], f.x),
+                          fmaf(scaling, c[k][i >> 1][2 + (i & 1)], f.y));
+      }
+      if (in && n < n_rows)
+        *reinterpret_cast<uint4*>(y + n * n_out + col) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 }
 
-// dB[o, j] = s sum_n g[n, o] t[n, j]: one thread per element; the sum over the rows is made of
-// sums over 128 rows, so that a long one does not lose its low bits
-__global__ void __launch_bounds__(256) grad_b_kernel(const __half* __restrict__ g, int64_t ld_g,
-                                                     const float* __restrict__ t, Shape s,
-                                                     float scaling, float* __restrict__ db) {
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (e >= s.n_out * s.rank) return;
-  const int64_t j = e / s.n_out, o = e % s.n_out;
-  float total = 0.0f;
-  for (int64_t n0 = 0; n0 < s.n_rows; n0 += 128) {
-    float part = 0.0f;
-    for (int64_t n = n0; n < n0 + 128 && n < s.n_rows; ++n)
-      part = fmaf(__half2float(g[n * ld_g + o]), t[n * s.rank + j], part);
-    total += part;
-  }
-  db[o * s.rank + j] = total * scaling;
-}
+// ---- outer: sums over the rows, and dx --------------------------------------------------------
+constexpr int OUTER_WARPS = 8;
 
-// dA[j, k] = f sum_n dt[n, j] keep x[n, k]: one thread per adapter row and eight columns
-__global__ void __launch_bounds__(256) grad_a_kernel(const __half* __restrict__ x, int64_t ld_x,
-                                                     const float* __restrict__ dt, Shape s,
-                                                     Dropout d, float* __restrict__ da) {
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  const int64_t chunks = s.n_in / 8;
-  if (e >= chunks * s.rank) return;
-  const int64_t j = e / chunks, k = (e % chunks) * 8;
-  const uint64_t key = d.drop ? static_cast<uint64_t>(*d.seed) : 0;
-  float total[8] = {};
-  for (int64_t n0 = 0; n0 < s.n_rows; n0 += 128) {
-    float part[8] = {};
-    for (int64_t n = n0; n < n0 + 128 && n < s.n_rows; ++n) {
-      float v[8];
-      masked8(x, ld_x, n, k, s.n_in, key, d, v);
-      const float w = dt[n * s.rank + j];
-      for (int i = 0; i < 8; ++i) part[i] = fmaf(v[i], w, part[i]);
+// part[split][j][c] = sum over the split's rows of T[n, j] (keep) x[n, c] (unless `part` is null),
+// and dx[n, c] = fp16(keep factor sum_j T[n, j] A[j, c]) (where DX). A CTA takes 64 columns and a
+// range of 16-row blocks, its warps every OUTER_WARPS-th of them. Lane (g, t) loads columns
+// 8 g .. 8 g + 7 of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9: two rows of a column make an operand
+// register by one byte permutation, and dx comes out of rank_product at the same places.
+template <int KS, bool MASK, bool DX>
+__global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kernel(
+    const __half* __restrict__ x, int64_t ld_x, int64_t n_rows, int n_cols, TParts tp, Dropout d,
+    const uint4* __restrict__ cols, int blocks_per_split, float* __restrict__ part,
+    __half* __restrict__ dx) {
+  extern __shared__ __align__(16) float outer_smem[];  // [OUTER_WARPS][16][64]
+  constexpr int RP = 16 * KS;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const int cb = blockIdx.x;
+  const int col = cb * 64 + 8 * g;
+  const bool in = col < n_cols;
+  const int64_t row_blocks = (n_rows + 15) / 16;
+  const int64_t rb0 = static_cast<int64_t>(blockIdx.y) * blocks_per_split;
+  const int64_t rb1 = min(row_blocks, rb0 + blocks_per_split);
+  const uint64_t key = MASK ? static_cast<uint64_t>(__ldg(d.seed)) : 0;
+  const uint32_t bias2 = keep_bias2(d.drop);
+  const uint4* my_cols = DX ? cols + static_cast<int64_t>(cb) * (4 * KS * 64) : nullptr;
+  const bool sums = part != nullptr;
+
+  auto load = [&](int64_t rb, uint4 (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t n = rb * 16 + row_of(i, t);
+      v[i] = in && n < n_rows && sums
+                 ? __ldg(reinterpret_cast<const uint4*>(x + n * ld_x + col))
+                 : make_uint4(0, 0, 0, 0);
     }
-    for (int i = 0; i < 8; ++i) total[i] += part[i];
+  };
+  float acc[KS][8][4] = {};
+  uint4 cur[4];
+  if (rb0 + warp < rb1) load(rb0 + warp, cur);
+  for (int64_t rb = rb0 + warp; rb < rb1; rb += OUTER_WARPS) {
+    uint4 next[4];
+    const bool more = rb + OUTER_WARPS < rb1;
+    if (more) load(rb + OUTER_WARPS, next);
+    uint4 keep[4];
+    if (MASK) {
+      const uint4 ones = make_uint4(~0u, ~0u, ~0u, ~0u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        keep[i] = masked(ones, rb * 16 + row_of(i, t), n_cols, col, key, bias2);
+        cur[i] = make_uint4(cur[i].x & keep[i].x, cur[i].y & keep[i].y, cur[i].z & keep[i].z,
+                            cur[i].w & keep[i].w);
+      }
+    }
+    if (sums) {
+      const float back = __ldg(tp.down + rb);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const uint4 hi = __ldg(tp.col + (rb * KS + k) * 64 + lane);
+        const uint4 lo = __ldg(tp.col + (rb * KS + k) * 64 + 32 + lane);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const uint32_t r0 = u == 0 ? cur[0].x : u == 1 ? cur[0].y : u == 2 ? cur[0].z : cur[0].w;
+          const uint32_t r1 = u == 0 ? cur[1].x : u == 1 ? cur[1].y : u == 2 ? cur[1].z : cur[1].w;
+          const uint32_t r2 = u == 0 ? cur[2].x : u == 1 ? cur[2].y : u == 2 ? cur[2].z : cur[2].w;
+          const uint32_t r3 = u == 0 ? cur[3].x : u == 1 ? cur[3].y : u == 2 ? cur[3].z : cur[3].w;
+#pragma unroll
+          for (int v = 0; v < 2; ++v) {  // column 8 g + 2 u + v
+            const uint32_t b0 = __byte_perm(r0, r1, v ? 0x7632 : 0x5410);
+            const uint32_t b1 = __byte_perm(r2, r3, v ? 0x7632 : 0x5410);
+            float c[4] = {};
+            mma_f16(c, lo.x, lo.y, lo.z, lo.w, b0, b1);
+            mma_f16(c, hi.x, hi.y, hi.z, hi.w, b0, b1);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[k][2 * u + v][q] = fmaf(back, c[q], acc[k][2 * u + v][q]);
+          }
+        }
+      }
+    }
+    if (DX) {
+      uint4 t_hi[KS], t_lo[KS];
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        t_hi[k] = __ldg(tp.row + (rb * KS + k) * 64 + lane);
+        t_lo[k] = __ldg(tp.row + (rb * KS + k) * 64 + 32 + lane);
+      }
+      float c[4][2][4];
+      rank_product<KS>(c, my_cols, t_hi, t_lo, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t n = rb * 16 + row_of(i, t);
+        uint32_t o[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          o[k] = pack_half2(d.factor * c[k][i >> 1][i & 1], d.factor * c[k][i >> 1][2 + (i & 1)]);
+        if (MASK) {
+          o[0] &= keep[i].x;
+          o[1] &= keep[i].y;
+          o[2] &= keep[i].z;
+          o[3] &= keep[i].w;
+        }
+        if (in && n < n_rows)
+          *reinterpret_cast<uint4*>(dx + n * n_cols + col) = make_uint4(o[0], o[1], o[2], o[3]);
+      }
+    }
+    if (more) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cur[i] = next[i];
+    }
   }
-  for (int i = 0; i < 8; ++i) da[j * s.n_in + k + i] = total[i] * d.factor;
+  if (!sums) return;
+  // the warps add their sums in warp order, 16 ranks at a time
+  float* out = part + static_cast<int64_t>(blockIdx.y) * RP * n_cols;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    __syncthreads();
+    float* mine = outer_smem + warp * (16 * 64);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {  // tile u: n index (2 t, 2 t + 1) stands for columns 8 n + u
+      mine[g * 64 + 8 * (2 * t) + u] = acc[k][u][0];
+      mine[g * 64 + 8 * (2 * t + 1) + u] = acc[k][u][1];
+      mine[(g + 8) * 64 + 8 * (2 * t) + u] = acc[k][u][2];
+      mine[(g + 8) * 64 + 8 * (2 * t + 1) + u] = acc[k][u][3];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * 64; i += 32 * OUTER_WARPS) {
+      const int c = cb * 64 + (i & 63);
+      float v = 0.0f;
+#pragma unroll
+      for (int q = 0; q < OUTER_WARPS; ++q) v += outer_smem[q * (16 * 64) + i];
+      if (c < n_cols) out[static_cast<int64_t>(16 * k + (i >> 6)) * n_cols + c] = v;
+    }
+  }
 }
 
-// dx[n, k] = fp16(keep f sum_j dt[n, j] A[j, k]): one thread per eight columns of a row
-__global__ void __launch_bounds__(256) grad_x_kernel(const float* __restrict__ dt,
-                                                     const float* __restrict__ a, Shape s,
-                                                     Dropout d, __half* __restrict__ dx) {
-  const int64_t q = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (8 * q >= s.n_rows * s.n_in) return;
-  const int64_t n = 8 * q / s.n_in, k = 8 * q % s.n_in;
-  float acc[8] = {};
-  for (int j = 0; j < s.rank; ++j) {
-    const float w = dt[n * s.rank + j];
-    for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, a[j * s.n_in + k + i], acc[i]);
+// out[j * out_j + c * out_c] = factor * (sum of the parts): the weights' gradients.
+__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ part, int splits,
+                                                        int rank, int rp, int n, float factor,
+                                                        int64_t out_j, int64_t out_c,
+                                                        float* __restrict__ out) {
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= static_cast<int64_t>(rank) * n) return;
+  const int64_t j = e / n, c = e % n;
+  float v = 0.0f;
+  for (int k = 0; k < splits; ++k) v += __ldg(part + (static_cast<int64_t>(k) * rp + j) * n + c);
+  out[j * out_j + c * out_c] = v * factor;
+}
+
+// ---- host: workspaces and launches ------------------------------------------------------------
+struct Carve {  // hands out 256-byte aligned pieces; counts them when there is no base
+  char* base;
+  size_t used;
+  template <class T>
+  T* take(size_t n) {
+    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += (n * sizeof(T) + 255) / 256 * 256;
+    return p;
   }
-  uint32_t c[4] = {};
-  if (d.drop) philox(static_cast<uint64_t>(q), static_cast<uint64_t>(*d.seed), c);
-  for (int i = 0; i < 8; ++i)
-    dx[8 * q + i] = __float2half_rn(kept(c, i, d.drop) ? acc[i] * d.factor : 0.0f);
+};
+
+constexpr int TARGET_CTAS = 296;  // two for each of 148 SMs
+
+// How `inner` divides its work: a CTA takes row_groups * 32 rows (few when there are few rows, so
+// that the warps share the columns instead) and steps_per_split 64-column steps.
+struct InnerPlan {
+  int row_groups, row_ctas, splits, steps_per_split;
+  InnerPlan(int64_t n_rows, int64_t n_cols, int rp) {
+    row_groups = n_rows <= 32 ? 1 : rp >= 64 ? 4 : 2;
+    row_ctas = static_cast<int>((n_rows + 32 * row_groups - 1) / (32 * row_groups));
+    const int steps = static_cast<int>((n_cols + 63) / 64);
+    int want = TARGET_CTAS / row_ctas;  // at least one step for each warp of a row group
+    const int most = (steps * row_groups + INNER_WARPS - 1) / INNER_WARPS;
+    if (want > most) want = most;
+    if (want > 32) want = 32;
+    if (want < 1) want = 1;
+    steps_per_split = (steps + want - 1) / want;
+    splits = (steps + steps_per_split - 1) / steps_per_split;
+  }
+};
+
+// How `outer` divides its work: a CTA takes 64 columns and blocks_per_split blocks of 16 rows.
+struct OuterPlan {
+  int col_ctas, splits, blocks_per_split;
+  OuterPlan(int64_t n_rows, int64_t n_cols) {
+    col_ctas = static_cast<int>((n_cols + 63) / 64);
+    const int64_t row_blocks = (n_rows + 15) / 16;
+    int64_t want = TARGET_CTAS / col_ctas;
+    const int64_t most = (row_blocks + OUTER_WARPS - 1) / OUTER_WARPS;
+    if (want > most) want = most;
+    if (want < 1) want = 1;
+    blocks_per_split = static_cast<int>((row_blocks + want - 1) / want);
+    splits = static_cast<int>((row_blocks + blocks_per_split - 1) / blocks_per_split);
+  }
+};
+
+struct TBuffers {
+  TParts parts;
+  TBuffers(Carve& c, int64_t n_rows, int rp) {
+    const size_t blocks = static_cast<size_t>((n_rows + 15) / 16);
+    parts.row = c.take<uint4>(blocks * (rp / 16) * 64);
+    parts.col = c.take<uint4>(blocks * (rp / 16) * 64);
+    parts.down = c.take<float>(blocks);
+  }
+};
+
+// The adapter's operands of one direction: the rows of one matrix, the columns of the other.
+struct Prepared {
+  Rows rows;
+  uint4* cols;
+  Prepared(Carve& c, int64_t n_rows_matrix, int64_t n_cols_matrix, int rp) {
+    rows.hi = c.take<__half>(static_cast<size_t>(rp) * n_rows_matrix);
+    rows.lo = c.take<__half>(static_cast<size_t>(rp) * n_rows_matrix);
+    rows.down = c.take<float>(rp);
+    cols = c.take<uint4>(static_cast<size_t>((n_cols_matrix + 63) / 64) * 4 * (rp / 16) * 64);
+  }
+};
+
+struct ForwardWork {
+  Carve carve;
+  Prepared prep;
+  float* part;
+  ForwardWork(void* base, const Shape& s, int rp)
+      : carve{static_cast<char*>(base), 0}, prep(carve, s.n_in, s.n_out, rp) {
+    const InnerPlan plan(s.n_rows, s.n_in, rp);
+    part = carve.take<float>(static_cast<size_t>(plan.splits) * s.n_rows * rp);
+  }
+};
+
+struct BackwardWork {
+  Carve carve;
+  Prepared prep;
+  TBuffers dt;
+  float *t_part, *b_part, *a_part;
+  BackwardWork(void* base, const Shape& s, int rp)
+      : carve{static_cast<char*>(base), 0},
+        prep(carve, s.n_out, s.n_in, rp),
+        dt(carve, s.n_rows, rp) {
+    const InnerPlan inner(s.n_rows, s.n_out, rp);
+    t_part = carve.take<float>(static_cast<size_t>(inner.splits) * s.n_rows * rp);
+    const OuterPlan ob(s.n_rows, s.n_out), oa(s.n_rows, s.n_in);
+    b_part = carve.take<float>(static_cast<size_t>(ob.splits) * rp * s.n_out);
+    a_part = carve.take<float>(static_cast<size_t>(oa.splits) * rp * s.n_in);
+  }
+};
+
+struct Saved {
+  Carve carve;
+  TBuffers t;
+  Saved(void* base, const Shape& s, int rp)
+      : carve{static_cast<char*>(base), 0}, t(carve, s.n_rows, rp) {}
+};
+
+template <class K>
+int allow_smem(K kernel, int bytes) {
+  // set on every call: a per-device record would cost as much as the call, which only notes it
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  return e == cudaSuccess ? TALM_OK : set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
+}
+
+void prepare(const float* m0, int64_t j0, int64_t c0, int64_t n0, const float* m1, int64_t j1,
+             int64_t c1, int64_t n1, const Prepared& p, int rank, int rp, cudaStream_t stream) {
+  const int64_t lanes = (n1 + 63) / 64 * 4 * (rp / 16) * 32;
+  const int64_t grid = rp + (lanes + PREP_THREADS - 1) / PREP_THREADS;
+  prepare_kernel<<<static_cast<unsigned>(grid), PREP_THREADS, 0, stream>>>(
+      m0, j0, c0, static_cast<int>(n0), p.rows, m1, j1, c1, static_cast<int>(n1), p.cols, rank,
+      rp);
+}
+
+template <int KS>
+int run_inner(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const Rows& rows,
+              const Dropout& d, float* part, float factor, const TParts& out,
+              cudaStream_t stream) {
+  const InnerPlan plan(n_rows, n_cols, 16 * KS);
+  const dim3 grid(static_cast<unsigned>(plan.row_ctas), static_cast<unsigned>(plan.splits), 1);
+  constexpr int smem = INNER_WARPS * 32 * 16 * KS * 4;
+  auto kernel = d.drop ? inner_kernel<2 * KS, true> : inner_kernel<2 * KS, false>;
+  if (smem > 48 * 1024) {
+    const int st = allow_smem(kernel, smem);
+    if (st != TALM_OK) return st;
+  }
+  kernel<<<grid, 32 * INNER_WARPS, smem, stream>>>(x, ld, n_rows, static_cast<int>(n_cols), rows, d,
+                                                   plan.row_groups, plan.steps_per_split, part);
+  const int64_t blocks = (n_rows + 15) / 16;
+  t_parts_kernel<KS><<<static_cast<unsigned>((blocks + 3) / 4), 128, 0, stream>>>(
+      part, plan.splits, n_rows, rows.down, factor, out);
+  return TALM_OK;
+}
+
+template <int KS>
+int run_forward(const __half* x, int64_t ld_x, const __half* base, int64_t ld_base,
+                const float* a, const float* b, const Shape& s, float scaling, const Dropout& d,
+                __half* y, void* saved, void* work, cudaStream_t stream) {
+  constexpr int RP = 16 * KS;
+  const ForwardWork w(work, s, RP);
+  const Saved keep(saved, s, RP);
+  prepare(a, s.n_in, 1, s.n_in, b, 1, s.rank, s.n_out, w.prep, s.rank, RP, stream);
+  const int st = run_inner<KS>(x, ld_x, s.n_rows, s.n_in, w.prep.rows, d, w.part, d.factor,
+                               keep.t.parts, stream);
+  if (st != TALM_OK) return st;
+  const int64_t col_blocks = (s.n_out + 63) / 64, row_blocks = (s.n_rows + 15) / 16;
+  int64_t shares = (int64_t{TARGET_CTAS} * 8 + col_blocks - 1) / col_blocks;
+  if (shares > row_blocks) shares = row_blocks;
+  up_kernel<KS><<<static_cast<unsigned>((col_blocks * shares + 7) / 8), 256, 0, stream>>>(
+      base, ld_base, keep.t.parts.row, w.prep.cols, s.n_rows, static_cast<int>(s.n_out), scaling,
+      static_cast<int>(shares), y);
+  return check_launch("adapter forward kernels");
+}
+
+template <int KS, bool MASK, bool DX>
+int launch_outer(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const TParts& t,
+                 const Dropout& d, const uint4* cols, float* part, __half* dx,
+                 cudaStream_t stream) {
+  const OuterPlan plan(n_rows, n_cols);
+  const dim3 grid(static_cast<unsigned>(plan.col_ctas), static_cast<unsigned>(plan.splits), 1);
+  constexpr int smem = OUTER_WARPS * 16 * 64 * 4;
+  outer_kernel<KS, MASK, DX><<<grid, 32 * OUTER_WARPS, smem, stream>>>(
+      x, ld, n_rows, static_cast<int>(n_cols), t, d, cols, plan.blocks_per_split, part, dx);
+  return TALM_OK;
+}
+
+void sum_parts(const float* part, int splits, int64_t n, int rank, int rp, float factor,
+               int64_t out_j, int64_t out_c, float* out, cudaStream_t stream) {
+  const int64_t total = rank * n;
+  sum_parts_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, stream>>>(
+      part, splits, rank, rp, static_cast<int>(n), factor, out_j, out_c, out);
+}
+
+template <int KS>
+int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, const float* a,
+                 const float* b, const Shape& s, float scaling, const Dropout& d,
+                 const void* saved, __half* dx, float* da, float* db, void* work,
+                 cudaStream_t stream) {
+  constexpr int RP = 16 * KS;
+  const BackwardWork w(work, s, RP);
+  const Saved keep(const_cast<void*>(saved), s, RP);
+  const Dropout none{nullptr, 0, 1.0f};
+  if (db) {
+    launch_outer<KS, false, false>(g, ld_g, s.n_rows, s.n_out, keep.t.parts, none, nullptr,
+                                   w.b_part, nullptr, stream);
+    sum_parts(w.b_part, OuterPlan(s.n_rows, s.n_out).splits, s.n_out, s.rank, RP, scaling, 1,
+              s.rank, db, stream);
+  }
+  if (da || dx) {
+    prepare(b, 1, s.rank, s.n_out, a, s.n_in, 1, s.n_in, w.prep, s.rank, RP, stream);
+    const int st = run_inner<KS>(g, ld_g, s.n_rows, s.n_out, w.prep.rows, none, w.t_part, scaling,
+                                 w.dt.parts, stream);
+    if (st != TALM_OK) return st;
+    float* part = da ? w.a_part : nullptr;
+    if (d.drop && dx)
+      launch_outer<KS, true, true>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, w.prep.cols, part, dx,
+                                   stream);
+    else if (d.drop)
+      launch_outer<KS, true, false>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, nullptr, part,
+                                    nullptr, stream);
+    else if (dx)
+      launch_outer<KS, false, true>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, w.prep.cols, part,
+                                    dx, stream);
+    else
+      launch_outer<KS, false, false>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, nullptr, part,
+                                     nullptr, stream);
+    if (da)
+      sum_parts(w.a_part, OuterPlan(s.n_rows, s.n_in).splits, s.n_in, s.rank, RP, d.factor,
+                s.n_in, 1, da, stream);
+  }
+  return check_launch("adapter backward kernels");
 }
 
 int check_dropout(int64_t drop, const int64_t* seed, Dropout* d) {
@@ -386,8 +1003,6 @@ bool rows_ok(const void* p, int64_t ld, int64_t cols) {
   return ld >= cols && ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
-unsigned blocks(int64_t threads) { return static_cast<unsigned>((threads + 255) / 256); }
-
 }  // namespace adapter
 }  // namespace talm
 
@@ -415,20 +1030,26 @@ int talm_dropout(const void* x, int64_t ld_x, int64_t n_rows, int64_t n_cols, in
 }
 
 int talm_lora_sizes(int64_t n_rows, int64_t n_in, int64_t n_out, int64_t rank, size_t* saved,
-                    size_t* backward_ws) {
+                    size_t* forward_ws, size_t* backward_ws) {
   using namespace talm;
-  const int st = adapter::check_shape(n_rows, n_in, n_out, rank);
+  using namespace talm::adapter;
+  const int st = check_shape(n_rows, n_in, n_out, rank);
   if (st != TALM_OK) return st;
-  if (!saved || !backward_ws) return set_error(TALM_EINVAL, "null pointer");
-  *saved = static_cast<size_t>(n_rows * rank) * 4;
-  *backward_ws = static_cast<size_t>(n_rows * rank) * 4;
+  if (!saved || !forward_ws || !backward_ws) return set_error(TALM_EINVAL, "null pointer");
+  const Shape s{n_rows, n_in, n_out, static_cast<int>(rank)};
+  const int rp = padded_rank(s.rank);
+  const bool none = n_rows == 0;
+  *saved = none ? 0 : Saved(nullptr, s, rp).carve.used;
+  *forward_ws = none ? 0 : ForwardWork(nullptr, s, rp).carve.used;
+  *backward_ws = none ? 0 : BackwardWork(nullptr, s, rp).carve.used;
   return TALM_OK;
 }
 
 int talm_lora_forward(const uint16_t* x, int64_t ld_x, const uint16_t* base, int64_t ld_base,
                       const float* lora_a, const float* lora_b, int64_t n_rows, int64_t n_in,
                       int64_t n_out, int64_t rank, float scaling, const int64_t* seed,
-                      int64_t drop, uint16_t* y, void* saved, size_t saved_bytes, void* stream_) {
+                      int64_t drop, uint16_t* y, void* saved, size_t saved_bytes,
+                      void* workspace, size_t ws_bytes, void* stream_) {
   using namespace talm;
   using namespace talm::adapter;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
@@ -436,23 +1057,23 @@ int talm_lora_forward(const uint16_t* x, int64_t ld_x, const uint16_t* base, int
   int st = check_shape(n_rows, n_in, n_out, rank);
   if (st == TALM_OK) st = check_dropout(drop, seed, &d);
   if (st != TALM_OK) return st;
-  size_t need = 0, need_ws = 0;
-  talm_lora_sizes(n_rows, n_in, n_out, rank, &need, &need_ws);
+  size_t need = 0, need_forward = 0, need_backward = 0;
+  talm_lora_sizes(n_rows, n_in, n_out, rank, &need, &need_forward, &need_backward);
   if (n_rows == 0) return TALM_OK;
-  if (!x || !base || !lora_a || !lora_b || !y || !saved)
+  if (!x || !base || !lora_a || !lora_b || !y || !saved || !workspace)
     return set_error(TALM_EINVAL, "null pointer");
-  if (!rows_ok(x, ld_x, n_in) || !rows_ok(base, ld_base, n_out) || !rows_ok(y, n_out, n_out))
+  if (!rows_ok(x, ld_x, n_in) || !rows_ok(base, ld_base, n_out) || !rows_ok(y, n_out, n_out) ||
+      ((reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(workspace)) & 15) != 0)
     return set_error(TALM_EINVAL, "rows must be 16-byte aligned with strides of 8 elements");
-  if (saved_bytes < need) return set_error(TALM_EINVAL, "saved buffer too small");
+  if (saved_bytes < need || ws_bytes < need_forward)
+    return set_error(TALM_EINVAL, "saved buffer or workspace too small");
   const Shape s{n_rows, n_in, n_out, static_cast<int>(rank)};
-  float* t = static_cast<float*>(saved);
   LaunchTimer timer(TALM_KERNEL_LORA_FORWARD, stream);
-  down_kernel<<<blocks(32 * n_rows), 256, 0, stream>>>(reinterpret_cast<const __half*>(x), ld_x,
-                                                       lora_a, s, d, t);
-  up_kernel<<<blocks(n_rows * n_out), 256, 0, stream>>>(reinterpret_cast<const __half*>(base),
-                                                        ld_base, t, lora_b, s, scaling,
-                                                        reinterpret_cast<__half*>(y));
-  return check_launch("adapter forward kernels");
+  const int rp = padded_rank(s.rank);
+  auto run = rp == 16 ? run_forward<1> : rp == 32 ? run_forward<2> : run_forward<4>;
+  return run(reinterpret_cast<const __half*>(x), ld_x, reinterpret_cast<const __half*>(base),
+             ld_base, lora_a, lora_b, s, scaling, d, reinterpret_cast<__half*>(y), saved, workspace,
+             stream);
 }
 
 int talm_lora_backward(const uint16_t* g, int64_t ld_g, const uint16_t* x, int64_t ld_x,
@@ -468,8 +1089,8 @@ int talm_lora_backward(const uint16_t* g, int64_t ld_g, const uint16_t* x, int64
   int st = check_shape(n_rows, n_in, n_out, rank);
   if (st == TALM_OK) st = check_dropout(drop, seed, &d);
   if (st != TALM_OK) return st;
-  size_t need = 0, need_ws = 0;
-  talm_lora_sizes(n_rows, n_in, n_out, rank, &need, &need_ws);
+  size_t need = 0, need_forward = 0, need_backward = 0;
+  talm_lora_sizes(n_rows, n_in, n_out, rank, &need, &need_forward, &need_backward);
   if (!dx && !grad_a && !grad_b) return TALM_OK;
   if (n_rows == 0) {  // no rows: the weights' gradients are zero
     cudaError_t e = cudaSuccess;
@@ -480,26 +1101,18 @@ int talm_lora_backward(const uint16_t* g, int64_t ld_g, const uint16_t* x, int64
   }
   if (!g || !x || !lora_a || !lora_b || !saved || !workspace)
     return set_error(TALM_EINVAL, "null pointer");
-  if (!rows_ok(g, ld_g, n_out) || !rows_ok(x, ld_x, n_in) || (dx && !rows_ok(dx, n_in, n_in)))
+  if (!rows_ok(g, ld_g, n_out) || !rows_ok(x, ld_x, n_in) || (dx && !rows_ok(dx, n_in, n_in)) ||
+      ((reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(workspace)) & 15) != 0)
     return set_error(TALM_EINVAL, "rows must be 16-byte aligned with strides of 8 elements");
-  if (saved_bytes < need || ws_bytes < need_ws)
+  if (saved_bytes < need || ws_bytes < need_backward)
     return set_error(TALM_EINVAL, "saved buffer or workspace too small");
   const Shape s{n_rows, n_in, n_out, static_cast<int>(rank)};
-  const float* t = static_cast<const float*>(saved);
-  float* dt = static_cast<float*>(workspace);
-  const __half* gh = reinterpret_cast<const __half*>(g);
   LaunchTimer timer(TALM_KERNEL_LORA_BACKWARD, stream);
-  if (dx || grad_a)
-    grad_t_kernel<<<blocks(32 * n_rows), 256, 0, stream>>>(gh, ld_g, lora_b, s, scaling, dt);
-  if (grad_b)
-    grad_b_kernel<<<blocks(n_out * rank), 256, 0, stream>>>(gh, ld_g, t, s, scaling, grad_b);
-  if (grad_a)
-    grad_a_kernel<<<blocks(n_in / 8 * rank), 256, 0, stream>>>(
-        reinterpret_cast<const __half*>(x), ld_x, dt, s, d, grad_a);
-  if (dx)
-    grad_x_kernel<<<blocks(n_rows * n_in / 8), 256, 0, stream>>>(dt, lora_a, s, d,
-                                                                 reinterpret_cast<__half*>(dx));
-  return check_launch("adapter backward kernels");
+  const int rp = padded_rank(s.rank);
+  auto run = rp == 16 ? run_backward<1> : rp == 32 ? run_backward<2> : run_backward<4>;
+  return run(reinterpret_cast<const __half*>(g), ld_g, reinterpret_cast<const __half*>(x), ld_x,
+             lora_a, lora_b, s, scaling, d, saved, reinterpret_cast<__half*>(dx), grad_a, grad_b,
+             workspace, stream);
 }
 
 }  // extern "C"

@@ -71,19 +71,20 @@ def test_c_entries_reject_bad_arguments(lib):
     assert drop(n_rows=1 << 40, n_cols=1 << 20, ld=1 << 20) == 3
 
     size = _lib._SZ(0)
-    assert lib.talm_lora_sizes(4, 64, 64, 16, size, size) == 0
+    assert lib.talm_lora_sizes(4, 64, 64, 16, size, size, size) == 0
     for bad in ((-1, 64, 64, 16), (4, 60, 64, 16), (4, 64, 60, 16), (4, 64, 64, 0),
                 (4, 64, 64, 65), (4, 0, 64, 16)):
-        assert lib.talm_lora_sizes(*bad, size, size) == 1, bad
-    assert lib.talm_lora_sizes(1 << 31, 64, 64, 16, size, size) == 3
+        assert lib.talm_lora_sizes(*bad, size, size, size) == 1, bad
+    assert lib.talm_lora_sizes(1 << 31, 64, 64, 16, size, size, size) == 3
 
-    def forward(n_rows=4, drop=0, seed=None, ptr=None, ld_x=64, saved=1 << 20):
+    def forward(n_rows=4, drop=0, seed=None, ptr=None, ld_x=64, saved=1 << 20, ws=1 << 24):
         return lib.talm_lora_forward(ptr, ld_x, ptr, 64, ptr, ptr, n_rows, 64, 64, 16, 1.0, seed,
-                                     drop, ptr, ptr, saved, None)
+                                     drop, ptr, ptr, saved, ptr, ws, None)
     assert forward() == 1 and forward(drop=5) == 1 and forward(n_rows=0) == 0
     assert forward(ptr=8) == 1                      # rows off their 16-byte boundary
     assert forward(ptr=16, ld_x=60) == 1 and forward(ptr=16, ld_x=68) == 1
     assert forward(ptr=16, saved=3) == 1 and b"too small" in lib.talm_last_error()
+    assert forward(ptr=16, ws=3) == 1
 
     def backward(n_rows=4, ptr=None, out=16, ws=1 << 24, ld_g=64):
         return lib.talm_lora_backward(ptr, ld_g, ptr, 64, ptr, ptr, ptr, 1 << 24, n_rows, 64, 64,
