@@ -21,6 +21,7 @@ replays it in the backward; its products run in fp16. Here sums are fp32 and eac
 rounded once. There is no CPU path.
 """
 
+import functools
 import math
 
 import torch
@@ -47,31 +48,45 @@ def drop_threshold(p):
 
 
 def _check_seed(seed, x):
-    if (not torch.is_tensor(seed) or seed.dtype != torch.int64 or seed.numel() != 1
+    if (not torch.is_tensor(seed) or seed.dtype is not torch.int64 or seed.numel() != 1
             or seed.get_device() != x.get_device()):
         raise ValueError("seed must be an int64 tensor of one element on the input's device")
 
 
 def _rows(t, cols):
     """`t` as [rows, cols] rows of unit stride that do not overlap (a view where its strides
-    allow it, else a copy)."""
+    allow it, else a copy), and their stride."""
+    if t.is_contiguous():
+        return t, cols
     t = t.reshape(-1, cols)
-    if t.stride(1) != 1 or (t.shape[0] > 1 and t.stride(0) < cols):
-        t = t.contiguous()
-    return t
+    ld, unit = t.stride()
+    if t.shape[0] == 1:
+        ld = cols
+    if (unit != 1 and cols > 1) or ld < cols:
+        t, ld = t.contiguous(), cols
+    return t, ld
 
 
 def _rows16(t, cols):
     """`_rows` on 16-byte boundaries, as the branch's kernels read them."""
-    t = _rows(t, cols)
-    if t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % 8):
-        t = t.clone(memory_format=torch.contiguous_format)
-    return t
+    t, ld = _rows(t, cols)
+    if t.data_ptr() % 16 or ld % 8:
+        t, ld = t.clone(memory_format=torch.contiguous_format), cols
+    return t, ld
 
 
-def _stride(t):
-    """The row stride of a 2-D tensor (its width where a single row leaves it undefined)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _run_dropout(x, seed, drop):
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    n = x.numel()
+    if n:
+        cols = x.shape[-1] if x.dim() else 1
+        rows, ld = _rows(x, cols)
+        with _lib.device_of(x):
+            _lib.check(_lib.load().talm_dropout(
+                rows.data_ptr(), ld, n // cols, cols, _DTYPES[x.dtype], seed.data_ptr(), drop,
+                y.data_ptr(), _lib.raw_stream(x)), "talm_dropout")
+        RAN["dropout"] += 1
+    return y
 
 
 class _Dropout(torch.autograd.Function):
@@ -79,22 +94,14 @@ class _Dropout(torch.autograd.Function):
     def forward(ctx, x, seed, drop):
         ctx.drop = drop
         ctx.save_for_backward(seed)
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        if x.numel() == 0:
-            return y
-        cols = x.shape[-1] if x.dim() else 1
-        rows = _rows(x, cols)
-        with _lib.device_of(x):
-            _lib.check(_lib.load().talm_dropout(
-                _lib.ptr(rows), _stride(rows), rows.shape[0], cols, _DTYPES[x.dtype],
-                _lib.ptr(seed), drop, _lib.ptr(y), _lib.raw_stream(x)), "talm_dropout")
-        RAN["dropout"] += 1
-        return y
+        return _run_dropout(x, seed, drop)
 
     @staticmethod
     def backward(ctx, grad):
         (seed,) = ctx.saved_tensors
-        return _Dropout.apply(grad, seed, ctx.drop), None, None
+        # the same map; through the node again only where its own gradient is wanted
+        run = _Dropout.apply if torch.is_grad_enabled() else _run_dropout
+        return run(grad, seed, ctx.drop), None, None
 
 
 def dropout(x, p, seed):
@@ -116,6 +123,7 @@ def branch_takes(x, base, rank):
             and x.shape[-1] % 8 == 0 and base.shape[-1] % 8 == 0 and 1 <= rank <= MAX_RANK)
 
 
+@functools.lru_cache(maxsize=256)
 def _sizes(n_rows, n_in, n_out, rank):
     saved, forward, backward = _lib._SZ(0), _lib._SZ(0), _lib._SZ(0)
     _lib.check(_lib.load().talm_lora_sizes(n_rows, n_in, n_out, rank, saved, forward, backward),
@@ -123,23 +131,27 @@ def _sizes(n_rows, n_in, n_out, rank):
     return saved.value, forward.value, backward.value
 
 
+def _bytes(n, x):
+    return torch.empty(n, dtype=torch.uint8, device=x.device)
+
+
 class _LoraBranch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, base, lora_a, lora_b, scaling, seed, drop):
         n_in, n_out, rank = x.shape[-1], base.shape[-1], lora_a.shape[0]
+        n_rows = base.numel() // n_out
         a, b = lora_a.contiguous(), lora_b.contiguous()
-        xr, br = _rows16(x, n_in), _rows16(base, n_out)
-        n_rows = xr.shape[0]
+        xr, ld_x = _rows16(x, n_in)
+        br, ld_b = _rows16(base, n_out)
         saved_bytes, work_bytes, ctx.work_bytes = _sizes(n_rows, n_in, n_out, rank)
-        y = torch.empty(base.shape, dtype=base.dtype, device=x.device)
-        saved = torch.empty(saved_bytes, dtype=torch.uint8, device=x.device)
-        work = torch.empty(work_bytes, dtype=torch.uint8, device=x.device)
+        y = torch.empty(base.shape, dtype=torch.float16, device=x.device)
+        saved, work = _bytes(saved_bytes, x), _bytes(work_bytes, x)
         with _lib.device_of(x):
             _lib.check(_lib.load().talm_lora_forward(
-                _lib.ptr(xr), _stride(xr), _lib.ptr(br), _stride(br), _lib.ptr(a), _lib.ptr(b),
-                n_rows, n_in, n_out, rank, scaling, _lib.ptr(seed), drop, _lib.ptr(y),
-                _lib.ptr(saved), saved_bytes, _lib.ptr(work), work_bytes, _lib.raw_stream(x)),
-                "talm_lora_forward")
+                xr.data_ptr(), ld_x, br.data_ptr(), ld_b, a.data_ptr(), b.data_ptr(), n_rows,
+                n_in, n_out, rank, scaling, None if seed is None else seed.data_ptr(), drop,
+                y.data_ptr(), saved.data_ptr(), saved_bytes, work.data_ptr(), work_bytes,
+                _lib.raw_stream(x)), "talm_lora_forward")
         ctx.scaling, ctx.drop = scaling, drop
         ctx.save_for_backward(x, lora_a, lora_b, seed, saved)
         RAN["lora"] += 1
@@ -150,21 +162,23 @@ class _LoraBranch(torch.autograd.Function):
     def backward(ctx, grad):
         x, lora_a, lora_b, seed, saved = ctx.saved_tensors
         need_x, need_base, need_a, need_b = ctx.needs_input_grad[:4]
-        n_in, n_out, rank = x.shape[-1], grad.shape[-1], lora_a.shape[0]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        da = torch.empty(rank, n_in, dtype=torch.float32, device=x.device) if need_a else None
-        db = torch.empty(n_out, rank, dtype=torch.float32, device=x.device) if need_b else None
+        dx = torch.empty(x.shape, dtype=torch.float16, device=x.device) if need_x else None
+        da = (torch.empty(lora_a.shape, dtype=torch.float32, device=x.device) if need_a else None)
+        db = (torch.empty(lora_b.shape, dtype=torch.float32, device=x.device) if need_b else None)
         if need_x or need_a or need_b:
+            n_in, n_out, rank = x.shape[-1], grad.shape[-1], lora_a.shape[0]
             a, b = lora_a.contiguous(), lora_b.contiguous()
-            xr, gr = _rows16(x, n_in), _rows16(grad, n_out)
-            work = torch.empty(ctx.work_bytes, dtype=torch.uint8, device=x.device)
+            xr, ld_x = _rows16(x, n_in)
+            gr, ld_g = _rows16(grad, n_out)
+            work = _bytes(ctx.work_bytes, x)
             with _lib.device_of(x):
                 _lib.check(_lib.load().talm_lora_backward(
-                    _lib.ptr(gr), _stride(gr), _lib.ptr(xr), _stride(xr), _lib.ptr(a),
-                    _lib.ptr(b), _lib.ptr(saved), saved.numel(), xr.shape[0], n_in, n_out, rank,
-                    ctx.scaling, _lib.ptr(seed), ctx.drop, _lib.ptr(dx), _lib.ptr(da),
-                    _lib.ptr(db), _lib.ptr(work), work.numel(), _lib.raw_stream(x)),
-                    "talm_lora_backward")
+                    gr.data_ptr(), ld_g, xr.data_ptr(), ld_x, a.data_ptr(), b.data_ptr(),
+                    saved.data_ptr(), saved.numel(), grad.numel() // n_out, n_in, n_out, rank,
+                    ctx.scaling, None if seed is None else seed.data_ptr(), ctx.drop,
+                    dx.data_ptr() if need_x else None, da.data_ptr() if need_a else None,
+                    db.data_ptr() if need_b else None, work.data_ptr(), ctx.work_bytes,
+                    _lib.raw_stream(x)), "talm_lora_backward")
         return dx, grad if need_base else None, da, db, None, None, None
 
 
@@ -174,9 +188,9 @@ def lora_branch(x, base, lora_A, lora_B, scaling, p=0.0, seed=None):
     lora_B [out, r]: fp32, r in 1..64; `in` and `out` multiples of 8. p > 0 takes a `seed`
     (`draw_seed`); the mask is that of `dropout(x, p, seed)`."""
     n_in, n_out = x.shape[-1], base.shape[-1]
-    if x.dtype != torch.float16 or base.dtype != torch.float16:
+    if x.dtype is not torch.float16 or base.dtype is not torch.float16:
         raise TypeError(f"lora_branch takes fp16 x and base, got {x.dtype} and {base.dtype}")
-    if lora_A.dtype != torch.float32 or lora_B.dtype != torch.float32:
+    if lora_A.dtype is not torch.float32 or lora_B.dtype is not torch.float32:
         raise TypeError("lora_A and lora_B must be fp32")
     if x.shape[:-1] != base.shape[:-1]:
         raise ValueError(f"x {tuple(x.shape)} and base {tuple(base.shape)} differ in their rows")
@@ -188,10 +202,11 @@ def lora_branch(x, base, lora_A, lora_B, scaling, p=0.0, seed=None):
         raise ValueError(f"lora_branch needs a rank of 1..{MAX_RANK} and widths of multiples of "
                          f"8, got rank {rank}, {n_in} -> {n_out}")
     drop = drop_threshold(p)
-    for t in (x, base, lora_A, lora_B):
-        _lib.ptr(t)
-        if t.get_device() != x.get_device():
-            raise ValueError("x, base and the adapter must be on one device")
+    device = x.get_device()
+    if device < 0:
+        raise RuntimeError("talm_b200 kernels run on CUDA tensors only (no CPU path)")
+    if not base.get_device() == lora_A.get_device() == lora_B.get_device() == device:
+        raise ValueError("x, base and the adapter must be on one device")
     if drop == 0:
         seed = None
     else:

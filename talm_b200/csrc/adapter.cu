@@ -272,8 +272,9 @@ __device__ __forceinline__ void power_scale(float m, float* up, float* down) {
 
 // ---- prepared operands -----------------------------------------------------------------------
 // RP: the rank rounded up to 16, 32 or 64, zeros behind it.
-//   Rows:  fp16 parts hi[RP][n], lo[RP][n] of an adapter matrix with the rank in the rows (A, B^T),
-//          each row scaled; down[RP] undoes the scale.
+//   Rows:  fp16 parts of an adapter matrix with the rank in the rows (A, B^T), each row scaled
+//          (down[RP] undoes it), as n operands: [n / 64][RP / 8][half][part][lane] uint4, lane (g, t)
+//          holding columns 8 t .. 8 t + 7 of the half's 32 for rank 8 * tile + g.
 //   Cols:  bf16 parts of the same matrix as 16 x 16 mma operands of 16 columns and 16 ranks:
 //          [n / 64][4][RP / 16][part][lane] uint4; tile i of a 64-column block holds, for m = g and
 //          g + 8, columns 8 g + 2 i and 8 g + 2 i + 1.
@@ -281,7 +282,7 @@ __device__ __forceinline__ void power_scale(float m, float* up, float* down) {
 //          [lane] uint4, and fp16 parts of the rows scaled together as the m operand, t_col of the
 //          same size, with t_down[rows / 16].
 struct Rows {
-  __half *hi, *lo;
+  uint4* parts;
   float* down;
 };
 struct TParts {
@@ -317,13 +318,20 @@ __global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(
     for (int i = 0; i < PREP_THREADS / 32; ++i) m = fmaxf(m, most[i]);
     float up, down;
     power_scale(m, &up, &down);
-    uint32_t* hi = reinterpret_cast<uint32_t*>(rows.hi + static_cast<int64_t>(j) * n0);
-    uint32_t* lo = reinterpret_cast<uint32_t*>(rows.lo + static_cast<int64_t>(j) * n0);
-    for (int c = 2 * tid; c < n0; c += 2 * PREP_THREADS) {  // n0 is even
-      uint32_t h = 0, l = 0;
-      if (j < rank) split_f16(__ldg(src + c * c0) * up, __ldg(src + (c + 1) * c0) * up, h, l);
-      hi[c >> 1] = h;
-      lo[c >> 1] = l;
+    const int groups = (n0 + 63) / 64 * 8;  // of eight columns
+    for (int q = tid; q < groups; q += PREP_THREADS) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = 8 * q + 2 * i;
+        const bool in = j < rank && c < n0;  // n0 is even
+        split_f16(in ? __ldg(src + c * c0) * up : 0.0f, in ? __ldg(src + (c + 1) * c0) * up : 0.0f,
+                  hi[i], lo[i]);
+      }
+      uint4* out = rows.parts + (static_cast<int64_t>(q >> 3) * (rp / 8) + (j >> 3)) * 128 +
+                   ((q >> 2) & 1) * 64 + (j & 7) * 4 + (q & 3);
+      out[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      out[32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
     if (tid == 0) rows.down[j] = down;
     return;
@@ -418,13 +426,8 @@ __global__ void __launch_bounds__(32 * INNER_WARPS, NT == 2 ? 2 : 1) inner_kerne
       float c[2][4] = {};
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int col = s * 64 + h * 32 + 8 * t;
-        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-        if (col < n_cols) {
-          const int64_t at = static_cast<int64_t>(nt * 8 + g) * n_cols + col;
-          hi = __ldg(reinterpret_cast<const uint4*>(w.hi + at));
-          lo = __ldg(reinterpret_cast<const uint4*>(w.lo + at));
-        }
+        const uint4* wp = w.parts + (static_cast<int64_t>(s) * NT + nt) * 128 + h * 64 + lane;
+        const uint4 hi = __ldg(wp), lo = __ldg(wp + 32);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           const uint4 &a = cur[2 * m][h], &b = cur[2 * m + 1][h];
@@ -470,39 +473,40 @@ __global__ void __launch_bounds__(32 * INNER_WARPS, NT == 2 ? 2 : 1) inner_kerne
 }
 
 // ---- the operands made of t (or dt) ----------------------------------------------------------
-// t[n, j] = factor * down[j] * (sum of the parts), one warp per 16 rows.
+// t[n, j] = factor * down[j] * (sum of the parts): a CTA of four warps per 16 rows.
 template <int KS>
 __global__ void __launch_bounds__(128) t_parts_kernel(const float* __restrict__ part, int splits,
                                                       int64_t n_rows, const float* __restrict__ down,
                                                       float factor, TParts out) {
   constexpr int RP = 16 * KS;
-  __shared__ float sh[4][16][RP + 1];
+  __shared__ float m[16][RP + 1];
+  __shared__ float warp_most[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
-  const int64_t block = static_cast<int64_t>(blockIdx.x) * 4 + warp;
-  if (block * 16 >= n_rows) return;
+  const int64_t block = blockIdx.x;
   float most = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 16 * RP / 32; ++i) {
-    const int e = i * 32 + lane, r = e / RP, j = e % RP;
+  for (int i = 0; i < 16 * RP / 128; ++i) {
+    const int e = i * 128 + threadIdx.x, r = e / RP, j = e % RP;
     const int64_t n = block * 16 + r;
     float v = 0.0f;
     if (n < n_rows) {
       const float* p = part + n * RP + j;
+#pragma unroll 8
       for (int k = 0; k < splits; ++k) v += __ldg(p + static_cast<int64_t>(k) * n_rows * RP);
       v *= __ldg(down + j) * factor;
     }
-    sh[warp][r][j] = v;
+    m[r][j] = v;
     most = fmaxf(most, fabsf(v));
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+  if (lane == 0) warp_most[warp] = most;
+  __syncthreads();
+  most = fmaxf(fmaxf(warp_most[0], warp_most[1]), fmaxf(warp_most[2], warp_most[3]));
   float up, back;
   power_scale(most, &up, &back);
-  __syncwarp();
-  const auto& m = sh[warp];
-#pragma unroll
-  for (int k = 0; k < KS; ++k) {
+  for (int k = warp; k < KS; k += 4) {
     const int64_t at = (block * KS + k) * 64 + lane;
     uint32_t hi[4], lo[4];
     // n operand: registers (rows g, rows 8 + g) x (ranks 2 t, 2 t + 8)
@@ -522,32 +526,34 @@ __global__ void __launch_bounds__(128) t_parts_kernel(const float* __restrict__ 
     out.col[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     out.col[at + 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  if (lane == 0) out.down[block] = back;
+  if (threadIdx.x == 0) out.down[block] = back;
 }
 
-// D tiles of rank-wide products: for 64 columns and 16 rows, c[i][h][..] = sum_j M[col, j] T[row, j]
-// with columns 8 g + 2 i, 8 g + 2 i + 1 and rows 8 h + 2 t, 8 h + 2 t + 1: lane (g, t) gets eight
-// consecutive columns of four rows.
-template <int KS>
-__device__ __forceinline__ void rank_product(float (&c)[4][2][4], const uint4* __restrict__ cols,
-                                             const uint4 (&t_hi)[KS], const uint4 (&t_lo)[KS],
-                                             int lane) {
+// Tile i of a rank-wide product for 64 columns and R blocks of 16 rows: c[r][h][..] = sum_j
+// M[col, j] T[row, j] with columns 8 g + 2 i, 8 g + 2 i + 1 and rows 8 h + 2 t, 8 h + 2 t + 1. Over
+// the four tiles, lane (g, t) gets eight consecutive columns of four rows.
+template <int KS, int R>
+__device__ __forceinline__ void rank_tile(float (&c)[R][2][4], const uint4* __restrict__ cols,
+                                          int i, const uint4 (&t_hi)[R][KS],
+                                          const uint4 (&t_lo)[R][KS], int lane) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int u = 0; u < 4; ++u) c[i][h][u] = 0.0f;
+      for (int u = 0; u < 4; ++u) c[r][h][u] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const uint4 hi = __ldg(cols + (i * KS + k) * 64 + lane);
-      const uint4 lo = __ldg(cols + (i * KS + k) * 64 + 32 + lane);
-      mma_bf16(c[i][0], lo, t_hi[k].x, t_hi[k].y);
-      mma_bf16(c[i][1], lo, t_hi[k].z, t_hi[k].w);
-      mma_bf16(c[i][0], hi, t_lo[k].x, t_lo[k].y);
-      mma_bf16(c[i][1], hi, t_lo[k].z, t_lo[k].w);
-      mma_bf16(c[i][0], hi, t_hi[k].x, t_hi[k].y);
-      mma_bf16(c[i][1], hi, t_hi[k].z, t_hi[k].w);
+  for (int k = 0; k < KS; ++k) {
+    const uint4 hi = __ldg(cols + (i * KS + k) * 64 + lane);
+    const uint4 lo = __ldg(cols + (i * KS + k) * 64 + 32 + lane);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      mma_bf16(c[r][0], lo, t_hi[r][k].x, t_hi[r][k].y);
+      mma_bf16(c[r][1], lo, t_hi[r][k].z, t_hi[r][k].w);
+      mma_bf16(c[r][0], hi, t_lo[r][k].x, t_lo[r][k].y);
+      mma_bf16(c[r][1], hi, t_lo[r][k].z, t_lo[r][k].w);
+      mma_bf16(c[r][0], hi, t_hi[r][k].x, t_hi[r][k].y);
+      mma_bf16(c[r][1], hi, t_hi[r][k].z, t_hi[r][k].w);
     }
   }
 }
@@ -556,13 +562,17 @@ __device__ __forceinline__ void rank_product(float (&c)[4][2][4], const uint4* _
 __device__ __forceinline__ int row_of(int i, int t) { return 2 * t + (i & 1) + 8 * (i >> 1); }
 
 // ---- up: y = fp16(base + s t B^T) ------------------------------------------------------------
-// A warp takes 64 columns and every `stride`-th block of 16 rows.
+// A warp takes 64 columns and every `shares`-th pair of 16-row blocks; a pair shares the loads of
+// the columns' operand.
+constexpr int UP_BLOCKS = 2;
+
 template <int KS>
 __global__ void __launch_bounds__(256) up_kernel(const __half* __restrict__ base, int64_t ld_base,
                                                  const uint4* __restrict__ t_row,
                                                  const uint4* __restrict__ cols, int64_t n_rows,
                                                  int n_out, float scaling, int shares,
                                                  __half* __restrict__ y) {
+  constexpr int R = UP_BLOCKS;
   const int lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -574,36 +584,51 @@ __global__ void __launch_bounds__(256) up_kernel(const __half* __restrict__ base
   const int col = cb * 64 + 8 * g;
   const bool in = col < n_out;
   const uint4* my_cols = cols + static_cast<int64_t>(cb) * (4 * KS * 64);
-  for (int64_t rb = share; rb < row_blocks; rb += shares) {
-    uint4 bv[4];
+  for (int64_t rb = share * R; rb < row_blocks; rb += int64_t{shares} * R) {
+    uint32_t v[R][4][4];  // base, then y: four rows of eight columns
+    uint4 t_hi[R][KS], t_lo[R][KS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t n = rb * 16 + row_of(i, t);
-      bv[i] = in && n < n_rows ? __ldg(reinterpret_cast<const uint4*>(base + n * ld_base + col))
-                               : make_uint4(0, 0, 0, 0);
-    }
-    uint4 t_hi[KS], t_lo[KS];
+    for (int r = 0; r < R; ++r) {
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      t_hi[k] = __ldg(t_row + (rb * KS + k) * 64 + lane);
-      t_lo[k] = __ldg(t_row + (rb * KS + k) * 64 + 32 + lane);
-    }
-    float c[4][2][4];
-    rank_product<KS>(c, my_cols, t_hi, t_lo, lane);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t n = rb * 16 + row_of(i, t);
-      const uint32_t w[4] = {bv[i].x, bv[i].y, bv[i].z, bv[i].w};
-      uint32_t o[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-        o[k] = pack_half2(fmaf(scaling, c[k][i >> 1][i & 1], f.x),
-                          fmaf(scaling, c[k][i >> 1][2 + (i & 1)], f.y));
+      for (int i = 0; i < 4; ++i) {
+        const int64_t n = (rb + r) * 16 + row_of(i, t);
+        const uint4 b = in && n < n_rows
+                            ? __ldg(reinterpret_cast<const uint4*>(base + n * ld_base + col))
+                            : make_uint4(0, 0, 0, 0);
+        v[r][i][0] = b.x;
+        v[r][i][1] = b.y;
+        v[r][i][2] = b.z;
+        v[r][i][3] = b.w;
       }
-      if (in && n < n_rows)
-        *reinterpret_cast<uint4*>(y + n * n_out + col) = make_uint4(o[0], o[1], o[2], o[3]);
+      const int64_t block = min(rb + r, row_blocks - 1);
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        t_hi[r][k] = __ldg(t_row + (block * KS + k) * 64 + lane);
+        t_lo[r][k] = __ldg(t_row + (block * KS + k) * 64 + 32 + lane);
+      }
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float c[R][2][4];
+      rank_tile<KS, R>(c, my_cols, k, t_hi, t_lo, lane);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[r][i][k]));
+          v[r][i][k] = pack_half2(fmaf(scaling, c[r][i >> 1][i & 1], f.x),
+                                  fmaf(scaling, c[r][i >> 1][2 + (i & 1)], f.y));
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int64_t n = (rb + r) * 16 + row_of(i, t);
+        if (in && n < n_rows)
+          *reinterpret_cast<uint4*>(y + n * n_out + col) =
+              make_uint4(v[r][i][0], v[r][i][1], v[r][i][2], v[r][i][3]);
+      }
   }
 }
 
@@ -614,7 +639,9 @@ constexpr int OUTER_WARPS = 8;
 // and dx[n, c] = fp16(keep factor sum_j T[n, j] A[j, c]) (where DX). A CTA takes 64 columns and a
 // range of 16-row blocks, its warps every OUTER_WARPS-th of them. Lane (g, t) loads columns
 // 8 g .. 8 g + 7 of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9: two rows of a column make an operand
-// register by one byte permutation, and dx comes out of rank_product at the same places.
+// register by one byte permutation, and dx comes out of rank_tile at the same places. A rank of
+// 64 is divided between the halves of the CTA's warps (64 sums in a lane's registers either way),
+// which read the same activations and take turns with dx.
 template <int KS, bool MASK, bool DX>
 __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kernel(
     const __half* __restrict__ x, int64_t ld_x, int64_t n_rows, int n_cols, TParts tp, Dropout d,
@@ -622,8 +649,11 @@ __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kerne
     __half* __restrict__ dx) {
   extern __shared__ __align__(16) float outer_smem[];  // [OUTER_WARPS][16][64]
   constexpr int RP = 16 * KS;
+  constexpr int HALVES = KS == 4 ? 2 : 1, MT = KS / HALVES;  // rank tiles of a warp
+  constexpr int LANES = OUTER_WARPS / HALVES;                // warps that take turns with the rows
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
+  const int half = warp / LANES, turn = warp % LANES;
   const int cb = blockIdx.x;
   const int col = cb * 64 + 8 * g;
   const bool in = col < n_cols;
@@ -644,13 +674,13 @@ __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kerne
                  : make_uint4(0, 0, 0, 0);
     }
   };
-  float acc[KS][8][4] = {};
+  float acc[MT][8][4] = {};
   uint4 cur[4];
-  if (rb0 + warp < rb1) load(rb0 + warp, cur);
-  for (int64_t rb = rb0 + warp; rb < rb1; rb += OUTER_WARPS) {
+  if (rb0 + turn < rb1) load(rb0 + turn, cur);
+  for (int64_t rb = rb0 + turn; rb < rb1; rb += LANES) {
     uint4 next[4];
-    const bool more = rb + OUTER_WARPS < rb1;
-    if (more) load(rb + OUTER_WARPS, next);
+    const bool more = rb + LANES < rb1;
+    if (more) load(rb + LANES, next);
     uint4 keep[4];
     if (MASK) {
       const uint4 ones = make_uint4(~0u, ~0u, ~0u, ~0u);
@@ -664,9 +694,9 @@ __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kerne
     if (sums) {
       const float back = __ldg(tp.down + rb);
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const uint4 hi = __ldg(tp.col + (rb * KS + k) * 64 + lane);
-        const uint4 lo = __ldg(tp.col + (rb * KS + k) * 64 + 32 + lane);
+      for (int k = 0; k < MT; ++k) {
+        const uint4* tc = tp.col + (rb * KS + half * MT + k) * 64 + lane;
+        const uint4 hi = __ldg(tc), lo = __ldg(tc + 32);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           const uint32_t r0 = u == 0 ? cur[0].x : u == 1 ? cur[0].y : u == 2 ? cur[0].z : cur[0].w;
@@ -686,30 +716,31 @@ __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kerne
         }
       }
     }
-    if (DX) {
-      uint4 t_hi[KS], t_lo[KS];
+    if (DX && (HALVES == 1 || (((rb - rb0) / LANES) & 1) == half)) {
+      uint4 t_hi[1][KS], t_lo[1][KS];
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        t_hi[k] = __ldg(tp.row + (rb * KS + k) * 64 + lane);
-        t_lo[k] = __ldg(tp.row + (rb * KS + k) * 64 + 32 + lane);
+        t_hi[0][k] = __ldg(tp.row + (rb * KS + k) * 64 + lane);
+        t_lo[0][k] = __ldg(tp.row + (rb * KS + k) * 64 + 32 + lane);
       }
-      float c[4][2][4];
-      rank_product<KS>(c, my_cols, t_hi, t_lo, lane);
+      uint32_t o[4][4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float c[1][2][4];
+        rank_tile<KS, 1>(c, my_cols, k, t_hi, t_lo, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[i][k] = pack_half2(d.factor * c[0][i >> 1][i & 1], d.factor * c[0][i >> 1][2 + (i & 1)]);
+          if (MASK)
+            o[i][k] &= k == 0 ? keep[i].x : k == 1 ? keep[i].y : k == 2 ? keep[i].z : keep[i].w;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int64_t n = rb * 16 + row_of(i, t);
-        uint32_t o[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          o[k] = pack_half2(d.factor * c[k][i >> 1][i & 1], d.factor * c[k][i >> 1][2 + (i & 1)]);
-        if (MASK) {
-          o[0] &= keep[i].x;
-          o[1] &= keep[i].y;
-          o[2] &= keep[i].z;
-          o[3] &= keep[i].w;
-        }
         if (in && n < n_rows)
-          *reinterpret_cast<uint4*>(dx + n * n_cols + col) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(dx + n * n_cols + col) =
+              make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
       }
     }
     if (more) {
@@ -718,10 +749,10 @@ __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kerne
     }
   }
   if (!sums) return;
-  // the warps add their sums in warp order, 16 ranks at a time
+  // the warps add their sums in warp order, 16 ranks of each half at a time
   float* out = part + static_cast<int64_t>(blockIdx.y) * RP * n_cols;
 #pragma unroll
-  for (int k = 0; k < KS; ++k) {
+  for (int k = 0; k < MT; ++k) {
     __syncthreads();
     float* mine = outer_smem + warp * (16 * 64);
 #pragma unroll
@@ -732,12 +763,14 @@ __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kerne
       mine[(g + 8) * 64 + 8 * (2 * t + 1) + u] = acc[k][u][3];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * 64; i += 32 * OUTER_WARPS) {
+    for (int i = threadIdx.x; i < HALVES * 16 * 64; i += 32 * OUTER_WARPS) {
+      const int hf = i >> 10, in_tile = i & 1023;
       const int c = cb * 64 + (i & 63);
       float v = 0.0f;
 #pragma unroll
-      for (int q = 0; q < OUTER_WARPS; ++q) v += outer_smem[q * (16 * 64) + i];
-      if (c < n_cols) out[static_cast<int64_t>(16 * k + (i >> 6)) * n_cols + c] = v;
+      for (int q = 0; q < LANES; ++q) v += outer_smem[(hf * LANES + q) * (16 * 64) + in_tile];
+      if (c < n_cols)
+        out[static_cast<int64_t>(16 * (hf * MT + k) + (in_tile >> 6)) * n_cols + c] = v;
     }
   }
 }
@@ -774,7 +807,7 @@ constexpr int TARGET_CTAS = 296;  // two for each of 148 SMs
 struct InnerPlan {
   int row_groups, row_ctas, splits, steps_per_split;
   InnerPlan(int64_t n_rows, int64_t n_cols, int rp) {
-    row_groups = n_rows <= 32 ? 1 : rp >= 64 ? 4 : 2;
+    row_groups = n_rows <= 32 ? 1 : rp / 8;  // a wide rank-wide operand serves more rows
     row_ctas = static_cast<int>((n_rows + 32 * row_groups - 1) / (32 * row_groups));
     const int steps = static_cast<int>((n_cols + 63) / 64);
     int want = TARGET_CTAS / row_ctas;  // at least one step for each warp of a row group
@@ -817,8 +850,7 @@ struct Prepared {
   Rows rows;
   uint4* cols;
   Prepared(Carve& c, int64_t n_rows_matrix, int64_t n_cols_matrix, int rp) {
-    rows.hi = c.take<__half>(static_cast<size_t>(rp) * n_rows_matrix);
-    rows.lo = c.take<__half>(static_cast<size_t>(rp) * n_rows_matrix);
+    rows.parts = c.take<uint4>(static_cast<size_t>((n_rows_matrix + 63) / 64) * (rp / 8) * 128);
     rows.down = c.take<float>(rp);
     cols = c.take<uint4>(static_cast<size_t>((n_cols_matrix + 63) / 64) * 4 * (rp / 16) * 64);
   }
@@ -891,7 +923,7 @@ int run_inner(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const
   kernel<<<grid, 32 * INNER_WARPS, smem, stream>>>(x, ld, n_rows, static_cast<int>(n_cols), rows, d,
                                                    plan.row_groups, plan.steps_per_split, part);
   const int64_t blocks = (n_rows + 15) / 16;
-  t_parts_kernel<KS><<<static_cast<unsigned>((blocks + 3) / 4), 128, 0, stream>>>(
+  t_parts_kernel<KS><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(
       part, plan.splits, n_rows, rows.down, factor, out);
   return TALM_OK;
 }
@@ -909,7 +941,8 @@ int run_forward(const __half* x, int64_t ld_x, const __half* base, int64_t ld_ba
   if (st != TALM_OK) return st;
   const int64_t col_blocks = (s.n_out + 63) / 64, row_blocks = (s.n_rows + 15) / 16;
   int64_t shares = (int64_t{TARGET_CTAS} * 8 + col_blocks - 1) / col_blocks;
-  if (shares > row_blocks) shares = row_blocks;
+  const int64_t pairs = (row_blocks + UP_BLOCKS - 1) / UP_BLOCKS;
+  if (shares > pairs) shares = pairs;
   up_kernel<KS><<<static_cast<unsigned>((col_blocks * shares + 7) / 8), 256, 0, stream>>>(
       base, ld_base, keep.t.parts.row, w.prep.cols, s.n_rows, static_cast<int>(s.n_out), scaling,
       static_cast<int>(shares), y);
