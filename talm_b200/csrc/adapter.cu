@@ -12,47 +12,10 @@
 // order, and the eight 16-bit halves of the four result words belong to the eight elements. The
 // low 15 bits u of its half keep an element when u >= d, d = round(p * 32768): 15 bits let two
 // elements be compared in one 32-bit register without a carry between them.
-#include "common.cuh"
+#include "adapter_gemm.cuh"
 
 namespace talm {
 namespace adapter {
-
-constexpr int MAX_RANK = 64;
-constexpr int DROP_ALL = 32768;
-
-struct Dropout {
-  const long long* seed;  // device; null: no dropout (drop must be 0)
-  uint32_t drop;          // 0..32768
-  float factor;           // 32768 / (32768 - drop), 0 when everything is dropped
-};
-
-__device__ __forceinline__ void philox_round(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
-  const uint32_t h0 = __umulhi(c[0], 0xD2511F53u), l0 = c[0] * 0xD2511F53u;
-  const uint32_t h1 = __umulhi(c[2], 0xCD9E8D57u), l1 = c[2] * 0xCD9E8D57u;
-  c[0] = h1 ^ c[1] ^ k0;
-  c[1] = l1;
-  c[2] = h0 ^ c[3] ^ k1;
-  c[3] = l0;
-}
-
-// The four words of group q (elements 8 q .. 8 q + 7).
-__device__ __forceinline__ void philox(uint64_t q, uint64_t key, uint32_t (&c)[4]) {
-  uint32_t k0 = static_cast<uint32_t>(key), k1 = static_cast<uint32_t>(key >> 32);
-  c[0] = static_cast<uint32_t>(q);
-  c[1] = static_cast<uint32_t>(q >> 32);
-  c[2] = 0;
-  c[3] = 0;
-#pragma unroll
-  for (int i = 0; i < 7; ++i) {
-    philox_round(c, k0, k1);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-}
-
-__device__ __forceinline__ bool kept(const uint32_t (&c)[4], int i, uint32_t drop) {
-  return ((c[i >> 1] >> (16 * (i & 1))) & 0x7FFFu) >= drop;
-}
 
 template <class T>
 __device__ __forceinline__ float to_f32(T v);
@@ -73,19 +36,6 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
-}
-
-// All ones in each half of the result whose element is kept: the 15-bit draws of a word plus
-// 0x8000 - drop carry into bit 15 of their own half exactly when they reach the threshold, and the
-// permutation copies that bit over the half.
-__device__ __forceinline__ uint32_t keep_mask2(uint32_t word, uint32_t bias2) {
-  const uint32_t sum = (word & 0x7FFF7FFFu) + bias2;
-  uint32_t mask;
-  asm("prmt.b32 %0, %1, 0, 0xBB99;" : "=r"(mask) : "r"(sum));
-  return mask;
-}
-__device__ __forceinline__ uint32_t keep_bias2(uint32_t drop) {
-  return (0x8000u - drop) * 0x10001u;
 }
 
 __device__ __forceinline__ uint32_t scale2(uint32_t v, float f, __half) {
@@ -208,10 +158,10 @@ int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, co
 //
 // Six products, three of them along the wide dimensions:
 //   inner   t = keep x A^T and dt = g B      (sums over the columns of a wide activation)
-//   outer   dA = dt^T keep x, dB = g^T t     (sums over its rows), with dx in dA's pass
-//   up      y = base + s t B^T               (sums over the rank; dx = keep dt A likewise)
+//   outer   dA = dt^T keep x, dB = g^T t     (sums over its rows)
+//   up      y = base + s t B^T and dx = keep dt A (sums over the rank): adapter_gemm.cuh
 // Every pass reads a wide activation once from HBM and keeps the rank-wide operand in registers
-// and caches; all of them run on mma.sync m16n8k16, whose fragments are loaded straight from global
+// and caches; inner and outer run on mma.sync m16n8k16, whose fragments are loaded straight from global
 // memory (16 bytes per lane and load, no shared memory): the reduction index of an mma may be
 // permuted, so the eight consecutive columns that a lane loads are used as they lie.
 //
@@ -237,56 +187,22 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&p);
-}
-// The two bf16 parts of a pair.
-__device__ __forceinline__ void split_bf16(float v0, float v1, uint32_t& hi, uint32_t& lo) {
-  hi = pack_bf16(v0, v1);
-  lo = pack_bf16(v0 - __uint_as_float(hi << 16), v1 - __uint_as_float(hi & 0xFFFF0000u));
-}
-// The two fp16 parts of a pair that has been scaled.
-__device__ __forceinline__ void split_f16(float v0, float v1, uint32_t& hi, uint32_t& lo) {
-  hi = pack_half2(v0, v1);
-  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-  lo = pack_half2(v0 - h.x, v1 - h.y);
-}
-// For a largest magnitude m: *up brings it to [2^14, 2^15), *down undoes that. Clamped so that both
-// are normal numbers; 1 for zero (and for what is not finite, which stays so).
-__device__ __forceinline__ void power_scale(float m, float* up, float* down) {
-  int e = static_cast<int>((__float_as_uint(m) >> 23) & 255) - 127 - 14;
-  if (m == 0.0f || !(m < __int_as_float(0x7F800000))) e = 0;
-  e = max(-112, min(112, e));
-  *up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  *down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-}
-
 // ---- prepared operands -----------------------------------------------------------------------
 // RP: the rank rounded up to 16, 32 or 64, zeros behind it.
 //   Rows:  fp16 parts of an adapter matrix with the rank in the rows (A, B^T), each row scaled
 //          (down[RP] undoes it), as n operands: [n / 64][RP / 8][half][part][lane] uint4, lane (g, t)
 //          holding columns 8 t .. 8 t + 7 of the half's 32 for rank 8 * tile + g.
-//   Cols:  bf16 parts of the same matrix as 16 x 16 mma operands of 16 columns and 16 ranks:
-//          [n / 64][4][RP / 16][part][lane] uint4; tile i of a 64-column block holds, for m = g and
-//          g + 8, columns 8 g + 2 i and 8 g + 2 i + 1.
-//   T:     of t or dt: bf16 parts as the n operand of 16 rows, t_row [rows / 16][RP / 16][part]
-//          [lane] uint4, and fp16 parts of the rows scaled together as the m operand, t_col of the
-//          same size, with t_down[rows / 16].
+//   Cat:   bf16 parts (hi | lo | hi) of an adapter matrix with the rank in the columns (B, A^T), rows
+//          of up::chunks(RP) * 64, zeros behind the third part.
+//   T:     of t or dt: cat, bf16 parts (hi | hi | lo) laid out likewise, and fp16 parts of 16 rows
+//          scaled together as the m operand, col [rows / 16][RP / 16][part][lane] uint4, with
+//          down[rows / 16].
 struct Rows {
   uint4* parts;
   float* down;
 };
 struct TParts {
-  uint4 *row, *col;
+  uint4 *cat, *col;
   float* down;
 };
 
@@ -296,11 +212,24 @@ __host__ __device__ constexpr int padded_rank(int rank) {
 
 constexpr int PREP_THREADS = 256;
 
+// Ranks j .. j + 7 of the three parts of row r of a concatenated operand; the first eight write the
+// zeros behind the parts too.
+__device__ __forceinline__ void put_cat(uint4* cat, int64_t r, int j, int rp, uint4 p0, uint4 p1,
+                                        uint4 p2) {
+  const int pieces = up::chunks(rp) * 8;  // of eight elements
+  uint4* row = cat + r * pieces;
+  row[j >> 3] = p0;
+  row[(rp + j) >> 3] = p1;
+  row[(2 * rp + j) >> 3] = p2;
+  if (j == 0)
+    for (int i = 3 * rp / 8; i < pieces; ++i) row[i] = make_uint4(0, 0, 0, 0);
+}
+
 // One CTA per padded rank builds its row of `rows` from m0 (element (j, c) at m0[j * j0 + c * c0]);
-// the others build `cols` from m1, a thread per lane of an operand.
+// the others build `cat` from m1, a thread per column and eight ranks.
 __global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(
     const float* __restrict__ m0, int64_t j0, int64_t c0, int n0, Rows rows,
-    const float* __restrict__ m1, int64_t j1, int64_t c1, int n1, uint4* __restrict__ cols,
+    const float* __restrict__ m1, int64_t j1, int64_t c1, int n1, uint4* __restrict__ cat,
     int rank, int rp) {
   const int tid = threadIdx.x;
   if (static_cast<int>(blockIdx.x) < rp) {
@@ -336,27 +265,21 @@ __global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(
     if (tid == 0) rows.down[j] = down;
     return;
   }
-  const int ks = rp / 16;
   const int64_t e = static_cast<int64_t>(blockIdx.x - rp) * PREP_THREADS + tid;
-  const int64_t blocks = (n1 + 63) / 64;
-  if (e >= blocks * 4 * ks * 32) return;
-  const int lane = static_cast<int>(e & 31), g = lane >> 2, t = lane & 3;
-  const int64_t tile = e >> 5;  // (block * 4 + i) * ks + k
-  const int k = static_cast<int>(tile % ks), i = static_cast<int>(tile / ks % 4);
-  const int64_t c = tile / ks / 4 * 64 + 8 * g + 2 * i;
+  const int64_t c = e % n1;
+  const int j = static_cast<int>(e / n1) * 8;
+  if (j >= rp) return;
   uint32_t hi[4], lo[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {  // registers: (m = g, g + 8) x (k low, k high)
-    const int64_t col = c + (r & 1);
-    const int j = 16 * k + 2 * t + 8 * (r >> 1);
+  for (int i = 0; i < 4; ++i) {
     float v[2];
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      v[u] = col < n1 && j + u < rank ? __ldg(m1 + (j + u) * j1 + col * c1) : 0.0f;
-    split_bf16(v[0], v[1], hi[r], lo[r]);
+      v[u] = j + 2 * i + u < rank ? __ldg(m1 + (j + 2 * i + u) * j1 + c * c1) : 0.0f;
+    split_bf16(v[0], v[1], hi[i], lo[i]);
   }
-  cols[tile * 64 + lane] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-  cols[tile * 64 + 32 + lane] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  put_cat(cat, c, j, rp, make_uint4(hi[0], hi[1], hi[2], hi[3]),
+          make_uint4(lo[0], lo[1], lo[2], lo[3]), make_uint4(hi[0], hi[1], hi[2], hi[3]));
 }
 
 // ---- inner: sums over the columns ------------------------------------------------------------
@@ -506,17 +429,18 @@ __global__ void __launch_bounds__(128) t_parts_kernel(const float* __restrict__ 
   most = fmaxf(fmaxf(warp_most[0], warp_most[1]), fmaxf(warp_most[2], warp_most[3]));
   float up, back;
   power_scale(most, &up, &back);
+  for (int i = threadIdx.x; i < 16 * RP / 8; i += 128) {  // a row's next eight ranks
+    const int r = i & 15, j = (i >> 4) * 8;
+    if (block * 16 + r >= n_rows) continue;
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split_bf16(m[r][j + 2 * k], m[r][j + 2 * k + 1], hi[k], lo[k]);
+    const uint4 h = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    put_cat(out.cat, block * 16 + r, j, RP, h, h, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+  }
   for (int k = warp; k < KS; k += 4) {
     const int64_t at = (block * KS + k) * 64 + lane;
     uint32_t hi[4], lo[4];
-    // n operand: registers (rows g, rows 8 + g) x (ranks 2 t, 2 t + 8)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int n = g + 8 * (r >> 1), j = 16 * k + 2 * t + 8 * (r & 1);
-      split_bf16(m[n][j], m[n][j + 1], hi[r], lo[r]);
-    }
-    out.row[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    out.row[at + 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     // m operand of the transpose: registers (ranks g, g + 8) x (rows 2 t, 2 t + 8)
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -529,124 +453,21 @@ __global__ void __launch_bounds__(128) t_parts_kernel(const float* __restrict__ 
   if (threadIdx.x == 0) out.down[block] = back;
 }
 
-// Tile i of a rank-wide product for 64 columns and R blocks of 16 rows: c[r][h][..] = sum_j
-// M[col, j] T[row, j] with columns 8 g + 2 i, 8 g + 2 i + 1 and rows 8 h + 2 t, 8 h + 2 t + 1. Over
-// the four tiles, lane (g, t) gets eight consecutive columns of four rows.
-template <int KS, int R>
-__device__ __forceinline__ void rank_tile(float (&c)[R][2][4], const uint4* __restrict__ cols,
-                                          int i, const uint4 (&t_hi)[R][KS],
-                                          const uint4 (&t_lo)[R][KS], int lane) {
-#pragma unroll
-  for (int r = 0; r < R; ++r)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) c[r][h][u] = 0.0f;
-#pragma unroll
-  for (int k = 0; k < KS; ++k) {
-    const uint4 hi = __ldg(cols + (i * KS + k) * 64 + lane);
-    const uint4 lo = __ldg(cols + (i * KS + k) * 64 + 32 + lane);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      mma_bf16(c[r][0], lo, t_hi[r][k].x, t_hi[r][k].y);
-      mma_bf16(c[r][1], lo, t_hi[r][k].z, t_hi[r][k].w);
-      mma_bf16(c[r][0], hi, t_lo[r][k].x, t_lo[r][k].y);
-      mma_bf16(c[r][1], hi, t_lo[r][k].z, t_lo[r][k].w);
-      mma_bf16(c[r][0], hi, t_hi[r][k].x, t_hi[r][k].y);
-      mma_bf16(c[r][1], hi, t_hi[r][k].z, t_hi[r][k].w);
-    }
-  }
-}
-
 // Where the rows of lane t lie in a block of 16: 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
 __device__ __forceinline__ int row_of(int i, int t) { return 2 * t + (i & 1) + 8 * (i >> 1); }
 
-// ---- up: y = fp16(base + s t B^T) ------------------------------------------------------------
-// A warp takes 64 columns and every `shares`-th pair of 16-row blocks; a pair shares the loads of
-// the columns' operand.
-constexpr int UP_BLOCKS = 2;
-
-template <int KS>
-__global__ void __launch_bounds__(256) up_kernel(const __half* __restrict__ base, int64_t ld_base,
-                                                 const uint4* __restrict__ t_row,
-                                                 const uint4* __restrict__ cols, int64_t n_rows,
-                                                 int n_out, float scaling, int shares,
-                                                 __half* __restrict__ y) {
-  constexpr int R = UP_BLOCKS;
-  const int lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int col_blocks = (n_out + 63) / 64;
-  const int cb = static_cast<int>(id % col_blocks);
-  const int64_t share = id / col_blocks;
-  const int64_t row_blocks = (n_rows + 15) / 16;
-  if (share >= shares) return;
-  const int col = cb * 64 + 8 * g;
-  const bool in = col < n_out;
-  const uint4* my_cols = cols + static_cast<int64_t>(cb) * (4 * KS * 64);
-  for (int64_t rb = share * R; rb < row_blocks; rb += int64_t{shares} * R) {
-    uint32_t v[R][4][4];  // base, then y: four rows of eight columns
-    uint4 t_hi[R][KS], t_lo[R][KS];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t n = (rb + r) * 16 + row_of(i, t);
-        const uint4 b = in && n < n_rows
-                            ? __ldg(reinterpret_cast<const uint4*>(base + n * ld_base + col))
-                            : make_uint4(0, 0, 0, 0);
-        v[r][i][0] = b.x;
-        v[r][i][1] = b.y;
-        v[r][i][2] = b.z;
-        v[r][i][3] = b.w;
-      }
-      const int64_t block = min(rb + r, row_blocks - 1);
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        t_hi[r][k] = __ldg(t_row + (block * KS + k) * 64 + lane);
-        t_lo[r][k] = __ldg(t_row + (block * KS + k) * 64 + 32 + lane);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float c[R][2][4];
-      rank_tile<KS, R>(c, my_cols, k, t_hi, t_lo, lane);
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[r][i][k]));
-          v[r][i][k] = pack_half2(fmaf(scaling, c[r][i >> 1][i & 1], f.x),
-                                  fmaf(scaling, c[r][i >> 1][2 + (i & 1)], f.y));
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t n = (rb + r) * 16 + row_of(i, t);
-        if (in && n < n_rows)
-          *reinterpret_cast<uint4*>(y + n * n_out + col) =
-              make_uint4(v[r][i][0], v[r][i][1], v[r][i][2], v[r][i][3]);
-      }
-  }
-}
-
-// ---- outer: sums over the rows, and dx --------------------------------------------------------
+// ---- outer: sums over the rows ----------------------------------------------------------------
 constexpr int OUTER_WARPS = 8;
 
-// part[split][j][c] = sum over the split's rows of T[n, j] (keep) x[n, c] (unless `part` is null),
-// and dx[n, c] = fp16(keep factor sum_j T[n, j] A[j, c]) (where DX). A CTA takes 64 columns and a
-// range of 16-row blocks, its warps every OUTER_WARPS-th of them. Lane (g, t) loads columns
-// 8 g .. 8 g + 7 of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9: two rows of a column make an operand
-// register by one byte permutation, and dx comes out of rank_tile at the same places. A rank of
-// 64 is divided between the halves of the CTA's warps (64 sums in a lane's registers either way),
-// which read the same activations and take turns with dx.
-template <int KS, bool MASK, bool DX>
+// part[split][j][c] = sum over the split's rows of T[n, j] (keep) x[n, c]. A CTA takes 64 columns
+// and a range of 16-row blocks, its warps take turns with those. Lane (g, t) loads columns 8 g ..
+// 8 g + 7 of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9: two rows of a column make an operand register by
+// one byte permutation. A rank of 64 is divided between the halves of the CTA's warps (64 sums in a
+// lane's registers at most), which read the same activations.
+template <int KS, bool MASK>
 __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kernel(
     const __half* __restrict__ x, int64_t ld_x, int64_t n_rows, int n_cols, TParts tp, Dropout d,
-    const uint4* __restrict__ cols, int blocks_per_split, float* __restrict__ part,
-    __half* __restrict__ dx) {
+    int blocks_per_split, float* __restrict__ part) {
   extern __shared__ __align__(16) float outer_smem[];  // [OUTER_WARPS][16][64]
   constexpr int RP = 16 * KS;
   constexpr int HALVES = KS == 4 ? 2 : 1, MT = KS / HALVES;  // rank tiles of a warp
@@ -662,14 +483,12 @@ __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kerne
   const int64_t rb1 = min(row_blocks, rb0 + blocks_per_split);
   const uint64_t key = MASK ? static_cast<uint64_t>(__ldg(d.seed)) : 0;
   const uint32_t bias2 = keep_bias2(d.drop);
-  const uint4* my_cols = DX ? cols + static_cast<int64_t>(cb) * (4 * KS * 64) : nullptr;
-  const bool sums = part != nullptr;
 
   auto load = [&](int64_t rb, uint4 (&v)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int64_t n = rb * 16 + row_of(i, t);
-      v[i] = in && n < n_rows && sums
+      v[i] = in && n < n_rows
                  ? __ldg(reinterpret_cast<const uint4*>(x + n * ld_x + col))
                  : make_uint4(0, 0, 0, 0);
     }
@@ -681,17 +500,12 @@ __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kerne
     uint4 next[4];
     const bool more = rb + LANES < rb1;
     if (more) load(rb + LANES, next);
-    uint4 keep[4];
     if (MASK) {
-      const uint4 ones = make_uint4(~0u, ~0u, ~0u, ~0u);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        keep[i] = masked(ones, rb * 16 + row_of(i, t), n_cols, col, key, bias2);
-        cur[i] = make_uint4(cur[i].x & keep[i].x, cur[i].y & keep[i].y, cur[i].z & keep[i].z,
-                            cur[i].w & keep[i].w);
-      }
+      for (int i = 0; i < 4; ++i)
+        cur[i] = masked(cur[i], rb * 16 + row_of(i, t), n_cols, col, key, bias2);
     }
-    if (sums) {
+    {
       const float back = __ldg(tp.down + rb);
 #pragma unroll
       for (int k = 0; k < MT; ++k) {
@@ -716,39 +530,11 @@ __global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kerne
         }
       }
     }
-    if (DX && (HALVES == 1 || (((rb - rb0) / LANES) & 1) == half)) {
-      uint4 t_hi[1][KS], t_lo[1][KS];
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        t_hi[0][k] = __ldg(tp.row + (rb * KS + k) * 64 + lane);
-        t_lo[0][k] = __ldg(tp.row + (rb * KS + k) * 64 + 32 + lane);
-      }
-      uint32_t o[4][4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float c[1][2][4];
-        rank_tile<KS, 1>(c, my_cols, k, t_hi, t_lo, lane);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          o[i][k] = pack_half2(d.factor * c[0][i >> 1][i & 1], d.factor * c[0][i >> 1][2 + (i & 1)]);
-          if (MASK)
-            o[i][k] &= k == 0 ? keep[i].x : k == 1 ? keep[i].y : k == 2 ? keep[i].z : keep[i].w;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int64_t n = rb * 16 + row_of(i, t);
-        if (in && n < n_rows)
-          *reinterpret_cast<uint4*>(dx + n * n_cols + col) =
-              make_uint4(o[i][0], o[i][1], o[i][2], o[i][3]);
-      }
-    }
     if (more) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) cur[i] = next[i];
     }
   }
-  if (!sums) return;
   // the warps add their sums in warp order, 16 ranks of each half at a time
   float* out = part + static_cast<int64_t>(blockIdx.y) * RP * n_cols;
 #pragma unroll
@@ -839,20 +625,20 @@ struct TBuffers {
   TParts parts;
   TBuffers(Carve& c, int64_t n_rows, int rp) {
     const size_t blocks = static_cast<size_t>((n_rows + 15) / 16);
-    parts.row = c.take<uint4>(blocks * (rp / 16) * 64);
+    parts.cat = c.take<uint4>(static_cast<size_t>(n_rows) * up::chunks(rp) * 8);
     parts.col = c.take<uint4>(blocks * (rp / 16) * 64);
     parts.down = c.take<float>(blocks);
   }
 };
 
-// The adapter's operands of one direction: the rows of one matrix, the columns of the other.
+// The adapter's operands of one direction: one matrix as rows, the other concatenated.
 struct Prepared {
   Rows rows;
-  uint4* cols;
+  uint4* cat;
   Prepared(Carve& c, int64_t n_rows_matrix, int64_t n_cols_matrix, int rp) {
     rows.parts = c.take<uint4>(static_cast<size_t>((n_rows_matrix + 63) / 64) * (rp / 8) * 128);
     rows.down = c.take<float>(rp);
-    cols = c.take<uint4>(static_cast<size_t>((n_cols_matrix + 63) / 64) * 4 * (rp / 16) * 64);
+    cat = c.take<uint4>(static_cast<size_t>(n_cols_matrix) * up::chunks(rp) * 8);
   }
 };
 
@@ -901,10 +687,9 @@ int allow_smem(K kernel, int bytes) {
 
 void prepare(const float* m0, int64_t j0, int64_t c0, int64_t n0, const float* m1, int64_t j1,
              int64_t c1, int64_t n1, const Prepared& p, int rank, int rp, cudaStream_t stream) {
-  const int64_t lanes = (n1 + 63) / 64 * 4 * (rp / 16) * 32;
-  const int64_t grid = rp + (lanes + PREP_THREADS - 1) / PREP_THREADS;
+  const int64_t grid = rp + (n1 * (rp / 8) + PREP_THREADS - 1) / PREP_THREADS;
   prepare_kernel<<<static_cast<unsigned>(grid), PREP_THREADS, 0, stream>>>(
-      m0, j0, c0, static_cast<int>(n0), p.rows, m1, j1, c1, static_cast<int>(n1), p.cols, rank,
+      m0, j0, c0, static_cast<int>(n0), p.rows, m1, j1, c1, static_cast<int>(n1), p.cat, rank,
       rp);
 }
 
@@ -939,26 +724,18 @@ int run_forward(const __half* x, int64_t ld_x, const __half* base, int64_t ld_ba
   const int st = run_inner<KS>(x, ld_x, s.n_rows, s.n_in, w.prep.rows, d, w.part, d.factor,
                                keep.t.parts, stream);
   if (st != TALM_OK) return st;
-  const int64_t col_blocks = (s.n_out + 63) / 64, row_blocks = (s.n_rows + 15) / 16;
-  int64_t shares = (int64_t{TARGET_CTAS} * 8 + col_blocks - 1) / col_blocks;
-  const int64_t pairs = (row_blocks + UP_BLOCKS - 1) / UP_BLOCKS;
-  if (shares > pairs) shares = pairs;
-  up_kernel<KS><<<static_cast<unsigned>((col_blocks * shares + 7) / 8), 256, 0, stream>>>(
-      base, ld_base, keep.t.parts.row, w.prep.cols, s.n_rows, static_cast<int>(s.n_out), scaling,
-      static_cast<int>(shares), y);
-  return check_launch("adapter forward kernels");
+  return up::launch<up::chunks(RP), false>(keep.t.parts.cat, w.prep.cat, base, ld_base, y, s.n_rows,
+                                           s.n_out, scaling, d, stream);
 }
 
-template <int KS, bool MASK, bool DX>
-int launch_outer(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const TParts& t,
-                 const Dropout& d, const uint4* cols, float* part, __half* dx,
-                 cudaStream_t stream) {
+template <int KS, bool MASK>
+void launch_outer(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const TParts& t,
+                  const Dropout& d, float* part, cudaStream_t stream) {
   const OuterPlan plan(n_rows, n_cols);
   const dim3 grid(static_cast<unsigned>(plan.col_ctas), static_cast<unsigned>(plan.splits), 1);
   constexpr int smem = OUTER_WARPS * 16 * 64 * 4;
-  outer_kernel<KS, MASK, DX><<<grid, 32 * OUTER_WARPS, smem, stream>>>(
-      x, ld, n_rows, static_cast<int>(n_cols), t, d, cols, plan.blocks_per_split, part, dx);
-  return TALM_OK;
+  outer_kernel<KS, MASK><<<grid, 32 * OUTER_WARPS, smem, stream>>>(
+      x, ld, n_rows, static_cast<int>(n_cols), t, d, plan.blocks_per_split, part);
 }
 
 void sum_parts(const float* part, int splits, int64_t n, int rank, int rp, float factor,
@@ -978,8 +755,7 @@ int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, c
   const Saved keep(const_cast<void*>(saved), s, RP);
   const Dropout none{nullptr, 0, 1.0f};
   if (db) {
-    launch_outer<KS, false, false>(g, ld_g, s.n_rows, s.n_out, keep.t.parts, none, nullptr,
-                                   w.b_part, nullptr, stream);
+    launch_outer<KS, false>(g, ld_g, s.n_rows, s.n_out, keep.t.parts, none, w.b_part, stream);
     sum_parts(w.b_part, OuterPlan(s.n_rows, s.n_out).splits, s.n_out, s.rank, RP, scaling, 1,
               s.rank, db, stream);
   }
@@ -988,19 +764,15 @@ int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, c
     const int st = run_inner<KS>(g, ld_g, s.n_rows, s.n_out, w.prep.rows, none, w.t_part, scaling,
                                  w.dt.parts, stream);
     if (st != TALM_OK) return st;
-    float* part = da ? w.a_part : nullptr;
-    if (d.drop && dx)
-      launch_outer<KS, true, true>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, w.prep.cols, part, dx,
-                                   stream);
-    else if (d.drop)
-      launch_outer<KS, true, false>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, nullptr, part,
-                                    nullptr, stream);
-    else if (dx)
-      launch_outer<KS, false, true>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, w.prep.cols, part,
-                                    dx, stream);
-    else
-      launch_outer<KS, false, false>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, nullptr, part,
-                                     nullptr, stream);
+    if (dx) {
+      const int st = up::launch<up::chunks(RP), true>(w.dt.parts.cat, w.prep.cat, nullptr, 0, dx,
+                                                      s.n_rows, s.n_in, d.factor, d, stream);
+      if (st != TALM_OK) return st;
+    }
+    if (da && d.drop)
+      launch_outer<KS, true>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, w.a_part, stream);
+    else if (da)
+      launch_outer<KS, false>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, w.a_part, stream);
     if (da)
       sum_parts(w.a_part, OuterPlan(s.n_rows, s.n_in).splits, s.n_in, s.rank, RP, d.factor,
                 s.n_in, 1, da, stream);

@@ -1,0 +1,86 @@
+// Parts that the adapter's kernels share: the dropout's generator and masks, and the splits of fp32
+// operands.
+#pragma once
+
+#include "common.cuh"
+
+namespace talm {
+namespace adapter {
+
+constexpr int MAX_RANK = 64;
+constexpr int DROP_ALL = 32768;
+
+struct Dropout {
+  const long long* seed;  // device; null: no dropout (drop must be 0)
+  uint32_t drop;          // 0..32768
+  float factor;           // 32768 / (32768 - drop), 0 when everything is dropped
+};
+
+__device__ __forceinline__ void philox_round(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
+  const uint32_t h0 = __umulhi(c[0], 0xD2511F53u), l0 = c[0] * 0xD2511F53u;
+  const uint32_t h1 = __umulhi(c[2], 0xCD9E8D57u), l1 = c[2] * 0xCD9E8D57u;
+  c[0] = h1 ^ c[1] ^ k0;
+  c[1] = l1;
+  c[2] = h0 ^ c[3] ^ k1;
+  c[3] = l0;
+}
+
+// The four words of group q (elements 8 q .. 8 q + 7).
+__device__ __forceinline__ void philox(uint64_t q, uint64_t key, uint32_t (&c)[4]) {
+  uint32_t k0 = static_cast<uint32_t>(key), k1 = static_cast<uint32_t>(key >> 32);
+  c[0] = static_cast<uint32_t>(q);
+  c[1] = static_cast<uint32_t>(q >> 32);
+  c[2] = 0;
+  c[3] = 0;
+#pragma unroll
+  for (int i = 0; i < 7; ++i) {
+    philox_round(c, k0, k1);
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+}
+
+__device__ __forceinline__ bool kept(const uint32_t (&c)[4], int i, uint32_t drop) {
+  return ((c[i >> 1] >> (16 * (i & 1))) & 0x7FFFu) >= drop;
+}
+
+// All ones in each half of the result whose element is kept: the 15-bit draws of a word plus
+// 0x8000 - drop carry into bit 15 of their own half exactly when they reach the threshold, and the
+// permutation copies that bit over the half.
+__device__ __forceinline__ uint32_t keep_mask2(uint32_t word, uint32_t bias2) {
+  const uint32_t sum = (word & 0x7FFF7FFFu) + bias2;
+  uint32_t mask;
+  asm("prmt.b32 %0, %1, 0, 0xBB99;" : "=r"(mask) : "r"(sum));
+  return mask;
+}
+__device__ __forceinline__ uint32_t keep_bias2(uint32_t drop) {
+  return (0x8000u - drop) * 0x10001u;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+// The two bf16 parts of a pair.
+__device__ __forceinline__ void split_bf16(float v0, float v1, uint32_t& hi, uint32_t& lo) {
+  hi = pack_bf16(v0, v1);
+  lo = pack_bf16(v0 - __uint_as_float(hi << 16), v1 - __uint_as_float(hi & 0xFFFF0000u));
+}
+// The two fp16 parts of a pair that has been scaled.
+__device__ __forceinline__ void split_f16(float v0, float v1, uint32_t& hi, uint32_t& lo) {
+  hi = pack_half2(v0, v1);
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  lo = pack_half2(v0 - h.x, v1 - h.y);
+}
+// For a largest magnitude m: *up brings it to [2^14, 2^15), *down undoes that. Clamped so that both
+// are normal numbers; 1 for zero (and for what is not finite, which stays so).
+__device__ __forceinline__ void power_scale(float m, float* up, float* down) {
+  int e = static_cast<int>((__float_as_uint(m) >> 23) & 255) - 127 - 14;
+  if (m == 0.0f || !(m < __int_as_float(0x7F800000))) e = 0;
+  e = max(-112, min(112, e));
+  *up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  *down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+}  // namespace adapter
+}  // namespace talm

@@ -1,0 +1,323 @@
+// The adapter's rank-wide product on tcgen05: for an activation of n_rows x n_cols,
+//   ADD:   y  = fp16(base + scale * T M^T)       (the branch's output: T = t, M = B)
+//   MASK:  dx = fp16(keep(...) * scale * T M^T)  (the input's gradient: T = dt, M = A^T)
+// T [n_rows, rank] and M [n_cols, rank] are fp32, each split in two bf16 parts; the three products
+// hi hi, hi lo and lo hi (the fourth is under 2^-16 of a term) are one GEMM over the
+// concatenated rank: rows of T' = (hi | hi | lo) and of M' = (hi | lo | hi), padded with zeros to
+// whole 64-column chunks. (The 16 x 8 x 16 mma.sync form of the same product needed 96 mma's and 40
+// 16-byte loads per 16 x 64 outputs at rank 64, and took 300 us for 16384 x 8960 outputs.)
+//
+// Bound by HBM: base is read and y written once (4 bytes per output). A persistent CTA walks 128 x
+// 128 tiles down the rows of a column tile, whose M' stays in shared memory:
+//   warp 0      TMA producer: M' when the column tile changes, T' (two stages), base in boxes of 64
+//               columns (four slots)
+//   warp 1      MMA issuer: 4 x tcgen05.mma (128 x 128 x 16) per chunk into one of two TMEM buffers
+//   warp 2      TMA stores of finished boxes; frees their slots
+//   warps 4-11  epilogue: two groups of 128 threads, a box each: TMEM -> fp32 -> + base (or mask) ->
+//               fp16, in place in the box's slot
+// Every wait is bounded; a wait that gives up ends the CTA's roles and records TALM_ETIMEOUT.
+#pragma once
+
+#include "adapter_common.cuh"
+
+namespace talm {
+namespace adapter {
+namespace up {
+
+constexpr int TILE = 128;
+constexpr int CHUNK_BYTES = TILE * 128;  // 128 rows of 64 bf16, 128-byte swizzle
+constexpr int BOX_BYTES = TILE * 128;    // 128 rows of 64 fp16
+constexpr int SLOTS = 4;
+constexpr int T_STAGES = 2;
+constexpr int EPI_WARPS = 8;
+constexpr int FIRST_EPI_WARP = 4;
+constexpr int THREADS = 32 * (FIRST_EPI_WARP + EPI_WARPS);
+
+// 64-column chunks of the concatenated rank
+__host__ __device__ constexpr int chunks(int rp) { return (3 * rp + 63) / 64; }
+__host__ __device__ constexpr int smem_bytes(int n_chunks) {
+  return (1 + T_STAGES) * n_chunks * CHUNK_BYTES + SLOTS * BOX_BYTES + 1024 + 512;
+}
+static_assert(smem_bytes(chunks(64)) <= 232448, "shared memory of one CTA");
+
+struct Ctl {
+  uint64_t m_full, m_empty;
+  uint64_t t_full[T_STAGES], t_empty[T_STAGES];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t box_full[SLOTS], box_done[SLOTS], box_empty[SLOTS];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct Params {
+  int64_t n_rows;
+  int n_cols, row_tiles;
+  int64_t n_tiles;
+  float scale;
+  Dropout drop;
+};
+
+template <int CHUNKS, bool MASK>
+__global__ void __launch_bounds__(THREADS, 1)
+    up_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_constant__ CUtensorMap tm_m,
+              const __grid_constant__ CUtensorMap tm_base,
+              const __grid_constant__ CUtensorMap tm_out, Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint8_t* m_s = smem;
+  uint8_t* t_s = m_s + CHUNKS * CHUNK_BYTES;
+  uint8_t* box_s = t_s + T_STAGES * CHUNKS * CHUNK_BYTES;
+  Ctl* ctl = reinterpret_cast<Ctl*>(box_s + SLOTS * BOX_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // this CTA's tiles, numbered down the rows of one column tile after another
+  const int64_t first = p.n_tiles * blockIdx.x / gridDim.x;
+  const int64_t last = p.n_tiles * (blockIdx.x + 1) / gridDim.x;
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_t);
+    prefetch_tmap(&tm_m);
+    prefetch_tmap(&tm_base);
+    prefetch_tmap(&tm_out);
+    mbar_init(&ctl->m_full, 1);
+    mbar_init(&ctl->m_empty, 1);
+    for (int i = 0; i < T_STAGES; ++i) {
+      mbar_init(&ctl->t_full[i], 1);
+      mbar_init(&ctl->t_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->acc_full[i], 1);
+      mbar_init(&ctl->acc_empty[i], EPI_WARPS);
+    }
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&ctl->box_full[i], 1);
+      mbar_init(&ctl->box_done[i], EPI_WARPS / 2);
+      mbar_init(&ctl->box_empty[i], 1);
+    }
+    mbar_init(&ctl->drain, 1);
+    ctl->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl->tmem_base, 2 * TILE);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = ctl->tmem_base;
+  volatile int* abort = &ctl->abort;
+
+  if (warp == 0) {
+    if (lane == 0) {  // producer
+      int64_t column = -1;
+      uint32_t m_phase = 0, m_n = 0, t_n[T_STAGES] = {}, box_n[SLOTS] = {};  // copies issued
+      int i = 0;  // tiles so far
+      for (int64_t tile = first; tile < last; ++tile, ++i) {
+        const int ct = static_cast<int>(tile / p.row_tiles);
+        const int row0 = static_cast<int>(tile % p.row_tiles) * TILE;
+        if (ct != column) {
+          if (column >= 0) {  // the MMAs of the column tile before are done with M'
+            if (!mbar_wait(&ctl->m_empty, m_phase, abort)) break;
+            m_phase ^= 1;
+          }
+          column = ct;
+          ++m_n;
+          mbar_arrive_expect_tx(&ctl->m_full, CHUNKS * CHUNK_BYTES);
+          for (int c = 0; c < CHUNKS; ++c)
+            tma_load_2d(m_s + c * CHUNK_BYTES, &tm_m, &ctl->m_full, c * 64, ct * TILE);
+        }
+        const int st = i % T_STAGES;
+        if (!mbar_wait(&ctl->t_empty[st], ((i / T_STAGES) & 1) ^ 1, abort)) break;
+        ++t_n[st];
+        mbar_arrive_expect_tx(&ctl->t_full[st], CHUNKS * CHUNK_BYTES);
+        for (int c = 0; c < CHUNKS; ++c)
+          tma_load_2d(t_s + (st * CHUNKS + c) * CHUNK_BYTES, &tm_t, &ctl->t_full[st], c * 64, row0);
+        if (!MASK) {
+          bool ok = true;
+          for (int q = 0; q < 2; ++q) {
+            const int slot = (2 * i + q) % SLOTS;
+            if (!mbar_wait(&ctl->box_empty[slot], ((i / (SLOTS / 2)) & 1) ^ 1, abort)) {
+              ok = false;
+              break;
+            }
+            ++box_n[slot];
+            // a box past the last column is filled with zeros and not stored
+            mbar_arrive_expect_tx(&ctl->box_full[slot], BOX_BYTES);
+            tma_load_2d(box_s + slot * BOX_BYTES, &tm_base, &ctl->box_full[slot],
+                        ct * TILE + q * 64, row0);
+          }
+          if (!ok) break;
+        }
+      }
+      // every copy issued lands before the CTA gives up its shared memory
+      if (m_n) mbar_drain(&ctl->m_full, (m_n - 1) & 1);
+      for (int k = 0; k < T_STAGES; ++k)
+        if (t_n[k]) mbar_drain(&ctl->t_full[k], (t_n[k] - 1) & 1);
+      for (int k = 0; k < SLOTS; ++k)
+        if (box_n[k]) mbar_drain(&ctl->box_full[k], (box_n[k] - 1) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {  // MMA issuer
+      constexpr uint32_t idesc = idesc_bf16_f32(TILE, TILE, false, false);
+      int64_t column = -1;
+      uint32_t m_phase = 0;
+      int i = 0;
+      for (int64_t tile = first; tile < last; ++tile, ++i) {
+        const int64_t ct = tile / p.row_tiles;
+        if (ct != column) {
+          if (!mbar_wait(&ctl->m_full, m_phase, abort)) break;
+          m_phase ^= 1;
+          column = ct;
+        }
+        const int st = i % T_STAGES, acc = i & 1;
+        if (!mbar_wait(&ctl->t_full[st], (i / T_STAGES) & 1, abort)) break;
+        if (!mbar_wait(&ctl->acc_empty[acc], ((i >> 1) & 1) ^ 1, abort)) break;
+        tc_fence_after();
+        const uint32_t a0 = smem_u32(t_s + st * CHUNKS * CHUNK_BYTES), b0 = smem_u32(m_s);
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem_base + acc * TILE,
+                     smem_desc_sw128(a0 + c * CHUNK_BYTES + k * 32, 16, 1024),
+                     smem_desc_sw128(b0 + c * CHUNK_BYTES + k * 32, 16, 1024), idesc,
+                     c != 0 || k != 0);
+        umma_commit(&ctl->t_empty[st]);
+        umma_commit(&ctl->acc_full[acc]);
+        if (tile + 1 < last && (tile + 1) / p.row_tiles != ct) umma_commit(&ctl->m_empty);
+      }
+      umma_commit(&ctl->drain);
+      mbar_drain(&ctl->drain, 0);
+    }
+  } else if (warp == 2) {
+    if (lane == 0) {  // stores
+      int i = 0;
+      for (int64_t tile = first; tile < last; ++tile, ++i) {
+        const int ct = static_cast<int>(tile / p.row_tiles);
+        const int row0 = static_cast<int>(tile % p.row_tiles) * TILE;
+        bool ok = true;
+        for (int q = 0; q < 2; ++q) {
+          const int slot = (2 * i + q) % SLOTS;
+          if (!mbar_wait(&ctl->box_done[slot], (i / (SLOTS / 2)) & 1, abort)) {
+            ok = false;
+            break;
+          }
+          if (ct * TILE + q * 64 < p.n_cols)
+            tma_store_2d(&tm_out, box_s + slot * BOX_BYTES, ct * TILE + q * 64, row0);
+          bulk_commit();
+          // the store before this one has read its slot: free it
+          bulk_wait_read<1>();
+          if (i > 0 || q > 0) mbar_arrive(&ctl->box_empty[(2 * i + q - 1) % SLOTS]);
+        }
+        if (!ok) break;
+      }
+      bulk_wait_all();
+    }
+  } else if (warp >= FIRST_EPI_WARP) {
+    const int quarter = warp & 3, q = (warp - FIRST_EPI_WARP) >> 2;
+    const int r = quarter * 32 + lane;
+    const uint64_t key = MASK && p.drop.drop ? static_cast<uint64_t>(__ldg(p.drop.seed)) : 0;
+    const uint32_t bias2 = keep_bias2(p.drop.drop);
+    int i = 0;
+    for (int64_t tile = first; tile < last; ++tile, ++i) {
+      const int ct = static_cast<int>(tile / p.row_tiles);
+      const int64_t row = tile % p.row_tiles * TILE + r;
+      const int slot = (2 * i + q) % SLOTS, acc = i & 1;
+      const uint32_t phase = (i / (SLOTS / 2)) & 1;
+      bool ok;
+      if (MASK)
+        ok = mbar_wait(&ctl->box_empty[slot], phase ^ 1, abort);
+      else
+        ok = mbar_wait(&ctl->box_full[slot], phase, abort);
+      if (ok) ok = mbar_wait(&ctl->acc_full[acc], (i >> 1) & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      uint8_t* box = box_s + slot * BOX_BYTES + r * 128;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t d[32];
+        tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * TILE +
+                               q * 64 + h * 32,
+                           d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {  // eight columns
+          uint4* at = reinterpret_cast<uint4*>(box + (((4 * h + c) ^ (r & 7)) << 4));
+          uint32_t o[4];
+          if (MASK) {
+            uint32_t w[4] = {};
+            if (p.drop.drop)
+              philox(static_cast<uint64_t>((row * p.n_cols + ct * TILE + q * 64 + h * 32 + c * 8) >> 3),
+                     key, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              o[k] = pack_half2(p.scale * __uint_as_float(d[8 * c + 2 * k]),
+                                p.scale * __uint_as_float(d[8 * c + 2 * k + 1])) &
+                     keep_mask2(w[k], bias2);
+          } else {
+            const uint4 b = *at;
+            const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&bw[k]));
+              o[k] = pack_half2(fmaf(p.scale, __uint_as_float(d[8 * c + 2 * k]), f.x),
+                                fmaf(p.scale, __uint_as_float(d[8 * c + 2 * k + 1]), f.y));
+            }
+          }
+          *at = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+      }
+      tc_fence_before();
+      fence_proxy_async_smem();  // the box is read by a bulk store
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&ctl->acc_empty[acc]);
+        mbar_arrive(&ctl->box_done[slot]);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, 2 * TILE);
+}
+
+// t_op [n_rows, 64 chunks], m_op [n_cols, 64 chunks]: the concatenated bf16 parts
+template <int CHUNKS, bool MASK>
+int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base, void* out,
+           int64_t n_rows, int64_t n_cols, float scale, const Dropout& d, cudaStream_t stream) {
+  CUtensorMap tm_t, tm_m, tm_base, tm_out;
+  int st = talm_make_tmap_2d_f16(&tm_t, t_op, CHUNKS * 64, n_rows, CHUNKS * 64, 64, TILE);
+  if (st == TALM_OK)
+    st = talm_make_tmap_2d_f16(&tm_m, m_op, CHUNKS * 64, n_cols, CHUNKS * 64, 64, TILE);
+  if (st == TALM_OK) st = talm_make_tmap_2d_f16(&tm_out, out, n_cols, n_rows, n_cols, 64, TILE);
+  if (st == TALM_OK)
+    st = MASK ? (tm_base = tm_out, TALM_OK)
+              : talm_make_tmap_2d_f16(&tm_base, base, n_cols, n_rows, ld_base, 64, TILE);
+  if (st != TALM_OK) return st;
+  constexpr int smem = smem_bytes(CHUNKS);
+  auto kernel = up_kernel<CHUNKS, MASK>;
+  // set on every call (it only notes the value): no per-device record to keep
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
+  Params p;
+  p.n_rows = n_rows;
+  p.n_cols = static_cast<int>(n_cols);
+  p.row_tiles = static_cast<int>((n_rows + TILE - 1) / TILE);
+  p.n_tiles = static_cast<int64_t>(p.row_tiles) * ((n_cols + TILE - 1) / TILE);
+  p.scale = scale;
+  p.drop = d;
+  const int sms = current_sm_count();
+  if (sms <= 0) return set_error(TALM_ENODEV, "no CUDA device");
+  const unsigned grid = static_cast<unsigned>(p.n_tiles < sms ? p.n_tiles : sms);
+  kernel<<<grid, THREADS, smem, stream>>>(tm_t, tm_m, tm_base, tm_out, p);
+  return check_launch("adapter up kernel");
+}
+
+}  // namespace up
+}  // namespace adapter
+}  // namespace talm
