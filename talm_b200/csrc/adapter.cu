@@ -156,53 +156,37 @@ int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, co
 // ------------------------------------------------------------------------------------------
 // the branch
 //
-// Six products, three of them along the wide dimensions:
-//   inner   t = keep x A^T and dt = g B      (sums over the columns of a wide activation)
-//   outer   dA = dt^T keep x, dB = g^T t     (sums over its rows)
-//   up      y = base + s t B^T and dx = keep dt A (sums over the rank): adapter_gemm.cuh
-// Every pass reads a wide activation once from HBM and keeps the rank-wide operand in registers
-// and caches; inner and outer run on mma.sync m16n8k16, whose fragments are loaded straight from global
-// memory (16 bytes per lane and load, no shared memory): the reduction index of an mma may be
-// permuted, so the eight consecutive columns that a lane loads are used as they lie.
-//
-// fp32 operands are split in two 16-bit parts. Where the other operand is an activation (t, dt,
-// dA, dB: fp32 results) they are fp16 parts of the operand scaled by a power of two that brings its
-// largest element to [2^14, 2^15): 2^-22 and better, at any size of the operand; the scale is one
-// per adapter row (A, B) or per 16 rows of the activation (t, dt). Where both operands are
-// fp32 and the result is fp16 (y, dx) they are bf16 parts without scale, and the product of the two
-// small parts is left out: 2^-16 of each term, under a sixteenth of the result's own rounding.
-// mma sums are moved into separate fp32 sums every 64 columns or 16 rows: the tensor core cuts its
-// sums off instead of rounding them, which would add up over a long chain.
+// Six products, each of a wide activation and a rank-wide operand (adapter_gemm.cuh):
+//   inner   t = keep x A^T and dt = s g B            sums over the activation's columns
+//   outer   dA = dt^T keep x and dB = s g^T t        sums over its rows
+//   up      y = base + s t B^T and dx = keep dt A    sums over the rank
+// and between them small kernels that turn the rank-wide fp32 operands into 16-bit parts for the
+// tensor cores. Where the other operand is an fp16 activation and the result fp32 (inner, outer) they
+// are two fp16 parts of the operand scaled by a power of two that brings its largest element to
+// [2^14, 2^15): 2^-22 and better, at any size of the operand; the scale is one per adapter row (A, B)
+// or per 128 rows of the activation (t, dt). Where both operands are fp32 and the result is fp16 (up)
+// they are two bf16 parts without scale, and the product of the two small ones is left out: under
+// 2^-16 of each term, a sixteenth of the result's own rounding.
 // ------------------------------------------------------------------------------------------
 struct Shape {
   int64_t n_rows, n_in, n_out;
   int rank;
 };
 
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                        uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // ---- prepared operands -----------------------------------------------------------------------
 // RP: the rank rounded up to 16, 32 or 64, zeros behind it.
 //   Rows:  fp16 parts of an adapter matrix with the rank in the rows (A, B^T), each row scaled
-//          (down[RP] undoes it), as n operands: [n / 64][RP / 8][half][part][lane] uint4, lane (g, t)
-//          holding columns 8 t .. 8 t + 7 of the half's 32 for rank 8 * tile + g.
-//   Cat:   bf16 parts (hi | lo | hi) of an adapter matrix with the rank in the columns (B, A^T), rows
+//          (down[RP] undoes it): [2 RP, n], the small parts behind the large ones.
+//   cat:   bf16 parts (hi | lo | hi) of an adapter matrix with the rank in the columns (B, A^T), rows
 //          of up::chunks(RP) * 64, zeros behind the third part.
-//   T:     of t or dt: cat, bf16 parts (hi | hi | lo) laid out likewise, and fp16 parts of 16 rows
-//          scaled together as the m operand, col [rows / 16][RP / 16][part][lane] uint4, with
-//          down[rows / 16].
+//   TParts, of t or dt: cat, bf16 parts (hi | hi | lo) laid out likewise, and pair, fp16 parts
+//          (hi | lo) in rows of sums::pair_width(RP), 128 rows scaled together (down undoes it).
 struct Rows {
-  uint4* parts;
+  __half* parts;
   float* down;
 };
 struct TParts {
-  uint4 *cat, *col;
+  uint4 *cat, *pair;
   float* down;
 };
 
@@ -247,20 +231,13 @@ __global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(
     for (int i = 0; i < PREP_THREADS / 32; ++i) m = fmaxf(m, most[i]);
     float up, down;
     power_scale(m, &up, &down);
-    const int groups = (n0 + 63) / 64 * 8;  // of eight columns
-    for (int q = tid; q < groups; q += PREP_THREADS) {
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int c = 8 * q + 2 * i;
-        const bool in = j < rank && c < n0;  // n0 is even
-        split_f16(in ? __ldg(src + c * c0) * up : 0.0f, in ? __ldg(src + (c + 1) * c0) * up : 0.0f,
-                  hi[i], lo[i]);
-      }
-      uint4* out = rows.parts + (static_cast<int64_t>(q >> 3) * (rp / 8) + (j >> 3)) * 128 +
-                   ((q >> 2) & 1) * 64 + (j & 7) * 4 + (q & 3);
-      out[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      out[32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    uint32_t* hi = reinterpret_cast<uint32_t*>(rows.parts + static_cast<int64_t>(j) * n0);
+    uint32_t* lo = reinterpret_cast<uint32_t*>(rows.parts + static_cast<int64_t>(rp + j) * n0);
+    for (int c = 2 * tid; c < n0; c += 2 * PREP_THREADS) {  // n0 is even
+      uint32_t h = 0, l = 0;
+      if (j < rank) split_f16(__ldg(src + c * c0) * up, __ldg(src + (c + 1) * c0) * up, h, l);
+      hi[c >> 1] = h;
+      lo[c >> 1] = l;
     }
     if (tid == 0) rows.down[j] = down;
     return;
@@ -282,136 +259,25 @@ __global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(
           make_uint4(lo[0], lo[1], lo[2], lo[3]), make_uint4(hi[0], hi[1], hi[2], hi[3]));
 }
 
-// ---- inner: sums over the columns ------------------------------------------------------------
-constexpr int INNER_WARPS = 8;
-
-// The four keep masks of the group of eight at (row n, column k).
-__device__ __forceinline__ uint4 masked(uint4 v, int64_t n, int64_t n_in, int k, uint64_t key,
-                                        uint32_t bias2) {
-  uint32_t c[4];
-  philox(static_cast<uint64_t>((n * n_in + k) >> 3), key, c);
-  return make_uint4(v.x & keep_mask2(c[0], bias2), v.y & keep_mask2(c[1], bias2),
-                    v.z & keep_mask2(c[2], bias2), v.w & keep_mask2(c[3], bias2));
-}
-
-// part[split][n][j] = sum over the split's columns of (keep) x[n, c] w[j, c], w the scaled rows. A
-// warp takes 32 rows and every KG-th 64-column step of its CTA's columns: per step, lane (g, t)
-// loads the columns 8 t .. 8 t + 7 of both 32-column halves for rows g, g + 8, g + 16, g + 24.
-template <int NT, bool MASK>
-__global__ void __launch_bounds__(32 * INNER_WARPS, NT == 2 ? 2 : 1) inner_kernel(
-    const __half* __restrict__ x, int64_t ld_x, int64_t n_rows, int n_cols, Rows w, Dropout d,
-    int row_groups, int steps_per_split, float* __restrict__ part) {
-  extern __shared__ __align__(16) float inner_smem[];  // [INNER_WARPS][32][8 NT]
-  constexpr int RP = 8 * NT;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int kg = INNER_WARPS / row_groups;  // warps that share a row group's columns
-  const int rg = warp / kg, kw = warp % kg;
-  const int64_t r0 = (static_cast<int64_t>(blockIdx.x) * row_groups + rg) * 32;
-  const int steps = (n_cols + 63) / 64;
-  const int s0 = blockIdx.y * steps_per_split;
-  const int s1 = min(steps, s0 + steps_per_split);
-  const uint64_t key = MASK ? static_cast<uint64_t>(__ldg(d.seed)) : 0;
-  const uint32_t bias2 = keep_bias2(d.drop);
-
-  const __half* xr[4];
-  int64_t row[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {  // rows past the end read the last one; they are not stored
-    row[i] = min(r0 + g + 8 * i, n_rows - 1);
-    xr[i] = x + row[i] * ld_x + 8 * t;
-  }
-  auto load = [&](int s, uint4 (&v)[4][2]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        v[i][h] = s * 64 + h * 32 + 8 * t < n_cols
-                      ? __ldg(reinterpret_cast<const uint4*>(xr[i] + s * 64 + h * 32))
-                      : make_uint4(0, 0, 0, 0);
-  };
-  float acc[2][NT][4] = {};
-  uint4 cur[4][2];
-  if (s0 + kw < s1) load(s0 + kw, cur);
-  for (int s = s0 + kw; s < s1; s += kg) {
-    uint4 next[4][2];
-    const bool more = s + kg < s1;
-    if (more) load(s + kg, next);
-    if (MASK) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          cur[i][h] = masked(cur[i][h], row[i], n_cols, s * 64 + h * 32 + 8 * t, key, bias2);
-    }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float c[2][4] = {};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint4* wp = w.parts + (static_cast<int64_t>(s) * NT + nt) * 128 + h * 64 + lane;
-        const uint4 hi = __ldg(wp), lo = __ldg(wp + 32);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const uint4 &a = cur[2 * m][h], &b = cur[2 * m + 1][h];
-          mma_f16(c[m], a.x, b.x, a.y, b.y, lo.x, lo.y);
-          mma_f16(c[m], a.z, b.z, a.w, b.w, lo.z, lo.w);
-          mma_f16(c[m], a.x, b.x, a.y, b.y, hi.x, hi.y);
-          mma_f16(c[m], a.z, b.z, a.w, b.w, hi.z, hi.w);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < 2; ++m)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][nt][i] += c[m][i];
-    }
-    if (more) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cur[i][0] = next[i][0];
-        cur[i][1] = next[i][1];
-      }
-    }
-  }
-  // the warps of a row group add their sums in warp order
-  float* mine = inner_smem + warp * (32 * RP);
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float* q = mine + (16 * m + g) * RP + nt * 8 + 2 * t;
-      *reinterpret_cast<float2*>(q) = make_float2(acc[m][nt][0], acc[m][nt][1]);
-      *reinterpret_cast<float2*>(q + 8 * RP) = make_float2(acc[m][nt][2], acc[m][nt][3]);
-    }
-  __syncthreads();
-  float* out = part + static_cast<int64_t>(blockIdx.y) * n_rows * RP;
-  for (int i = threadIdx.x; i < row_groups * 32 * RP; i += 32 * INNER_WARPS) {
-    const int grp = i / (32 * RP), in = i % (32 * RP);
-    const int64_t n = (static_cast<int64_t>(blockIdx.x) * row_groups + grp) * 32 + in / RP;
-    if (n >= n_rows) continue;
-    float v = 0.0f;
-    for (int k = 0; k < kg; ++k) v += inner_smem[(grp * kg + k) * (32 * RP) + in];
-    out[n * RP + in % RP] = v;
-  }
-}
-
 // ---- the operands made of t (or dt) ----------------------------------------------------------
-// t[n, j] = factor * down[j] * (sum of the parts): a CTA of four warps per 16 rows.
-template <int KS>
-__global__ void __launch_bounds__(128) t_parts_kernel(const float* __restrict__ part, int splits,
-                                                      int64_t n_rows, const float* __restrict__ down,
-                                                      float factor, TParts out) {
-  constexpr int RP = 16 * KS;
+// t[n, j] = factor * down[j] * (sum of the parts): a CTA of four warps per 16 rows, a cluster of
+// eight per 128 rows, which find their common scale through each other's shared memory.
+constexpr int T_CLUSTER = 8;
+
+template <int RP>
+__global__ void __cluster_dims__(T_CLUSTER, 1, 1) __launch_bounds__(128)
+    t_parts_kernel(const float* __restrict__ part, int splits, int64_t n_rows,
+                   const float* __restrict__ down, float factor, TParts out) {
   __shared__ float m[16][RP + 1];
   __shared__ float warp_most[4];
+  __shared__ float cta_most;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int64_t block = blockIdx.x;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 16;
   float most = 0.0f;
 #pragma unroll
   for (int i = 0; i < 16 * RP / 128; ++i) {
     const int e = i * 128 + threadIdx.x, r = e / RP, j = e % RP;
-    const int64_t n = block * 16 + r;
+    const int64_t n = row0 + r;
     float v = 0.0f;
     if (n < n_rows) {
       const float* p = part + n * RP + j;
@@ -426,139 +292,38 @@ __global__ void __launch_bounds__(128) t_parts_kernel(const float* __restrict__ 
   for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
   if (lane == 0) warp_most[warp] = most;
   __syncthreads();
-  most = fmaxf(fmaxf(warp_most[0], warp_most[1]), fmaxf(warp_most[2], warp_most[3]));
+  if (threadIdx.x == 0)
+    cta_most = fmaxf(fmaxf(warp_most[0], warp_most[1]), fmaxf(warp_most[2], warp_most[3]));
+  cluster_sync();
+  const uint32_t at = smem_u32(&cta_most);
+#pragma unroll
+  for (int c = 0; c < T_CLUSTER; ++c) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(at, c)));
+    most = fmaxf(most, v);
+  }
   float up, back;
   power_scale(most, &up, &back);
-  for (int i = threadIdx.x; i < 16 * RP / 8; i += 128) {  // a row's next eight ranks
-    const int r = i & 15, j = (i >> 4) * 8;
-    if (block * 16 + r >= n_rows) continue;
+  constexpr int PIECES = RP / 8;  // of eight ranks
+  for (int i = threadIdx.x; i < 16 * PIECES; i += 128) {
+    const int r = i / PIECES, j = (i % PIECES) * 8;
+    const int64_t n = row0 + r;
+    if (n >= n_rows) continue;
     uint32_t hi[4], lo[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) split_bf16(m[r][j + 2 * k], m[r][j + 2 * k + 1], hi[k], lo[k]);
     const uint4 h = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    put_cat(out.cat, block * 16 + r, j, RP, h, h, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+    put_cat(out.cat, n, j, RP, h, h, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      split_f16(m[r][j + 2 * k] * up, m[r][j + 2 * k + 1] * up, hi[k], lo[k]);
+    uint4* row = out.pair + n * (sums::pair_width(RP) / 8);
+    row[j / 8] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    row[PIECES + j / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  for (int k = warp; k < KS; k += 4) {
-    const int64_t at = (block * KS + k) * 64 + lane;
-    uint32_t hi[4], lo[4];
-    // m operand of the transpose: registers (ranks g, g + 8) x (rows 2 t, 2 t + 8)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int j = 16 * k + g + 8 * (r & 1), n = 2 * t + 8 * (r >> 1);
-      split_f16(m[n][j] * up, m[n + 1][j] * up, hi[r], lo[r]);
-    }
-    out.col[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    out.col[at + 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-  }
-  if (threadIdx.x == 0) out.down[block] = back;
-}
-
-// Where the rows of lane t lie in a block of 16: 2 t, 2 t + 1, 2 t + 8, 2 t + 9.
-__device__ __forceinline__ int row_of(int i, int t) { return 2 * t + (i & 1) + 8 * (i >> 1); }
-
-// ---- outer: sums over the rows ----------------------------------------------------------------
-constexpr int OUTER_WARPS = 8;
-
-// part[split][j][c] = sum over the split's rows of T[n, j] (keep) x[n, c]. A CTA takes 64 columns
-// and a range of 16-row blocks, its warps take turns with those. Lane (g, t) loads columns 8 g ..
-// 8 g + 7 of rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9: two rows of a column make an operand register by
-// one byte permutation. A rank of 64 is divided between the halves of the CTA's warps (64 sums in a
-// lane's registers at most), which read the same activations.
-template <int KS, bool MASK>
-__global__ void __launch_bounds__(32 * OUTER_WARPS, KS == 1 ? 2 : 1) outer_kernel(
-    const __half* __restrict__ x, int64_t ld_x, int64_t n_rows, int n_cols, TParts tp, Dropout d,
-    int blocks_per_split, float* __restrict__ part) {
-  extern __shared__ __align__(16) float outer_smem[];  // [OUTER_WARPS][16][64]
-  constexpr int RP = 16 * KS;
-  constexpr int HALVES = KS == 4 ? 2 : 1, MT = KS / HALVES;  // rank tiles of a warp
-  constexpr int LANES = OUTER_WARPS / HALVES;                // warps that take turns with the rows
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, t = lane & 3;
-  const int half = warp / LANES, turn = warp % LANES;
-  const int cb = blockIdx.x;
-  const int col = cb * 64 + 8 * g;
-  const bool in = col < n_cols;
-  const int64_t row_blocks = (n_rows + 15) / 16;
-  const int64_t rb0 = static_cast<int64_t>(blockIdx.y) * blocks_per_split;
-  const int64_t rb1 = min(row_blocks, rb0 + blocks_per_split);
-  const uint64_t key = MASK ? static_cast<uint64_t>(__ldg(d.seed)) : 0;
-  const uint32_t bias2 = keep_bias2(d.drop);
-
-  auto load = [&](int64_t rb, uint4 (&v)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t n = rb * 16 + row_of(i, t);
-      v[i] = in && n < n_rows
-                 ? __ldg(reinterpret_cast<const uint4*>(x + n * ld_x + col))
-                 : make_uint4(0, 0, 0, 0);
-    }
-  };
-  float acc[MT][8][4] = {};
-  uint4 cur[4];
-  if (rb0 + turn < rb1) load(rb0 + turn, cur);
-  for (int64_t rb = rb0 + turn; rb < rb1; rb += LANES) {
-    uint4 next[4];
-    const bool more = rb + LANES < rb1;
-    if (more) load(rb + LANES, next);
-    if (MASK) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        cur[i] = masked(cur[i], rb * 16 + row_of(i, t), n_cols, col, key, bias2);
-    }
-    {
-      const float back = __ldg(tp.down + rb);
-#pragma unroll
-      for (int k = 0; k < MT; ++k) {
-        const uint4* tc = tp.col + (rb * KS + half * MT + k) * 64 + lane;
-        const uint4 hi = __ldg(tc), lo = __ldg(tc + 32);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const uint32_t r0 = u == 0 ? cur[0].x : u == 1 ? cur[0].y : u == 2 ? cur[0].z : cur[0].w;
-          const uint32_t r1 = u == 0 ? cur[1].x : u == 1 ? cur[1].y : u == 2 ? cur[1].z : cur[1].w;
-          const uint32_t r2 = u == 0 ? cur[2].x : u == 1 ? cur[2].y : u == 2 ? cur[2].z : cur[2].w;
-          const uint32_t r3 = u == 0 ? cur[3].x : u == 1 ? cur[3].y : u == 2 ? cur[3].z : cur[3].w;
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {  // column 8 g + 2 u + v
-            const uint32_t b0 = __byte_perm(r0, r1, v ? 0x7632 : 0x5410);
-            const uint32_t b1 = __byte_perm(r2, r3, v ? 0x7632 : 0x5410);
-            float c[4] = {};
-            mma_f16(c, lo.x, lo.y, lo.z, lo.w, b0, b1);
-            mma_f16(c, hi.x, hi.y, hi.z, hi.w, b0, b1);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) acc[k][2 * u + v][q] = fmaf(back, c[q], acc[k][2 * u + v][q]);
-          }
-        }
-      }
-    }
-    if (more) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cur[i] = next[i];
-    }
-  }
-  // the warps add their sums in warp order, 16 ranks of each half at a time
-  float* out = part + static_cast<int64_t>(blockIdx.y) * RP * n_cols;
-#pragma unroll
-  for (int k = 0; k < MT; ++k) {
-    __syncthreads();
-    float* mine = outer_smem + warp * (16 * 64);
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {  // tile u: n index (2 t, 2 t + 1) stands for columns 8 n + u
-      mine[g * 64 + 8 * (2 * t) + u] = acc[k][u][0];
-      mine[g * 64 + 8 * (2 * t + 1) + u] = acc[k][u][1];
-      mine[(g + 8) * 64 + 8 * (2 * t) + u] = acc[k][u][2];
-      mine[(g + 8) * 64 + 8 * (2 * t + 1) + u] = acc[k][u][3];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < HALVES * 16 * 64; i += 32 * OUTER_WARPS) {
-      const int hf = i >> 10, in_tile = i & 1023;
-      const int c = cb * 64 + (i & 63);
-      float v = 0.0f;
-#pragma unroll
-      for (int q = 0; q < LANES; ++q) v += outer_smem[(hf * LANES + q) * (16 * 64) + in_tile];
-      if (c < n_cols)
-        out[static_cast<int64_t>(16 * (hf * MT + k) + (in_tile >> 6)) * n_cols + c] = v;
-    }
-  }
+  if (threadIdx.x == 0 && (blockIdx.x & (T_CLUSTER - 1)) == 0)
+    out.down[blockIdx.x / T_CLUSTER] = back;
+  cluster_sync();  // the cluster's largest values have been read
 }
 
 // out[j * out_j + c * out_c] = factor * (sum of the parts): the weights' gradients.
@@ -586,48 +351,12 @@ struct Carve {  // hands out 256-byte aligned pieces; counts them when there is 
   }
 };
 
-constexpr int TARGET_CTAS = 296;  // two for each of 148 SMs
-
-// How `inner` divides its work: a CTA takes row_groups * 32 rows (few when there are few rows, so
-// that the warps share the columns instead) and steps_per_split 64-column steps.
-struct InnerPlan {
-  int row_groups, row_ctas, splits, steps_per_split;
-  InnerPlan(int64_t n_rows, int64_t n_cols, int rp) {
-    row_groups = n_rows <= 32 ? 1 : rp / 8;  // a wide rank-wide operand serves more rows
-    row_ctas = static_cast<int>((n_rows + 32 * row_groups - 1) / (32 * row_groups));
-    const int steps = static_cast<int>((n_cols + 63) / 64);
-    int want = TARGET_CTAS / row_ctas;  // at least one step for each warp of a row group
-    const int most = (steps * row_groups + INNER_WARPS - 1) / INNER_WARPS;
-    if (want > most) want = most;
-    if (want > 32) want = 32;
-    if (want < 1) want = 1;
-    steps_per_split = (steps + want - 1) / want;
-    splits = (steps + steps_per_split - 1) / steps_per_split;
-  }
-};
-
-// How `outer` divides its work: a CTA takes 64 columns and blocks_per_split blocks of 16 rows.
-struct OuterPlan {
-  int col_ctas, splits, blocks_per_split;
-  OuterPlan(int64_t n_rows, int64_t n_cols) {
-    col_ctas = static_cast<int>((n_cols + 63) / 64);
-    const int64_t row_blocks = (n_rows + 15) / 16;
-    int64_t want = TARGET_CTAS / col_ctas;
-    const int64_t most = (row_blocks + OUTER_WARPS - 1) / OUTER_WARPS;
-    if (want > most) want = most;
-    if (want < 1) want = 1;
-    blocks_per_split = static_cast<int>((row_blocks + want - 1) / want);
-    splits = static_cast<int>((row_blocks + blocks_per_split - 1) / blocks_per_split);
-  }
-};
-
 struct TBuffers {
   TParts parts;
   TBuffers(Carve& c, int64_t n_rows, int rp) {
-    const size_t blocks = static_cast<size_t>((n_rows + 15) / 16);
     parts.cat = c.take<uint4>(static_cast<size_t>(n_rows) * up::chunks(rp) * 8);
-    parts.col = c.take<uint4>(blocks * (rp / 16) * 64);
-    parts.down = c.take<float>(blocks);
+    parts.pair = c.take<uint4>(static_cast<size_t>(n_rows) * (sums::pair_width(rp) / 8));
+    parts.down = c.take<float>(static_cast<size_t>((n_rows + 127) / 128));
   }
 };
 
@@ -636,7 +365,7 @@ struct Prepared {
   Rows rows;
   uint4* cat;
   Prepared(Carve& c, int64_t n_rows_matrix, int64_t n_cols_matrix, int rp) {
-    rows.parts = c.take<uint4>(static_cast<size_t>((n_rows_matrix + 63) / 64) * (rp / 8) * 128);
+    rows.parts = c.take<__half>(static_cast<size_t>(2 * rp) * n_rows_matrix);
     rows.down = c.take<float>(rp);
     cat = c.take<uint4>(static_cast<size_t>(n_cols_matrix) * up::chunks(rp) * 8);
   }
@@ -648,7 +377,7 @@ struct ForwardWork {
   float* part;
   ForwardWork(void* base, const Shape& s, int rp)
       : carve{static_cast<char*>(base), 0}, prep(carve, s.n_in, s.n_out, rp) {
-    const InnerPlan plan(s.n_rows, s.n_in, rp);
+    const sums::Plan plan(false, s.n_rows, s.n_in);
     part = carve.take<float>(static_cast<size_t>(plan.splits) * s.n_rows * rp);
   }
 };
@@ -662,9 +391,9 @@ struct BackwardWork {
       : carve{static_cast<char*>(base), 0},
         prep(carve, s.n_out, s.n_in, rp),
         dt(carve, s.n_rows, rp) {
-    const InnerPlan inner(s.n_rows, s.n_out, rp);
+    const sums::Plan inner(false, s.n_rows, s.n_out);
     t_part = carve.take<float>(static_cast<size_t>(inner.splits) * s.n_rows * rp);
-    const OuterPlan ob(s.n_rows, s.n_out), oa(s.n_rows, s.n_in);
+    const sums::Plan ob(true, s.n_rows, s.n_out), oa(true, s.n_rows, s.n_in);
     b_part = carve.take<float>(static_cast<size_t>(ob.splits) * rp * s.n_out);
     a_part = carve.take<float>(static_cast<size_t>(oa.splits) * rp * s.n_in);
   }
@@ -677,14 +406,6 @@ struct Saved {
       : carve{static_cast<char*>(base), 0}, t(carve, s.n_rows, rp) {}
 };
 
-template <class K>
-int allow_smem(K kernel, int bytes) {
-  // set on every call: a per-device record would cost as much as the call, which only notes it
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  return e == cudaSuccess ? TALM_OK : set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
-}
-
 void prepare(const float* m0, int64_t j0, int64_t c0, int64_t n0, const float* m1, int64_t j1,
              int64_t c1, int64_t n1, const Prepared& p, int rank, int rp, cudaStream_t stream) {
   const int64_t grid = rp + (n1 * (rp / 8) + PREP_THREADS - 1) / PREP_THREADS;
@@ -693,49 +414,34 @@ void prepare(const float* m0, int64_t j0, int64_t c0, int64_t n0, const float* m
       rp);
 }
 
-template <int KS>
+// t or dt of an activation: the inner sums and the operands made of them.
+template <int RP>
 int run_inner(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const Rows& rows,
               const Dropout& d, float* part, float factor, const TParts& out,
               cudaStream_t stream) {
-  const InnerPlan plan(n_rows, n_cols, 16 * KS);
-  const dim3 grid(static_cast<unsigned>(plan.row_ctas), static_cast<unsigned>(plan.splits), 1);
-  constexpr int smem = INNER_WARPS * 32 * 16 * KS * 4;
-  auto kernel = d.drop ? inner_kernel<2 * KS, true> : inner_kernel<2 * KS, false>;
-  if (smem > 48 * 1024) {
-    const int st = allow_smem(kernel, smem);
-    if (st != TALM_OK) return st;
-  }
-  kernel<<<grid, 32 * INNER_WARPS, smem, stream>>>(x, ld, n_rows, static_cast<int>(n_cols), rows, d,
-                                                   plan.row_groups, plan.steps_per_split, part);
-  const int64_t blocks = (n_rows + 15) / 16;
-  t_parts_kernel<KS><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(
-      part, plan.splits, n_rows, rows.down, factor, out);
+  const int st = d.drop ? sums::launch<RP, false, true>(x, ld, n_rows, n_cols, rows.parts, nullptr,
+                                                        d, part, stream)
+                        : sums::launch<RP, false, false>(x, ld, n_rows, n_cols, rows.parts, nullptr,
+                                                         d, part, stream);
+  if (st != TALM_OK) return st;
+  const unsigned grid = static_cast<unsigned>((n_rows + 127) / 128 * T_CLUSTER);
+  t_parts_kernel<RP><<<grid, 128, 0, stream>>>(part, sums::Plan(false, n_rows, n_cols).splits,
+                                               n_rows, rows.down, factor, out);
   return TALM_OK;
 }
 
-template <int KS>
+template <int RP>
 int run_forward(const __half* x, int64_t ld_x, const __half* base, int64_t ld_base,
                 const float* a, const float* b, const Shape& s, float scaling, const Dropout& d,
                 __half* y, void* saved, void* work, cudaStream_t stream) {
-  constexpr int RP = 16 * KS;
   const ForwardWork w(work, s, RP);
   const Saved keep(saved, s, RP);
   prepare(a, s.n_in, 1, s.n_in, b, 1, s.rank, s.n_out, w.prep, s.rank, RP, stream);
-  const int st = run_inner<KS>(x, ld_x, s.n_rows, s.n_in, w.prep.rows, d, w.part, d.factor,
+  const int st = run_inner<RP>(x, ld_x, s.n_rows, s.n_in, w.prep.rows, d, w.part, d.factor,
                                keep.t.parts, stream);
   if (st != TALM_OK) return st;
   return up::launch<up::chunks(RP), false>(keep.t.parts.cat, w.prep.cat, base, ld_base, y, s.n_rows,
                                            s.n_out, scaling, d, stream);
-}
-
-template <int KS, bool MASK>
-void launch_outer(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const TParts& t,
-                  const Dropout& d, float* part, cudaStream_t stream) {
-  const OuterPlan plan(n_rows, n_cols);
-  const dim3 grid(static_cast<unsigned>(plan.col_ctas), static_cast<unsigned>(plan.splits), 1);
-  constexpr int smem = OUTER_WARPS * 16 * 64 * 4;
-  outer_kernel<KS, MASK><<<grid, 32 * OUTER_WARPS, smem, stream>>>(
-      x, ld, n_rows, static_cast<int>(n_cols), t, d, plan.blocks_per_split, part);
 }
 
 void sum_parts(const float* part, int splits, int64_t n, int rank, int rp, float factor,
@@ -745,23 +451,24 @@ void sum_parts(const float* part, int splits, int64_t n, int rank, int rp, float
       part, splits, rank, rp, static_cast<int>(n), factor, out_j, out_c, out);
 }
 
-template <int KS>
+template <int RP>
 int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, const float* a,
                  const float* b, const Shape& s, float scaling, const Dropout& d,
                  const void* saved, __half* dx, float* da, float* db, void* work,
                  cudaStream_t stream) {
-  constexpr int RP = 16 * KS;
   const BackwardWork w(work, s, RP);
   const Saved keep(const_cast<void*>(saved), s, RP);
   const Dropout none{nullptr, 0, 1.0f};
   if (db) {
-    launch_outer<KS, false>(g, ld_g, s.n_rows, s.n_out, keep.t.parts, none, w.b_part, stream);
-    sum_parts(w.b_part, OuterPlan(s.n_rows, s.n_out).splits, s.n_out, s.rank, RP, scaling, 1,
+    const int st = sums::launch<RP, true, false>(g, ld_g, s.n_rows, s.n_out, keep.t.parts.pair,
+                                                 keep.t.parts.down, none, w.b_part, stream);
+    if (st != TALM_OK) return st;
+    sum_parts(w.b_part, sums::Plan(true, s.n_rows, s.n_out).splits, s.n_out, s.rank, RP, scaling, 1,
               s.rank, db, stream);
   }
   if (da || dx) {
     prepare(b, 1, s.rank, s.n_out, a, s.n_in, 1, s.n_in, w.prep, s.rank, RP, stream);
-    const int st = run_inner<KS>(g, ld_g, s.n_rows, s.n_out, w.prep.rows, none, w.t_part, scaling,
+    const int st = run_inner<RP>(g, ld_g, s.n_rows, s.n_out, w.prep.rows, none, w.t_part, scaling,
                                  w.dt.parts, stream);
     if (st != TALM_OK) return st;
     if (dx) {
@@ -769,13 +476,16 @@ int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, c
                                                       s.n_rows, s.n_in, d.factor, d, stream);
       if (st != TALM_OK) return st;
     }
-    if (da && d.drop)
-      launch_outer<KS, true>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, w.a_part, stream);
-    else if (da)
-      launch_outer<KS, false>(x, ld_x, s.n_rows, s.n_in, w.dt.parts, d, w.a_part, stream);
-    if (da)
-      sum_parts(w.a_part, OuterPlan(s.n_rows, s.n_in).splits, s.n_in, s.rank, RP, d.factor,
+    if (da) {
+      const TParts& t = w.dt.parts;
+      const int st = d.drop ? sums::launch<RP, true, true>(x, ld_x, s.n_rows, s.n_in, t.pair,
+                                                           t.down, d, w.a_part, stream)
+                            : sums::launch<RP, true, false>(x, ld_x, s.n_rows, s.n_in, t.pair,
+                                                            t.down, d, w.a_part, stream);
+      if (st != TALM_OK) return st;
+      sum_parts(w.a_part, sums::Plan(true, s.n_rows, s.n_in).splits, s.n_in, s.rank, RP, d.factor,
                 s.n_in, 1, da, stream);
+    }
   }
   return check_launch("adapter backward kernels");
 }
@@ -875,7 +585,7 @@ int talm_lora_forward(const uint16_t* x, int64_t ld_x, const uint16_t* base, int
   const Shape s{n_rows, n_in, n_out, static_cast<int>(rank)};
   LaunchTimer timer(TALM_KERNEL_LORA_FORWARD, stream);
   const int rp = padded_rank(s.rank);
-  auto run = rp == 16 ? run_forward<1> : rp == 32 ? run_forward<2> : run_forward<4>;
+  auto run = rp == 16 ? run_forward<16> : rp == 32 ? run_forward<32> : run_forward<64>;
   return run(reinterpret_cast<const __half*>(x), ld_x, reinterpret_cast<const __half*>(base),
              ld_base, lora_a, lora_b, s, scaling, d, reinterpret_cast<__half*>(y), saved, workspace,
              stream);
@@ -914,7 +624,7 @@ int talm_lora_backward(const uint16_t* g, int64_t ld_g, const uint16_t* x, int64
   const Shape s{n_rows, n_in, n_out, static_cast<int>(rank)};
   LaunchTimer timer(TALM_KERNEL_LORA_BACKWARD, stream);
   const int rp = padded_rank(s.rank);
-  auto run = rp == 16 ? run_backward<1> : rp == 32 ? run_backward<2> : run_backward<4>;
+  auto run = rp == 16 ? run_backward<16> : rp == 32 ? run_backward<32> : run_backward<64>;
   return run(reinterpret_cast<const __half*>(g), ld_g, reinterpret_cast<const __half*>(x), ld_x,
              lora_a, lora_b, s, scaling, d, saved, reinterpret_cast<__half*>(dx), grad_a, grad_b,
              workspace, stream);

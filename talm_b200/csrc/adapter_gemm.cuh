@@ -289,6 +289,13 @@ __global__ void __launch_bounds__(THREADS, 1)
 template <int CHUNKS, bool MASK>
 int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base, void* out,
            int64_t n_rows, int64_t n_cols, float scale, const Dropout& d, cudaStream_t stream) {
+  constexpr int smem = smem_bytes(CHUNKS);
+  auto kernel = up_kernel<CHUNKS, MASK>;
+  // Set on every call: it only notes the value, and it makes the device's context current in a
+  // thread that has made no CUDA call yet (autograd's), which the tensor map encoder asks for.
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
   CUtensorMap tm_t, tm_m, tm_base, tm_out;
   int st = talm_make_tmap_2d_f16(&tm_t, t_op, CHUNKS * 64, n_rows, CHUNKS * 64, 64, TILE);
   if (st == TALM_OK)
@@ -298,12 +305,6 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
     st = MASK ? (tm_base = tm_out, TALM_OK)
               : talm_make_tmap_2d_f16(&tm_base, base, n_cols, n_rows, ld_base, 64, TILE);
   if (st != TALM_OK) return st;
-  constexpr int smem = smem_bytes(CHUNKS);
-  auto kernel = up_kernel<CHUNKS, MASK>;
-  // set on every call (it only notes the value): no per-device record to keep
-  const cudaError_t e =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
   Params p;
   p.n_rows = n_rows;
   p.n_cols = static_cast<int>(n_cols);
@@ -319,5 +320,292 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
 }
 
 }  // namespace up
+
+// The adapter's sums over an activation X [n_rows, n_cols] on tcgen05, X optionally dropped out:
+//   INNER:  part[split][n][j] = sum over the split's columns of X[n, c] W[j, c]
+//   OUTER:  part[split][j][c] = sum over the split's rows of X[n, c] T[n, j]
+// W (an adapter matrix) and T (t or dt) are fp32, scaled by powers of two and split in two fp16
+// parts that stand side by side as the n operand (N = 2 RP), so that X passes the tensor core once;
+// the epilogue adds the two halves of the result. X is the 128-row m operand as it lies in memory:
+// rows of K-major for INNER, columns of it, MN-major, for OUTER.
+//
+// Bound by HBM: X is read once (2 bytes per element, 4 RP flops). One CTA per 128 rows (INNER) or
+// columns (OUTER) and split, stages of 64 of the reduction:
+//   warp 0        TMA producer           warp 1      MMA issuer, into one of two TMEM buffers
+//   warps 4-11    epilogue: two groups of 128 threads, half the ranks each. The buffer is moved
+//                 into fp32 registers every FLUSH stages: the tensor core's long sums are not
+//                 rounded to nearest, and OUTER's T has a scale of its own for every 128 rows.
+//   warps 12-19   (MASK) drop X in shared memory before it is multiplied: a 16-byte piece is one
+//                 group of the generator
+namespace sums {
+
+constexpr int TILE = 128;
+constexpr int X_BYTES = 16384;  // 64 x 128 fp16
+constexpr int EPI_WARPS = 8, MASK_WARPS = 8;
+constexpr int FIRST_EPI_WARP = 4, FIRST_MASK_WARP = FIRST_EPI_WARP + EPI_WARPS;
+constexpr int MAX_STAGES = 6;
+
+__host__ __device__ constexpr int pair_width(int rp) { return 2 * rp < 64 ? 64 : 2 * rp; }
+template <int RP, bool OUTER>
+__host__ __device__ constexpr int other_bytes() {  // of the n operand per stage
+  return OUTER ? pair_width(RP) * 64 * 2 : 2 * RP * 128;
+}
+template <int RP, bool OUTER, bool MASK>
+__host__ __device__ constexpr int stages() {  // two CTAs per SM, or one with its mask warps
+  return MASK ? MAX_STAGES : 98304 / (X_BYTES + other_bytes<RP, OUTER>());
+}
+template <int RP, bool OUTER, bool MASK>
+__host__ __device__ constexpr int smem_bytes() {
+  return stages<RP, OUTER, MASK>() * (X_BYTES + other_bytes<RP, OUTER>()) + 1024 + 512;
+}
+__host__ __device__ constexpr int threads(bool mask) { return 32 * (FIRST_MASK_WARP + (mask ? MASK_WARPS : 0)); }
+
+struct Ctl {
+  uint64_t full[MAX_STAGES], masked[MAX_STAGES], empty[MAX_STAGES];
+  uint64_t acc_full[2], acc_empty[2];
+  uint64_t drain;
+  uint32_t tmem_base;
+  int abort;
+};
+
+struct Params {
+  int64_t n_rows;
+  int n_cols;
+  int steps, steps_per_split;  // 64-wide stages of the whole reduction, and of a split
+  const float* down;           // OUTER: the scale of every 128 rows of T
+  float* part;
+  Dropout drop;
+};
+
+template <int RP, bool OUTER, bool MASK>
+__global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
+    sums_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_o,
+                Params p) {
+  constexpr int STAGES = stages<RP, OUTER, MASK>();
+  constexpr int O_BYTES = other_bytes<RP, OUTER>();
+  constexpr int N = 2 * RP;
+  constexpr int COLS = N < 32 ? 32 : N;  // TMEM columns of a buffer
+  constexpr int FLUSH = OUTER ? 2 : 8;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* x_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                            ~uintptr_t(1023));
+  uint8_t* o_s = x_s + STAGES * X_BYTES;
+  Ctl* ctl = reinterpret_cast<Ctl*>(o_s + STAGES * O_BYTES);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t origin = static_cast<int64_t>(blockIdx.x) * TILE;  // first row / column
+  const int s0 = blockIdx.y * p.steps_per_split;
+  const int n_steps = min(p.steps, s0 + p.steps_per_split) - s0;  // at least one
+
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_o);
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&ctl->full[i], 1);
+      mbar_init(&ctl->masked[i], MASK_WARPS);
+      mbar_init(&ctl->empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl->acc_full[i], 1);
+      mbar_init(&ctl->acc_empty[i], EPI_WARPS);
+    }
+    mbar_init(&ctl->drain, 1);
+    ctl->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&ctl->tmem_base, 2 * COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = ctl->tmem_base;
+  volatile int* abort = &ctl->abort;
+
+  if (warp == 0) {
+    if (lane == 0) {  // producer
+      int i = 0;
+      for (; i < n_steps; ++i) {
+        const int st = i % STAGES;
+        if (!mbar_wait(&ctl->empty[st], ((i / STAGES) & 1) ^ 1, abort)) break;
+        const int at = (s0 + i) * 64, o = static_cast<int>(origin);
+        uint8_t* x = x_s + st * X_BYTES;
+        uint8_t* w = o_s + st * O_BYTES;
+        mbar_arrive_expect_tx(&ctl->full[st], X_BYTES + O_BYTES);
+        if (OUTER) {  // 64 rows of 2 x 64 columns; the parts' 64 rows
+          tma_load_2d(x, &tm_x, &ctl->full[st], o, at);
+          tma_load_2d(x + 8192, &tm_x, &ctl->full[st], o + 64, at);
+          for (int b = 0; b < O_BYTES / 8192; ++b)
+            tma_load_2d(w + b * 8192, &tm_o, &ctl->full[st], b * 64, at);
+        } else {  // 128 rows of 64 columns; the parts' 64 columns
+          tma_load_2d(x, &tm_x, &ctl->full[st], at, o);
+          tma_load_2d(w, &tm_o, &ctl->full[st], at, 0);
+        }
+      }
+      for (int k = 0; k < STAGES; ++k) {  // every copy issued lands before the CTA ends
+        const int n = (i - k + STAGES - 1) / STAGES;
+        if (i > k) mbar_drain(&ctl->full[k], (n - 1) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {  // MMA issuer
+      constexpr uint32_t idesc = idesc_f16_f32(TILE, N, OUTER, OUTER);
+      for (int i = 0; i < n_steps; ++i) {
+        const int st = i % STAGES, f = i / FLUSH;
+        if (i % FLUSH == 0 &&
+            !mbar_wait(&ctl->acc_empty[f & 1], ((f >> 1) & 1) ^ 1, abort)) break;
+        if (!mbar_wait(&ctl->full[st], (i / STAGES) & 1, abort)) break;
+        if (MASK && !mbar_wait(&ctl->masked[st], (i / STAGES) & 1, abort)) break;
+        tc_fence_after();
+        const uint32_t a = smem_u32(x_s + st * X_BYTES), b = smem_u32(o_s + st * O_BYTES);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          // MN-major: 16 rows of 128 bytes further, 8 KiB between groups of 64 columns;
+          // K-major: 32 bytes further
+          const uint64_t ad = OUTER ? smem_desc_sw128(a + k * 2048, 8192, 1024)
+                                    : smem_desc_sw128(a + k * 32, 16, 1024);
+          const uint64_t bd = OUTER ? smem_desc_sw128(b + k * 2048, 8192, 1024)
+                                    : smem_desc_sw128(b + k * 32, 16, 1024);
+          umma_f16(tmem_base + (f & 1) * COLS, ad, bd, idesc, i % FLUSH != 0 || k != 0);
+        }
+        umma_commit(&ctl->empty[st]);
+        if (i % FLUSH == FLUSH - 1 || i + 1 == n_steps) umma_commit(&ctl->acc_full[f & 1]);
+      }
+      umma_commit(&ctl->drain);
+      mbar_drain(&ctl->drain, 0);
+    }
+  } else if (warp >= FIRST_EPI_WARP && warp < FIRST_MASK_WARP) {
+    constexpr int HR = RP / 2;  // ranks of a group
+    const int quarter = warp & 3, q = (warp - FIRST_EPI_WARP) >> 2;
+    const int r = quarter * 32 + lane;
+    float acc[HR] = {};
+    const int flushes = (n_steps + FLUSH - 1) / FLUSH;
+    bool ok = true;
+    for (int f = 0; f < flushes; ++f) {
+      const float back = OUTER ? __ldg(p.down + s0 / FLUSH + f) : 1.0f;
+      ok = mbar_wait(&ctl->acc_full[f & 1], (f >> 1) & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t ta = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                          (f & 1) * COLS + q * HR;
+      constexpr int STEP = HR < 16 ? HR : 16;
+#pragma unroll
+      for (int j = 0; j < HR; j += STEP) {
+        uint32_t hi[STEP], lo[STEP];
+#pragma unroll
+        for (int u = 0; u < STEP; u += 8) {
+          tmem_ld_32x32b_x8(ta + j + u, hi + u);
+          tmem_ld_32x32b_x8(ta + RP + j + u, lo + u);
+        }
+        tmem_wait_ld();
+#pragma unroll
+        for (int u = 0; u < STEP; ++u)
+          acc[j + u] = fmaf(back, __uint_as_float(hi[u]) + __uint_as_float(lo[u]), acc[j + u]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->acc_empty[f & 1]);
+    }
+    const int64_t at = origin + r;
+    if (ok && at < (OUTER ? p.n_cols : p.n_rows)) {
+      if (OUTER) {
+        float* out = p.part + (static_cast<int64_t>(blockIdx.y) * RP + q * HR) * p.n_cols + at;
+#pragma unroll
+        for (int j = 0; j < HR; ++j) out[static_cast<int64_t>(j) * p.n_cols] = acc[j];
+      } else {
+        float4* out = reinterpret_cast<float4*>(
+            p.part + (static_cast<int64_t>(blockIdx.y) * p.n_rows + at) * RP + q * HR);
+#pragma unroll
+        for (int j = 0; j < HR; j += 4)
+          out[j / 4] = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+      }
+    }
+  } else if (MASK && warp >= FIRST_MASK_WARP) {
+    const int id = threadIdx.x - 32 * FIRST_MASK_WARP;
+    const uint64_t key = static_cast<uint64_t>(__ldg(p.drop.seed));
+    const uint32_t bias2 = keep_bias2(p.drop.drop);
+    for (int i = 0; i < n_steps; ++i) {
+      const int st = i % STAGES;
+      const bool ok = mbar_wait(&ctl->full[st], (i / STAGES) & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      uint8_t* x = x_s + st * X_BYTES;
+#pragma unroll
+      for (int u = 0; u < X_BYTES / 16 / (32 * MASK_WARPS); ++u) {
+        const int e = u * (32 * MASK_WARPS) + id;  // piece e: row line e / 8 of 128 bytes
+        const int line = e >> 3, c = e & 7;
+        // INNER: line = row, 64 columns; OUTER: line = row + 64 * (column group)
+        const int64_t row = OUTER ? static_cast<int64_t>(s0 + i) * 64 + (line & 63) : origin + line;
+        const int64_t col = OUTER ? origin + (line >> 6) * 64 + c * 8
+                                  : static_cast<int64_t>(s0 + i) * 64 + c * 8;
+        uint4* at = reinterpret_cast<uint4*>(x + line * 128 + ((c ^ (line & 7)) << 4));
+        uint32_t w[4];
+        philox(static_cast<uint64_t>((row * p.n_cols + col) >> 3), key, w);
+        uint4 v = *at;
+        v.x &= keep_mask2(w[0], bias2);
+        v.y &= keep_mask2(w[1], bias2);
+        v.z &= keep_mask2(w[2], bias2);
+        v.w &= keep_mask2(w[3], bias2);
+        *at = v;
+      }
+      fence_proxy_async_smem();  // the tensor core reads it
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl->masked[st]);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, 2 * COLS);
+}
+
+// How the reduction is divided: about two CTAs for each of 148 SMs, at least three stages (INNER)
+// or two 128-row blocks (OUTER) for a CTA, and whole blocks.
+struct Plan {
+  int tiles, steps, steps_per_split, splits;
+  Plan(bool outer, int64_t n_rows, int64_t n_cols) {
+    tiles = static_cast<int>(((outer ? n_cols : n_rows) + TILE - 1) / TILE);
+    const int64_t length = outer ? n_rows : n_cols;
+    const int unit = outer ? 2 : 1;
+    steps = static_cast<int>((length + 63) / 64);
+    const int units = (steps + unit - 1) / unit;
+    int want = 296 / tiles;
+    const int most = outer ? (units + 1) / 2 : (units + 2) / 3;
+    if (want > most) want = most;
+    if (want > 32) want = 32;
+    if (want < 1) want = 1;
+    steps_per_split = (units + want - 1) / want * unit;
+    splits = (steps + steps_per_split - 1) / steps_per_split;
+  }
+};
+
+// x: the activation; other: W parts [2 RP, n_cols] (INNER) or T parts [n_rows, pair_width] (OUTER)
+template <int RP, bool OUTER, bool MASK>
+int launch(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void* other,
+           const float* down, const Dropout& d, float* part, cudaStream_t stream) {
+  constexpr int smem = smem_bytes<RP, OUTER, MASK>();
+  static_assert(smem <= 232448 && (MASK || 2 * smem <= 232448), "shared memory");
+  auto kernel = sums_kernel<RP, OUTER, MASK>;
+  // before the tensor maps, as in up::launch
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
+  const Plan plan(OUTER, n_rows, n_cols);
+  CUtensorMap tm_x, tm_o;
+  int st = talm_make_tmap_2d_f16(&tm_x, x, n_cols, n_rows, ld, 64, OUTER ? 64 : TILE);
+  if (st == TALM_OK)
+    st = OUTER ? talm_make_tmap_2d_f16(&tm_o, other, pair_width(RP), n_rows, pair_width(RP), 64, 64)
+               : talm_make_tmap_2d_f16(&tm_o, other, n_cols, 2 * RP, n_cols, 64, 2 * RP);
+  if (st != TALM_OK) return st;
+  const Params p{n_rows, static_cast<int>(n_cols), plan.steps, plan.steps_per_split, down, part, d};
+  kernel<<<dim3(static_cast<unsigned>(plan.tiles), static_cast<unsigned>(plan.splits), 1),
+           threads(MASK), smem, stream>>>(tm_x, tm_o, p);
+  return check_launch("adapter sums kernel");
+}
+
+}  // namespace sums
 }  // namespace adapter
 }  // namespace talm

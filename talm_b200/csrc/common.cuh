@@ -255,6 +255,16 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
       : "memory");
 }
 
+// 32 lanes x 8 consecutive 32-bit columns (no wait).
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7])
+      : "r"(taddr)
+      : "memory");
+}
+
 // Shared-memory matrix descriptor, 128-byte swizzle (sm_100 layout: version 1, base offset 0).
 //   K-major tiles: rows of 128 B (64 fp16 of K), 8-row atoms -> SBO = 1024, LBO unused (1).
 //   MN-major tiles: K-rows of 128 B (64 fp16 of MN), 8-row atoms -> SBO = 1024 between
