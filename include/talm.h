@@ -190,8 +190,8 @@ int talm_lora_sizes(int64_t n_rows, int64_t n_in, int64_t n_out, int64_t rank, s
  *   x, base, y : fp16 [n_rows, n_in], [n_rows, n_out], [n_rows, n_out] (y contiguous), rows 16-byte
  *                aligned with strides of a multiple of 8 elements
  *   lora_a, lora_b : fp32 [rank, n_in], [n_out, rank], contiguous
- *   saved : talm_lora_sizes bytes, 16-byte aligned, kept for the backward; workspace likewise,
- *           free again once the call's work is done
+ *   saved : talm_lora_sizes bytes, 16-byte aligned, kept for the backward (NULL: none is wanted);
+ *   workspace : likewise, free again once the call's work is done
  * Preconditions: n_in and n_out multiples of 8, 1 <= rank <= 64. */
 int talm_lora_forward(const uint16_t* x, int64_t ld_x, const uint16_t* base, int64_t ld_base,
                       const float* lora_a, const float* lora_b, int64_t n_rows, int64_t n_in,
@@ -203,12 +203,11 @@ int talm_lora_forward(const uint16_t* x, int64_t ld_x, const uint16_t* base, int
  *   dt = scaling g lora_b, grad_b = scaling g^T t, grad_a = dt^T dropout(x),
  *   dx = fp16(mask * (dt lora_a))      (base's gradient is g itself)
  * in fp32 sums taken in an order that does not depend on timing. dx (fp16 [n_rows, n_in],
- * contiguous), grad_a and grad_b (fp32, overwritten) may each be NULL. `saved` is the forward's;
- * x, seed and drop are the forward's arguments.
+ * contiguous), grad_a and grad_b (fp32, overwritten) may each be NULL. `saved` is the forward's (it
+ * holds the adapter as it was then); x, seed and drop are the forward's arguments.
  * Replaces solution/lora.py:151-231 (LoraProjectionTorch.backward). */
 int talm_lora_backward(const uint16_t* g, int64_t ld_g, const uint16_t* x, int64_t ld_x,
-                       const float* lora_a, const float* lora_b, const void* saved,
-                       size_t saved_bytes, int64_t n_rows, int64_t n_in, int64_t n_out,
+                       const void* saved, size_t saved_bytes, int64_t n_rows, int64_t n_in, int64_t n_out,
                        int64_t rank, float scaling, const int64_t* seed, int64_t drop,
                        uint16_t* dx, float* grad_a, float* grad_b, void* workspace,
                        size_t ws_bytes, void* stream);

@@ -41,8 +41,8 @@ SIGNATURES = {
                                ctypes.POINTER(_SZ), ctypes.POINTER(_SZ)]),
     "talm_lora_forward": (_INT, [_P, _I64, _P, _I64, _P, _P, _I64, _I64, _I64, _I64, _F32, _P,
                                  _I64, _P, _P, _SZ, _P, _SZ, _P]),
-    "talm_lora_backward": (_INT, [_P, _I64, _P, _I64, _P, _P, _P, _SZ, _I64, _I64, _I64, _I64,
-                                  _F32, _P, _I64, _P, _P, _P, _P, _SZ, _P]),
+    "talm_lora_backward": (_INT, [_P, _I64, _P, _I64, _P, _SZ, _I64, _I64, _I64, _I64, _F32,
+                                   _P, _I64, _P, _P, _P, _P, _SZ, _P]),
     "talm_head_workspace_size": (_INT, [_I64, _I64, _I64, _I64, _I64, ctypes.POINTER(_SZ)]),
     "talm_head_shard": (_INT, [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P,
                                _P, _P, _SZ, _P]),

@@ -144,38 +144,45 @@ class _LoraBranch(torch.autograd.Function):
         xr, ld_x = _rows16(x, n_in)
         br, ld_b = _rows16(base, n_out)
         saved_bytes, work_bytes, ctx.work_bytes = _sizes(n_rows, n_in, n_out, rank)
+        need_x, _, need_a, need_b = ctx.needs_input_grad[:4]
         y = torch.empty(base.shape, dtype=torch.float16, device=x.device)
-        saved, work = _bytes(saved_bytes, x), _bytes(work_bytes, x)
+        saved = _bytes(saved_bytes, x) if need_x or need_a or need_b else None
+        work = _bytes(work_bytes, x)
         with _lib.device_of(x):
             _lib.check(_lib.load().talm_lora_forward(
                 xr.data_ptr(), ld_x, br.data_ptr(), ld_b, a.data_ptr(), b.data_ptr(), n_rows,
                 n_in, n_out, rank, scaling, None if seed is None else seed.data_ptr(), drop,
-                y.data_ptr(), saved.data_ptr(), saved_bytes, work.data_ptr(), work_bytes,
-                _lib.raw_stream(x)), "talm_lora_forward")
-        ctx.scaling, ctx.drop = scaling, drop
-        ctx.save_for_backward(x, lora_a, lora_b, seed, saved)
+                y.data_ptr(), None if saved is None else saved.data_ptr(), saved_bytes,
+                work.data_ptr(), work_bytes, _lib.raw_stream(x)), "talm_lora_forward")
+        if saved is not None:  # `saved` holds the adapter as it is now, in the kernels' parts
+            ctx.scaling, ctx.drop, ctx.rank = scaling, drop, rank
+            ctx.save_for_backward(x, seed, saved)
         RAN["lora"] += 1
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        x, lora_a, lora_b, seed, saved = ctx.saved_tensors
         need_x, need_base, need_a, need_b = ctx.needs_input_grad[:4]
-        dx = torch.empty(x.shape, dtype=torch.float16, device=x.device) if need_x else None
-        da = (torch.empty(lora_a.shape, dtype=torch.float32, device=x.device) if need_a else None)
-        db = (torch.empty(lora_b.shape, dtype=torch.float32, device=x.device) if need_b else None)
+        dx = da = db = None
         if need_x or need_a or need_b:
-            n_in, n_out, rank = x.shape[-1], grad.shape[-1], lora_a.shape[0]
-            a, b = lora_a.contiguous(), lora_b.contiguous()
+            x, seed, saved = ctx.saved_tensors
+            n_in, n_out, rank = x.shape[-1], grad.shape[-1], ctx.rank
+            device = x.device
+            if need_x:
+                dx = torch.empty(x.shape, dtype=torch.float16, device=device)
+            if need_a:
+                da = torch.empty((rank, n_in), dtype=torch.float32, device=device)
+            if need_b:
+                db = torch.empty((n_out, rank), dtype=torch.float32, device=device)
             xr, ld_x = _rows16(x, n_in)
             gr, ld_g = _rows16(grad, n_out)
             work = _bytes(ctx.work_bytes, x)
             with _lib.device_of(x):
                 _lib.check(_lib.load().talm_lora_backward(
-                    gr.data_ptr(), ld_g, xr.data_ptr(), ld_x, a.data_ptr(), b.data_ptr(),
-                    saved.data_ptr(), saved.numel(), grad.numel() // n_out, n_in, n_out, rank,
-                    ctx.scaling, None if seed is None else seed.data_ptr(), ctx.drop,
+                    gr.data_ptr(), ld_g, xr.data_ptr(), ld_x, saved.data_ptr(), saved.numel(),
+                    grad.numel() // n_out, n_in, n_out, rank, ctx.scaling,
+                    None if seed is None else seed.data_ptr(), ctx.drop,
                     dx.data_ptr() if need_x else None, da.data_ptr() if need_a else None,
                     db.data_ptr() if need_b else None, work.data_ptr(), ctx.work_bytes,
                     _lib.raw_stream(x)), "talm_lora_backward")

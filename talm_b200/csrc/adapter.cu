@@ -163,8 +163,8 @@ int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, co
 // and between them small kernels that turn the rank-wide fp32 operands into 16-bit parts for the
 // tensor cores. Where the other operand is an fp16 activation and the result fp32 (inner, outer) they
 // are two fp16 parts of the operand scaled by a power of two that brings its largest element to
-// [2^14, 2^15): 2^-22 and better, at any size of the operand; the scale is one per adapter row (A, B)
-// or per 128 rows of the activation (t, dt). Where both operands are fp32 and the result is fp16 (up)
+// [2^14, 2^15): 2^-22 and better, at any size of the operand; the scale is one per 128 elements of the
+// reduction (and per adapter row for A and B). Where both operands are fp32 and the result is fp16 (up)
 // they are two bf16 parts without scale, and the product of the two small ones is left out: under
 // 2^-16 of each term, a sixteenth of the result's own rounding.
 // ------------------------------------------------------------------------------------------
@@ -175,8 +175,9 @@ struct Shape {
 
 // ---- prepared operands -----------------------------------------------------------------------
 // RP: the rank rounded up to 16, 32 or 64, zeros behind it.
-//   Rows:  fp16 parts of an adapter matrix with the rank in the rows (A, B^T), each row scaled
-//          (down[RP] undoes it): [2 RP, n], the small parts behind the large ones.
+//   Rows:  fp16 parts of an adapter matrix with the rank in the rows (A, B^T), 128 columns of a row
+//          scaled together: parts [2 RP, n], the small parts behind the large ones; down [ceil(n /
+//          128)][RP] undoes the scale.
 //   cat:   bf16 parts (hi | lo | hi) of an adapter matrix with the rank in the columns (B, A^T), rows
 //          of up::chunks(RP) * 64, zeros behind the third part.
 //   TParts, of t or dt: cat, bf16 parts (hi | hi | lo) laid out likewise, and pair, fp16 parts
@@ -209,134 +210,193 @@ __device__ __forceinline__ void put_cat(uint4* cat, int64_t r, int j, int rp, ui
     for (int i = 3 * rp / 8; i < pieces; ++i) row[i] = make_uint4(0, 0, 0, 0);
 }
 
-// One CTA per padded rank builds its row of `rows` from m0 (element (j, c) at m0[j * j0 + c * c0]);
-// the others build `cat` from m1, a thread per column and eight ranks.
-__global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(
-    const float* __restrict__ m0, int64_t j0, int64_t c0, int n0, Rows rows,
-    const float* __restrict__ m1, int64_t j1, int64_t c1, int n1, uint4* __restrict__ cat,
-    int rank, int rp) {
-  const int tid = threadIdx.x;
-  if (static_cast<int>(blockIdx.x) < rp) {
-    __shared__ float most[PREP_THREADS / 32];
-    const int j = blockIdx.x;
-    const float* src = m0 + j * j0;
-    float m = 0.0f;
-    if (j < rank)
-      for (int c = tid; c < n0; c += PREP_THREADS) m = fmaxf(m, fabsf(__ldg(src + c * c0)));
+// An adapter matrix: element (rank j, column c) at m[j * dj + c * dc].
+struct Matrix {
+  const float* m;
+  int64_t dj, dc;
+  int n;
+};
+
+// The operands of one matrix: rows for the sums, cat for the rank-wide product; null where it is not
+// wanted.
+struct Operands {
+  Rows rows;
+  uint4* cat;
+};
+
+// A CTA takes 128 columns of A or of B^T into shared memory and builds both of its operands.
+template <int RP>
+__global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(Matrix a, Matrix b, Operands of_a,
+                                                               Operands of_b, int rank) {
+  constexpr int LD = 128 + 1;
+  extern __shared__ float tile[];  // [RP][LD]
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int a_ctas = (a.n + 127) / 128;
+  const bool is_a = static_cast<int>(blockIdx.x) < a_ctas;
+  const Matrix& s = is_a ? a : b;
+  const Operands& out = is_a ? of_a : of_b;
+  const int block = is_a ? blockIdx.x : blockIdx.x - a_ctas;
+  const int c0 = block * 128;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // neighbours read neighbours: A's columns, B's ranks
+#pragma unroll 8
+  for (int i = tid; i < RP * 128; i += PREP_THREADS) {
+    const int j = is_a ? i >> 7 : i % RP, c = is_a ? i & 127 : i / RP;
+    tile[j * LD + c] =
+        j < rank && c0 + c < s.n ? __ldg(s.m + j * s.dj + (c0 + c) * s.dc) : 0.0f;
+  }
+  __syncthreads();
+  if (out.rows.parts != nullptr) {
+    uint32_t* parts = reinterpret_cast<uint32_t*>(out.rows.parts);
+    const int64_t ld = s.n / 2;  // pairs; n is even
+    for (int j = warp; j < RP; j += PREP_THREADS / 32) {
+      const float* row = tile + j * LD;
+      float v[2][2], most = 0.0f;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    if ((tid & 31) == 0) most[tid >> 5] = m;
-    __syncthreads();
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int i = 0; i < PREP_THREADS / 32; ++i) m = fmaxf(m, most[i]);
-    float up, down;
-    power_scale(m, &up, &down);
-    uint32_t* hi = reinterpret_cast<uint32_t*>(rows.parts + static_cast<int64_t>(j) * n0);
-    uint32_t* lo = reinterpret_cast<uint32_t*>(rows.parts + static_cast<int64_t>(rp + j) * n0);
-    for (int c = 2 * tid; c < n0; c += 2 * PREP_THREADS) {  // n0 is even
-      uint32_t h = 0, l = 0;
-      if (j < rank) split_f16(__ldg(src + c * c0) * up, __ldg(src + (c + 1) * c0) * up, h, l);
-      hi[c >> 1] = h;
-      lo[c >> 1] = l;
+        for (int u = 0; u < 2; ++u) {
+          v[h][u] = row[64 * h + 2 * lane + u];
+          most = fmaxf(most, fabsf(v[h][u]));
+        }
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+      float up, down;
+      power_scale(most, &up, &down);
+      if (lane == 0) out.rows.down[block * RP + j] = down;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t c = c0 / 2 + 32 * h + lane;
+        if (c >= ld) continue;
+        uint32_t hi, lo;
+        split_f16(v[h][0] * up, v[h][1] * up, hi, lo);
+        parts[j * ld + c] = hi;
+        parts[(RP + j) * ld + c] = lo;
+      }
     }
-    if (tid == 0) rows.down[j] = down;
-    return;
   }
-  const int64_t e = static_cast<int64_t>(blockIdx.x - rp) * PREP_THREADS + tid;
-  const int64_t c = e % n1;
-  const int j = static_cast<int>(e / n1) * 8;
-  if (j >= rp) return;
-  uint32_t hi[4], lo[4];
+  if (out.cat != nullptr) {
+    constexpr int PIECES = RP / 8;
+    for (int i = tid; i < 128 * PIECES; i += PREP_THREADS) {
+      const int c = i / PIECES, j = (i % PIECES) * 8;
+      if (c0 + c >= s.n) break;  // so are the columns behind it
+      uint32_t hi[4], lo[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float v[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      v[u] = j + 2 * i + u < rank ? __ldg(m1 + (j + 2 * i + u) * j1 + c * c1) : 0.0f;
-    split_bf16(v[0], v[1], hi[i], lo[i]);
+      for (int k = 0; k < 4; ++k)
+        split_bf16(tile[(j + 2 * k) * LD + c], tile[(j + 2 * k + 1) * LD + c], hi[k], lo[k]);
+      const uint4 h = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      put_cat(out.cat, c0 + c, j, RP, h, make_uint4(lo[0], lo[1], lo[2], lo[3]), h);
+    }
   }
-  put_cat(cat, c, j, rp, make_uint4(hi[0], hi[1], hi[2], hi[3]),
-          make_uint4(lo[0], lo[1], lo[2], lo[3]), make_uint4(hi[0], hi[1], hi[2], hi[3]));
 }
 
 // ---- the operands made of t (or dt) ----------------------------------------------------------
-// t[n, j] = factor * down[j] * (sum of the parts): a CTA of four warps per 16 rows, a cluster of
-// eight per 128 rows, which find their common scale through each other's shared memory.
-constexpr int T_CLUSTER = 8;
+// t[n, j] = factor * (sum of the parts): a CTA per 128 rows, which share a scale. The pair is built
+// where it is wanted (out.pair not null).
+constexpr int T_THREADS = 1024;
 
 template <int RP>
-__global__ void __cluster_dims__(T_CLUSTER, 1, 1) __launch_bounds__(128)
+__global__ void __launch_bounds__(T_THREADS)
     t_parts_kernel(const float* __restrict__ part, int splits, int64_t n_rows,
-                   const float* __restrict__ down, float factor, TParts out) {
-  __shared__ float m[16][RP + 1];
-  __shared__ float warp_most[4];
-  __shared__ float cta_most;
+                   float factor, TParts out) {
+  extern __shared__ float t_smem[];  // [128][RP + 1]
+  __shared__ float warp_most[T_THREADS / 32];
+  grid_launch_dependents();
+  grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * 128;
+  constexpr int E = 128 * RP / T_THREADS, U = 8 / E;  // elements of a thread; eight loads at a time
+  float v[E] = {};
+  const int64_t live = (n_rows - row0 < 128 ? n_rows - row0 : 128) * RP;
+  const float* p = part + row0 * RP + threadIdx.x;
+  for (int k0 = 0; k0 < splits; k0 += U) {
+    float x[E][U];
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        x[i][u] = k0 + u < splits && i * T_THREADS + threadIdx.x < live
+                      ? __ldcg(p + static_cast<int64_t>(k0 + u) * n_rows * RP + i * T_THREADS)
+                      : 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[i] += x[i][u];
+  }
   float most = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 16 * RP / 128; ++i) {
-    const int e = i * 128 + threadIdx.x, r = e / RP, j = e % RP;
-    const int64_t n = row0 + r;
-    float v = 0.0f;
-    if (n < n_rows) {
-      const float* p = part + n * RP + j;
-#pragma unroll 8
-      for (int k = 0; k < splits; ++k) v += __ldg(p + static_cast<int64_t>(k) * n_rows * RP);
-      v *= __ldg(down + j) * factor;
-    }
-    m[r][j] = v;
-    most = fmaxf(most, fabsf(v));
+  for (int i = 0; i < E; ++i) {
+    const int e = i * T_THREADS + threadIdx.x;
+    t_smem[e / RP * (RP + 1) + e % RP] = v[i] * factor;
+    most = fmaxf(most, fabsf(v[i] * factor));
   }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
   if (lane == 0) warp_most[warp] = most;
   __syncthreads();
-  if (threadIdx.x == 0)
-    cta_most = fmaxf(fmaxf(warp_most[0], warp_most[1]), fmaxf(warp_most[2], warp_most[3]));
-  cluster_sync();
-  const uint32_t at = smem_u32(&cta_most);
 #pragma unroll
-  for (int c = 0; c < T_CLUSTER; ++c) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(at, c)));
-    most = fmaxf(most, v);
-  }
+  for (int i = 0; i < T_THREADS / 32; ++i) most = fmaxf(most, warp_most[i]);
   float up, back;
   power_scale(most, &up, &back);
   constexpr int PIECES = RP / 8;  // of eight ranks
-  for (int i = threadIdx.x; i < 16 * PIECES; i += 128) {
+  for (int i = threadIdx.x; i < 128 * PIECES; i += T_THREADS) {
     const int r = i / PIECES, j = (i % PIECES) * 8;
     const int64_t n = row0 + r;
-    if (n >= n_rows) continue;
+    if (n >= n_rows) break;  // so are the rows behind it
+    const float* m = t_smem + r * (RP + 1) + j;
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) split_bf16(m[r][j + 2 * k], m[r][j + 2 * k + 1], hi[k], lo[k]);
+    for (int k = 0; k < 4; ++k) split_bf16(m[2 * k], m[2 * k + 1], hi[k], lo[k]);
     const uint4 h = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     put_cat(out.cat, n, j, RP, h, h, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+    if (out.pair == nullptr) continue;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      split_f16(m[r][j + 2 * k] * up, m[r][j + 2 * k + 1] * up, hi[k], lo[k]);
+    for (int k = 0; k < 4; ++k) split_f16(m[2 * k] * up, m[2 * k + 1] * up, hi[k], lo[k]);
     uint4* row = out.pair + n * (sums::pair_width(RP) / 8);
     row[j / 8] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     row[PIECES + j / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  if (threadIdx.x == 0 && (blockIdx.x & (T_CLUSTER - 1)) == 0)
-    out.down[blockIdx.x / T_CLUSTER] = back;
-  cluster_sync();  // the cluster's largest values have been read
+  if (threadIdx.x == 0 && out.pair != nullptr) out.down[blockIdx.x] = back;
 }
 
-// out[j * out_j + c * out_c] = factor * (sum of the parts): the weights' gradients.
-__global__ void __launch_bounds__(256) sum_parts_kernel(const float* __restrict__ part, int splits,
-                                                        int rank, int rp, int n, float factor,
-                                                        int64_t out_j, int64_t out_c,
-                                                        float* __restrict__ out) {
-  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (e >= static_cast<int64_t>(rank) * n) return;
-  const int64_t j = e / n, c = e % n;
-  float v = 0.0f;
-  for (int k = 0; k < splits; ++k) v += __ldg(part + (static_cast<int64_t>(k) * rp + j) * n + c);
-  out[j * out_j + c * out_c] = v * factor;
+// The weights' gradients: factor * (sum of the parts) as [rank, n] (A) or [n, rank] (B).
+struct PartSum {
+  const float* part;  // [splits, RP, n]
+  int splits, n;
+  float factor;
+  float* out;  // null: not wanted
+};
+
+// A CTA per 32 columns of one of them.
+__global__ void __launch_bounds__(256) sum_parts_kernel(PartSum a, PartSum b, int rank, int rp) {
+  __shared__ float turned[32][64 + 1];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int a_ctas = a.out ? (a.n + 31) / 32 : 0;
+  const bool is_a = static_cast<int>(blockIdx.x) < a_ctas;
+  const PartSum& s = is_a ? a : b;
+  const int c0 = (is_a ? blockIdx.x : blockIdx.x - a_ctas) * 32;
+  const int c = threadIdx.x & 31, live = min(32, s.n - c0);
+  const int64_t step = static_cast<int64_t>(rp) * s.n;
+  for (int j = threadIdx.x >> 5; j < rank; j += 8) {
+    const float* p = s.part + static_cast<int64_t>(j) * s.n + c0 + c;
+    float v = 0.0f;
+    for (int k0 = 0; k0 < s.splits; k0 += 8) {
+      float x[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        x[u] = k0 + u < s.splits && c < live ? __ldcg(p + (k0 + u) * step) : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += x[u];
+    }
+    if (is_a && c < live) s.out[static_cast<int64_t>(j) * s.n + c0 + c] = v * s.factor;
+    if (!is_a) turned[c][j] = v * s.factor;
+  }
+  if (is_a) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < live * rank; i += 256)
+    s.out[static_cast<int64_t>(c0) * rank + i] = turned[i / rank][i % rank];
 }
 
 // ---- host: workspaces and launches ------------------------------------------------------------
@@ -351,83 +411,69 @@ struct Carve {  // hands out 256-byte aligned pieces; counts them when there is 
   }
 };
 
-struct TBuffers {
-  TParts parts;
-  TBuffers(Carve& c, int64_t n_rows, int rp) {
-    parts.cat = c.take<uint4>(static_cast<size_t>(n_rows) * up::chunks(rp) * 8);
-    parts.pair = c.take<uint4>(static_cast<size_t>(n_rows) * (sums::pair_width(rp) / 8));
-    parts.down = c.take<float>(static_cast<size_t>((n_rows + 127) / 128));
-  }
-};
-
-// The adapter's operands of one direction: one matrix as rows, the other concatenated.
-struct Prepared {
-  Rows rows;
-  uint4* cat;
-  Prepared(Carve& c, int64_t n_rows_matrix, int64_t n_cols_matrix, int rp) {
-    rows.parts = c.take<__half>(static_cast<size_t>(2 * rp) * n_rows_matrix);
-    rows.down = c.take<float>(rp);
-    cat = c.take<uint4>(static_cast<size_t>(n_cols_matrix) * up::chunks(rp) * 8);
+// What the forward pass leaves for the backward pass: t's pair and the adapter's other operands.
+struct Saved {
+  Carve carve;
+  TParts t;
+  Rows b_rows;
+  uint4* a_cat;
+  Saved(void* base, const Shape& s, int rp) : carve{static_cast<char*>(base), 0} {
+    t.cat = nullptr;
+    t.pair = carve.take<uint4>(static_cast<size_t>(s.n_rows) * (sums::pair_width(rp) / 8));
+    t.down = carve.take<float>(static_cast<size_t>((s.n_rows + 127) / 128));
+    b_rows.parts = carve.take<__half>(static_cast<size_t>(2 * rp) * s.n_out);
+    b_rows.down = carve.take<float>(static_cast<size_t>((s.n_out + 127) / 128) * rp);
+    a_cat = carve.take<uint4>(static_cast<size_t>(s.n_in) * up::chunks(rp) * 8);
   }
 };
 
 struct ForwardWork {
   Carve carve;
-  Prepared prep;
+  Rows a_rows;
+  uint4 *b_cat, *t_cat;
   float* part;
-  ForwardWork(void* base, const Shape& s, int rp)
-      : carve{static_cast<char*>(base), 0}, prep(carve, s.n_in, s.n_out, rp) {
-    const sums::Plan plan(false, s.n_rows, s.n_in);
-    part = carve.take<float>(static_cast<size_t>(plan.splits) * s.n_rows * rp);
+  ForwardWork(void* base, const Shape& s, int rp) : carve{static_cast<char*>(base), 0} {
+    a_rows.parts = carve.take<__half>(static_cast<size_t>(2 * rp) * s.n_in);
+    a_rows.down = carve.take<float>(static_cast<size_t>((s.n_in + 127) / 128) * rp);
+    b_cat = carve.take<uint4>(static_cast<size_t>(s.n_out) * up::chunks(rp) * 8);
+    t_cat = carve.take<uint4>(static_cast<size_t>(s.n_rows) * up::chunks(rp) * 8);
+    part = carve.take<float>(static_cast<size_t>(sums::Plan(false, s.n_rows, s.n_in).splits) *
+                             s.n_rows * rp);
   }
 };
 
 struct BackwardWork {
   Carve carve;
-  Prepared prep;
-  TBuffers dt;
+  TParts dt;
   float *t_part, *b_part, *a_part;
-  BackwardWork(void* base, const Shape& s, int rp)
-      : carve{static_cast<char*>(base), 0},
-        prep(carve, s.n_out, s.n_in, rp),
-        dt(carve, s.n_rows, rp) {
-    const sums::Plan inner(false, s.n_rows, s.n_out);
-    t_part = carve.take<float>(static_cast<size_t>(inner.splits) * s.n_rows * rp);
-    const sums::Plan ob(true, s.n_rows, s.n_out), oa(true, s.n_rows, s.n_in);
-    b_part = carve.take<float>(static_cast<size_t>(ob.splits) * rp * s.n_out);
-    a_part = carve.take<float>(static_cast<size_t>(oa.splits) * rp * s.n_in);
+  BackwardWork(void* base, const Shape& s, int rp) : carve{static_cast<char*>(base), 0} {
+    dt.cat = carve.take<uint4>(static_cast<size_t>(s.n_rows) * up::chunks(rp) * 8);
+    dt.pair = carve.take<uint4>(static_cast<size_t>(s.n_rows) * (sums::pair_width(rp) / 8));
+    dt.down = carve.take<float>(static_cast<size_t>((s.n_rows + 127) / 128));
+    t_part = carve.take<float>(static_cast<size_t>(sums::Plan(false, s.n_rows, s.n_out).splits) *
+                               s.n_rows * rp);
+    b_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, s.n_rows, s.n_out).splits) *
+                               rp * s.n_out);
+    a_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, s.n_rows, s.n_in).splits) *
+                               rp * s.n_in);
   }
 };
-
-struct Saved {
-  Carve carve;
-  TBuffers t;
-  Saved(void* base, const Shape& s, int rp)
-      : carve{static_cast<char*>(base), 0}, t(carve, s.n_rows, rp) {}
-};
-
-void prepare(const float* m0, int64_t j0, int64_t c0, int64_t n0, const float* m1, int64_t j1,
-             int64_t c1, int64_t n1, const Prepared& p, int rank, int rp, cudaStream_t stream) {
-  const int64_t grid = rp + (n1 * (rp / 8) + PREP_THREADS - 1) / PREP_THREADS;
-  prepare_kernel<<<static_cast<unsigned>(grid), PREP_THREADS, 0, stream>>>(
-      m0, j0, c0, static_cast<int>(n0), p.rows, m1, j1, c1, static_cast<int>(n1), p.cat, rank,
-      rp);
-}
 
 // t or dt of an activation: the inner sums and the operands made of them.
 template <int RP>
 int run_inner(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const Rows& rows,
               const Dropout& d, float* part, float factor, const TParts& out,
               cudaStream_t stream) {
-  const int st = d.drop ? sums::launch<RP, false, true>(x, ld, n_rows, n_cols, rows.parts, nullptr,
-                                                        d, part, stream)
-                        : sums::launch<RP, false, false>(x, ld, n_rows, n_cols, rows.parts, nullptr,
-                                                         d, part, stream);
+  const int st = d.drop ? sums::launch<RP, false, true>(x, ld, n_rows, n_cols, rows.parts,
+                                                        rows.down, d, part, stream)
+                        : sums::launch<RP, false, false>(x, ld, n_rows, n_cols, rows.parts,
+                                                         rows.down, d, part, stream);
   if (st != TALM_OK) return st;
-  const unsigned grid = static_cast<unsigned>((n_rows + 127) / 128 * T_CLUSTER);
-  t_parts_kernel<RP><<<grid, 128, 0, stream>>>(part, sums::Plan(false, n_rows, n_cols).splits,
-                                               n_rows, rows.down, factor, out);
-  return TALM_OK;
+  constexpr int smem = 128 * (RP + 1) * 4;
+  static_assert(smem <= 48 * 1024, "no opt-in");
+  return launch_dependent(t_parts_kernel<RP>, static_cast<unsigned>((n_rows + 127) / 128),
+                          T_THREADS, smem, stream, part,
+                          sums::Plan(false, n_rows, n_cols).splits, n_rows, factor, out);
 }
 
 template <int RP>
@@ -436,58 +482,55 @@ int run_forward(const __half* x, int64_t ld_x, const __half* base, int64_t ld_ba
                 __half* y, void* saved, void* work, cudaStream_t stream) {
   const ForwardWork w(work, s, RP);
   const Saved keep(saved, s, RP);
-  prepare(a, s.n_in, 1, s.n_in, b, 1, s.rank, s.n_out, w.prep, s.rank, RP, stream);
-  const int st = run_inner<RP>(x, ld_x, s.n_rows, s.n_in, w.prep.rows, d, w.part, d.factor,
-                               keep.t.parts, stream);
+  const Matrix ma{a, s.n_in, 1, static_cast<int>(s.n_in)};
+  const Matrix mb{b, 1, s.rank, static_cast<int>(s.n_out)};
+  const Operands of_a{w.a_rows, keep.a_cat};
+  const Operands of_b{saved ? keep.b_rows : Rows{nullptr, nullptr}, w.b_cat};
+  constexpr int smem = RP * 129 * 4;
+  static_assert(smem <= 48 * 1024, "no opt-in");
+  int st = launch_dependent(prepare_kernel<RP>,
+                            static_cast<unsigned>((s.n_in + 127) / 128 + (s.n_out + 127) / 128),
+                            PREP_THREADS, smem, stream, ma, mb, of_a, of_b, s.rank);
+  const TParts t{w.t_cat, saved ? keep.t.pair : nullptr, saved ? keep.t.down : nullptr};
+  if (st == TALM_OK)
+    st = run_inner<RP>(x, ld_x, s.n_rows, s.n_in, w.a_rows, d, w.part, d.factor, t, stream);
   if (st != TALM_OK) return st;
-  return up::launch<up::chunks(RP), false>(keep.t.parts.cat, w.prep.cat, base, ld_base, y, s.n_rows,
-                                           s.n_out, scaling, d, stream);
-}
-
-void sum_parts(const float* part, int splits, int64_t n, int rank, int rp, float factor,
-               int64_t out_j, int64_t out_c, float* out, cudaStream_t stream) {
-  const int64_t total = rank * n;
-  sum_parts_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, stream>>>(
-      part, splits, rank, rp, static_cast<int>(n), factor, out_j, out_c, out);
+  return up::launch<up::chunks(RP), false>(w.t_cat, w.b_cat, base, ld_base, y, s.n_rows, s.n_out,
+                                           scaling, d, stream);
 }
 
 template <int RP>
-int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, const float* a,
-                 const float* b, const Shape& s, float scaling, const Dropout& d,
-                 const void* saved, __half* dx, float* da, float* db, void* work,
-                 cudaStream_t stream) {
+int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, const Shape& s,
+                 float scaling, const Dropout& d, const void* saved, __half* dx, float* da,
+                 float* db, void* work, cudaStream_t stream) {
   const BackwardWork w(work, s, RP);
   const Saved keep(const_cast<void*>(saved), s, RP);
   const Dropout none{nullptr, 0, 1.0f};
-  if (db) {
-    const int st = sums::launch<RP, true, false>(g, ld_g, s.n_rows, s.n_out, keep.t.parts.pair,
-                                                 keep.t.parts.down, none, w.b_part, stream);
-    if (st != TALM_OK) return st;
-    sum_parts(w.b_part, sums::Plan(true, s.n_rows, s.n_out).splits, s.n_out, s.rank, RP, scaling, 1,
-              s.rank, db, stream);
+  int st = TALM_OK;
+  if (da || dx)
+    st = run_inner<RP>(g, ld_g, s.n_rows, s.n_out, keep.b_rows, none, w.t_part, scaling, w.dt,
+                       stream);
+  if (db && st == TALM_OK)
+    st = sums::launch<RP, true, false>(g, ld_g, s.n_rows, s.n_out, keep.t.pair, keep.t.down, none,
+                                       w.b_part, stream);
+  if (da && st == TALM_OK)
+    st = d.drop ? sums::launch<RP, true, true>(x, ld_x, s.n_rows, s.n_in, w.dt.pair, w.dt.down, d,
+                                               w.a_part, stream)
+                : sums::launch<RP, true, false>(x, ld_x, s.n_rows, s.n_in, w.dt.pair, w.dt.down, d,
+                                                w.a_part, stream);
+  if (dx && st == TALM_OK)
+    st = up::launch<up::chunks(RP), true>(w.dt.cat, keep.a_cat, nullptr, 0, dx, s.n_rows, s.n_in,
+                                          d.factor, d, stream);
+  if ((da || db) && st == TALM_OK) {
+    const PartSum sa{w.a_part, sums::Plan(true, s.n_rows, s.n_in).splits,
+                     static_cast<int>(s.n_in), d.factor, da};
+    const PartSum sb{w.b_part, sums::Plan(true, s.n_rows, s.n_out).splits,
+                     static_cast<int>(s.n_out), scaling, db};
+    const int64_t ctas = (da ? (s.n_in + 31) / 32 : 0) + (db ? (s.n_out + 31) / 32 : 0);
+    st = launch_dependent(sum_parts_kernel, static_cast<unsigned>(ctas), 256, 0, stream, sa, sb,
+                          s.rank, RP);
   }
-  if (da || dx) {
-    prepare(b, 1, s.rank, s.n_out, a, s.n_in, 1, s.n_in, w.prep, s.rank, RP, stream);
-    const int st = run_inner<RP>(g, ld_g, s.n_rows, s.n_out, w.prep.rows, none, w.t_part, scaling,
-                                 w.dt.parts, stream);
-    if (st != TALM_OK) return st;
-    if (dx) {
-      const int st = up::launch<up::chunks(RP), true>(w.dt.parts.cat, w.prep.cat, nullptr, 0, dx,
-                                                      s.n_rows, s.n_in, d.factor, d, stream);
-      if (st != TALM_OK) return st;
-    }
-    if (da) {
-      const TParts& t = w.dt.parts;
-      const int st = d.drop ? sums::launch<RP, true, true>(x, ld_x, s.n_rows, s.n_in, t.pair,
-                                                           t.down, d, w.a_part, stream)
-                            : sums::launch<RP, true, false>(x, ld_x, s.n_rows, s.n_in, t.pair,
-                                                            t.down, d, w.a_part, stream);
-      if (st != TALM_OK) return st;
-      sum_parts(w.a_part, sums::Plan(true, s.n_rows, s.n_in).splits, s.n_in, s.rank, RP, d.factor,
-                s.n_in, 1, da, stream);
-    }
-  }
-  return check_launch("adapter backward kernels");
+  return st;
 }
 
 int check_dropout(int64_t drop, const int64_t* seed, Dropout* d) {
@@ -575,12 +618,12 @@ int talm_lora_forward(const uint16_t* x, int64_t ld_x, const uint16_t* base, int
   size_t need = 0, need_forward = 0, need_backward = 0;
   talm_lora_sizes(n_rows, n_in, n_out, rank, &need, &need_forward, &need_backward);
   if (n_rows == 0) return TALM_OK;
-  if (!x || !base || !lora_a || !lora_b || !y || !saved || !workspace)
+  if (!x || !base || !lora_a || !lora_b || !y || !workspace)
     return set_error(TALM_EINVAL, "null pointer");
   if (!rows_ok(x, ld_x, n_in) || !rows_ok(base, ld_base, n_out) || !rows_ok(y, n_out, n_out) ||
       ((reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(workspace)) & 15) != 0)
     return set_error(TALM_EINVAL, "rows must be 16-byte aligned with strides of 8 elements");
-  if (saved_bytes < need || ws_bytes < need_forward)
+  if ((saved && saved_bytes < need) || ws_bytes < need_forward)
     return set_error(TALM_EINVAL, "saved buffer or workspace too small");
   const Shape s{n_rows, n_in, n_out, static_cast<int>(rank)};
   LaunchTimer timer(TALM_KERNEL_LORA_FORWARD, stream);
@@ -592,8 +635,7 @@ int talm_lora_forward(const uint16_t* x, int64_t ld_x, const uint16_t* base, int
 }
 
 int talm_lora_backward(const uint16_t* g, int64_t ld_g, const uint16_t* x, int64_t ld_x,
-                       const float* lora_a, const float* lora_b, const void* saved,
-                       size_t saved_bytes, int64_t n_rows, int64_t n_in, int64_t n_out,
+                       const void* saved, size_t saved_bytes, int64_t n_rows, int64_t n_in, int64_t n_out,
                        int64_t rank, float scaling, const int64_t* seed, int64_t drop,
                        uint16_t* dx, float* grad_a, float* grad_b, void* workspace,
                        size_t ws_bytes, void* stream_) {
@@ -614,7 +656,7 @@ int talm_lora_backward(const uint16_t* g, int64_t ld_g, const uint16_t* x, int64
       e = cudaMemsetAsync(grad_b, 0, static_cast<size_t>(rank * n_out) * 4, stream);
     return e == cudaSuccess ? TALM_OK : set_error(TALM_ECUDA, "memset: %s", cudaGetErrorString(e));
   }
-  if (!g || !x || !lora_a || !lora_b || !saved || !workspace)
+  if (!g || !x || !saved || !workspace)
     return set_error(TALM_EINVAL, "null pointer");
   if (!rows_ok(g, ld_g, n_out) || !rows_ok(x, ld_x, n_in) || (dx && !rows_ok(dx, n_in, n_in)) ||
       ((reinterpret_cast<uintptr_t>(saved) | reinterpret_cast<uintptr_t>(workspace)) & 15) != 0)
@@ -626,8 +668,7 @@ int talm_lora_backward(const uint16_t* g, int64_t ld_g, const uint16_t* x, int64
   const int rp = padded_rank(s.rank);
   auto run = rp == 16 ? run_backward<16> : rp == 32 ? run_backward<32> : run_backward<64>;
   return run(reinterpret_cast<const __half*>(g), ld_g, reinterpret_cast<const __half*>(x), ld_x,
-             lora_a, lora_b, s, scaling, d, saved, reinterpret_cast<__half*>(dx), grad_a, grad_b,
-             workspace, stream);
+             s, scaling, d, saved, reinterpret_cast<__half*>(dx), grad_a, grad_b, workspace, stream);
 }
 
 }  // extern "C"

@@ -82,5 +82,26 @@ __device__ __forceinline__ void power_scale(float m, float* up, float* down) {
   *down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
+// The kernels of one branch follow one another closely: each may start its set-up while the one
+// before it ends (programmatic stream serialization) and waits in grid_dependency_wait before it
+// touches global memory.
+template <class... Params, class... Args>
+int launch_dependent(void (*kernel)(Params...), dim3 grid, int threads, int smem,
+                     cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
+  if (e != cudaSuccess) return set_error(TALM_ECUDA, "adapter kernel: %s", cudaGetErrorString(e));
+  return TALM_OK;
+}
+
 }  // namespace adapter
 }  // namespace talm

@@ -106,6 +106,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_launch_dependents();
+  grid_dependency_wait();
   const uint32_t tmem_base = ctl->tmem_base;
   volatile int* abort = &ctl->abort;
 
@@ -226,6 +228,18 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int64_t row = tile % p.row_tiles * TILE + r;
       const int slot = (2 * i + q) % SLOTS, acc = i & 1;
       const uint32_t phase = (i / (SLOTS / 2)) & 1;
+      // the tile's masks while its product is made: eight groups of eight columns
+      uint32_t keep[MASK ? 32 : 1];
+      if (MASK) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t w[4] = {};
+          if (p.drop.drop)
+            philox(static_cast<uint64_t>((row * p.n_cols + ct * TILE + q * 64 + c * 8) >> 3), key, w);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) keep[4 * c + k] = keep_mask2(w[k], bias2);
+        }
+      }
       bool ok;
       if (MASK)
         ok = mbar_wait(&ctl->box_empty[slot], phase ^ 1, abort);
@@ -247,15 +261,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           uint4* at = reinterpret_cast<uint4*>(box + (((4 * h + c) ^ (r & 7)) << 4));
           uint32_t o[4];
           if (MASK) {
-            uint32_t w[4] = {};
-            if (p.drop.drop)
-              philox(static_cast<uint64_t>((row * p.n_cols + ct * TILE + q * 64 + h * 32 + c * 8) >> 3),
-                     key, w);
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               o[k] = pack_half2(p.scale * __uint_as_float(d[8 * c + 2 * k]),
                                 p.scale * __uint_as_float(d[8 * c + 2 * k + 1])) &
-                     keep_mask2(w[k], bias2);
+                     keep[4 * (4 * h + c) + k];
           } else {
             const uint4 b = *at;
             const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
@@ -315,8 +325,7 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
   const int sms = current_sm_count();
   if (sms <= 0) return set_error(TALM_ENODEV, "no CUDA device");
   const unsigned grid = static_cast<unsigned>(p.n_tiles < sms ? p.n_tiles : sms);
-  kernel<<<grid, THREADS, smem, stream>>>(tm_t, tm_m, tm_base, tm_out, p);
-  return check_launch("adapter up kernel");
+  return launch_dependent(kernel, grid, THREADS, smem, stream, tm_t, tm_m, tm_base, tm_out, p);
 }
 
 }  // namespace up
@@ -324,8 +333,8 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
 // The adapter's sums over an activation X [n_rows, n_cols] on tcgen05, X optionally dropped out:
 //   INNER:  part[split][n][j] = sum over the split's columns of X[n, c] W[j, c]
 //   OUTER:  part[split][j][c] = sum over the split's rows of X[n, c] T[n, j]
-// W (an adapter matrix) and T (t or dt) are fp32, scaled by powers of two and split in two fp16
-// parts that stand side by side as the n operand (N = 2 RP), so that X passes the tensor core once;
+// W (an adapter matrix) and T (t or dt) are fp32, scaled by powers of two (a scale for every 128 of the
+// reduction, for W one for each rank) and split in two fp16 parts that stand side by side as the n operand (N = 2 RP), so that X passes the tensor core once;
 // the epilogue adds the two halves of the result. X is the 128-row m operand as it lies in memory:
 // rows of K-major for INNER, columns of it, MN-major, for OUTER.
 //
@@ -333,8 +342,8 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
 // columns (OUTER) and split, stages of 64 of the reduction:
 //   warp 0        TMA producer           warp 1      MMA issuer, into one of two TMEM buffers
 //   warps 4-11    epilogue: two groups of 128 threads, half the ranks each. The buffer is moved
-//                 into fp32 registers every FLUSH stages: the tensor core's long sums are not
-//                 rounded to nearest, and OUTER's T has a scale of its own for every 128 rows.
+//                 into fp32 registers every two stages, which share a scale; the tensor core's
+//                 sums, which are not rounded to nearest, stay short by that.
 //   warps 12-19   (MASK) drop X in shared memory before it is multiplied: a 16-byte piece is one
 //                 group of the generator
 namespace sums {
@@ -372,7 +381,7 @@ struct Params {
   int64_t n_rows;
   int n_cols;
   int steps, steps_per_split;  // 64-wide stages of the whole reduction, and of a split
-  const float* down;           // OUTER: the scale of every 128 rows of T
+  const float* down;           // what undoes the scales: [blocks of 128] of T, [blocks][RP] of W
   float* part;
   Dropout drop;
 };
@@ -385,7 +394,7 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
   constexpr int O_BYTES = other_bytes<RP, OUTER>();
   constexpr int N = 2 * RP;
   constexpr int COLS = N < 32 ? 32 : N;  // TMEM columns of a buffer
-  constexpr int FLUSH = OUTER ? 2 : 8;
+  constexpr int FLUSH = 2;  // stages of a scale
   extern __shared__ uint8_t smem_raw[];
   uint8_t* x_s = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                             ~uintptr_t(1023));
@@ -419,6 +428,8 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_launch_dependents();
+  grid_dependency_wait();
   const uint32_t tmem_base = ctl->tmem_base;
   volatile int* abort = &ctl->abort;
 
@@ -482,7 +493,7 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
     const int flushes = (n_steps + FLUSH - 1) / FLUSH;
     bool ok = true;
     for (int f = 0; f < flushes; ++f) {
-      const float back = OUTER ? __ldg(p.down + s0 / FLUSH + f) : 1.0f;
+      const float* down = p.down + (s0 / FLUSH + f) * (OUTER ? 1 : RP) + (OUTER ? 0 : q * HR);
       ok = mbar_wait(&ctl->acc_full[f & 1], (f >> 1) & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
@@ -503,7 +514,8 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
         tmem_wait_ld();
 #pragma unroll
         for (int u = 0; u < STEP; ++u)
-          acc[j + u] = fmaf(back, __uint_as_float(hi[u]) + __uint_as_float(lo[u]), acc[j + u]);
+          acc[j + u] = fmaf(__ldg(down + (OUTER ? 0 : j + u)),
+                            __uint_as_float(hi[u]) + __uint_as_float(lo[u]), acc[j + u]);
       }
       tc_fence_before();
       __syncwarp();
@@ -562,22 +574,21 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
   if (warp == 1) tmem_dealloc(tmem_base, 2 * COLS);
 }
 
-// How the reduction is divided: about two CTAs for each of 148 SMs, at least three stages (INNER)
-// or two 128-row blocks (OUTER) for a CTA, and whole blocks.
+// How the reduction is divided: about two CTAs for each of 148 SMs, two blocks of 128 (which share a
+// scale) for a CTA at least.
 struct Plan {
   int tiles, steps, steps_per_split, splits;
   Plan(bool outer, int64_t n_rows, int64_t n_cols) {
     tiles = static_cast<int>(((outer ? n_cols : n_rows) + TILE - 1) / TILE);
     const int64_t length = outer ? n_rows : n_cols;
-    const int unit = outer ? 2 : 1;
     steps = static_cast<int>((length + 63) / 64);
-    const int units = (steps + unit - 1) / unit;
+    const int blocks = (steps + 1) / 2;
     int want = 296 / tiles;
-    const int most = outer ? (units + 1) / 2 : (units + 2) / 3;
+    const int most = (blocks + 1) / 2;
     if (want > most) want = most;
     if (want > 32) want = 32;
     if (want < 1) want = 1;
-    steps_per_split = (units + want - 1) / want * unit;
+    steps_per_split = (blocks + want - 1) / want * 2;
     splits = (steps + steps_per_split - 1) / steps_per_split;
   }
 };
@@ -601,9 +612,9 @@ int launch(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void
                : talm_make_tmap_2d_f16(&tm_o, other, n_cols, 2 * RP, n_cols, 64, 2 * RP);
   if (st != TALM_OK) return st;
   const Params p{n_rows, static_cast<int>(n_cols), plan.steps, plan.steps_per_split, down, part, d};
-  kernel<<<dim3(static_cast<unsigned>(plan.tiles), static_cast<unsigned>(plan.splits), 1),
-           threads(MASK), smem, stream>>>(tm_x, tm_o, p);
-  return check_launch("adapter sums kernel");
+  return launch_dependent(
+      kernel, dim3(static_cast<unsigned>(plan.tiles), static_cast<unsigned>(plan.splits), 1),
+      threads(MASK), smem, stream, tm_x, tm_o, p);
 }
 
 }  // namespace sums

@@ -87,8 +87,8 @@ def test_c_entries_reject_bad_arguments(lib):
     assert forward(ptr=16, ws=3) == 1
 
     def backward(n_rows=4, ptr=None, out=16, ws=1 << 24, ld_g=64):
-        return lib.talm_lora_backward(ptr, ld_g, ptr, 64, ptr, ptr, ptr, 1 << 24, n_rows, 64, 64,
-                                      16, 1.0, None, 0, out, None, None, ptr, ws, None)
+        return lib.talm_lora_backward(ptr, ld_g, ptr, 64, ptr, 1 << 24, n_rows, 64, 64, 16,
+                                       1.0, None, 0, out, None, None, ptr, ws, None)
     assert backward() == 1
     assert backward(out=None) == 0                  # nothing asked for
     assert backward(ptr=16, ld_g=60) == 1 and backward(ptr=16, ws=3) == 1
