@@ -195,7 +195,7 @@ __host__ __device__ constexpr int padded_rank(int rank) {
   return rank <= 16 ? 16 : rank <= 32 ? 32 : 64;
 }
 
-constexpr int PREP_THREADS = 256;
+constexpr int PREP_THREADS = 1024;
 
 // Ranks j .. j + 7 of the three parts of row r of a concatenated operand; the first eight write the
 // zeros behind the parts too.
@@ -368,8 +368,10 @@ struct PartSum {
   float* out;  // null: not wanted
 };
 
-// A CTA per 32 columns of one of them.
-__global__ void __launch_bounds__(256) sum_parts_kernel(PartSum a, PartSum b, int rank, int rp) {
+// A CTA per 32 columns of one of them, a warp per rank.
+constexpr int SUM_THREADS = 1024;
+
+__global__ void __launch_bounds__(SUM_THREADS) sum_parts_kernel(PartSum a, PartSum b, int rank, int rp) {
   __shared__ float turned[32][64 + 1];
   grid_launch_dependents();
   grid_dependency_wait();
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(PartSum a, PartSum b, in
   const int c0 = (is_a ? blockIdx.x : blockIdx.x - a_ctas) * 32;
   const int c = threadIdx.x & 31, live = min(32, s.n - c0);
   const int64_t step = static_cast<int64_t>(rp) * s.n;
-  for (int j = threadIdx.x >> 5; j < rank; j += 8) {
+  for (int j = threadIdx.x >> 5; j < rank; j += SUM_THREADS / 32) {
     const float* p = s.part + static_cast<int64_t>(j) * s.n + c0 + c;
     float v = 0.0f;
     for (int k0 = 0; k0 < s.splits; k0 += 8) {
@@ -395,7 +397,7 @@ __global__ void __launch_bounds__(256) sum_parts_kernel(PartSum a, PartSum b, in
   }
   if (is_a) return;
   __syncthreads();
-  for (int i = threadIdx.x; i < live * rank; i += 256)
+  for (int i = threadIdx.x; i < live * rank; i += SUM_THREADS)
     s.out[static_cast<int64_t>(c0) * rank + i] = turned[i / rank][i % rank];
 }
 
@@ -437,8 +439,9 @@ struct ForwardWork {
     a_rows.down = carve.take<float>(static_cast<size_t>((s.n_in + 127) / 128) * rp);
     b_cat = carve.take<uint4>(static_cast<size_t>(s.n_out) * up::chunks(rp) * 8);
     t_cat = carve.take<uint4>(static_cast<size_t>(s.n_rows) * up::chunks(rp) * 8);
-    part = carve.take<float>(static_cast<size_t>(sums::Plan(false, s.n_rows, s.n_in).splits) *
-                             s.n_rows * rp);
+    // without a mask there are at least as many splits
+    part = carve.take<float>(
+        static_cast<size_t>(sums::Plan(false, false, s.n_rows, s.n_in).splits) * s.n_rows * rp);
   }
 };
 
@@ -450,11 +453,11 @@ struct BackwardWork {
     dt.cat = carve.take<uint4>(static_cast<size_t>(s.n_rows) * up::chunks(rp) * 8);
     dt.pair = carve.take<uint4>(static_cast<size_t>(s.n_rows) * (sums::pair_width(rp) / 8));
     dt.down = carve.take<float>(static_cast<size_t>((s.n_rows + 127) / 128));
-    t_part = carve.take<float>(static_cast<size_t>(sums::Plan(false, s.n_rows, s.n_out).splits) *
+    t_part = carve.take<float>(static_cast<size_t>(sums::Plan(false, false, s.n_rows, s.n_out).splits) *
                                s.n_rows * rp);
-    b_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, s.n_rows, s.n_out).splits) *
+    b_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, false, s.n_rows, s.n_out).splits) *
                                rp * s.n_out);
-    a_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, s.n_rows, s.n_in).splits) *
+    a_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, false, s.n_rows, s.n_in).splits) *
                                rp * s.n_in);
   }
 };
@@ -473,7 +476,7 @@ int run_inner(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const
   static_assert(smem <= 48 * 1024, "no opt-in");
   return launch_dependent(t_parts_kernel<RP>, static_cast<unsigned>((n_rows + 127) / 128),
                           T_THREADS, smem, stream, part,
-                          sums::Plan(false, n_rows, n_cols).splits, n_rows, factor, out);
+                          sums::Plan(false, d.drop != 0, n_rows, n_cols).splits, n_rows, factor, out);
 }
 
 template <int RP>
@@ -522,12 +525,12 @@ int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, c
     st = up::launch<up::chunks(RP), true>(w.dt.cat, keep.a_cat, nullptr, 0, dx, s.n_rows, s.n_in,
                                           d.factor, d, stream);
   if ((da || db) && st == TALM_OK) {
-    const PartSum sa{w.a_part, sums::Plan(true, s.n_rows, s.n_in).splits,
+    const PartSum sa{w.a_part, sums::Plan(true, d.drop != 0, s.n_rows, s.n_in).splits,
                      static_cast<int>(s.n_in), d.factor, da};
-    const PartSum sb{w.b_part, sums::Plan(true, s.n_rows, s.n_out).splits,
+    const PartSum sb{w.b_part, sums::Plan(true, false, s.n_rows, s.n_out).splits,
                      static_cast<int>(s.n_out), scaling, db};
     const int64_t ctas = (da ? (s.n_in + 31) / 32 : 0) + (db ? (s.n_out + 31) / 32 : 0);
-    st = launch_dependent(sum_parts_kernel, static_cast<unsigned>(ctas), 256, 0, stream, sa, sb,
+    st = launch_dependent(sum_parts_kernel, static_cast<unsigned>(ctas), SUM_THREADS, 0, stream, sa, sb,
                           s.rank, RP);
   }
   return st;

@@ -13,8 +13,8 @@
 //               columns (four slots)
 //   warp 1      MMA issuer: 4 x tcgen05.mma (128 x 128 x 16) per chunk into one of two TMEM buffers
 //   warp 2      TMA stores of finished boxes; frees their slots
-//   warps 4-11  epilogue: two groups of 128 threads, a box each: TMEM -> fp32 -> + base (or mask) ->
-//               fp16, in place in the box's slot
+//   warps 4-19  epilogue: four groups of 128 threads, half a box each: TMEM -> fp32 -> + base (or
+//               mask) -> fp16, in place in the box's slot
 // Every wait is bounded; a wait that gives up ends the CTA's roles and records TALM_ETIMEOUT.
 #pragma once
 
@@ -29,7 +29,7 @@ constexpr int CHUNK_BYTES = TILE * 128;  // 128 rows of 64 bf16, 128-byte swizzl
 constexpr int BOX_BYTES = TILE * 128;    // 128 rows of 64 fp16
 constexpr int SLOTS = 4;
 constexpr int T_STAGES = 2;
-constexpr int EPI_WARPS = 8;
+constexpr int EPI_WARPS = 16;
 constexpr int FIRST_EPI_WARP = 4;
 constexpr int THREADS = 32 * (FIRST_EPI_WARP + EPI_WARPS);
 
@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       bulk_wait_all();
     }
   } else if (warp >= FIRST_EPI_WARP) {
-    const int quarter = warp & 3, q = (warp - FIRST_EPI_WARP) >> 2;
+    const int quarter = warp & 3, group = (warp - FIRST_EPI_WARP) >> 2;
+    const int q = group >> 1, h = group & 1;  // box, and which 32 columns of it
     const int r = quarter * 32 + lane;
     const uint64_t key = MASK && p.drop.drop ? static_cast<uint64_t>(__ldg(p.drop.seed)) : 0;
     const uint32_t bias2 = keep_bias2(p.drop.drop);
@@ -228,14 +229,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int64_t row = tile % p.row_tiles * TILE + r;
       const int slot = (2 * i + q) % SLOTS, acc = i & 1;
       const uint32_t phase = (i / (SLOTS / 2)) & 1;
-      // the tile's masks while its product is made: eight groups of eight columns
-      uint32_t keep[MASK ? 32 : 1];
+      // the masks of these columns while the product is made
+      uint32_t keep[MASK ? 16 : 1];
       if (MASK) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
+        for (int c = 0; c < 4; ++c) {
           uint32_t w[4] = {};
           if (p.drop.drop)
-            philox(static_cast<uint64_t>((row * p.n_cols + ct * TILE + q * 64 + c * 8) >> 3), key, w);
+            philox(static_cast<uint64_t>(
+                       (row * p.n_cols + ct * TILE + q * 64 + h * 32 + c * 8) >> 3),
+                   key, w);
 #pragma unroll
           for (int k = 0; k < 4; ++k) keep[4 * c + k] = keep_mask2(w[k], bias2);
         }
@@ -249,35 +252,32 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
       uint8_t* box = box_s + slot * BOX_BYTES + r * 128;
+      uint32_t d[32];
+      tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * TILE +
+                             q * 64 + h * 32,
+                         d);
+      tmem_wait_ld();
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t d[32];
-        tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * TILE +
-                               q * 64 + h * 32,
-                           d);
-        tmem_wait_ld();
+      for (int c = 0; c < 4; ++c) {  // eight columns
+        uint4* at = reinterpret_cast<uint4*>(box + (((4 * h + c) ^ (r & 7)) << 4));
+        uint32_t o[4];
+        if (MASK) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {  // eight columns
-          uint4* at = reinterpret_cast<uint4*>(box + (((4 * h + c) ^ (r & 7)) << 4));
-          uint32_t o[4];
-          if (MASK) {
+          for (int k = 0; k < 4; ++k)
+            o[k] = pack_half2(p.scale * __uint_as_float(d[8 * c + 2 * k]),
+                              p.scale * __uint_as_float(d[8 * c + 2 * k + 1])) &
+                   keep[4 * c + k];
+        } else {
+          const uint4 b = *at;
+          const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              o[k] = pack_half2(p.scale * __uint_as_float(d[8 * c + 2 * k]),
-                                p.scale * __uint_as_float(d[8 * c + 2 * k + 1])) &
-                     keep[4 * (4 * h + c) + k];
-          } else {
-            const uint4 b = *at;
-            const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&bw[k]));
-              o[k] = pack_half2(fmaf(p.scale, __uint_as_float(d[8 * c + 2 * k]), f.x),
-                                fmaf(p.scale, __uint_as_float(d[8 * c + 2 * k + 1]), f.y));
-            }
+          for (int k = 0; k < 4; ++k) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&bw[k]));
+            o[k] = pack_half2(fmaf(p.scale, __uint_as_float(d[8 * c + 2 * k]), f.x),
+                              fmaf(p.scale, __uint_as_float(d[8 * c + 2 * k + 1]), f.y));
           }
-          *at = make_uint4(o[0], o[1], o[2], o[3]);
         }
+        *at = make_uint4(o[0], o[1], o[2], o[3]);
       }
       tc_fence_before();
       fence_proxy_async_smem();  // the box is read by a bulk store
@@ -539,27 +539,33 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
     const int id = threadIdx.x - 32 * FIRST_MASK_WARP;
     const uint64_t key = static_cast<uint64_t>(__ldg(p.drop.seed));
     const uint32_t bias2 = keep_bias2(p.drop.drop);
+    constexpr int U = X_BYTES / 16 / (32 * MASK_WARPS);  // pieces of a thread
     for (int i = 0; i < n_steps; ++i) {
       const int st = i % STAGES;
-      const bool ok = mbar_wait(&ctl->full[st], (i / STAGES) & 1, abort);
-      if (!__all_sync(0xffffffffu, ok)) break;
       uint8_t* x = x_s + st * X_BYTES;
+      uint32_t w[U][4];  // the masks while the stage is on its way
 #pragma unroll
-      for (int u = 0; u < X_BYTES / 16 / (32 * MASK_WARPS); ++u) {
-        const int e = u * (32 * MASK_WARPS) + id;  // piece e: row line e / 8 of 128 bytes
-        const int line = e >> 3, c = e & 7;
-        // INNER: line = row, 64 columns; OUTER: line = row + 64 * (column group)
+      for (int u = 0; u < U; ++u) {
+        const int e = u * (32 * MASK_WARPS) + id, line = e >> 3, c = e & 7;
+        // a line is 128 bytes: a row of INNER's 64 columns; OUTER: row + 64 * (column group)
         const int64_t row = OUTER ? static_cast<int64_t>(s0 + i) * 64 + (line & 63) : origin + line;
         const int64_t col = OUTER ? origin + (line >> 6) * 64 + c * 8
                                   : static_cast<int64_t>(s0 + i) * 64 + c * 8;
+        philox(static_cast<uint64_t>((row * p.n_cols + col) >> 3), key, w[u]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[u][k] = keep_mask2(w[u][k], bias2);
+      }
+      const bool ok = mbar_wait(&ctl->full[st], (i / STAGES) & 1, abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int e = u * (32 * MASK_WARPS) + id, line = e >> 3, c = e & 7;
         uint4* at = reinterpret_cast<uint4*>(x + line * 128 + ((c ^ (line & 7)) << 4));
-        uint32_t w[4];
-        philox(static_cast<uint64_t>((row * p.n_cols + col) >> 3), key, w);
         uint4 v = *at;
-        v.x &= keep_mask2(w[0], bias2);
-        v.y &= keep_mask2(w[1], bias2);
-        v.z &= keep_mask2(w[2], bias2);
-        v.w &= keep_mask2(w[3], bias2);
+        v.x &= w[u][0];
+        v.y &= w[u][1];
+        v.z &= w[u][2];
+        v.w &= w[u][3];
         *at = v;
       }
       fence_proxy_async_smem();  // the tensor core reads it
@@ -574,16 +580,16 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
   if (warp == 1) tmem_dealloc(tmem_base, 2 * COLS);
 }
 
-// How the reduction is divided: about two CTAs for each of 148 SMs, two blocks of 128 (which share a
-// scale) for a CTA at least.
+// How the reduction is divided: as many CTAs as 148 SMs hold at a time (two of them, one with its mask
+// warps), two blocks of 128 (which share a scale) for a CTA at least.
 struct Plan {
   int tiles, steps, steps_per_split, splits;
-  Plan(bool outer, int64_t n_rows, int64_t n_cols) {
+  Plan(bool outer, bool mask, int64_t n_rows, int64_t n_cols) {
     tiles = static_cast<int>(((outer ? n_cols : n_rows) + TILE - 1) / TILE);
     const int64_t length = outer ? n_rows : n_cols;
     steps = static_cast<int>((length + 63) / 64);
     const int blocks = (steps + 1) / 2;
-    int want = 296 / tiles;
+    int want = (mask ? 148 : 296) / tiles;
     const int most = (blocks + 1) / 2;
     if (want > most) want = most;
     if (want > 32) want = 32;
@@ -604,7 +610,7 @@ int launch(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
-  const Plan plan(OUTER, n_rows, n_cols);
+  const Plan plan(OUTER, MASK, n_rows, n_cols);
   CUtensorMap tm_x, tm_o;
   int st = talm_make_tmap_2d_f16(&tm_x, x, n_cols, n_rows, ld, 64, OUTER ? 64 : TILE);
   if (st == TALM_OK)
