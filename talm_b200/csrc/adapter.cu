@@ -178,10 +178,10 @@ struct Shape {
 //   Rows:  fp16 parts of an adapter matrix with the rank in the rows (A, B^T), 128 columns of a row
 //          scaled together: parts [2 RP, n], the small parts behind the large ones; down [ceil(n /
 //          128)][RP] undoes the scale.
-//   cat:   bf16 parts (hi | lo | hi) of an adapter matrix with the rank in the columns (B, A^T), rows
-//          of up::chunks(RP) * 64, zeros behind the third part.
-//   TParts, of t or dt: cat, bf16 parts (hi | hi | lo) laid out likewise, and pair, fp16 parts
-//          (hi | lo) in rows of sums::pair_width(RP), 128 rows scaled together (down undoes it).
+//   cat:   bf16 parts (hi | lo) of an adapter matrix with the rank in the columns (B, A^T), or of t or
+//          dt, in rows of up::chunks(RP) * 64 (what is behind the parts is not read).
+//   pair:  fp16 parts (hi | lo) of t or dt in rows of sums::pair_width(RP) (likewise), 128 rows scaled
+//          together; down [ceil(rows / 128)] undoes it.
 struct Rows {
   __half* parts;
   float* down;
@@ -197,17 +197,14 @@ __host__ __device__ constexpr int padded_rank(int rank) {
 
 constexpr int PREP_THREADS = 1024;
 
-// Ranks j .. j + 7 of the three parts of row r of a concatenated operand; the first eight write the
-// zeros behind the parts too.
-__device__ __forceinline__ void put_cat(uint4* cat, int64_t r, int j, int rp, uint4 p0, uint4 p1,
-                                        uint4 p2) {
-  const int pieces = up::chunks(rp) * 8;  // of eight elements
-  uint4* row = cat + r * pieces;
-  row[j >> 3] = p0;
-  row[(rp + j) >> 3] = p1;
-  row[(2 * rp + j) >> 3] = p2;
-  if (j == 0)
-    for (int i = 3 * rp / 8; i < pieces; ++i) row[i] = make_uint4(0, 0, 0, 0);
+// Ranks j .. j + 7 of row r of a cat: both parts of eight values.
+__device__ __forceinline__ void put_cat(uint4* cat, int64_t r, int j, int rp, const float (&v)[8]) {
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) split_bf16(v[2 * k], v[2 * k + 1], hi[k], lo[k]);
+  uint4* row = cat + r * (up::chunks(rp) * 8);
+  row[j / 8] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  row[(rp + j) / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
 }
 
 // An adapter matrix: element (rank j, column c) at m[j * dj + c * dc].
@@ -281,12 +278,10 @@ __global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(Matrix a, Matrix 
     for (int i = tid; i < 128 * PIECES; i += PREP_THREADS) {
       const int c = i / PIECES, j = (i % PIECES) * 8;
       if (c0 + c >= s.n) break;  // so are the columns behind it
-      uint32_t hi[4], lo[4];
+      float v[8];
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        split_bf16(tile[(j + 2 * k) * LD + c], tile[(j + 2 * k + 1) * LD + c], hi[k], lo[k]);
-      const uint4 h = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      put_cat(out.cat, c0 + c, j, RP, h, make_uint4(lo[0], lo[1], lo[2], lo[3]), h);
+      for (int k = 0; k < 8; ++k) v[k] = tile[(j + k) * LD + c];
+      put_cat(out.cat, c0 + c, j, RP, v);
     }
   }
 }
@@ -344,13 +339,12 @@ __global__ void __launch_bounds__(T_THREADS)
     const int r = i / PIECES, j = (i % PIECES) * 8;
     const int64_t n = row0 + r;
     if (n >= n_rows) break;  // so are the rows behind it
-    const float* m = t_smem + r * (RP + 1) + j;
-    uint32_t hi[4], lo[4];
+    float m[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) split_bf16(m[2 * k], m[2 * k + 1], hi[k], lo[k]);
-    const uint4 h = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    put_cat(out.cat, n, j, RP, h, h, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+    for (int k = 0; k < 8; ++k) m[k] = t_smem[r * (RP + 1) + j + k];
+    put_cat(out.cat, n, j, RP, m);
     if (out.pair == nullptr) continue;
+    uint32_t hi[4], lo[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) split_f16(m[2 * k] * up, m[2 * k + 1] * up, hi[k], lo[k]);
     uint4* row = out.pair + n * (sums::pair_width(RP) / 8);
@@ -498,7 +492,7 @@ int run_forward(const __half* x, int64_t ld_x, const __half* base, int64_t ld_ba
   if (st == TALM_OK)
     st = run_inner<RP>(x, ld_x, s.n_rows, s.n_in, w.a_rows, d, w.part, d.factor, t, stream);
   if (st != TALM_OK) return st;
-  return up::launch<up::chunks(RP), false>(w.t_cat, w.b_cat, base, ld_base, y, s.n_rows, s.n_out,
+  return up::launch<RP, false>(w.t_cat, w.b_cat, base, ld_base, y, s.n_rows, s.n_out,
                                            scaling, d, stream);
 }
 
@@ -522,7 +516,7 @@ int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, c
                 : sums::launch<RP, true, false>(x, ld_x, s.n_rows, s.n_in, w.dt.pair, w.dt.down, d,
                                                 w.a_part, stream);
   if (dx && st == TALM_OK)
-    st = up::launch<up::chunks(RP), true>(w.dt.cat, keep.a_cat, nullptr, 0, dx, s.n_rows, s.n_in,
+    st = up::launch<RP, true>(w.dt.cat, keep.a_cat, nullptr, 0, dx, s.n_rows, s.n_in,
                                           d.factor, d, stream);
   if ((da || db) && st == TALM_OK) {
     const PartSum sa{w.a_part, sums::Plan(true, d.drop != 0, s.n_rows, s.n_in).splits,

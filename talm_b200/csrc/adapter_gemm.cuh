@@ -1,17 +1,17 @@
 // The adapter's rank-wide product on tcgen05: for an activation of n_rows x n_cols,
 //   ADD:   y  = fp16(base + scale * T M^T)       (the branch's output: T = t, M = B)
 //   MASK:  dx = fp16(keep(...) * scale * T M^T)  (the input's gradient: T = dt, M = A^T)
-// T [n_rows, rank] and M [n_cols, rank] are fp32, each split in two bf16 parts; the three products
-// hi hi, hi lo and lo hi (the fourth is under 2^-16 of a term) are one GEMM over the
-// concatenated rank: rows of T' = (hi | hi | lo) and of M' = (hi | lo | hi), padded with zeros to
-// whole 64-column chunks. (The 16 x 8 x 16 mma.sync form of the same product needed 96 mma's and 40
+// T [n_rows, rank] and M [n_cols, rank] are fp32, each split in two bf16 parts that stand side by side
+// in rows (hi | lo); a 16-rank slice is three tcgen05 steps, lo hi + hi lo + hi hi (the fourth is
+// under 2^-16 of a term). (The 16 x 8 x 16 mma.sync form of the same product needed 96 mma's and 40
 // 16-byte loads per 16 x 64 outputs at rank 64, and took 300 us for 16384 x 8960 outputs.)
 //
 // Bound by HBM: base is read and y written once (4 bytes per output). A persistent CTA walks 128 x
-// 128 tiles down the rows of a column tile, whose M' stays in shared memory:
-//   warp 0      TMA producer: M' when the column tile changes, T' (two stages), base in boxes of 64
-//               columns (four slots)
-//   warp 1      MMA issuer: 4 x tcgen05.mma (128 x 128 x 16) per chunk into one of two TMEM buffers
+// 128 tiles down the rows of a column tile, whose M stays in shared memory:
+//   warp 0      TMA producer: M when the column tile changes, T (three stages), base in boxes of 64
+//               columns (six slots)
+//   warp 1      MMA issuer: 3 x tcgen05.mma (128 x 128 x 16) per 16 ranks into one of two TMEM
+//               buffers
 //   warp 2      TMA stores of finished boxes; frees their slots
 //   warps 4-19  epilogue: four groups of 128 threads, half a box each: TMEM -> fp32 -> + base (or
 //               mask) -> fp16, in place in the box's slot
@@ -27,18 +27,22 @@ namespace up {
 constexpr int TILE = 128;
 constexpr int CHUNK_BYTES = TILE * 128;  // 128 rows of 64 bf16, 128-byte swizzle
 constexpr int BOX_BYTES = TILE * 128;    // 128 rows of 64 fp16
-constexpr int SLOTS = 4;
-constexpr int T_STAGES = 2;
+constexpr int SLOTS = 6;
+constexpr int T_STAGES = 3;
 constexpr int EPI_WARPS = 16;
 constexpr int FIRST_EPI_WARP = 4;
 constexpr int THREADS = 32 * (FIRST_EPI_WARP + EPI_WARPS);
 
-// 64-column chunks of the concatenated rank
-__host__ __device__ constexpr int chunks(int rp) { return (3 * rp + 63) / 64; }
-__host__ __device__ constexpr int smem_bytes(int n_chunks) {
-  return (1 + T_STAGES) * n_chunks * CHUNK_BYTES + SLOTS * BOX_BYTES + 1024 + 512;
+// 64-column chunks of an operand's row (hi | lo)
+__host__ __device__ constexpr int chunks(int rp) { return (2 * rp + 63) / 64; }
+__host__ __device__ constexpr int smem_bytes(int rp) {
+  return (1 + T_STAGES) * chunks(rp) * CHUNK_BYTES + SLOTS * BOX_BYTES + 1024 + 512;
 }
-static_assert(smem_bytes(chunks(64)) <= 232448, "shared memory of one CTA");
+static_assert(smem_bytes(64) <= 232448, "shared memory of one CTA");
+// where 16 columns from `col` start in a staged operand (chunks of 128-byte rows)
+__host__ __device__ constexpr int slice(int col) {
+  return col / 64 * CHUNK_BYTES + col % 64 * 2;
+}
 
 struct Ctl {
   uint64_t m_full, m_empty;
@@ -58,11 +62,12 @@ struct Params {
   Dropout drop;
 };
 
-template <int CHUNKS, bool MASK>
+template <int RP, bool MASK>
 __global__ void __launch_bounds__(THREADS, 1)
     up_kernel(const __grid_constant__ CUtensorMap tm_t, const __grid_constant__ CUtensorMap tm_m,
               const __grid_constant__ CUtensorMap tm_base,
               const __grid_constant__ CUtensorMap tm_out, Params p) {
+  constexpr int CHUNKS = chunks(RP);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -120,7 +125,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int ct = static_cast<int>(tile / p.row_tiles);
         const int row0 = static_cast<int>(tile % p.row_tiles) * TILE;
         if (ct != column) {
-          if (column >= 0) {  // the MMAs of the column tile before are done with M'
+          if (column >= 0) {  // the MMAs of the column tile before are done with M
             if (!mbar_wait(&ctl->m_empty, m_phase, abort)) break;
             m_phase ^= 1;
           }
@@ -178,14 +183,17 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (!mbar_wait(&ctl->acc_empty[acc], ((i >> 1) & 1) ^ 1, abort)) break;
         tc_fence_after();
         const uint32_t a0 = smem_u32(t_s + st * CHUNKS * CHUNK_BYTES), b0 = smem_u32(m_s);
+        const uint32_t d = tmem_base + acc * TILE;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16(tmem_base + acc * TILE,
-                     smem_desc_sw128(a0 + c * CHUNK_BYTES + k * 32, 16, 1024),
-                     smem_desc_sw128(b0 + c * CHUNK_BYTES + k * 32, 16, 1024), idesc,
-                     c != 0 || k != 0);
+        for (int j = 0; j < RP; j += 16) {
+          const uint64_t t_hi = smem_desc_sw128(a0 + slice(j), 16, 1024);
+          const uint64_t t_lo = smem_desc_sw128(a0 + slice(RP + j), 16, 1024);
+          const uint64_t m_hi = smem_desc_sw128(b0 + slice(j), 16, 1024);
+          const uint64_t m_lo = smem_desc_sw128(b0 + slice(RP + j), 16, 1024);
+          umma_f16(d, t_lo, m_hi, idesc, j != 0);
+          umma_f16(d, t_hi, m_lo, idesc, 1);
+          umma_f16(d, t_hi, m_hi, idesc, 1);
+        }
         umma_commit(&ctl->t_empty[st]);
         umma_commit(&ctl->acc_full[acc]);
         if (tile + 1 < last && (tile + 1) / p.row_tiles != ct) umma_commit(&ctl->m_empty);
@@ -295,12 +303,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 1) tmem_dealloc(tmem_base, 2 * TILE);
 }
 
-// t_op [n_rows, 64 chunks], m_op [n_cols, 64 chunks]: the concatenated bf16 parts
-template <int CHUNKS, bool MASK>
+// t_op [n_rows, 64 chunks(RP)], m_op [n_cols, 64 chunks(RP)]: the bf16 parts (hi | lo)
+template <int RP, bool MASK>
 int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base, void* out,
            int64_t n_rows, int64_t n_cols, float scale, const Dropout& d, cudaStream_t stream) {
-  constexpr int smem = smem_bytes(CHUNKS);
-  auto kernel = up_kernel<CHUNKS, MASK>;
+  constexpr int smem = smem_bytes(RP), CHUNKS = chunks(RP);
+  auto kernel = up_kernel<RP, MASK>;
   // Set on every call: it only notes the value, and it makes the device's context current in a
   // thread that has made no CUDA call yet (autograd's), which the tensor map encoder asks for.
   const cudaError_t e =
