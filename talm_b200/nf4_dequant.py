@@ -63,8 +63,7 @@ def nf4_matvec(x, packed, absmax, blocksize, out=None, bias=None, adapter=None):
     n_cols = x.shape[-1]
     if absmax.dtype != torch.float32 or packed.dtype != torch.uint8:
         raise ValueError("packed must be uint8 and absmax fp32")
-    packed = packed.contiguous().view(-1)
-    absmax = absmax.contiguous()
+    packed, absmax = packed.contiguous(), absmax.contiguous()
     n = 2 * packed.numel()
     if n_cols == 0 or n % n_cols:
         raise ValueError(f"{n} packed weights are not rows of {n_cols}")
@@ -76,7 +75,7 @@ def nf4_matvec(x, packed, absmax, blocksize, out=None, bias=None, adapter=None):
         else out
     qgroup.run_matvec(a, packed, None, absmax, None, None, None, None, 0, n_rows, n_cols,
                       int(blocksize), 1, bias, adapter, y)
-    return y.view(*x.shape[:-1], n_rows) if out is None else out
+    return y if out is not None or x.dim() == 2 else y.view(*x.shape[:-1], n_rows)
 
 
 def _self_check(original_impl):

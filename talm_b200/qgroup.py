@@ -349,19 +349,31 @@ def _few_rows(x, n_cols):
     return x
 
 
+_NO_ADAPTER = (None, None, 0, 0.0, None)
+
+
 def run_matvec(x, packed, absmax8, absmax, code, absmax2, offset2, levels, row0, n_rows, n_cols,
                blocksize, qblock2, bias, adapter, out):
     """The call of talm_nf4_matvec behind `launch_matvec`, `matvec` and `nf4_dequant.nf4_matvec`:
     x [rows, n_cols] from `_few_rows`, out [rows, n_rows], the weight's arrays checked by those."""
-    ptr = _lib.ptr
     n, device = x.shape[0], x.get_device()
-    ld_y = n_rows
     if out.dtype is not torch.float16 or out.shape != (n, n_rows):
         raise ValueError(f"out must be fp16 [{n}, {n_rows}]")
+    ld_y = n_rows
     if not out.is_contiguous():
         ld_y = out.stride(0) if n > 1 else n_rows
         if (n_rows > 1 and out.stride(1) != 1) or ld_y < n_rows:
             raise ValueError("out must have rows of unit stride that do not overlap")
+    apart = not packed.get_device() == out.get_device() == device
+    if absmax8 is None:
+        apart = apart or absmax.get_device() != device
+        scales = (None, absmax.data_ptr(), None, None, None, None)
+    else:
+        apart = apart or not (absmax8.get_device() == code.get_device() == absmax2.get_device()
+                              == offset2.get_device() == levels.get_device() == device)
+        scales = (absmax8.data_ptr(), None, code.data_ptr(), absmax2.data_ptr(),
+                  offset2.data_ptr(), levels.data_ptr())
+    extra = _NO_ADAPTER
     if adapter is not None:
         lora_a, lora_b, scaling = adapter
         rank = lora_a.shape[0]
@@ -370,31 +382,26 @@ def run_matvec(x, packed, absmax8, absmax, code, absmax2, offset2, levels, row0,
         if lora_a.shape != (rank, n_cols) or lora_b.shape != (n_rows, rank):
             raise ValueError(f"adapter {tuple(lora_a.shape)}, {tuple(lora_b.shape)} does not map "
                              f"{n_cols} to {n_rows}")
-    if absmax8 is None:
-        scales = (None, ptr(absmax), None, None, None, None)
-        apart = absmax.get_device() != device
-    else:
-        scales = (ptr(absmax8), None, ptr(code), ptr(absmax2), ptr(offset2), ptr(levels))
-        apart = not (absmax8.get_device() == code.get_device() == absmax2.get_device()
-                     == offset2.get_device() == levels.get_device() == device)
-    extra = (None, None, 0, 0.0, None)
-    if adapter is not None:
+        apart = apart or not lora_a.get_device() == lora_b.get_device() == device
         lora_a, lora_b = lora_a.contiguous(), lora_b.contiguous()
         down = torch.empty(8 * n * rank, dtype=torch.float32, device=x.device)
-        extra = (ptr(lora_a), ptr(lora_b), rank, scaling, ptr(down))
-        apart = apart or not lora_a.get_device() == lora_b.get_device() == device
+        extra = (lora_a.data_ptr(), lora_b.data_ptr(), rank, scaling, down.data_ptr())
+    bias_ptr = None
     if bias is not None:
         if bias.dtype is not torch.float16 or bias.shape != (n_rows,):
             raise ValueError(f"the bias must be fp16 [{n_rows}]")
-        bias = bias.contiguous()
         apart = apart or bias.get_device() != device
-    if apart or not packed.get_device() == out.get_device() == device:
+        bias = bias.contiguous()
+        bias_ptr = bias.data_ptr()
+    if device < 0:
+        raise RuntimeError("talm_b200 kernels run on CUDA tensors only (no CPU path)")
+    if apart:
         raise ValueError("the operands of the few-row product must be on one device")
     with _lib.device_of(x):
         _lib.check(_lib.load().talm_nf4_matvec(
-            ptr(x), x.stride(0) if n > 1 else n_cols, n, ptr(packed), *scales, row0, n_rows,
-            n_cols, blocksize, qblock2, None if bias is None else ptr(bias), *extra, ptr(out),
-            ld_y, _lib.raw_stream(x)), "talm_nf4_matvec")
+            x.data_ptr(), x.stride(0) if n > 1 else n_cols, n, packed.data_ptr(), *scales, row0,
+            n_rows, n_cols, blocksize, qblock2, bias_ptr, *extra, out.data_ptr(), ld_y,
+            _lib.raw_stream(x)), "talm_nf4_matvec")
     RAN["matvec"] += 1
     return out
 
