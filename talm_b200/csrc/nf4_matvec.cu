@@ -37,9 +37,9 @@ struct Weight {
 
 struct Epilogue {
   const __half* bias;   // null: none
-  const float* t;       // [parts, n_rows, rank] (t is the sum over the parts) or null
+  const float* t;       // [n_rows, rank] or null
   const float* lora_b;  // [n_out, rank]
-  int rank, parts;
+  int rank;
   float scaling;
 };
 
@@ -51,16 +51,16 @@ __device__ __forceinline__ void split_tf32(float v, uint32_t& hi, uint32_t& lo) 
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// t = x A^T in DOWN_PARTS or fewer partial sums over the columns (the product that reads t adds
-// them up): CTA (j, p) takes 16 rows of A and part p of the columns, its warps share those. fp16
-// x is exact in tf32, A is split in two.
+// t = x A^T: a cluster takes 16 rows of A, its CTAs (DOWN_PARTS or fewer) a part of the columns
+// each, their warps share those; the CTAs add up their sums in rank order through each other's shared
+// memory. fp16 x is exact in tf32, A is split in two.
 constexpr int DOWN_WARPS = 16;
 constexpr int DOWN_PARTS = 8;
 
@@ -137,12 +137,28 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 16 * n_rows; i += blockDim.x) {
-    const int n = i >> 4, j = j0 + (i & 15);
     float sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < DOWN_WARPS; ++v) sum += part[v][i];
-    if (j < rank) t_out[(int64_t{blockIdx.y} * n_rows + n) * rank + j] = sum;
+    part[0][i] = sum;
   }
+  const int parts = gridDim.y, me = static_cast<int>(cluster_ctarank());
+  if (parts > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  for (int i = me * blockDim.x + threadIdx.x; i < 16 * n_rows; i += parts * blockDim.x) {
+    const int j = j0 + (i & 15);
+    const uint32_t at = smem_u32(&part[0][i]);
+    float sum = 0.0f;
+    for (int c = 0; c < parts; ++c) {
+      float v;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(at, c)));
+      sum += v;
+    }
+    if (j < rank) t_out[(i >> 4) * rank + j] = sum;
+  }
+  if (parts > 1) cluster_sync();  // every CTA has read the others' sums
 }
 
 // ------------------------------------------------------------------------------------------
@@ -150,13 +166,14 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 // weight as the 16-row operand, up to 8 NT rows of x as the n operand).
 //
 // A warp takes tiles of 16 weight rows; lane (g, t) = (lane / 4, lane % 4) reads 8 packed bytes of
-// rows g and g + 8 per block (a quad reads a row's 32 bytes) and turns each byte into the fp16
+// rows g and g + 8 per block (a quad reads a row's 32 bytes: lane t bytes 4 t .. 4 t + 3 of both
+// halves) and turns each byte into the fp16
 // pair of its two levels by one shared-memory read: a table of 256 pairs, one copy per lane, so
 // that no two lanes meet in a bank. Entries lie 256 bytes apart (the second 128 are not used), so
 // that one byte permutation makes the address: the packed byte above the lane's own four-byte
 // offset. The reduction index may be permuted as long as both operands
-// agree, so a lane's 16 consecutive weights go into four mma's as they are and the matching
-// operand is 32 consecutive bytes of x. A block's 64 columns have one scale per row: its four
+// agree, so a lane's two runs of eight consecutive weights go into four mma's as they are and the
+// matching operand is two 16-byte pieces of x, a quad's pieces side by side. A block's 64 columns have one scale per row: its four
 // mma's start from zero and their result is added to the fp32 sum with one FMA per value, times
 // the scale.
 //
@@ -178,7 +195,7 @@ constexpr int mma_smem() {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -187,7 +204,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4],
                                               uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%10, %10, %10, %10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -227,15 +244,12 @@ __device__ __forceinline__ void load_scales(ScaleIn& in, const Weight& w, const 
   }
 }
 
-// x of rows 8 q + g, the 16 columns of lane t in block b
-template <int NT>
-__device__ __forceinline__ void load_x(uint4 (&v)[NT][2], const __half* const (&xp)[NT], int b) {
-#pragma unroll
-  for (int q = 0; q < NT; ++q) {
-    const uint4* p = reinterpret_cast<const uint4*>(xp[q] + b * 64);
-    v[q][0] = __ldg(p);
-    v[q][1] = __ldg(p + 1);
-  }
+// x of one row (xp: at lane t's columns), the 16 columns of lane t in block b: 8 t .. 8 t + 7 of
+// both halves
+__device__ __forceinline__ void load_x(uint4 (&v)[2], const __half* xp, int b) {
+  const uint4* p = reinterpret_cast<const uint4*>(xp + b * 64);
+  v[0] = __ldg(p);
+  v[1] = __ldg(p + 4);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -326,7 +340,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
 #pragma unroll
   for (int q = 0; q < NT; ++q)
     // rows past n_rows read the last one: their columns of the result are not stored
-    xp[q] = x + min(q * 8 + g, n_rows - 1) * ld_x + t * 16;
+    xp[q] = x + min(q * 8 + g, n_rows - 1) * ld_x + t * 8;
   int64_t e[2];  // of the tile whose scales are loaded: the flattened index of rows g and g + 8
   auto first_of = [&](int tile) {
     e[0] = row_of(tile, g) * w.n_in;
@@ -337,7 +351,8 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
   if (any) {
     first_of(first_tile);
     load_scales<GROUPED>(cur, w, sp, e, min(b_first + t, b_last - 1));
-    load_x<NT>(xv, xp, b_first);
+#pragma unroll
+    for (int q = 0; q < NT; ++q) load_x(xv[q], xp[q], b_first);
   }
   static_assert(32 * WARPS == 512, "two threads fill the 32 copies of a table entry");
   {
@@ -358,7 +373,7 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
   auto level_pair = [&](uint32_t v, int i) {
     return *reinterpret_cast<const uint32_t*>(lut_bytes + __byte_perm(v, lane4, 0x5504 | (i << 4)));
   };
-  const uint8_t* my_ring = rings + warp * (STAGES * STAGE_BYTES) + g * 128 + (t & 1) * 8;
+  const uint8_t* my_ring = rings + warp * (STAGES * STAGE_BYTES) + g * 128 + t * 4;
 
   int stage = 0;
   // every warp of a cluster makes the same rounds, those without a tile in the last one too
@@ -391,59 +406,47 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
         mine[h] = s * (1.0f / LEVEL_GAIN);
       }
       const uint8_t* st = my_ring + stage * STAGE_BYTES;
-      // block b + i of this step with its x in xv
-      auto block = [&](int i, const uint4 (&xb)[NT][2]) {
+      // block b + i of this step with its x in xv, which then gets that of block `ahead`
+      auto block = [&](int i, int ahead) {
         const float s0 = __shfl_sync(0xffffffffu, mine[0], i, 4);
         const float s1 = __shfl_sync(0xffffffffu, mine[1], i, 4);
-        const int at = ((2 * i + (t >> 1)) ^ g) << 4;
-        const uint2 wa2 = *reinterpret_cast<const uint2*>(st + at);
-        const uint2 wb2 = *reinterpret_cast<const uint2*>(st + 8 * 128 + at);
-        float c[NT][4];
+        uint32_t a[4][4];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const uint32_t wa = m < 2 ? wa2.x : wa2.y, wb = m < 2 ? wb2.x : wb2.y;
-          const uint32_t a[4] = {level_pair(wa, 2 * (m & 1)), level_pair(wb, 2 * (m & 1)),
-                                 level_pair(wa, 2 * (m & 1) + 1), level_pair(wb, 2 * (m & 1) + 1)};
+        for (int half = 0; half < 2; ++half) {
+          const uint8_t* at = st + (((2 * i + half) ^ g) << 4);
+          const uint32_t wa = *reinterpret_cast<const uint32_t*>(at);
+          const uint32_t wb = *reinterpret_cast<const uint32_t*>(at + 8 * 128);
 #pragma unroll
-          for (int q = 0; q < NT; ++q) {
-            const uint4& h = xb[q][m >> 1];
-            if (m == 0)
-              mma_f16_first(c[q], a, h.x, h.y);
-            else
-              mma_f16(c[q], a, m & 1 ? h.z : h.x, m & 1 ? h.w : h.y);
+          for (int m = 0; m < 2; ++m) {
+            a[2 * half + m][0] = level_pair(wa, 2 * m);
+            a[2 * half + m][1] = level_pair(wb, 2 * m);
+            a[2 * half + m][2] = level_pair(wa, 2 * m + 1);
+            a[2 * half + m][3] = level_pair(wb, 2 * m + 1);
           }
         }
 #pragma unroll
         for (int q = 0; q < NT; ++q) {
-          acc[q][0] = fmaf(s0, c[q][0], acc[q][0]);
-          acc[q][1] = fmaf(s0, c[q][1], acc[q][1]);
-          acc[q][2] = fmaf(s1, c[q][2], acc[q][2]);
-          acc[q][3] = fmaf(s1, c[q][3], acc[q][3]);
+          float c[4];
+          mma_f16_first(c, a[0], xv[q][0].x, xv[q][0].y);
+          mma_f16(c, a[1], xv[q][0].z, xv[q][0].w);
+          mma_f16(c, a[2], xv[q][1].x, xv[q][1].y);
+          mma_f16(c, a[3], xv[q][1].z, xv[q][1].w);
+          load_x(xv[q], xp[q], ahead);
+          acc[q][0] = fmaf(s0, c[0], acc[q][0]);
+          acc[q][1] = fmaf(s0, c[1], acc[q][1]);
+          acc[q][2] = fmaf(s1, c[2], acc[q][2]);
+          acc[q][3] = fmaf(s1, c[3], acc[q][3]);
         }
       };
-      const int ahead = more ? n_b : b;  // whose x is loaded behind this step's
+      const int behind = more ? n_b : b;  // whose x is loaded behind this step's
       if (b + STEP_BLOCKS <= b_last) {
-        uint4 xw[NT][2];
-        load_x<NT>(xw, xp, b + 1);
-        block(0, xv);
-        load_x<NT>(xv, xp, b + 2);
-        block(1, xw);
-        load_x<NT>(xw, xp, b + 3);
-        block(2, xv);
-        load_x<NT>(xv, xp, ahead);
-        block(3, xw);
+        block(0, b + 1);
+        block(1, b + 2);
+        block(2, b + 3);
+        block(3, behind);
       } else {  // the share's ragged end
 #pragma unroll 1
-        for (int i = 0; b + i < b_last; ++i) {
-          uint4 xw[NT][2];
-          load_x<NT>(xw, xp, b + i + 1 < b_last ? b + i + 1 : ahead);
-          block(i, xv);
-#pragma unroll
-          for (int q = 0; q < NT; ++q) {
-            xv[q][0] = xw[q][0];
-            xv[q][1] = xw[q][1];
-          }
-        }
+        for (int i = 0; b + i < b_last; ++i) block(i, b + i + 1 < b_last ? b + i + 1 : behind);
       }
       __syncwarp();  // the stage has been read; the next fetch may fill it
       stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -474,12 +477,9 @@ __global__ void __launch_bounds__(32 * WARPS, 1)
 #pragma unroll
         for (int q = 0; q < NT; ++q) {
           const int n = min(q * 8 + g, n_rows - 1);
-          float tv[2] = {};
-          for (int k = 0; k < ep.parts; ++k) {
-            const float* tp = ep.t + (static_cast<int64_t>(k) * n_rows + n) * ep.rank + j + 2 * t;
-            if (j + 2 * t < ep.rank) tv[0] += __ldcg(tp);
-            if (j + 2 * t + 1 < ep.rank) tv[1] += __ldcg(tp + 1);
-          }
+          const float* tp = ep.t + n * ep.rank + j + 2 * t;
+          const float tv[2] = {j + 2 * t < ep.rank ? __ldcg(tp) : 0.0f,
+                               j + 2 * t + 1 < ep.rank ? __ldcg(tp + 1) : 0.0f};
           uint32_t t_hi[2], t_lo[2];
           split_tf32(tv[0], t_hi[0], t_lo[0]);
           split_tf32(tv[1], t_hi[1], t_lo[1]);
@@ -649,12 +649,8 @@ __global__ void __launch_bounds__(256) nf4_matvec_any_kernel(const __half* __res
       if (n0 + n >= n_rows) break;
       float extra = 0.0f;
       if (ep.t != nullptr)
-        for (int j = lane; j < ep.rank; j += 32) {
-          float t = 0.0f;
-          for (int k = 0; k < ep.parts; ++k)
-            t += ep.t[(static_cast<int64_t>(k) * n_rows + n0 + n) * ep.rank + j];
-          extra = fmaf(t, ep.lora_b[o * ep.rank + j], extra);
-        }
+        for (int j = lane; j < ep.rank; j += 32)
+          extra = fmaf(ep.t[(n0 + n) * ep.rank + j], ep.lora_b[o * ep.rank + j], extra);
       float v = fmaf(ep.scaling, extra, acc[n]);
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
@@ -707,26 +703,35 @@ int talm_nf4_matvec(const uint16_t* x, int64_t ld_x, int64_t n_rows, const uint8
   const Weight w{packed, absmax8, absmax,      code,      absmax2, offset2,
                  levels, absmax_row0, blocksize, qblock2, w_rows,  w_cols};
   const __half* xh = reinterpret_cast<const __half*>(x);
-  int parts = 0;
   if (rank > 0) {
     LaunchTimer timer(TALM_KERNEL_ADAPTER_DOWN, stream);
     // as many parts as leave each a thousand columns
-    parts = static_cast<int>(w_cols / 1024 < 1 ? 1 : w_cols / 1024);
+    int parts = static_cast<int>(w_cols / 1024 < 1 ? 1 : w_cols / 1024);
     parts = parts < DOWN_PARTS ? parts : DOWN_PARTS;
-    const dim3 grid(static_cast<unsigned>((rank + 15) / 16), static_cast<unsigned>(parts), 1);
     const bool vec = w_cols % 4 == 0 && ld_x % 4 == 0 &&
                      (reinterpret_cast<uintptr_t>(x) & 7) == 0 &&
                      (reinterpret_cast<uintptr_t>(lora_a) & 15) == 0;
     auto kernel = n_rows <= 8 ? (vec ? adapter_down_kernel<1, true> : adapter_down_kernel<1, false>)
                               : (vec ? adapter_down_kernel<4, true> : adapter_down_kernel<4, false>);
-    kernel<<<grid, 32 * DOWN_WARPS, 0, stream>>>(xh, ld_x, lora_a, static_cast<int>(w_cols),
-                                                 static_cast<int>(n_rows),
-                                                 static_cast<int>(rank), down);
-    const int st = check_launch("adapter down kernel");
-    if (st != TALM_OK) return st;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((rank + 15) / 16), static_cast<unsigned>(parts), 1);
+    cfg.blockDim = dim3(32 * DOWN_WARPS, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = static_cast<unsigned>(parts);
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e =
+        cudaLaunchKernelEx(&cfg, kernel, xh, ld_x, lora_a, static_cast<int>(w_cols),
+                           static_cast<int>(n_rows), static_cast<int>(rank), down);
+    if (e != cudaSuccess)
+      return set_error(TALM_ECUDA, "adapter down kernel: %s", cudaGetErrorString(e));
   }
   const Epilogue ep{reinterpret_cast<const __half*>(bias), rank > 0 ? down : nullptr, lora_b,
-                    static_cast<int>(rank), parts, scaling};
+                    static_cast<int>(rank), scaling};
   LaunchTimer timer(TALM_KERNEL_NF4_MATVEC, stream);
   // The tensor-core kernel takes whole 64-column blocks of one scale each, on the boundaries of its
   // wide loads; anything else the byte-wise kernel.

@@ -18,7 +18,7 @@ that the patch takes over are that file's.
 
 import torch
 
-from . import _lib
+from . import _lib, qgroup
 from .engaged import FELL_BACK, ON, RAN
 from .state import DISABLED, fallback
 
@@ -58,10 +58,8 @@ def nf4_matvec(x, packed, absmax, blocksize, out=None, bias=None, adapter=None):
     GEMM would give, with the weight read packed, not rounded to fp16, and never written. packed:
     uint8 of any shape, absmax: fp32 [ceil(n / blocksize)], bias: fp16 [out], adapter: (lora_A,
     lora_B, scaling) as in `qgroup.matvec`; out: fp16 [rows, out] to write into."""
-    from . import qgroup
-
     n_cols = x.shape[-1]
-    if absmax.dtype != torch.float32 or packed.dtype != torch.uint8:
+    if absmax.dtype is not torch.float32 or packed.dtype is not torch.uint8:
         raise ValueError("packed must be uint8 and absmax fp32")
     packed, absmax = packed.contiguous(), absmax.contiguous()
     n = 2 * packed.numel()

@@ -384,7 +384,7 @@ def run_matvec(x, packed, absmax8, absmax, code, absmax2, offset2, levels, row0,
                              f"{n_cols} to {n_rows}")
         apart = apart or not lora_a.get_device() == lora_b.get_device() == device
         lora_a, lora_b = lora_a.contiguous(), lora_b.contiguous()
-        down = torch.empty(8 * n * rank, dtype=torch.float32, device=x.device)
+        down = torch.empty(n * rank, dtype=torch.float32, device=x.device)
         extra = (lora_a.data_ptr(), lora_b.data_ptr(), rank, scaling, down.data_ptr())
     bias_ptr = None
     if bias is not None:
