@@ -137,16 +137,15 @@ def _bytes(n, x):
 
 class _LoraBranch(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, base, lora_a, lora_b, scaling, seed, drop):
+    def forward(ctx, x, base, lora_a, lora_b, scaling, seed, drop, want_grad):
         n_in, n_out, rank = x.shape[-1], base.shape[-1], lora_a.shape[0]
         n_rows = base.numel() // n_out
         a, b = lora_a.contiguous(), lora_b.contiguous()
         xr, ld_x = _rows16(x, n_in)
         br, ld_b = _rows16(base, n_out)
         saved_bytes, work_bytes, ctx.work_bytes = _sizes(n_rows, n_in, n_out, rank)
-        need_x, _, need_a, need_b = ctx.needs_input_grad[:4]
         y = torch.empty(base.shape, dtype=torch.float16, device=x.device)
-        saved = _bytes(saved_bytes, x) if need_x or need_a or need_b else None
+        saved = _bytes(saved_bytes, x) if want_grad else None
         work = _bytes(work_bytes, x)
         with _lib.device_of(x):
             _lib.check(_lib.load().talm_lora_forward(
@@ -154,7 +153,7 @@ class _LoraBranch(torch.autograd.Function):
                 n_in, n_out, rank, scaling, None if seed is None else seed.data_ptr(), drop,
                 y.data_ptr(), None if saved is None else saved.data_ptr(), saved_bytes,
                 work.data_ptr(), work_bytes, _lib.raw_stream(x)), "talm_lora_forward")
-        if saved is not None:  # `saved` holds the adapter as it is now, in the kernels' parts
+        if want_grad:  # `saved` holds the adapter as it is now, in the kernels' parts
             ctx.scaling, ctx.drop, ctx.rank = scaling, drop, rank
             ctx.save_for_backward(x, seed, saved)
         RAN["lora"] += 1
@@ -186,7 +185,7 @@ class _LoraBranch(torch.autograd.Function):
                     dx.data_ptr() if need_x else None, da.data_ptr() if need_a else None,
                     db.data_ptr() if need_b else None, work.data_ptr(), ctx.work_bytes,
                     _lib.raw_stream(x)), "talm_lora_backward")
-        return dx, grad if need_base else None, da, db, None, None, None
+        return dx, grad if need_base else None, da, db, None, None, None, None
 
 
 def lora_branch(x, base, lora_A, lora_B, scaling, p=0.0, seed=None):
@@ -220,4 +219,6 @@ def lora_branch(x, base, lora_A, lora_B, scaling, p=0.0, seed=None):
         if seed is None:
             raise ValueError("dropout needs a seed (adapter.draw_seed)")
         _check_seed(seed, x)
-    return _LoraBranch.apply(x, base, lora_A, lora_B, float(scaling), seed, drop)
+    want_grad = torch.is_grad_enabled() and (x.requires_grad or lora_A.requires_grad
+                                             or lora_B.requires_grad)
+    return _LoraBranch.apply(x, base, lora_A, lora_B, float(scaling), seed, drop, want_grad)

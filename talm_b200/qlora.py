@@ -250,11 +250,11 @@ def train_step(model, optimizer, batch):
 
 @torch.no_grad()
 def generate(model, input_ids, new_tokens):
-    """Greedy decoding of `new_tokens` tokens after the prompts input_ids [B, S] (B at most 32 rows
-    of one length): one pass over the prompt, then one token of every row per pass with the
-    decoder's key-value cache. Passes of at most 32 tokens run under `qgroup.serving`: each 4-bit
-    projection is a few-row product with the packed weights, its adapter included. The model is
-    put into evaluation mode for the call. Returns [B, S + new_tokens]."""
+    """Greedy decoding of `new_tokens` tokens after the prompts input_ids [B, S] (rows of one length):
+    one pass over the prompt, then one token of every row per pass with the decoder's key-value
+    cache, under `qgroup.serving`: in passes of at most 32 tokens each 4-bit projection is a few-row
+    product with the packed weights, its adapter included. The model is in evaluation mode during
+    the call. Returns [B, S + new_tokens]."""
     was_training = model.training
     model.eval()
     try:

@@ -17,6 +17,7 @@ COMPONENTS = {
     "fused_head": "fused output head + cross-entropy (fused_head.py)",
     "qgroup": "grouped NF4 dequantisation of a decoder layer (qgroup.py)",
     "nf4_dequant": "per-projection NF4 dequantisation (nf4_dequant.py)",
+    "adapter": "LoRA branch and counter-based dropout (adapter.py)",
 }
 
 

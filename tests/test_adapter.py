@@ -441,6 +441,86 @@ def test_branch_same_bits_on_streams_and_in_graphs():
     assert all(torch.equal(u, v) for u, v in zip(half, (graphs[1][2], *graphs[1][3])))
 
 
+@pytest.mark.gpu
+def test_branch_saves_its_input_and_rank_wide_operands_only():
+    """What a call keeps for its backward: x as it is (changing it in place is an error, as is
+    changing the seed), the rank-wide parts, no mask and no dropped copy; nothing without grad."""
+    x, base, a, b, g = _branch_inputs(4096, 1536, 64, 16, 3)
+    a.requires_grad_()
+    b.requires_grad_()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        y = adapter.lora_branch(x, base, a, b, 1.0, 0.1, _seed(1))
+    assert y.grad_fn is None
+    assert torch.cuda.memory_allocated() - before <= y.numel() * 2 + 4096
+    del y
+    seed = _seed(1)
+    before = torch.cuda.memory_allocated()
+    y = adapter.lora_branch(x, base, a, b, 1.0, 0.1, seed)
+    kept = torch.cuda.memory_allocated() - before - y.numel() * 2
+    # t's parts (128 bytes a row), the parts of A and B for the backward pass
+    assert kept <= 4096 * 128 + 16 * 2 * 2 * 64 + 1536 * 128 + (1 << 15) < x.numel() // 8
+    seed.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward(g)
+    y = adapter.lora_branch(x, base, a, b, 1.0, 0.1, _seed(1))
+    x.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward(g)
+
+
+@pytest.mark.gpu
+def test_branch_past_32_bit_offsets():
+    """Rows whose elements lie beyond 2^32: their masks and products, forward and backward."""
+    cols, rank = 8960, 4
+    rows = (1 << 32) // cols + 200
+    g = torch.Generator("cuda").manual_seed(2)
+    x = torch.empty(rows, cols, dtype=torch.float16, device="cuda")
+    x[:1000].normal_(generator=g)
+    at = [0, 1, rows - 150, rows - 1]
+    for i in at:
+        x[i].normal_(generator=g)
+    x[1000:rows - 200] = 0
+    x[rows - 200:].normal_(generator=g)
+    base = torch.zeros(rows, 8, dtype=torch.float16, device="cuda")
+    a = (torch.rand(rank, cols, generator=g, device="cuda") - 0.5) * 0.02
+    b = torch.randn(8, rank, generator=g, device="cuda")
+    dy = torch.randn(rows, 8, generator=g, device="cuda").half()
+    x.requires_grad_()
+    y = adapter.lora_branch(x, base, a, b, 1.0, 0.3, _seed(8))
+    dx, = torch.autograd.grad(y, x, dy)
+    for i in at:
+        kept, factor = oracle.keep_mask(cols, 0.3, 8, first=i * cols)
+        m = torch.from_numpy(kept).cuda().double() * factor
+        want = ((x[i].double() * m) @ a.double().t()) @ b.double().t()
+        scale = ((x[i].double() * m).abs() @ a.double().abs().t()) @ b.double().abs().t()
+        assert ((y[i].double() - want).abs() <= 2.0 ** -11 * want.abs() + 2.0 ** -16 * scale).all()
+        want = (dy[i].double() @ b.double() @ a.double()) * m
+        scale = (dy[i].double().abs() @ b.double().abs() @ a.double().abs()) * m
+        err = (dx[i].double() - want).abs()
+        assert (err <= 2.0 ** -11 * want.abs() + 2.0 ** -25 + 2.0 ** -16 * scale).all()
+
+
+@pytest.mark.gpu
+def test_branches_on_two_streams_at_once():
+    """Calls that overlap on the GPU: each has workspaces of its own."""
+    cases = [_branch_inputs(1500, 1536, 520, 16, 4), _branch_inputs(900, 520, 1536, 64, 5)]
+    want = [_run_branch(*c[:4], 1.0, 0.2, 3, c[4]) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, (c, stream) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(stream):
+                got[i].append(_run_branch(*c[:4], 1.0, 0.2, 3, c[4]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for out in got[i]:
+            assert all(torch.equal(u, v) for u, v in zip(want[i], out))
+    assert _lib.device_status() == 0
+
+
 # ------------------------------------------------------------------------------------------
 # the branch in its module and in the training step
 # ------------------------------------------------------------------------------------------
