@@ -49,7 +49,9 @@ __device__ __forceinline__ uint32_t scale2(uint32_t v, float f, __nv_bfloat16) {
 }
 
 // The flattened tensor on 16-byte boundaries: a thread takes UNROLL groups of eight elements, their
-// loads first.
+// loads first. Bound by HBM: 16384 x 8960 bf16, forward and backward, 206 us (1.17 GB, 5.7 TB/s, 0.87 of
+// the measured copy); a group costs 14 multiplications and about 100 operations in all, 46 % of the
+// ALU's rate at that speed (10 rounds, or 32 bits per element, would be the bound themselves).
 template <class T, int UNROLL>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, int64_t n,
                                                       Dropout d, T* __restrict__ y) {
@@ -167,6 +169,11 @@ int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, co
 // reduction (and per adapter row for A and B). Where both operands are fp32 and the result is fp16 (up)
 // they are two bf16 parts without scale, and the product of the two small ones is left out: under
 // 2^-16 of each term, a sixteenth of the result's own rounding.
+//
+// Measured on one B200, forward and backward replayed in a graph: q_proj of 2048 rows, rank 16, 42 us (38
+// MB; ten launches of about 4 us each are the bound), 16384 x 1536 to 8960, rank 64, 313 us (1.04 GB,
+// 3.3 TB/s, 0.51 of the measured copy: g is read twice, once for dt and once for dB, 45 us that the
+// floor does not have; the passes themselves run at 0.8 to 0.95).
 // ------------------------------------------------------------------------------------------
 struct Shape {
   int64_t n_rows, n_in, n_out;

@@ -16,6 +16,11 @@
 //   warps 4-19  epilogue: four groups of 128 threads, half a box each: TMEM -> fp32 -> + base (or
 //               mask) -> fp16, in place in the box's slot
 // Every wait is bounded; a wait that gives up ends the CTA's roles and records TALM_ETIMEOUT.
+//
+// Measured: ADD 16384 x 8960 at rank 64 100 us (587 MB, 5.9 TB/s, 0.90 of the measured copy); with T
+// loaded three parts wide and two stages it was 118 us, the MMA issuer waiting for T a third of the
+// time. MASK 16384 x 1536 25 us: 7.7 us of bytes; the generator and the conversions of 128 x 128 outputs
+// per CTA take the rest.
 #pragma once
 
 #include "adapter_common.cuh"
@@ -354,6 +359,11 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
 //                 sums, which are not rounded to nearest, stay short by that.
 //   warps 12-19   (MASK) drop X in shared memory before it is multiplied: a 16-byte piece is one
 //                 group of the generator
+//
+// Measured at rank 64: dB of 16384 x 8960 47 us (294 MB, 6.2 TB/s, 0.95 of the measured copy), dt 55 us
+// (its W, 2.3 MB, is read again by every 128 rows), with the dropout of 16384 x 1536 t 28 us and dA 24
+// us (7.7 us of bytes: the generator, one CTA per SM). The mma.sync form of the same sums took 276,
+// 171, 70 and 74 us.
 namespace sums {
 
 constexpr int TILE = 128;

@@ -8,6 +8,12 @@
 // an fp32 absmax, or fp32(fp32(code2[absmax8] * absmax2) + offset2) as in nf4.cu. Products and
 // sums are fp32 and the result is rounded once: the weight itself is not rounded to fp16, which
 // the dequantised copy of a weight is.
+//
+// Measured on one B200, calls replayed in a graph over two sets of inputs (29 MB: L2 holds them):
+// gate + up of the Qwen2.5-1.5B layer (17920 x 1536) for one row 7.9 us (14.2 MB, 1.8 TB/s; the floor
+// at the measured copy bandwidth is 2.2 us), k_proj 3.6 us, down_proj for 13 rows 10.4 us, down_proj
+// for 32 rows with an adapter of rank 64 18.1 us. Dequantising the layer and multiplying moves 117 MB
+// for the same 23 MB of weights.
 #include "common.cuh"
 
 namespace talm {
