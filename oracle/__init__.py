@@ -14,3 +14,13 @@ Pinning: both are checked against golden vectors that tests/golden/make_golden.p
 importing the reference's own Python functions (`_nf4_manual`, `reference_head`,
 `_head_reference`, `labelled_first`, `LayerGroup` packing) on CPU.
 """
+
+import multiprocessing
+import multiprocessing.util
+import time
+
+if multiprocessing.parent_process() is not None:
+    # A rank of a CPU test puts its tensors on a queue and exits, but the parent fetches them by file
+    # descriptor from the sender: a rank that has already gone leaves it without. The sender stays
+    # for a moment after its queue has been flushed (finalizers of a lower priority run later).
+    multiprocessing.util.Finalize(None, time.sleep, args=(3,), exitpriority=-100)
