@@ -172,20 +172,25 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 // weight as the 16-row operand, up to 8 NT rows of x as the n operand).
 //
 // A warp takes tiles of 16 weight rows; lane (g, t) = (lane / 4, lane % 4) reads 8 packed bytes of
-// rows g and g + 8 per block (a quad reads a row's 32 bytes: lane t bytes 4 t .. 4 t + 3 of both
-// halves) and turns each byte into the fp16
-// pair of its two levels by one shared-memory read: a table of 256 pairs, one copy per lane, so
-// that no two lanes meet in a bank. Entries lie 256 bytes apart (the second 128 are not used), so
-// that one byte permutation makes the address: the packed byte above the lane's own four-byte
-// offset. The reduction index may be permuted as long as both operands
+// rows g and g + 8 per block (a quad reads a row's 32 bytes, lane t bytes 4 t .. 4 t + 3 of both
+// halves) and turns each byte into the fp16 pair of its two levels by one shared-memory read: a table
+// of 256 pairs, one copy per lane, so that no two lanes meet in a bank. Entries lie 256 bytes apart
+// (the second 128 are not used), so that one byte permutation makes the address: the packed byte
+// above the lane's own four-byte offset. The reduction index may be permuted as long as both operands
 // agree, so a lane's two runs of eight consecutive weights go into four mma's as they are and the
-// matching operand is two 16-byte pieces of x, a quad's pieces side by side. A block's 64 columns have one scale per row: its four
-// mma's start from zero and their result is added to the fp32 sum with one FMA per value, times
-// the scale.
+// matching operand is two 16-byte pieces of x, a quad's pieces side by side. A block's 64 columns have
+// one scale per row: its four mma's start from zero and their result is added to the fp32 sum with one
+// FMA per value, times the scale.
 //
 // The table holds fp16(LEVEL_GAIN * level) and the scale takes 1 / LEVEL_GAIN: the gain is the one
 // in [1, 2) whose 16 rounded levels are nearest to the true ones (6.2e-5 in the mean square
 // against 1.56e-4 without it and 2.1e-4 for the result's own rounding).
+//
+// What bounds it (one row of gate + up, cycles of an instrumented copy): 2.9k of 12.4k are set-up
+// (first loads, the table), 8.7k the 12 blocks of each of 16 warps, 45 per block and warp: the
+// table's 16 shared-memory reads per 1024 weights and the reads of x and of the ring take 24, the
+// rest is their latency at four warps per scheduler. 32 warps of 64 registers were slower (9.7 us
+// against 7.9, spills), and so were table entries 128 bytes apart (two operations per address, 8.8).
 // ------------------------------------------------------------------------------------------
 constexpr int WARPS = 16;
 constexpr int STEP_BLOCKS = 4;  // blocks of 64 columns that a warp loads ahead

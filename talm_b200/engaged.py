@@ -1,7 +1,8 @@
 """Host counters of which fast paths ran (mirror of solution/engaged.py:65-68).
 
 The keys are the reference's: `vchunk`, `compact` (fused head), `group`, `split` (grouped NF4
-dequantisation), `nf4_dequant` (per-projection NF4). Plain Python integers bumped where a call
+dequantisation), `nf4_dequant` (per-projection NF4); beside them `matvec` (few-row products), `lora`
+and `dropout` (adapter.py). Plain Python integers bumped where a call
 takes its fast path or declines it; no device sync, no kernel.
 """
 
