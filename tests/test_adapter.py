@@ -332,6 +332,29 @@ def test_branch_has_dropouts_mask_and_the_formulas_gradient():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rank", [16, 32, 64])
+@pytest.mark.parametrize("p", [0.0, 0.1])
+def test_branch_of_many_tiles(rank, p):
+    """Enough rows that every CTA walks over many tiles and stages of its rings several times, against
+    fp64 products on the GPU: relative norms within half a step of fp16 (y, dx) and 2^-20 (dA, dB)."""
+    x, base, a, b, g = _branch_inputs(20000, 1032, 1160, rank, 17)
+    y, dx, da, db = _run_branch(x, base, a, b, 0.5, p, 33, g)
+    mask = adapter.dropout(torch.ones_like(x), p, _seed(33)).bool().double()
+    mask *= 32768 / (32768 - adapter.drop_threshold(p))
+    a64, b64, g64 = a.double(), b.double(), g.double()
+    xd = x.double() * mask
+    t, dt = xd @ a64.t(), 0.5 * g64 @ b64
+    for got, want, tol in ((y, base.double() + 0.5 * t @ b64.t(), 2.0 ** -11),
+                           (dx, (dt @ a64) * mask, 2.0 ** -11), (da, dt.t() @ xd, 2.0 ** -20),
+                           (db, 0.5 * g64.t() @ t, 2.0 ** -20)):
+        rows = (got.double() - want).norm(dim=1) / want.norm(dim=1).clamp(min=1e-30)
+        assert float(rows.max()) < tol, float(rows.max())
+    again = _run_branch(x, base, a, b, 0.5, p, 33, g)
+    assert all(torch.equal(u, v) for u, v in zip((y, dx, da, db), again))
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
 def test_branch_layouts():
     """Leading dimensions, rows of wider tensors, odd offsets and strides, broadcast gradients, a
     frozen input or adapter."""

@@ -182,6 +182,17 @@ def test_matches_the_oracle(rows, shape, form):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 9, 32])
+@pytest.mark.parametrize("shape", [(60011, 64), (40000, 192), (17920, 1536)],
+                         ids=lambda s: f"{s[0]}x{s[1]}")
+def test_many_tiles(shape, rows):
+    """More tiles than the GPU's warps: every warp walks over several, its ring many times around."""
+    for form, rank in (("group", 0), ("absmax", 16)):
+        c = _Case(rows, *shape, form, seed=rows + shape[1], bias=True, rank=rank, block=64, row0=5)
+        c.check(c.run())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("block", [2, 6, 64, 96, 128, 256, 4096])
 @pytest.mark.parametrize("n_in", [64, 192, 250])
 def test_block_sizes(block, n_in):
