@@ -558,20 +558,29 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
     const uint64_t key = static_cast<uint64_t>(__ldg(p.drop.seed));
     const uint32_t bias2 = keep_bias2(p.drop.drop);
     constexpr int U = X_BYTES / 16 / (32 * MASK_WARPS);  // pieces of a thread
+    constexpr int LINES = 32 * MASK_WARPS / 8;           // between a thread's pieces
+    // A piece is a group of eight columns of line id / 8 + u * LINES of the stage; a line is 128 bytes:
+    // a row of INNER's 64 columns; OUTER: row + 64 * (column group). q[u]: the group's number, which
+    // moves on by a constant from stage to stage.
+    const int64_t row_groups = p.n_cols / 8;
+    int64_t q[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int line = id / 8 + u * LINES;
+      q[u] = OUTER ? (static_cast<int64_t>(s0) * 64 + (line & 63)) * row_groups + origin / 8 +
+                         (line >> 6) * 8 + (id & 7)
+                   : (origin + line) * row_groups + s0 * 8 + (id & 7);
+    }
     for (int i = 0; i < n_steps; ++i) {
       const int st = i % STAGES;
       uint8_t* x = x_s + st * X_BYTES;
       uint32_t w[U][4];  // the masks while the stage is on its way
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int e = u * (32 * MASK_WARPS) + id, line = e >> 3, c = e & 7;
-        // a line is 128 bytes: a row of INNER's 64 columns; OUTER: row + 64 * (column group)
-        const int64_t row = OUTER ? static_cast<int64_t>(s0 + i) * 64 + (line & 63) : origin + line;
-        const int64_t col = OUTER ? origin + (line >> 6) * 64 + c * 8
-                                  : static_cast<int64_t>(s0 + i) * 64 + c * 8;
-        philox(static_cast<uint64_t>((row * p.n_cols + col) >> 3), key, w[u]);
+        philox(static_cast<uint64_t>(q[u]), key, w[u]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) w[u][k] = keep_mask2(w[u][k], bias2);
+        q[u] += OUTER ? 64 * row_groups : 8;
       }
       const bool ok = mbar_wait(&ctl->full[st], (i / STAGES) & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) break;
