@@ -463,21 +463,14 @@ struct BackwardWork {
   }
 };
 
-// t or dt of an activation: the inner sums and the operands made of them.
+// The operands made of the inner sums of an activation.
 template <int RP>
-int run_inner(const __half* x, int64_t ld, int64_t n_rows, int64_t n_cols, const Rows& rows,
-              const Dropout& d, float* part, float factor, const TParts& out,
-              cudaStream_t stream) {
-  const int st = d.drop ? sums::launch<RP, false, true>(x, ld, n_rows, n_cols, rows.parts,
-                                                        rows.down, d, part, stream)
-                        : sums::launch<RP, false, false>(x, ld, n_rows, n_cols, rows.parts,
-                                                         rows.down, d, part, stream);
-  if (st != TALM_OK) return st;
+int make_t_parts(const float* part, int splits, int64_t n_rows, float factor, const TParts& out,
+                 cudaStream_t stream) {
   constexpr int smem = 128 * (RP + 1) * 4;
   static_assert(smem <= 48 * 1024, "no opt-in");
   return launch_dependent(t_parts_kernel<RP>, static_cast<unsigned>((n_rows + 127) / 128),
-                          T_THREADS, smem, stream, part,
-                          sums::Plan(false, d.drop != 0, n_rows, n_cols).splits, n_rows, factor, out);
+                          T_THREADS, smem, stream, part, splits, n_rows, factor, out);
 }
 
 template <int RP>
@@ -497,7 +490,13 @@ int run_forward(const __half* x, int64_t ld_x, const __half* base, int64_t ld_ba
                             PREP_THREADS, smem, stream, ma, mb, of_a, of_b, s.rank);
   const TParts t{w.t_cat, saved ? keep.t.pair : nullptr, saved ? keep.t.down : nullptr};
   if (st == TALM_OK)
-    st = run_inner<RP>(x, ld_x, s.n_rows, s.n_in, w.a_rows, d, w.part, d.factor, t, stream);
+    st = d.drop ? sums::launch<RP, false, true>(x, ld_x, s.n_rows, s.n_in, w.a_rows.parts,
+                                                w.a_rows.down, d, w.part, stream)
+                : sums::launch<RP, false, false>(x, ld_x, s.n_rows, s.n_in, w.a_rows.parts,
+                                                 w.a_rows.down, d, w.part, stream);
+  if (st == TALM_OK)
+    st = make_t_parts<RP>(w.part, sums::Plan(false, d.drop != 0, s.n_rows, s.n_in).splits,
+                          s.n_rows, d.factor, t, stream);
   if (st != TALM_OK) return st;
   return up::launch<RP, false>(w.t_cat, w.b_cat, base, ld_base, y, s.n_rows, s.n_out,
                                            scaling, d, stream);
@@ -511,12 +510,19 @@ int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, c
   const Saved keep(const_cast<void*>(saved), s, RP);
   const Dropout none{nullptr, 0, 1.0f};
   int st = TALM_OK;
-  if (da || dx)
-    st = run_inner<RP>(g, ld_g, s.n_rows, s.n_out, keep.b_rows, none, w.t_part, scaling, w.dt,
-                       stream);
-  if (db && st == TALM_OK)
+  const bool want_dt = da || dx;
+  if (want_dt && db)
+    st = sums::launch_pair<RP>(g, ld_g, s.n_rows, s.n_out, keep.b_rows.parts, keep.b_rows.down,
+                               w.t_part, keep.t.pair, keep.t.down, w.b_part, stream);
+  else if (want_dt)
+    st = sums::launch<RP, false, false>(g, ld_g, s.n_rows, s.n_out, keep.b_rows.parts,
+                                        keep.b_rows.down, none, w.t_part, stream);
+  else
     st = sums::launch<RP, true, false>(g, ld_g, s.n_rows, s.n_out, keep.t.pair, keep.t.down, none,
                                        w.b_part, stream);
+  if (want_dt && st == TALM_OK)
+    st = make_t_parts<RP>(w.t_part, sums::Plan(false, false, s.n_rows, s.n_out).splits, s.n_rows,
+                          scaling, w.dt, stream);
   if (da && st == TALM_OK)
     st = d.drop ? sums::launch<RP, true, true>(x, ld_x, s.n_rows, s.n_in, w.dt.pair, w.dt.down, d,
                                                w.a_part, stream)

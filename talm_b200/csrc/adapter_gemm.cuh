@@ -404,10 +404,10 @@ struct Params {
   Dropout drop;
 };
 
+// One CTA: the tile's split `split`.
 template <int RP, bool OUTER, bool MASK>
-__global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
-    sums_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_o,
-                Params p) {
+__device__ __forceinline__ void sums_cta(const CUtensorMap& tm_x, const CUtensorMap& tm_o,
+                                         const Params& p, int tile, int split) {
   constexpr int STAGES = stages<RP, OUTER, MASK>();
   constexpr int O_BYTES = other_bytes<RP, OUTER>();
   constexpr int N = 2 * RP;
@@ -419,8 +419,8 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
   uint8_t* o_s = x_s + STAGES * X_BYTES;
   Ctl* ctl = reinterpret_cast<Ctl*>(o_s + STAGES * O_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t origin = static_cast<int64_t>(blockIdx.x) * TILE;  // first row / column
-  const int s0 = blockIdx.y * p.steps_per_split;
+  const int64_t origin = static_cast<int64_t>(tile) * TILE;  // first row / column
+  const int s0 = split * p.steps_per_split;
   const int n_steps = min(p.steps, s0 + p.steps_per_split) - s0;  // at least one
 
   if (threadIdx.x == 0) {
@@ -542,12 +542,12 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
     const int64_t at = origin + r;
     if (ok && at < (OUTER ? p.n_cols : p.n_rows)) {
       if (OUTER) {
-        float* out = p.part + (static_cast<int64_t>(blockIdx.y) * RP + q * HR) * p.n_cols + at;
+        float* out = p.part + (static_cast<int64_t>(split) * RP + q * HR) * p.n_cols + at;
 #pragma unroll
         for (int j = 0; j < HR; ++j) out[static_cast<int64_t>(j) * p.n_cols] = acc[j];
       } else {
         float4* out = reinterpret_cast<float4*>(
-            p.part + (static_cast<int64_t>(blockIdx.y) * p.n_rows + at) * RP + q * HR);
+            p.part + (static_cast<int64_t>(split) * p.n_rows + at) * RP + q * HR);
 #pragma unroll
         for (int j = 0; j < HR; j += 4)
           out[j / 4] = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
@@ -607,10 +607,35 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
   if (warp == 1) tmem_dealloc(tmem_base, 2 * COLS);
 }
 
+template <int RP, bool OUTER, bool MASK>
+__global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
+    sums_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_o,
+                const __grid_constant__ Params p) {
+  sums_cta<RP, OUTER, MASK>(tm_x, tm_o, p, blockIdx.x, blockIdx.y);
+}
+
+// dt and dB, which read the same gradient and do not wait for one another, in one launch: the first
+// `inner_ctas` CTAs work on dt.
+template <int RP>
+__global__ void __launch_bounds__(threads(false), 2)
+    sums_pair_kernel(const __grid_constant__ CUtensorMap in_x,
+                     const __grid_constant__ CUtensorMap in_o, const __grid_constant__ Params in_p,
+                     int inner_ctas, int inner_tiles, const __grid_constant__ CUtensorMap out_x,
+                     const __grid_constant__ CUtensorMap out_o,
+                     const __grid_constant__ Params out_p, int outer_tiles) {
+  const int id = blockIdx.x;
+  if (id < inner_ctas)
+    sums_cta<RP, false, false>(in_x, in_o, in_p, id % inner_tiles, id / inner_tiles);
+  else
+    sums_cta<RP, true, false>(out_x, out_o, out_p, (id - inner_ctas) % outer_tiles,
+                              (id - inner_ctas) / outer_tiles);
+}
+
 // How the reduction is divided: as many CTAs as 148 SMs hold at a time (two of them, one with its mask
 // warps), two blocks of 128 (which share a scale) for a CTA at least.
 struct Plan {
-  int tiles, steps, steps_per_split, splits;
+  int tiles = 0, steps = 0, steps_per_split = 0, splits = 0;
+  Plan() = default;
   Plan(bool outer, bool mask, int64_t n_rows, int64_t n_cols) {
     tiles = static_cast<int>(((outer ? n_cols : n_rows) + TILE - 1) / TILE);
     const int64_t length = outer ? n_rows : n_cols;
@@ -626,7 +651,28 @@ struct Plan {
   }
 };
 
-// x: the activation; other: W parts [2 RP, n_cols] (INNER) or T parts [n_rows, pair_width] (OUTER)
+// The arguments of a launch. x: the activation; other: W parts [2 RP, n_cols] (INNER) or T parts
+// [n_rows, pair_width] (OUTER).
+struct Call {
+  CUtensorMap tm_x, tm_o;
+  Params p;
+  Plan plan;
+};
+
+template <int RP, bool OUTER, bool MASK>
+int make_call(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void* other,
+              const float* down, const Dropout& d, float* part, Call* c) {
+  c->plan = Plan(OUTER, MASK, n_rows, n_cols);
+  c->p = Params{n_rows, static_cast<int>(n_cols), c->plan.steps, c->plan.steps_per_split,
+                down,   part,                     d};
+  int st = talm_make_tmap_2d_f16(&c->tm_x, x, n_cols, n_rows, ld, 64, OUTER ? 64 : TILE);
+  if (st == TALM_OK)
+    st = OUTER ? talm_make_tmap_2d_f16(&c->tm_o, other, pair_width(RP), n_rows, pair_width(RP), 64,
+                                       64)
+               : talm_make_tmap_2d_f16(&c->tm_o, other, n_cols, 2 * RP, n_cols, 64, 2 * RP);
+  return st;
+}
+
 template <int RP, bool OUTER, bool MASK>
 int launch(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void* other,
            const float* down, const Dropout& d, float* part, cudaStream_t stream) {
@@ -637,17 +683,36 @@ int launch(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void
   const cudaError_t e =
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
-  const Plan plan(OUTER, MASK, n_rows, n_cols);
-  CUtensorMap tm_x, tm_o;
-  int st = talm_make_tmap_2d_f16(&tm_x, x, n_cols, n_rows, ld, 64, OUTER ? 64 : TILE);
-  if (st == TALM_OK)
-    st = OUTER ? talm_make_tmap_2d_f16(&tm_o, other, pair_width(RP), n_rows, pair_width(RP), 64, 64)
-               : talm_make_tmap_2d_f16(&tm_o, other, n_cols, 2 * RP, n_cols, 64, 2 * RP);
+  Call c;
+  const int st = make_call<RP, OUTER, MASK>(x, ld, n_rows, n_cols, other, down, d, part, &c);
   if (st != TALM_OK) return st;
-  const Params p{n_rows, static_cast<int>(n_cols), plan.steps, plan.steps_per_split, down, part, d};
   return launch_dependent(
-      kernel, dim3(static_cast<unsigned>(plan.tiles), static_cast<unsigned>(plan.splits), 1),
-      threads(MASK), smem, stream, tm_x, tm_o, p);
+      kernel, dim3(static_cast<unsigned>(c.plan.tiles), static_cast<unsigned>(c.plan.splits), 1),
+      threads(MASK), smem, stream, c.tm_x, c.tm_o, c.p);
+}
+
+// dt = g B and dB = g^T t (see sums_pair_kernel).
+template <int RP>
+int launch_pair(const void* g, int64_t ld, int64_t n_rows, int64_t n_cols, const void* w_parts,
+                const float* w_down, float* dt_part, const void* t_parts, const float* t_down,
+                float* db_part, cudaStream_t stream) {
+  constexpr int a = smem_bytes<RP, false, false>(), b = smem_bytes<RP, true, false>();
+  constexpr int smem = a > b ? a : b;
+  auto kernel = sums_pair_kernel<RP>;
+  const cudaError_t e =
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
+  const Dropout none{nullptr, 0, 1.0f};
+  Call in, out;
+  int st = make_call<RP, false, false>(g, ld, n_rows, n_cols, w_parts, w_down, none, dt_part, &in);
+  if (st == TALM_OK)
+    st = make_call<RP, true, false>(g, ld, n_rows, n_cols, t_parts, t_down, none, db_part, &out);
+  if (st != TALM_OK) return st;
+  const int inner = in.plan.tiles * in.plan.splits;
+  return launch_dependent(kernel,
+                          dim3(static_cast<unsigned>(inner + out.plan.tiles * out.plan.splits)),
+                          threads(false), smem, stream, in.tm_x, in.tm_o, in.p, inner,
+                          in.plan.tiles, out.tm_x, out.tm_o, out.p, out.plan.tiles);
 }
 
 }  // namespace sums
