@@ -748,7 +748,7 @@ int talm_nf4_matvec(const uint16_t* x, int64_t ld_x, int64_t n_rows, const uint8
   // wide loads; anything else the byte-wise kernel.
   const int shift = log2_exact(blocksize), shift2 = absmax8 ? log2_exact(qblock2) : 0;
   if (w_cols % 64 == 0 && shift >= 6 && shift2 >= 0 && ld_x % 8 == 0 &&
-      (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(packed) & 7) == 0) {
+      ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(packed)) & 15) == 0) {
     const Split sp{0, 1, static_cast<int>((w_rows + 15) / 16), static_cast<int>(w_cols / 64), shift,
                    shift2};
     __half* yh = reinterpret_cast<__half*>(y);

@@ -232,6 +232,20 @@ def test_strides_alignment_and_untouched_neighbours():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("offset", [16, 8, 4, 1])
+def test_packed_bytes_on_any_boundary(offset):
+    """The wide copies want rows on 16-byte boundaries; weights that start elsewhere (behind an odd
+    one in the same buffer) take the other kernel."""
+    for rows, shape in ((1, (37, 128)), (9, (256, 1536))):
+        c = _Case(rows, *shape, "group", seed=offset, bias=True, rank=8)
+        whole = torch.empty(c.packed.numel() + 32, dtype=torch.uint8, device="cuda")
+        assert whole.data_ptr() % 16 == 0
+        moved = whole[offset:offset + c.packed.numel()]
+        c.packed = moved.copy_(c.packed)
+        c.check(c.run())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows", [1, 9])
 def test_extreme_values(rows):
     """Zero scales, an input of zeros, the largest fp16 inputs (an infinite result where the sum
