@@ -413,6 +413,8 @@ def launch_matvec(x, packed, absmax8, code, absmax2, offset2, levels, out, row0,
     index of its first absmax row, which the second level is indexed by), into `out` [rows, n_rows]
     fp16. The raw form of `matvec`, as `launch` is of `dequantize_all`; adapter = (lora_A [r,
     n_cols], lora_B [n_rows, r], scaling), fp32."""
+    if qblock < 1 or qblock2 < 1 or row0 < 0 or n_rows < 0:
+        raise ValueError("block sizes must be positive, row counts and indices not negative")
     n = n_rows * n_cols
     blocks = -(-n // qblock)
     if 2 * packed.numel() < n or absmax8.numel() < blocks or code.numel() != 256 or (

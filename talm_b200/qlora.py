@@ -55,9 +55,10 @@ class LoraLinear(torch.nn.Module):
 
     With `fused` the branch runs through `adapter.lora_branch` (fp32 adapter weights and sums, one
     rounding, dropout from a counter: other masks than torch's for the same torch seed, no mask
-    and no dropped copy kept); a branch that it does not take (another type, a rank over 64) through
-    `adapter.dropout` and the products above. Under `qgroup.serving`, a call without gradients and
-    without dropout on a few rows is one product with base, bias and adapter in it."""
+    and no dropped copy kept); a branch that it does not take (another type, an adapter cast to
+    fp16, a rank over 64) through `adapter.dropout` and the products above. Under `qgroup.serving`,
+    a call without gradients and without dropout on a few rows is one product with base, bias and
+    (fp32) adapter in it."""
 
     def __init__(self, base, r, alpha, dropout, generator=None, b_std=0.0, fused=False):
         super().__init__()
@@ -83,13 +84,14 @@ class LoraLinear(torch.nn.Module):
 
     def forward(self, x):
         p = self.dropout if self.training else 0.0
-        if p == 0 and self.r <= adapter.MAX_RANK and isinstance(self.base, nf4_format.NF4Linear) \
-                and qgroup.takes_matvec(x):
+        fp32 = self.lora_A.dtype is torch.float32 is self.lora_B.dtype  # what the kernels take
+        if p == 0 and fp32 and self.r <= adapter.MAX_RANK \
+                and isinstance(self.base, nf4_format.NF4Linear) and qgroup.takes_matvec(x):
             return self.base.matvec(x, (self.lora_A, self.lora_B, self.scaling))
         out = self.base(x)
         if self.fused:
             seed = adapter.draw_seed(x.device) if p > 0 else None
-            if adapter.branch_takes(x, out, self.r):
+            if fp32 and adapter.branch_takes(x, out, self.r):
                 return adapter.lora_branch(x, out, self.lora_A, self.lora_B, self.scaling, p, seed)
             xd = adapter.dropout(x, p, seed) if p > 0 else x
         else:

@@ -547,6 +547,46 @@ def test_branches_on_two_streams_at_once():
 # ------------------------------------------------------------------------------------------
 # the branch in its module and in the training step
 # ------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_branch_captured_behind_copies_and_joined_streams():
+    """Captured behind a copy (a node that is no kernel) and behind two streams that have been
+    joined (two nodes), forward and backward apart on their own graphs' inputs."""
+    x, base, a, b, g = _branch_inputs(140, 136, 264, 8, 21)
+    want = _run_branch(x, base, a, b, 2.0, 0.1, 31, g)
+    seed = _seed(31)
+    leaves = [torch.zeros_like(t).requires_grad_() for t in (x, base, a, b)]
+    gs, doubled = torch.zeros_like(g), torch.zeros_like(g)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.no_grad():
+            for t, v in zip(leaves, (x, base, a, b)):
+                t.copy_(v)
+            with torch.cuda.stream(side):
+                gs.copy_(g)
+        torch.cuda.current_stream().wait_stream(side)
+        y = adapter.lora_branch(*leaves, 2.0, 0.1, seed)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            doubled.copy_(gs).mul_(2)
+        torch.cuda.current_stream().wait_stream(side)
+        grads = torch.autograd.grad(y, (leaves[0], leaves[2], leaves[3]), gs)
+        after = y.detach().clone()
+    for _ in range(2):
+        graph.replay()
+    assert all(torch.equal(u, v) for u, v in zip(want, (after, *grads)))
+    assert torch.equal(doubled, 2 * g)
+
+
+@pytest.mark.gpu
+def test_branch_that_drops_everything():
+    x, base, a, b, g = _branch_inputs(70, 136, 72, 8, 22)
+    x[3, 5] = float("inf")
+    y, dx, da, db = _run_branch(x, base, a, b, 2.0, 1.0, 31, g)
+    assert torch.equal(y, base) and not dx.any() and not da.any() and not db.any()
+
+
 TINY = dict(vocab_size=1000, hidden_size=512, intermediate_size=1024, num_hidden_layers=2,
             num_attention_heads=8, num_key_value_heads=2)
 
@@ -578,6 +618,30 @@ def test_fused_module_and_its_unfused_way_share_their_mask():
     module.eval()
     quiet = call(x)
     assert torch.equal(quiet, call(x))
+
+
+@pytest.mark.gpu
+def test_adapters_cast_to_fp16_keep_working():
+    """model.half() makes the adapters fp16, which the kernels do not take: the fused module and the
+    served one go through the stock products and give what those give."""
+    model = qlora.build_model(qlora.qwen25_15b_config(**TINY), "cuda", lora_fused=True, seed=5,
+                              lora_dropout=0.0, lora_b_std=0.05)
+    layer = model.model.layers[0]
+    module = layer.self_attn.q_proj
+    module.lora_A.data, module.lora_B.data = module.lora_A.data.half(), module.lora_B.data.half()
+    x = torch.randn(4, 512, device="cuda").half()
+
+    def call():
+        layer._talm_layer_group.start_forward()
+        return module(x)
+    got = call()
+    module.fused = False
+    want = call()
+    assert torch.equal(got, want)
+    with torch.no_grad(), qgroup.serving():
+        served = call()
+    # the base's weights rounded or not: 2^-11 of each term, and of the result
+    assert (served.float() - want.float()).norm() < 2e-3 * want.float().norm()
 
 
 @pytest.mark.gpu

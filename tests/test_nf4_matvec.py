@@ -137,6 +137,10 @@ def test_python_entries_refuse_what_the_kernel_does_not_take():
                              torch.empty(2, 8).half(), 256, 8, 64, 64, 256)
     with pytest.raises(ValueError, match="out must be"):
         c.run(out=torch.empty(2, 9).half())
+    for row0, block, block2 in ((0, 0, 256), (0, 64, 0), (-1, 64, 256)):
+        with pytest.raises(ValueError, match="positive"):
+            qgroup.launch_matvec(c.x, c.packed, c.absmax8, c.code, c.absmax2, c.offset2, c.levels,
+                                 torch.empty(2, 8).half(), row0, 8, 64, block, block2)
     d = _Case(2, 8, 64, "absmax", 0, device="cpu")
     with pytest.raises(ValueError, match="scales for"):
         nf4_dequant.nf4_matvec(d.x, d.packed, d.absmax[:-1], 64)
@@ -208,6 +212,15 @@ def test_block_sizes(block, n_in):
 def test_adapter_in_the_epilogue(rows, n_out, n_in, rank):
     for form in ("group", "absmax"):
         c = _Case(rows, n_out, n_in, form, seed=rank + n_out, bias=rank % 2 == 0, rank=rank)
+        c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_in", [1024, 2560, 3584, 4096, 5120, 6144, 7168, 8192, 14336])
+def test_adapter_widths(n_in):
+    """One to eight CTAs share the columns of x A^T."""
+    for rows in (1, 20):
+        c = _Case(rows, 48, n_in, "group", seed=n_in, rank=24)
         c.check(c.run())
 
 
