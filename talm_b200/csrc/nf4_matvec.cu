@@ -10,9 +10,9 @@
 // the dequantised copy of a weight is.
 //
 // Measured on one B200, calls replayed in a graph over two sets of inputs (29 MB: L2 holds them):
-// gate + up of the Qwen2.5-1.5B layer (17920 x 1536) for one row 7.9 us (14.2 MB, 1.8 TB/s; the floor
-// at the measured copy bandwidth is 2.2 us), k_proj 3.6 us, down_proj for 13 rows 10.4 us, down_proj
-// for 32 rows with an adapter of rank 64 18.1 us. Dequantising the layer and multiplying moves 117 MB
+// gate + up of the Qwen2.5-1.5B layer (17920 x 1536) for one row 7.7 us (14.2 MB, 1.8 TB/s; the floor
+// at the measured copy bandwidth is 2.2 us), k_proj 3.5 us, down_proj for 13 rows 9.7 us, down_proj
+// for 32 rows with an adapter of rank 64 15.2 us. Dequantising the layer and multiplying moves 117 MB
 // for the same 23 MB of weights.
 #include "common.cuh"
 
@@ -181,6 +181,11 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 // matching operand is two 16-byte pieces of x, a quad's pieces side by side. A block's 64 columns have
 // one scale per row: its four mma's start from zero and their result is added to the fp32 sum with one
 // FMA per value, times the scale.
+//
+// From nine rows on (NT 2 and 4) a warp takes two such tiles, 32 weight rows, against the same x, and
+// a CTA has half as many warps with twice the registers: x is read half as often, and next to nothing spills
+// (17920 x 1536: 16 rows 13.1 -> 11.9 us, 32 rows 19.6 -> 17.9; one row would gain 0.3 us there, but
+// k_proj lose as much and down_proj 3). A second block of x ahead changed nothing.
 //
 // The table holds fp16(LEVEL_GAIN * level) and the scale takes 1 / LEVEL_GAIN: the gain is the one
 // in [1, 2) whose 16 rounded levels are nearest to the true ones (6.2e-5 in the mean square
@@ -481,8 +486,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1)
     if (ep.t != nullptr && has) {
       // scaling * t B^T, eight columns of the rank per share, as tf32 products of split operands
       // (without the product of the two rests): lane columns j + 2 t and j + 2 t + 1. The loads of
-      // UNROLL such steps go out together, B's before the wait for t: one latency for all of them (17920
-      // x 1536 at rank 64, one row 14.9 -> NEW us, eight 21.5 -> NEW, with t read through L1 as well).
+      // UNROLL such steps go out together, B's before the wait for t: one latency for all of them
+      // (17920 x 1536 at rank 64: one row 14.9 -> 10.6 us, eight 21.5 -> 12.1, with t read through
+      // L1 as well).
       constexpr int UNROLL = NT == 4 ? 2 : 4;  // (registers)
       for (int j0 = 8 * place; j0 < ep.rank; j0 += UNROLL * 8 * shares) {
         float bv[UNROLL][4 * MT];
@@ -614,12 +620,15 @@ int run_mma(const __half* x, int64_t ld_x, int n_rows, const Weight& w, Split sp
   }
   const int sms = current_sm_count();
   if (sms <= 0) return set_error(TALM_ENODEV, "no CUDA device");
-  // How many warps (and CTAs) share a tile's columns: the least time by a model in units of one
-  // block of one warp, ~720 cycles at 16 warps per SM: the blocks a warp runs one after another in
-  // every round of tiles, three more for the epilogue, two for a cluster's barriers, and the rows of
-  // x that a CTA reads from L2 (64 bytes per cycle) for its share of the columns. (gate + up of
-  // one row, 1120 tiles of 24 blocks: W = 2 one round of 12 + 3, W = 4 two of 6 + 3; down_proj of
-  // 32 rows: a cluster of 4 reads a quarter of 573 KB per CTA.) Clusters of 4 find 33 places.
+  // How many warps (and CTAs) share a tile's columns: the least time by a model in cycles, fitted to
+  // ten shapes with every choice forced. In each round of tiles a warp works through its blocks
+  // one after another, finishes the tile (its outputs divided over the warps that share it, whose
+  // sums each of them reads) and, in a cluster, meets the other CTAs twice. (17920 x 1536, 32 rows:
+  // W = 2, one round of 12 blocks, 15.0 us; W = 4, two rounds of 6, 17.0. 1536 x 8960, 32 rows:
+  // clusters of 4 13.4 us, none 18.7. 3000 x 4096, 32 rows: none 11.6, clusters of 4 13.2.)
+  // Clusters of 4 find 33 places.
+  constexpr int BLOCK = NT == 1 ? 640 : NT == 2 ? 910 : 1490, ROUND = NT == 1 ? 1600 : 2800;
+  constexpr int OUTPUTS = 200, JOIN = NT == 1 ? 50 : 150, MEET = NT == 2 ? 2300 : 3200;
   int64_t least = -1;
   int groups = 1, clusters = 1;
   for (int c = 1; c <= (NT == 1 ? 1 : 4); c *= 2) {
@@ -628,8 +637,8 @@ int run_mma(const __half* x, int64_t ld_x, int n_rows, const Weight& w, Split sp
       const int64_t slots = (places > 0 ? places : 1) * (WARPS >> lw);
       const int64_t rounds = (sp.n_tiles + slots - 1) / slots;
       const int64_t blocks = (sp.n_blocks + (c << lw) - 1) / (c << lw);
-      const int64_t x_read = int64_t{n_rows} * sp.n_blocks * 128 / c / (64 * 720);
-      const int64_t cost = rounds * (blocks * (NT == 4 ? 3 : 1) + 3 + (c > 1 ? 2 : 0) + x_read);
+      const int64_t cost = rounds * (blocks * BLOCK + ROUND + OUTPUTS * n_rows / (c << lw) +
+                                     (JOIN << lw) + (c > 1 ? MEET : 0));
       if (least < 0 || cost < least) {
         least = cost;
         sp.log_w = lw;
