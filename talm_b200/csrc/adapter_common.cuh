@@ -16,9 +16,21 @@ struct Dropout {
   float factor;           // 32768 / (32768 - drop), 0 when everything is dropped
 };
 
+// WIDE: one 64-bit product instead of its two halves. Fewer instructions, which counts where the
+// generator runs beside HBM at full rate, but a longer wait for each: dropout of 16384 x 8960 bf16
+// (forward and backward) 206.7 -> 200.1 us, of 2048 x 1536 fp16 6.5 -> 6.9, the branch 306 -> 310.
+template <bool WIDE>
 __device__ __forceinline__ void philox_round(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
-  const uint32_t h0 = __umulhi(c[0], 0xD2511F53u), l0 = c[0] * 0xD2511F53u;
-  const uint32_t h1 = __umulhi(c[2], 0xCD9E8D57u), l1 = c[2] * 0xCD9E8D57u;
+  uint32_t h0, l0, h1, l1;
+  if (WIDE) {
+    const uint64_t p0 = static_cast<uint64_t>(c[0]) * 0xD2511F53u;
+    const uint64_t p1 = static_cast<uint64_t>(c[2]) * 0xCD9E8D57u;
+    h0 = static_cast<uint32_t>(p0 >> 32), l0 = static_cast<uint32_t>(p0);
+    h1 = static_cast<uint32_t>(p1 >> 32), l1 = static_cast<uint32_t>(p1);
+  } else {
+    h0 = __umulhi(c[0], 0xD2511F53u), l0 = c[0] * 0xD2511F53u;
+    h1 = __umulhi(c[2], 0xCD9E8D57u), l1 = c[2] * 0xCD9E8D57u;
+  }
   c[0] = h1 ^ c[1] ^ k0;
   c[1] = l1;
   c[2] = h0 ^ c[3] ^ k1;
@@ -26,6 +38,7 @@ __device__ __forceinline__ void philox_round(uint32_t (&c)[4], uint32_t k0, uint
 }
 
 // The four words of group q (elements 8 q .. 8 q + 7).
+template <bool WIDE = false>
 __device__ __forceinline__ void philox(uint64_t q, uint64_t key, uint32_t (&c)[4]) {
   uint32_t k0 = static_cast<uint32_t>(key), k1 = static_cast<uint32_t>(key >> 32);
   c[0] = static_cast<uint32_t>(q);
@@ -34,7 +47,7 @@ __device__ __forceinline__ void philox(uint64_t q, uint64_t key, uint32_t (&c)[4
   c[3] = 0;
 #pragma unroll
   for (int i = 0; i < 7; ++i) {
-    philox_round(c, k0, k1);
+    philox_round<WIDE>(c, k0, k1);
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }

@@ -244,6 +244,17 @@ def test_dropout_past_32_bit_offsets():
         assert torch.equal(y[row], want), row
 
 
+@pytest.mark.gpu
+def test_dropout_mask_does_not_depend_on_the_type_or_the_size():
+    """One seed's mask over long, odd-sized tensors of each type, and over their first elements."""
+    n = 75_000_003
+    masks = [adapter.dropout(torch.ones(n, dtype=t, device="cuda"), 0.3, _seed(9)) != 0
+             for t in (torch.bfloat16, torch.float16, torch.float32)]
+    few = adapter.dropout(torch.ones(100_001, device="cuda").half(), 0.3, _seed(9)) != 0
+    assert torch.equal(masks[0], masks[1]) and torch.equal(masks[0], masks[2])
+    assert torch.equal(masks[0][:100_001], few)
+
+
 # ------------------------------------------------------------------------------------------
 # the branch
 # ------------------------------------------------------------------------------------------
