@@ -176,10 +176,10 @@ int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, co
 // they are two bf16 parts without scale, and the product of the two small ones is left out: under
 // 2^-16 of each term, a sixteenth of the result's own rounding.
 //
-// Measured on one B200, forward and backward replayed in a graph: q_proj of 2048 rows, rank 16, 42 us (38
-// MB; ten launches of about 4 us each are the bound), 16384 x 1536 to 8960, rank 64, 313 us (1.04 GB,
-// 3.3 TB/s, 0.51 of the measured copy: g is read twice, once for dt and once for dB, 45 us that the
-// floor does not have; the passes themselves run at 0.8 to 0.95).
+// Measured on one B200, forward and backward replayed in a graph: q_proj of 2048 rows, rank 16, 39 us (38
+// MB; nine launches of about 4 us each are the bound), 16384 x 1536 to 8960, rank 64, 306 us (1.04 GB,
+// 3.4 TB/s, 0.52 of the measured copy: g is read twice, once for dt and once for dB, 45 us that the
+// floor does not have, and the masked passes by the generator; the others run at 0.8 to 0.95).
 // ------------------------------------------------------------------------------------------
 struct Shape {
   int64_t n_rows, n_in, n_out;

@@ -347,9 +347,10 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
 //   INNER:  part[split][n][j] = sum over the split's columns of X[n, c] W[j, c]
 //   OUTER:  part[split][j][c] = sum over the split's rows of X[n, c] T[n, j]
 // W (an adapter matrix) and T (t or dt) are fp32, scaled by powers of two (a scale for every 128 of the
-// reduction, for W one for each rank) and split in two fp16 parts that stand side by side as the n operand (N = 2 RP), so that X passes the tensor core once;
-// the epilogue adds the two halves of the result. X is the 128-row m operand as it lies in memory:
-// rows of K-major for INNER, columns of it, MN-major, for OUTER.
+// reduction, for W one for each rank) and split in two fp16 parts that stand side by side as the n
+// operand (N = 2 RP), so that X passes the tensor core once; the epilogue adds the two halves of the
+// result. X is the 128-row m operand as it lies in memory: rows of it, K-major, for INNER, columns of
+// it, MN-major, for OUTER.
 //
 // Bound by HBM: X is read once (2 bytes per element, 4 RP flops). One CTA per 128 rows (INNER) or
 // columns (OUTER) and split, stages of 64 of the reduction:
@@ -361,9 +362,10 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
 //                 group of the generator
 //
 // Measured at rank 64: dB of 16384 x 8960 47 us (294 MB, 6.2 TB/s, 0.95 of the measured copy), dt 55 us
-// (its W, 2.3 MB, is read again by every 128 rows), with the dropout of 16384 x 1536 t 28 us and dA 24
-// us (7.7 us of bytes: the generator, one CTA per SM). The mma.sync form of the same sums took 276,
-// 171, 70 and 74 us.
+// (its W, 2.3 MB, is read again by every 128 rows), both in one launch 100 us; with the dropout of 16384
+// x 1536 t 28 us and dA 22 us (7.7 us of bytes; of the 1600 cycles a stage takes a mask warp, 850 are the
+// generator's and 380 the and; 16 mask warps or its products as whole 64-bit ones changed nothing). The
+// mma.sync form of the same sums took 276, 171, 70 and 74 us.
 namespace sums {
 
 constexpr int TILE = 128;
@@ -385,7 +387,9 @@ template <int RP, bool OUTER, bool MASK>
 __host__ __device__ constexpr int smem_bytes() {
   return stages<RP, OUTER, MASK>() * (X_BYTES + other_bytes<RP, OUTER>()) + 1024 + 512;
 }
-__host__ __device__ constexpr int threads(bool mask) { return 32 * (FIRST_MASK_WARP + (mask ? MASK_WARPS : 0)); }
+__host__ __device__ constexpr int threads(bool mask) {
+  return 32 * (FIRST_MASK_WARP + (mask ? MASK_WARPS : 0));
+}
 
 struct Ctl {
   uint64_t full[MAX_STAGES], masked[MAX_STAGES], empty[MAX_STAGES];

@@ -183,9 +183,9 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 // FMA per value, times the scale.
 //
 // From nine rows on (NT 2 and 4) a warp takes two such tiles, 32 weight rows, against the same x, and
-// a CTA has half as many warps with twice the registers: x is read half as often, and next to nothing spills
-// (17920 x 1536: 16 rows 13.1 -> 11.9 us, 32 rows 19.6 -> 17.9; one row would gain 0.3 us there, but
-// k_proj lose as much and down_proj 3). A second block of x ahead changed nothing.
+// a CTA has half as many warps with twice the registers: x is read half as often, and next to nothing
+// spills (17920 x 1536: 16 rows 13.1 -> 11.9 us, 32 rows 19.6 -> 17.9; one row would gain 0.3 us there,
+// but k_proj lose as much and down_proj 3). A second block of x ahead changed nothing.
 //
 // The table holds fp16(LEVEL_GAIN * level) and the scale takes 1 / LEVEL_GAIN: the gain is the one
 // in [1, 2) whose 16 rounded levels are nearest to the true ones (6.2e-5 in the mean square
