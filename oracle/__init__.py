@@ -22,5 +22,6 @@ import time
 if multiprocessing.parent_process() is not None:
     # A rank of a CPU test puts its tensors on a queue and exits, but the parent fetches them by file
     # descriptor from the sender: a rank that has already gone leaves it without. The sender stays
-    # for a moment after its queue has been flushed (finalizers of a lower priority run later).
-    multiprocessing.util.Finalize(None, time.sleep, args=(3,), exitpriority=-100)
+    # for a moment after its queue has been told to finish (10) and before the socket that the parent
+    # connects to is unlinked (0; finalizers of a lower priority run later).
+    multiprocessing.util.Finalize(None, time.sleep, args=(5,), exitpriority=5)
