@@ -177,7 +177,7 @@ int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, co
 // 2^-16 of each term, a sixteenth of the result's own rounding.
 //
 // Measured on one B200, forward and backward replayed in a graph: q_proj of 2048 rows, rank 16, 39 us (38
-// MB; nine launches of about 4 us each are the bound), 16384 x 1536 to 8960, rank 64, 306 us (1.04 GB,
+// MB; nine launches of about 4 us each are the bound), 16384 x 1536 to 8960, rank 64, 304 us (1.04 GB,
 // 3.4 TB/s, 0.52 of the measured copy: g is read twice, once for dt and once for dB, 45 us that the
 // floor does not have, and the masked passes by the generator; the others run at 0.8 to 0.95).
 // ------------------------------------------------------------------------------------------
@@ -462,7 +462,7 @@ struct BackwardWork {
     dt.down = carve.take<float>(static_cast<size_t>((s.n_rows + 127) / 128));
     t_part = carve.take<float>(static_cast<size_t>(sums::Plan(false, false, s.n_rows, s.n_out).splits) *
                                s.n_rows * rp);
-    b_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, false, s.n_rows, s.n_out).splits) *
+    b_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, true, s.n_rows, s.n_out).splits) *
                                rp * s.n_out);
     a_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, false, s.n_rows, s.n_in).splits) *
                                rp * s.n_in);
@@ -494,15 +494,15 @@ int run_forward(const __half* x, int64_t ld_x, const __half* base, int64_t ld_ba
   int st = launch_dependent(prepare_kernel<RP>,
                             static_cast<unsigned>((s.n_in + 127) / 128 + (s.n_out + 127) / 128),
                             PREP_THREADS, smem, stream, ma, mb, of_a, of_b, s.rank);
+  const sums::Plan plan(false, d.drop != 0, s.n_rows, s.n_in);
   const TParts t{w.t_cat, saved ? keep.t.pair : nullptr, saved ? keep.t.down : nullptr};
   if (st == TALM_OK)
-    st = d.drop ? sums::launch<RP, false, true>(x, ld_x, s.n_rows, s.n_in, w.a_rows.parts,
+    st = d.drop ? sums::launch<RP, false, true>(plan, x, ld_x, s.n_rows, s.n_in, w.a_rows.parts,
                                                 w.a_rows.down, d, w.part, stream)
-                : sums::launch<RP, false, false>(x, ld_x, s.n_rows, s.n_in, w.a_rows.parts,
+                : sums::launch<RP, false, false>(plan, x, ld_x, s.n_rows, s.n_in, w.a_rows.parts,
                                                  w.a_rows.down, d, w.part, stream);
   if (st == TALM_OK)
-    st = make_t_parts<RP>(w.part, sums::Plan(false, d.drop != 0, s.n_rows, s.n_in).splits,
-                          s.n_rows, d.factor, t, stream);
+    st = make_t_parts<RP>(w.part, plan.splits, s.n_rows, d.factor, t, stream);
   if (st != TALM_OK) return st;
   return up::launch<RP, false>(w.t_cat, w.b_cat, base, ld_base, y, s.n_rows, s.n_out,
                                            scaling, d, stream);
@@ -517,31 +517,31 @@ int run_backward(const __half* g, int64_t ld_g, const __half* x, int64_t ld_x, c
   const Dropout none{nullptr, 0, 1.0f};
   int st = TALM_OK;
   const bool want_dt = da || dx;
+  const sums::Plan dt_plan(false, false, s.n_rows, s.n_out), db_plan(true, true, s.n_rows, s.n_out);
+  const sums::Plan da_plan(true, d.drop != 0, s.n_rows, s.n_in);
   if (want_dt && db)
-    st = sums::launch_pair<RP>(g, ld_g, s.n_rows, s.n_out, keep.b_rows.parts, keep.b_rows.down,
-                               w.t_part, keep.t.pair, keep.t.down, w.b_part, stream);
+    st = sums::launch_pair<RP>(dt_plan, db_plan, g, ld_g, s.n_rows, s.n_out, keep.b_rows.parts,
+                               keep.b_rows.down, w.t_part, keep.t.pair, keep.t.down, w.b_part,
+                               stream);
   else if (want_dt)
-    st = sums::launch<RP, false, false>(g, ld_g, s.n_rows, s.n_out, keep.b_rows.parts,
+    st = sums::launch<RP, false, false>(dt_plan, g, ld_g, s.n_rows, s.n_out, keep.b_rows.parts,
                                         keep.b_rows.down, none, w.t_part, stream);
   else
-    st = sums::launch<RP, true, false>(g, ld_g, s.n_rows, s.n_out, keep.t.pair, keep.t.down, none,
-                                       w.b_part, stream);
+    st = sums::launch<RP, true, false>(db_plan, g, ld_g, s.n_rows, s.n_out, keep.t.pair,
+                                       keep.t.down, none, w.b_part, stream);
   if (want_dt && st == TALM_OK)
-    st = make_t_parts<RP>(w.t_part, sums::Plan(false, false, s.n_rows, s.n_out).splits, s.n_rows,
-                          scaling, w.dt, stream);
+    st = make_t_parts<RP>(w.t_part, dt_plan.splits, s.n_rows, scaling, w.dt, stream);
   if (da && st == TALM_OK)
-    st = d.drop ? sums::launch<RP, true, true>(x, ld_x, s.n_rows, s.n_in, w.dt.pair, w.dt.down, d,
-                                               w.a_part, stream)
-                : sums::launch<RP, true, false>(x, ld_x, s.n_rows, s.n_in, w.dt.pair, w.dt.down, d,
-                                                w.a_part, stream);
+    st = d.drop ? sums::launch<RP, true, true>(da_plan, x, ld_x, s.n_rows, s.n_in, w.dt.pair,
+                                               w.dt.down, d, w.a_part, stream)
+                : sums::launch<RP, true, false>(da_plan, x, ld_x, s.n_rows, s.n_in, w.dt.pair,
+                                                w.dt.down, d, w.a_part, stream);
   if (dx && st == TALM_OK)
     st = up::launch<RP, true>(w.dt.cat, keep.a_cat, nullptr, 0, dx, s.n_rows, s.n_in,
                                           d.factor, d, stream);
   if ((da || db) && st == TALM_OK) {
-    const PartSum sa{w.a_part, sums::Plan(true, d.drop != 0, s.n_rows, s.n_in).splits,
-                     static_cast<int>(s.n_in), d.factor, da};
-    const PartSum sb{w.b_part, sums::Plan(true, false, s.n_rows, s.n_out).splits,
-                     static_cast<int>(s.n_out), scaling, db};
+    const PartSum sa{w.a_part, da_plan.splits, static_cast<int>(s.n_in), d.factor, da};
+    const PartSum sb{w.b_part, db_plan.splits, static_cast<int>(s.n_out), scaling, db};
     const int64_t ctas = (da ? (s.n_in + 31) / 32 : 0) + (db ? (s.n_out + 31) / 32 : 0);
     st = launch_dependent(sum_parts_kernel, static_cast<unsigned>(ctas), SUM_THREADS, 0, stream, sa, sb,
                           s.rank, RP);

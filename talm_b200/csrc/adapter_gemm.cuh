@@ -618,34 +618,34 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
   sums_cta<RP, OUTER, MASK>(tm_x, tm_o, p, blockIdx.x, blockIdx.y);
 }
 
-// dt and dB, which read the same gradient and do not wait for one another, in one launch: the first
-// `inner_ctas` CTAs work on dt.
+// dt and dB, which read the same gradient and do not wait for one another, in one launch. dB's CTAs come
+// first, one per SM, and a row tile's splits side by side (16384 x 1536 to 8960, forward and backward:
+// rank 16 269 -> 262 us, rank 64 307 -> 304, against dt first and dB with two CTAs per SM).
 template <int RP>
 __global__ void __launch_bounds__(threads(false), 2)
     sums_pair_kernel(const __grid_constant__ CUtensorMap in_x,
                      const __grid_constant__ CUtensorMap in_o, const __grid_constant__ Params in_p,
-                     int inner_ctas, int inner_tiles, const __grid_constant__ CUtensorMap out_x,
+                     int inner_splits, const __grid_constant__ CUtensorMap out_x,
                      const __grid_constant__ CUtensorMap out_o,
-                     const __grid_constant__ Params out_p, int outer_tiles) {
-  const int id = blockIdx.x;
-  if (id < inner_ctas)
-    sums_cta<RP, false, false>(in_x, in_o, in_p, id % inner_tiles, id / inner_tiles);
+                     const __grid_constant__ Params out_p, int outer_tiles, int outer_ctas) {
+  const int id = blockIdx.x, inner = id - outer_ctas;
+  if (inner >= 0)
+    sums_cta<RP, false, false>(in_x, in_o, in_p, inner / inner_splits, inner % inner_splits);
   else
-    sums_cta<RP, true, false>(out_x, out_o, out_p, (id - inner_ctas) % outer_tiles,
-                              (id - inner_ctas) / outer_tiles);
+    sums_cta<RP, true, false>(out_x, out_o, out_p, id % outer_tiles, id / outer_tiles);
 }
 
-// How the reduction is divided: as many CTAs as 148 SMs hold at a time (two of them, one with its mask
-// warps), two blocks of 128 (which share a scale) for a CTA at least.
+// How the reduction is divided: as many CTAs as 148 SMs hold at a time (two of them, or `one` per SM: with
+// its mask warps, and for dB beside dt), two blocks of 128 (which share a scale) for a CTA at least.
 struct Plan {
   int tiles = 0, steps = 0, steps_per_split = 0, splits = 0;
   Plan() = default;
-  Plan(bool outer, bool mask, int64_t n_rows, int64_t n_cols) {
+  Plan(bool outer, bool one, int64_t n_rows, int64_t n_cols) {
     tiles = static_cast<int>(((outer ? n_cols : n_rows) + TILE - 1) / TILE);
     const int64_t length = outer ? n_rows : n_cols;
     steps = static_cast<int>((length + 63) / 64);
     const int blocks = (steps + 1) / 2;
-    int want = (mask ? 148 : 296) / tiles;
+    int want = (one ? 148 : 296) / tiles;
     const int most = (blocks + 1) / 2;
     if (want > most) want = most;
     if (want > 32) want = 32;
@@ -664,9 +664,9 @@ struct Call {
 };
 
 template <int RP, bool OUTER, bool MASK>
-int make_call(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void* other,
-              const float* down, const Dropout& d, float* part, Call* c) {
-  c->plan = Plan(OUTER, MASK, n_rows, n_cols);
+int make_call(const Plan& plan, const void* x, int64_t ld, int64_t n_rows, int64_t n_cols,
+              const void* other, const float* down, const Dropout& d, float* part, Call* c) {
+  c->plan = plan;
   c->p = Params{n_rows, static_cast<int>(n_cols), c->plan.steps, c->plan.steps_per_split,
                 down,   part,                     d};
   int st = talm_make_tmap_2d_f16(&c->tm_x, x, n_cols, n_rows, ld, 64, OUTER ? 64 : TILE);
@@ -678,8 +678,9 @@ int make_call(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const v
 }
 
 template <int RP, bool OUTER, bool MASK>
-int launch(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void* other,
-           const float* down, const Dropout& d, float* part, cudaStream_t stream) {
+int launch(const Plan& plan, const void* x, int64_t ld, int64_t n_rows, int64_t n_cols,
+           const void* other, const float* down, const Dropout& d, float* part,
+           cudaStream_t stream) {
   constexpr int smem = smem_bytes<RP, OUTER, MASK>();
   static_assert(smem <= 232448 && (MASK || 2 * smem <= 232448), "shared memory");
   auto kernel = sums_kernel<RP, OUTER, MASK>;
@@ -688,7 +689,7 @@ int launch(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
   Call c;
-  const int st = make_call<RP, OUTER, MASK>(x, ld, n_rows, n_cols, other, down, d, part, &c);
+  const int st = make_call<RP, OUTER, MASK>(plan, x, ld, n_rows, n_cols, other, down, d, part, &c);
   if (st != TALM_OK) return st;
   return launch_dependent(
       kernel, dim3(static_cast<unsigned>(c.plan.tiles), static_cast<unsigned>(c.plan.splits), 1),
@@ -697,9 +698,9 @@ int launch(const void* x, int64_t ld, int64_t n_rows, int64_t n_cols, const void
 
 // dt = g B and dB = g^T t (see sums_pair_kernel).
 template <int RP>
-int launch_pair(const void* g, int64_t ld, int64_t n_rows, int64_t n_cols, const void* w_parts,
-                const float* w_down, float* dt_part, const void* t_parts, const float* t_down,
-                float* db_part, cudaStream_t stream) {
+int launch_pair(const Plan& dt_plan, const Plan& db_plan, const void* g, int64_t ld, int64_t n_rows,
+                int64_t n_cols, const void* w_parts, const float* w_down, float* dt_part,
+                const void* t_parts, const float* t_down, float* db_part, cudaStream_t stream) {
   constexpr int a = smem_bytes<RP, false, false>(), b = smem_bytes<RP, true, false>();
   constexpr int smem = a > b ? a : b;
   auto kernel = sums_pair_kernel<RP>;
@@ -708,15 +709,16 @@ int launch_pair(const void* g, int64_t ld, int64_t n_rows, int64_t n_cols, const
   if (e != cudaSuccess) return set_error(TALM_ECUDA, "smem: %s", cudaGetErrorString(e));
   const Dropout none{nullptr, 0, 1.0f};
   Call in, out;
-  int st = make_call<RP, false, false>(g, ld, n_rows, n_cols, w_parts, w_down, none, dt_part, &in);
+  int st = make_call<RP, false, false>(dt_plan, g, ld, n_rows, n_cols, w_parts, w_down, none,
+                                       dt_part, &in);
   if (st == TALM_OK)
-    st = make_call<RP, true, false>(g, ld, n_rows, n_cols, t_parts, t_down, none, db_part, &out);
+    st = make_call<RP, true, false>(db_plan, g, ld, n_rows, n_cols, t_parts, t_down, none, db_part,
+                                    &out);
   if (st != TALM_OK) return st;
-  const int inner = in.plan.tiles * in.plan.splits;
-  return launch_dependent(kernel,
-                          dim3(static_cast<unsigned>(inner + out.plan.tiles * out.plan.splits)),
-                          threads(false), smem, stream, in.tm_x, in.tm_o, in.p, inner,
-                          in.plan.tiles, out.tm_x, out.tm_o, out.p, out.plan.tiles);
+  const int inner = dt_plan.tiles * dt_plan.splits, outer = db_plan.tiles * db_plan.splits;
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(inner + outer)), threads(false), smem,
+                          stream, in.tm_x, in.tm_o, in.p, dt_plan.splits, out.tm_x, out.tm_o, out.p,
+                          db_plan.tiles, outer);
 }
 
 }  // namespace sums
