@@ -394,6 +394,20 @@ def test_branch_layouts():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("p", [0.0, 0.1])
+def test_branch_each_gradient_alone(p):
+    """A gradient asked for by itself (another choice of launches) has the bits it has among all."""
+    x, base, a, b, g = _branch_inputs(1500, 264, 1032, 12, 6)
+    _, *want = _run_branch(x, base, a, b, 1.0, p, 2, g)
+    want.insert(1, g)
+    for alone in range(4):
+        leaves = [t.clone().requires_grad_(i == alone) for i, t in enumerate((x, base, a, b))]
+        y = adapter.lora_branch(*leaves, 1.0, p, _seed(2) if p else None)
+        got, = torch.autograd.grad(y, leaves[alone], g)
+        assert torch.equal(got, want[alone]), alone
+
+
+@pytest.mark.gpu
 def test_branch_of_no_rows():
     x, base, a, b, _ = _branch_inputs(1, 64, 48, 8, 5)
     leaves = [t.clone().requires_grad_() for t in (x[:0], base[:0], a, b)]
