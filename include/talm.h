@@ -141,7 +141,8 @@ int talm_nf4_linear(const uint16_t* a, int64_t ld_a, int64_t n_rows, const uint8
  *   y[n, o] = fp16( sum_k level[code(o, k)] * scale(o, k) * x[n, k] + bias[o]
  *                   + scaling * sum_j (sum_k x[n, k] lora_a[j, k]) * lora_b[o, j] )
  * with fp32 products and sums and one rounding (the weight itself is not rounded to fp16, as the
- * dequantised copy is). Stands in for the dequantisation + product of solution/qgroup.py:346-355
+ * dequantised copy is; a level keeps 2^-22 of itself where it is at least 2^-17 of the largest one, any
+ * finite table). Stands in for the dequantisation + product of solution/qgroup.py:346-355
  * (GroupLinear) and the adapter of solution/lora.py:151-231 where there are few rows.
  *   x        : fp16 [n_rows, w_cols], row stride ld_x elements
  *   packed   : w_rows * w_cols / 2 bytes, row-major

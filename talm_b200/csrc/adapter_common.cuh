@@ -85,16 +85,6 @@ __device__ __forceinline__ void split_f16(float v0, float v1, uint32_t& hi, uint
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   lo = pack_half2(v0 - h.x, v1 - h.y);
 }
-// For a largest magnitude m: *up brings it to [2^14, 2^15), *down undoes that. Clamped so that both
-// are normal numbers; 1 for zero (and for what is not finite, which stays so).
-__device__ __forceinline__ void power_scale(float m, float* up, float* down) {
-  int e = static_cast<int>((__float_as_uint(m) >> 23) & 255) - 127 - 14;
-  if (m == 0.0f || !(m < __int_as_float(0x7F800000))) e = 0;
-  e = max(-112, min(112, e));
-  *up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  *down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-}
-
 // The kernels of one branch follow one another closely: each may start its set-up while the one
 // before it ends (programmatic stream serialization) and waits in grid_dependency_wait before it
 // touches global memory.

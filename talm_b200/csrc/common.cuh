@@ -428,6 +428,19 @@ __device__ __forceinline__ void umma_commit(uint64_t* bar) {
 }
 
 // ------------------------------------------------------------------------------------------
+// fp32 in two 16-bit parts
+// ------------------------------------------------------------------------------------------
+// For a largest magnitude m: *up brings it to [2^14, 2^15), *down undoes that. Clamped so that both
+// are normal numbers; 1 for zero (and for what is not finite, which stays so).
+__device__ __forceinline__ void power_scale(float m, float* up, float* down) {
+  int e = static_cast<int>((__float_as_uint(m) >> 23) & 255) - 127 - 14;
+  if (m == 0.0f || !(m < __int_as_float(0x7F800000))) e = 0;
+  e = max(-112, min(112, e));
+  *up = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  *down = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+
+// ------------------------------------------------------------------------------------------
 // memory helpers
 // ------------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t ld_stream_u32(const uint32_t* p) {

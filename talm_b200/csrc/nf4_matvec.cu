@@ -7,12 +7,12 @@
 // L are the 16 levels, S the scale of the block that the flattened weight element o * K + k is in:
 // an fp32 absmax, or fp32(fp32(code2[absmax8] * absmax2) + offset2) as in nf4.cu. Products and
 // sums are fp32 and the result is rounded once: the weight itself is not rounded to fp16, which
-// the dequantised copy of a weight is.
+// the dequantised copy of a weight is, and its levels keep 22 bits and more of their fp32 values.
 //
 // Measured on one B200, calls replayed in a graph over two sets of inputs (29 MB: L2 holds them):
-// gate + up of the Qwen2.5-1.5B layer (17920 x 1536) for one row 7.7 us (14.2 MB, 1.8 TB/s; the floor
-// at the measured copy bandwidth is 2.2 us), k_proj 3.5 us, down_proj for 13 rows 9.7 us, down_proj
-// for 32 rows with an adapter of rank 64 15.2 us. Dequantising the layer and multiplying moves 117 MB
+// gate + up of the Qwen2.5-1.5B layer (17920 x 1536) for one row 9.6 us (14.2 MB, 1.5 TB/s; the floor
+// at the measured copy bandwidth is 2.2 us), k_proj 3.9 us, down_proj for 13 rows 11.5 us, down_proj
+// for 32 rows with an adapter of rank 64 21.1 us. Dequantising the layer and multiplying moves 117 MB
 // for the same 23 MB of weights.
 #include "common.cuh"
 
@@ -173,35 +173,39 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 //
 // A warp takes tiles of 16 weight rows; lane (g, t) = (lane / 4, lane % 4) reads 8 packed bytes of
 // rows g and g + 8 per block (a quad reads a row's 32 bytes, lane t bytes 4 t .. 4 t + 3 of both
-// halves) and turns each byte into the fp16 pair of its two levels by one shared-memory read: a table
-// of 256 pairs, one copy per lane, so that no two lanes meet in a bank. Entries lie 256 bytes apart
-// (the second 128 are not used), so that one byte permutation makes the address: the packed byte
-// above the lane's own four-byte offset. The reduction index may be permuted as long as both operands
-// agree, so a lane's two runs of eight consecutive weights go into four mma's as they are and the
-// matching operand is two 16-byte pieces of x, a quad's pieces side by side. A block's 64 columns have
-// one scale per row: its four mma's start from zero and their result is added to the fp32 sum with one
-// FMA per value, times the scale.
+// halves) and turns each byte into the fp16 pairs of its two levels by one 64-bit shared-memory read: a
+// table of 256 entries, sixteen copies side by side, so that no two lanes of the half warp that such a
+// read takes at a time meet in a bank. Entries lie 256 bytes apart (the second 128 are not used), so that
+// one byte permutation makes the address: the packed byte above the lane's own eight-byte offset. The
+// reduction index may be permuted as long as both operands agree, so a lane's two runs of eight
+// consecutive weights go into four steps as they are and the matching operand is two 16-byte pieces of
+// x, a quad's pieces side by side. A block's 64 columns have one scale per row: its mma's start from
+// zero and their result is added to the fp32 sum with one FMA per value, times the scale.
+//
+// A level has 24 bits and an fp16 operand 11, so a level is two parts (split_levels) and a step two mma's
+// against the same x. With one part, under the best common gain, outputs were 4 to 7 % farther from the exact
+// ones than their own rounding puts them, and a table other than NF4's could be off by 2^-11 of a term
+// or pass fp16's range; the second part costs twice the table's bytes and the mma's (17920 x 1536: one row
+// 7.6 -> 9.6 us, 32 rows 14.8 -> 21.6). The levels take a power of two that brings the largest to [2^14,
+// 2^15), undone by the scales: parts are exact to 2^-22 of a level that is at least 2^-17 of the largest, and
+// to 2^-40 of the largest below.
 //
 // From nine rows on (NT 2 and 4) a warp takes two such tiles, 32 weight rows, against the same x, and
 // a CTA has half as many warps with twice the registers: x is read half as often, and next to nothing
-// spills (17920 x 1536: 16 rows 13.1 -> 11.9 us, 32 rows 19.6 -> 17.9; one row would gain 0.3 us there,
-// but k_proj lose as much and down_proj 3). A second block of x ahead changed nothing.
+// spills (17920 x 1536: 16 rows 15.5 us with one tile and 16 warps, 12.4 with two, 32 rows 23.4 and
+// 21.6). The table reads of a step are made before the mma's of the step before it, and each half of x is
+// replaced as soon as the block is done with it (32 rows 22.2 -> 21.6, one row 9.7 -> 9.6).
 //
-// The table holds fp16(LEVEL_GAIN * level) and the scale takes 1 / LEVEL_GAIN: the gain is the one
-// in [1, 2) whose 16 rounded levels are nearest to the true ones (6.2e-5 in the mean square
-// against 1.56e-4 without it and 2.1e-4 for the result's own rounding).
-//
-// What bounds it (one row of gate + up, cycles of an instrumented copy): 2.9k of 12.4k are set-up
-// (first loads, the table), 8.7k the 12 blocks of each of 16 warps, 45 per block and warp: the
-// table's 16 shared-memory reads per 1024 weights and the reads of x and of the ring take 24, the
-// rest is their latency at four warps per scheduler. 32 warps of 64 registers were slower (9.7 us
-// against 7.9, spills), and so were table entries 128 bytes apart (two operations per address, 8.8).
+// What bounds it: one row, the latency of dependent shared-memory reads at four warps per scheduler (by
+// count a block of a warp is 40 cycles of the SM's shared memory, 32 of them the table's: 7.3k of gate +
+// up's 18.6k); 32 rows, that and 64 mma's per 32 x 64 weights at two warps per scheduler (128 cycles of the
+// tensor cores: 11.6k of 41k). 32 warps of 64 registers were slower with half the table reads (9.7 us
+// against 7.9, spills), and so were entries 128 bytes apart (two operations per address).
 // ------------------------------------------------------------------------------------------
 // 16-row tiles of a warp, and the warps of a CTA
 __host__ __device__ constexpr int tiles_of(int nt) { return nt >= 2 ? 2 : 1; }
 __host__ __device__ constexpr int warps_of(int nt) { return 16 / tiles_of(nt); }
 constexpr int STEP_BLOCKS = 4;  // blocks of 64 columns that a warp loads ahead
-constexpr float LEVEL_GAIN = 1.6776883602142334f;
 constexpr int LUT_BYTES = 256 * 256;
 constexpr int STAGES = 4;       // a warp's ring of steps
 constexpr int TILE_STAGE_BYTES = 16 * 32 * STEP_BLOCKS;
@@ -213,7 +217,7 @@ constexpr int mma_smem() {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
-  asm(
+  asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -222,11 +226,27 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4],
                                               uint32_t b0, uint32_t b1) {
-  asm(
+  asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%10, %10, %10, %10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// The fp16 parts of two scaled levels: cut towards zero, and the rest (2^-22 of the level and better).
+// The rest of a level that fp16 holds exactly is one step instead of zero, so that both parts have the
+// level's sign: an infinite input then gives an infinity of the right sign, where a rest of zero or of
+// the other sign would make NaN.
+__device__ __forceinline__ float below_exact(float v) {
+  const uint32_t bits = __float_as_uint(v);
+  return __uint_as_float((bits & 0x1FFFu) == 0 && v != 0.0f ? bits - 1 : bits);
+}
+__device__ __forceinline__ void split_levels(float v0, float v1, uint32_t& hi, uint32_t& lo) {
+  v0 = below_exact(v0);
+  v1 = below_exact(v1);
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(v1), "f"(v0));
+  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  lo = pack_half2(v0 - h.x, v1 - h.y);
 }
 
 struct Split {
@@ -263,12 +283,9 @@ __device__ __forceinline__ void load_scales(ScaleIn<H>& in, const Weight& w, con
   }
 }
 
-// x of one row (xp: at lane t's columns), the 16 columns of lane t in block b: 8 t .. 8 t + 7 of
-// both halves
-__device__ __forceinline__ void load_x(uint4 (&v)[2], const __half* xp, int b) {
-  const uint4* p = reinterpret_cast<const uint4*>(xp + b * 64);
-  v[0] = __ldg(p);
-  v[1] = __ldg(p + 4);
+// x of one row (xp: at lane t's columns), the 8 columns of lane t in a half of block b: 8 t .. 8 t + 7
+__device__ __forceinline__ uint4 load_x(const __half* xp, int b, int half) {
+  return __ldg(reinterpret_cast<const uint4*>(xp + b * 64) + 4 * half);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -375,27 +392,37 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1)
     first_of(first_tile);
     load_scales<GROUPED>(cur, w, sp, e, min(b_first + t, b_last - 1));
 #pragma unroll
-    for (int q = 0; q < NT; ++q) load_x(xv[q], xp[q], b_first);
+    for (int q = 0; q < NT; ++q) {
+      xv[q][0] = load_x(xp[q], b_first, 0);
+      xv[q][1] = load_x(xp[q], b_first, 1);
+    }
   }
+  // the levels' own scale: the largest magnitude to [2^14, 2^15), undone by the blocks' scales
+  float most = fabsf(w.levels ? __ldg(w.levels + (lane & 15)) : kNf4Levels[lane & 15]);
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+  float level_up, level_down;
+  power_scale(most, &level_up, &level_down);
   static_assert(32 * WARPS == 512 || 32 * WARPS == 256, "threads fill halves of the table's rows");
 #pragma unroll
   for (int half = threadIdx.x >> 8; half < 2; half += WARPS / 8) {
     const int i = threadIdx.x & 255;
-    const float hi = w.levels ? __ldg(w.levels + (i >> 4)) : kNf4Levels[i >> 4];
-    const float lo = w.levels ? __ldg(w.levels + (i & 15)) : kNf4Levels[i & 15];
-    const uint32_t pair = pack_half2(LEVEL_GAIN * hi, LEVEL_GAIN * lo);
-    const uint4 four = make_uint4(pair, pair, pair, pair);
+    const float v0 = w.levels ? __ldg(w.levels + (i >> 4)) : kNf4Levels[i >> 4];
+    const float v1 = w.levels ? __ldg(w.levels + (i & 15)) : kNf4Levels[i & 15];
+    uint32_t hi, lo;
+    split_levels(level_up * v0, level_up * v1, hi, lo);
+    const uint4 two = make_uint4(hi, lo, hi, lo);
 #pragma unroll
     for (int k = 0; k < 4; ++k)  // eight neighbours write eight different bank groups
-      reinterpret_cast<uint4*>(lut)[i * 16 + ((4 * half + k + i) & 7)] = four;
+      reinterpret_cast<uint4*>(lut)[i * 16 + ((4 * half + k + i) & 7)] = two;
     if (GROUPED && half == 0) code_s[i] = __ldg(w.code + i);
   }
   __syncthreads();
   // the pair of byte i of v: bytes (lane * 4, v.i, 0, 0) are the entry's offset
   const char* const lut_bytes = reinterpret_cast<const char*>(mv_smem);
-  const uint32_t lane4 = lane * 4;
+  const uint32_t lane8 = (lane & 15) * 8;  // a 64-bit read takes half a warp at a time
   auto level_pair = [&](uint32_t v, int i) {
-    return *reinterpret_cast<const uint32_t*>(lut_bytes + __byte_perm(v, lane4, 0x5504 | (i << 4)));
+    return *reinterpret_cast<const uint2*>(lut_bytes + __byte_perm(v, lane8, 0x5504 | (i << 4)));
   };
   const uint8_t* my_ring = rings + warp * (STAGES * STAGE_BYTES) + g * 128 + t * 4;
 
@@ -427,41 +454,56 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1)
           s = __fadd_rn(__fmul_rn(code_s[cur.a8[h]], cur.a2[h]), cur.o2[h]);
         else
           s = cur.s[h];
-        mine[h] = s * (1.0f / LEVEL_GAIN);
+        mine[h] = s * level_down;
       }
       const uint8_t* st = my_ring + stage * STAGE_BYTES;
       // block b + i of this step with its x in xv, which then gets that of block `ahead`
       auto block = [&](int i, int ahead) {
+        float c[NT][4];
+        uint2 e[2][4];
+        auto look = [&](int u) {  // the lookups of step u % 4 of row tile u / 4
+          const uint8_t* at = st + (u / 4) * TILE_STAGE_BYTES + (((2 * i + u % 4 / 2) ^ g) << 4);
+          const uint32_t wa = *reinterpret_cast<const uint32_t*>(at);
+          const uint32_t wb = *reinterpret_cast<const uint32_t*>(at + 8 * 128);
+          const int m = 2 * (u & 1);
+          e[u & 1][0] = level_pair(wa, m);
+          e[u & 1][1] = level_pair(wb, m);
+          e[u & 1][2] = level_pair(wa, m + 1);
+          e[u & 1][3] = level_pair(wb, m + 1);
+        };
+        look(0);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const float s0 = __shfl_sync(0xffffffffu, mine[2 * mt], i, 4);
-          const float s1 = __shfl_sync(0xffffffffu, mine[2 * mt + 1], i, 4);
-          uint32_t a[4][4];
+        for (int u = 0; u < 4 * MT; ++u) {
+          const int mt = u / 4, step = u % 4;
+          if (u + 1 < 4 * MT) look(u + 1);
+          const uint2* f = e[u & 1];
+          const uint32_t hi[4] = {f[0].x, f[1].x, f[2].x, f[3].x};
+          const uint32_t lo[4] = {f[0].y, f[1].y, f[2].y, f[3].y};
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint8_t* at = st + mt * TILE_STAGE_BYTES + (((2 * i + half) ^ g) << 4);
-            const uint32_t wa = *reinterpret_cast<const uint32_t*>(at);
-            const uint32_t wb = *reinterpret_cast<const uint32_t*>(at + 8 * 128);
+          for (int part = 0; part < 2; ++part)
 #pragma unroll
-            for (int m = 0; m < 2; ++m) {
-              a[2 * half + m][0] = level_pair(wa, 2 * m);
-              a[2 * half + m][1] = level_pair(wb, 2 * m);
-              a[2 * half + m][2] = level_pair(wa, 2 * m + 1);
-              a[2 * half + m][3] = level_pair(wb, 2 * m + 1);
+            for (int q = 0; q < NT; ++q) {
+              const uint4 v = xv[q][step / 2];
+              const uint32_t b0 = step & 1 ? v.z : v.x, b1 = step & 1 ? v.w : v.y;
+              if (step == 0 && part == 0)
+                mma_f16_first(c[q], lo, b0, b1);
+              else
+                mma_f16(c[q], part == 0 ? lo : hi, b0, b1);
             }
-          }
+          // this half of x is done with: that of the next block, which is needed half a block later
+          if (mt == MT - 1 && step % 2 == 1)
 #pragma unroll
-          for (int q = 0; q < NT; ++q) {
-            float c[4];
-            mma_f16_first(c, a[0], xv[q][0].x, xv[q][0].y);
-            mma_f16(c, a[1], xv[q][0].z, xv[q][0].w);
-            mma_f16(c, a[2], xv[q][1].x, xv[q][1].y);
-            mma_f16(c, a[3], xv[q][1].z, xv[q][1].w);
-            if (mt == MT - 1) load_x(xv[q], xp[q], ahead);
-            acc[mt][q][0] = fmaf(s0, c[0], acc[mt][q][0]);
-            acc[mt][q][1] = fmaf(s0, c[1], acc[mt][q][1]);
-            acc[mt][q][2] = fmaf(s1, c[2], acc[mt][q][2]);
-            acc[mt][q][3] = fmaf(s1, c[3], acc[mt][q][3]);
+            for (int q = 0; q < NT; ++q) xv[q][step / 2] = load_x(xp[q], ahead, step / 2);
+          if (step == 3) {
+            const float s0 = __shfl_sync(0xffffffffu, mine[2 * mt], i, 4);
+            const float s1 = __shfl_sync(0xffffffffu, mine[2 * mt + 1], i, 4);
+#pragma unroll
+            for (int q = 0; q < NT; ++q) {
+              acc[mt][q][0] = fmaf(s0, c[q][0], acc[mt][q][0]);
+              acc[mt][q][1] = fmaf(s0, c[q][1], acc[mt][q][1]);
+              acc[mt][q][2] = fmaf(s1, c[q][2], acc[mt][q][2]);
+              acc[mt][q][3] = fmaf(s1, c[q][3], acc[mt][q][3]);
+            }
           }
         }
       };
@@ -624,8 +666,8 @@ int run_mma(const __half* x, int64_t ld_x, int n_rows, const Weight& w, Split sp
   // ten shapes with every choice forced. In each round of tiles a warp works through its blocks
   // one after another, finishes the tile (its outputs divided over the warps that share it, whose
   // sums each of them reads) and, in a cluster, meets the other CTAs twice. (17920 x 1536, 32 rows:
-  // W = 2, one round of 12 blocks, 15.0 us; W = 4, two rounds of 6, 17.0. 1536 x 8960, 32 rows:
-  // clusters of 4 13.4 us, none 18.7. 3000 x 4096, 32 rows: none 11.6, clusters of 4 13.2.)
+  // W = 2, one round of 12 blocks, 21.6 us; W = 4, two rounds of 6, 23.9. 1536 x 8960, 32 rows:
+  // clusters of 2 18.7 us, none 28.6. 3000 x 4096, 32 rows: none 15.7, clusters of 2 17.3.)
   // Clusters of 4 find 33 places.
   constexpr int BLOCK = NT == 1 ? 640 : NT == 2 ? 910 : 1490, ROUND = NT == 1 ? 1600 : 2800;
   constexpr int OUTPUTS = 200, JOIN = NT == 1 ? 50 : 150, MEET = NT == 2 ? 2300 : 3200;
