@@ -171,8 +171,9 @@ int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, co
 // and between them small kernels that turn the rank-wide fp32 operands into 16-bit parts for the
 // tensor cores. Where the other operand is an fp16 activation and the result fp32 (inner, outer) they
 // are two fp16 parts of the operand scaled by a power of two that brings its largest element to
-// [2^14, 2^15): 2^-22 and better, at any size of the operand; the scale is one per 128 elements of the
-// reduction (and per adapter row for A and B). Where both operands are fp32 and the result is fp16 (up)
+// [2^14, 2^15), one for every rank and 128 elements of the reduction: 2^-22 of an element that is at least
+// 2^-17 of the largest of its 128, 2^-40 of that largest below, at any size of a rank beside the others (one
+// scale for all ranks of 128 rows left a rank of 2^-24 of its neighbour 2^-16 wrong). Where both operands are fp32 and the result is fp16 (up)
 // they are two bf16 parts without scale, and the product of the two small ones is left out: under
 // 2^-16 of each term, a sixteenth of the result's own rounding.
 //
@@ -193,8 +194,8 @@ struct Shape {
 //          128)][RP] undoes the scale.
 //   cat:   bf16 parts (hi | lo) of an adapter matrix with the rank in the columns (B, A^T), or of t or
 //          dt, in rows of up::chunks(RP) * 64 (what is behind the parts is not read).
-//   pair:  fp16 parts (hi | lo) of t or dt in rows of sums::pair_width(RP) (likewise), 128 rows scaled
-//          together; down [ceil(rows / 128)] undoes it.
+//   pair:  fp16 parts (hi | lo) of t or dt in rows of sums::pair_width(RP) (likewise), 128 rows of a rank
+//          scaled together; down [ceil(rows / 128)][RP] undoes it.
 struct Rows {
   __half* parts;
   float* down;
@@ -300,8 +301,8 @@ __global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(Matrix a, Matrix 
 }
 
 // ---- the operands made of t (or dt) ----------------------------------------------------------
-// t[n, j] = factor * (sum of the parts): a CTA per 128 rows, which share a scale. The pair is built
-// where it is wanted (out.pair not null).
+// t[n, j] = factor * (sum of the parts): a CTA per 128 rows, of which each rank has its own scale. The
+// pair is built where it is wanted (out.pair not null).
 constexpr int T_THREADS = 1024;
 
 template <int RP>
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(T_THREADS)
     t_parts_kernel(const float* __restrict__ part, int splits, int64_t n_rows,
                    float factor, TParts out) {
   extern __shared__ float t_smem[];  // [128][RP + 1]
-  __shared__ float warp_most[T_THREADS / 32];
+  __shared__ float scale_up[RP];
   grid_launch_dependents();
   grid_dependency_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -332,39 +333,49 @@ __global__ void __launch_bounds__(T_THREADS)
 #pragma unroll
       for (int u = 0; u < U; ++u) v[i] += x[i][u];
   }
-  float most = 0.0f;
 #pragma unroll
   for (int i = 0; i < E; ++i) {
     const int e = i * T_THREADS + threadIdx.x;
     t_smem[e / RP * (RP + 1) + e % RP] = v[i] * factor;
-    most = fmaxf(most, fabsf(v[i] * factor));
   }
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-  if (lane == 0) warp_most[warp] = most;
   __syncthreads();
+  if (out.pair != nullptr)
+    for (int j = warp; j < RP; j += T_THREADS / 32) {  // a warp per rank
+      float most = 0.0f;
 #pragma unroll
-  for (int i = 0; i < T_THREADS / 32; ++i) most = fmaxf(most, warp_most[i]);
-  float up, back;
-  power_scale(most, &up, &back);
+      for (int r = 0; r < 128; r += 32) most = fmaxf(most, fabsf(t_smem[(r + lane) * (RP + 1) + j]));
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+      float up, back;
+      power_scale(most, &up, &back);
+      if (lane == 0) {
+        scale_up[j] = up;
+        out.down[static_cast<int64_t>(blockIdx.x) * RP + j] = back;
+      }
+    }
   constexpr int PIECES = RP / 8;  // of eight ranks
   for (int i = threadIdx.x; i < 128 * PIECES; i += T_THREADS) {
     const int r = i / PIECES, j = (i % PIECES) * 8;
-    const int64_t n = row0 + r;
-    if (n >= n_rows) break;  // so are the rows behind it
+    if (row0 + r >= n_rows) break;  // so are the rows behind it
     float m[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) m[k] = t_smem[r * (RP + 1) + j + k];
-    put_cat(out.cat, n, j, RP, m);
-    if (out.pair == nullptr) continue;
+    put_cat(out.cat, row0 + r, j, RP, m);
+  }
+  if (out.pair == nullptr) return;
+  __syncthreads();
+  for (int i = threadIdx.x; i < 128 * PIECES; i += T_THREADS) {
+    const int r = i / PIECES, j = (i % PIECES) * 8;
+    if (row0 + r >= n_rows) break;
+    const float *m = t_smem + r * (RP + 1) + j, *up = scale_up + j;
     uint32_t hi[4], lo[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) split_f16(m[2 * k] * up, m[2 * k + 1] * up, hi[k], lo[k]);
-    uint4* row = out.pair + n * (sums::pair_width(RP) / 8);
+    for (int k = 0; k < 4; ++k)
+      split_f16(m[2 * k] * up[2 * k], m[2 * k + 1] * up[2 * k + 1], hi[k], lo[k]);
+    uint4* row = out.pair + (row0 + r) * (sums::pair_width(RP) / 8);
     row[j / 8] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
     row[PIECES + j / 8] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
-  if (threadIdx.x == 0 && out.pair != nullptr) out.down[blockIdx.x] = back;
 }
 
 // The weights' gradients: factor * (sum of the parts) as [rank, n] (A) or [n, rank] (B).
@@ -429,7 +440,7 @@ struct Saved {
   Saved(void* base, const Shape& s, int rp) : carve{static_cast<char*>(base), 0} {
     t.cat = nullptr;
     t.pair = carve.take<uint4>(static_cast<size_t>(s.n_rows) * (sums::pair_width(rp) / 8));
-    t.down = carve.take<float>(static_cast<size_t>((s.n_rows + 127) / 128));
+    t.down = carve.take<float>(static_cast<size_t>((s.n_rows + 127) / 128) * rp);
     b_rows.parts = carve.take<__half>(static_cast<size_t>(2 * rp) * s.n_out);
     b_rows.down = carve.take<float>(static_cast<size_t>((s.n_out + 127) / 128) * rp);
     a_cat = carve.take<uint4>(static_cast<size_t>(s.n_in) * up::chunks(rp) * 8);
@@ -459,7 +470,7 @@ struct BackwardWork {
   BackwardWork(void* base, const Shape& s, int rp) : carve{static_cast<char*>(base), 0} {
     dt.cat = carve.take<uint4>(static_cast<size_t>(s.n_rows) * up::chunks(rp) * 8);
     dt.pair = carve.take<uint4>(static_cast<size_t>(s.n_rows) * (sums::pair_width(rp) / 8));
-    dt.down = carve.take<float>(static_cast<size_t>((s.n_rows + 127) / 128));
+    dt.down = carve.take<float>(static_cast<size_t>((s.n_rows + 127) / 128) * rp);
     t_part = carve.take<float>(static_cast<size_t>(sums::Plan(false, false, s.n_rows, s.n_out).splits) *
                                s.n_rows * rp);
     b_part = carve.take<float>(static_cast<size_t>(sums::Plan(true, true, s.n_rows, s.n_out).splits) *

@@ -347,7 +347,7 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
 //   INNER:  part[split][n][j] = sum over the split's columns of X[n, c] W[j, c]
 //   OUTER:  part[split][j][c] = sum over the split's rows of X[n, c] T[n, j]
 // W (an adapter matrix) and T (t or dt) are fp32, scaled by powers of two (a scale for every 128 of the
-// reduction, for W one for each rank) and split in two fp16 parts that stand side by side as the n
+// reduction and each rank) and split in two fp16 parts that stand side by side as the n
 // operand (N = 2 RP), so that X passes the tensor core once; the epilogue adds the two halves of the
 // result. X is the 128-row m operand as it lies in memory: rows of it, K-major, for INNER, columns of
 // it, MN-major, for OUTER.
@@ -403,7 +403,7 @@ struct Params {
   int64_t n_rows;
   int n_cols;
   int steps, steps_per_split;  // 64-wide stages of the whole reduction, and of a split
-  const float* down;           // what undoes the scales: [blocks of 128] of T, [blocks][RP] of W
+  const float* down;           // what undoes the scales: [blocks of 128][RP]
   float* part;
   Dropout drop;
 };
@@ -515,7 +515,8 @@ __device__ __forceinline__ void sums_cta(const CUtensorMap& tm_x, const CUtensor
     const int flushes = (n_steps + FLUSH - 1) / FLUSH;
     bool ok = true;
     for (int f = 0; f < flushes; ++f) {
-      const float* down = p.down + (s0 / FLUSH + f) * (OUTER ? 1 : RP) + (OUTER ? 0 : q * HR);
+      const float4* down = reinterpret_cast<const float4*>(
+          p.down + static_cast<int64_t>(s0 / FLUSH + f) * RP + q * HR);
       ok = mbar_wait(&ctl->acc_full[f & 1], (f >> 1) & 1, abort);
       if (!__all_sync(0xffffffffu, ok)) {
         ok = false;
@@ -535,9 +536,14 @@ __device__ __forceinline__ void sums_cta(const CUtensorMap& tm_x, const CUtensor
         }
         tmem_wait_ld();
 #pragma unroll
-        for (int u = 0; u < STEP; ++u)
-          acc[j + u] = fmaf(__ldg(down + (OUTER ? 0 : j + u)),
-                            __uint_as_float(hi[u]) + __uint_as_float(lo[u]), acc[j + u]);
+        for (int u = 0; u < STEP; u += 4) {
+          const float4 scale = __ldg(down + (j + u) / 4);
+          const float by[4] = {scale.x, scale.y, scale.z, scale.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            acc[j + u + k] = fmaf(by[k], __uint_as_float(hi[u + k]) + __uint_as_float(lo[u + k]),
+                                  acc[j + u + k]);
+        }
       }
       tc_fence_before();
       __syncwarp();
