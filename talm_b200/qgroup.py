@@ -22,6 +22,7 @@ exact behaviour; the CUDA kernels they call are this package's own.
 """
 
 import contextlib
+import contextvars
 import os
 import weakref
 
@@ -446,22 +447,42 @@ def matvec(x, group, first, last=None, bias=None, adapter=None):
     return out.view(*x.shape[:-1], rows)
 
 
-_SERVING = {"rows": 0}
+class _Serving:
+    """The `serving` blocks that the current thread (or asyncio task) is in, the last entered one last.
+    ["rows"]: the limit that holds now."""
+
+    def __init__(self):
+        self._blocks = contextvars.ContextVar("talm_serving", default=())
+
+    def __getitem__(self, key):
+        blocks = self._blocks.get()
+        return blocks[-1][key] if blocks else 0
+
+    def enter(self, rows):
+        block = {"rows": rows}
+        self._blocks.set((*self._blocks.get(), block))
+        return block
+
+    def leave(self, block):
+        self._blocks.set(tuple(b for b in self._blocks.get() if b is not block))
+
+
+_SERVING = _Serving()
 
 
 @contextlib.contextmanager
 def serving(rows=MATVEC_MAX_ROWS):
-    """Within it, 4-bit projections called without gradients on at most `rows` rows take `matvec`
-    instead of the layer's dequantised buffer (`NF4Linear`, and `LoraLinear` with its adapter in
-    the same call). For the whole process, as torch's global switches are."""
+    """Within it, the 4-bit projections that ask for it (`NF4Linear`, and `LoraLinear` with its adapter in
+    the same call) take `matvec` instead of the layer's dequantised buffer where they are called without
+    gradients on at most `rows` rows. For the thread (or asyncio task) that enters it, as torch.no_grad
+    is: other threads keep their own route, whatever the order in which their blocks end."""
     if not 0 <= rows <= MATVEC_MAX_ROWS:
         raise ValueError(f"the few-row product takes 0..{MATVEC_MAX_ROWS} rows, got {rows}")
-    before = _SERVING["rows"]
-    _SERVING["rows"] = rows
+    block = _SERVING.enter(rows)
     try:
         yield
     finally:
-        _SERVING["rows"] = before
+        _SERVING.leave(block)
 
 
 def takes_matvec(x):
