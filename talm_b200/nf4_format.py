@@ -188,6 +188,17 @@ class NF4Linear(torch.nn.Module):
         return f"in_features={self.in_features}, out_features={self.out_features}, nf4"
 
 
+def is_plain(module):
+    """Whether calling `module` is NF4Linear.forward and nothing else: no forward hooks, its own or
+    torch's global ones, and no other forward on the class or the instance."""
+    hooks = torch.nn.modules.module
+    return (type(module).__call__ is torch.nn.Module.__call__
+            and getattr(type(module), "forward", None) is NF4Linear.forward
+            and "forward" not in module.__dict__
+            and not (module._forward_hooks or module._forward_pre_hooks
+                     or hooks._global_forward_hooks or hooks._global_forward_pre_hooks))
+
+
 def load_layer(source, prefix, device, projections=qgroup.PROJECTIONS):
     """The seven projections of the decoder layer stored under `prefix` ("model.layers.3."), as
     `NF4Linear` modules packed into one `LayerGroup` on `device`.

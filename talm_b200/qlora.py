@@ -58,7 +58,8 @@ class LoraLinear(torch.nn.Module):
     and no dropped copy kept); a branch that it does not take (another type, an adapter cast to
     fp16, a rank over 64) through `adapter.dropout` and the products above. Under `qgroup.serving`,
     a call without gradients and without dropout on a few rows is one product with base, bias and
-    (fp32) adapter in it."""
+    (fp32) adapter in it; a base with forward hooks (or a forward of its own) is called as a module, so
+    that they run, and the branch is added to its result."""
 
     def __init__(self, base, r, alpha, dropout, generator=None, b_std=0.0, fused=False):
         super().__init__()
@@ -85,8 +86,8 @@ class LoraLinear(torch.nn.Module):
     def forward(self, x):
         p = self.dropout if self.training else 0.0
         fp32 = self.lora_A.dtype is torch.float32 is self.lora_B.dtype  # what the kernels take
-        if p == 0 and fp32 and self.r <= adapter.MAX_RANK \
-                and isinstance(self.base, nf4_format.NF4Linear) and qgroup.takes_matvec(x):
+        if p == 0 and fp32 and self.r <= adapter.MAX_RANK and qgroup.takes_matvec(x) \
+                and nf4_format.is_plain(self.base):
             return self.base.matvec(x, (self.lora_A, self.lora_B, self.scaling))
         out = self.base(x)
         if self.fused:

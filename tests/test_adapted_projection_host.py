@@ -4,9 +4,10 @@ is refused, what a call leaves behind."""
 import threading
 from types import SimpleNamespace
 
+import pytest
 import torch
 
-from talm_b200 import qgroup
+from talm_b200 import nf4_format, qgroup, qlora
 
 
 def _served(rows=1):
@@ -62,3 +63,76 @@ def test_serving_blocks_that_end_out_of_order():
     assert _served(8)
     inner.__exit__(None, None, None)
     assert not _served()
+
+
+# ------------------------------------------------------------------------------------------
+# an adapted projection under serving
+# ------------------------------------------------------------------------------------------
+@pytest.fixture
+def served(monkeypatch):
+    """An adapted projection whose few-row product is a dense one on the CPU; `.calls` holds the
+    adapters it was given."""
+    g = torch.Generator().manual_seed(0)
+    w = torch.randn(8, 64, generator=g).half()
+    calls = []
+
+    def matvec(x, group, first, last=None, bias=None, adapter=None):
+        calls.append(adapter)
+        y = x.float() @ w.float().t()
+        if adapter is not None:
+            y = y + adapter[2] * (x.float() @ adapter[0].t()) @ adapter[1].t()
+        return y.half()
+
+    monkeypatch.setattr(qgroup, "matvec", matvec)
+    monkeypatch.setattr(qgroup, "takes_matvec", lambda x: not torch.is_grad_enabled())
+    base = nf4_format.NF4Linear(torch.zeros(8 * 32, dtype=torch.uint8),
+                                SimpleNamespace(shape=(8, 64)))
+    base._talm_group = (SimpleNamespace(biases=[None]), 0)
+    module = qlora.LoraLinear(base, 4, 8, 0.0, generator=g, b_std=0.1).eval()
+    module.calls = calls
+    return module
+
+
+def _call(module, x):
+    with torch.no_grad():
+        return module(x)
+
+
+def test_served_projection_is_one_product(served):
+    x = torch.randn(2, 64).half()
+    _call(served, x)
+    assert len(served.calls) == 1 and served.calls[0] is not None
+
+
+@pytest.mark.parametrize("kind", ["forward", "pre", "global", "global pre", "instance"])
+def test_served_projection_runs_the_base_hooks(served, kind):
+    """Hooks of the base projection see its call and its result, and what they return counts."""
+    x = torch.randn(2, 64).half()
+    seen = []
+    branch = _call(served, x).float()
+    base = served.base
+    calls = torch.nn.modules.module
+    if kind == "forward":
+        handle = base.register_forward_hook(lambda m, a, out: (seen.append(m), out * 0)[1])
+    elif kind == "pre":
+        handle = base.register_forward_pre_hook(lambda m, a: (seen.append(m), (a[0] * 0,))[1])
+    elif kind == "global":
+        handle = calls.register_module_forward_hook(
+            lambda m, a, out: (seen.append(m), out * 0)[1] if m is base else None)
+    elif kind == "global pre":
+        handle = calls.register_module_forward_pre_hook(
+            lambda m, a: (seen.append(m), (a[0] * 0,))[1] if m is base else None)
+    else:
+        forward = base.forward
+        base.forward = lambda v: (seen.append(base), forward(v) * 0)[1]
+        handle = SimpleNamespace(remove=lambda: base.__dict__.pop("forward"))
+    try:
+        got = _call(served, x).float()
+    finally:
+        handle.remove()
+    want = served.scaling * (x.float() @ served.lora_A.t()) @ served.lora_B.t()
+    assert seen == [base]
+    assert served.calls[-1] is None  # the base alone: the branch is added to what the hook returned
+    assert (got - want).norm() < 1e-2 * want.norm() < branch.norm()
+    _call(served, x)
+    assert served.calls[-1] is not None
