@@ -57,7 +57,7 @@ def nf4_matvec(x, packed, absmax, blocksize, out=None, bias=None, adapter=None):
     NF4 weight [out, in] (sizes from the packed bytes): the product that `nf4_dequantize` and a
     GEMM would give, with the weight read packed, not rounded to fp16, and never written. packed:
     uint8 of any shape, absmax: fp32 [ceil(n / blocksize)], bias: fp16 [out], adapter: (lora_A,
-    lora_B, scaling) as in `qgroup.matvec`; out: fp16 [rows, out] to write into."""
+    lora_B, scaling) as in `qgroup.matvec`; out: fp16 [rows, out] to write into. No gradient, as there."""
     n_cols = x.shape[-1]
     if absmax.dtype is not torch.float32 or packed.dtype is not torch.uint8:
         raise ValueError("packed must be uint8 and absmax fp32")

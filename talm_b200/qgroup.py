@@ -358,6 +358,11 @@ def run_matvec(x, packed, absmax8, absmax, code, absmax2, offset2, levels, row0,
     """The call of talm_nf4_matvec behind `launch_matvec`, `matvec` and `nf4_dequant.nf4_matvec`:
     x [rows, n_cols] from `_few_rows`, out [rows, n_rows], the weight's arrays checked by those."""
     n, device = x.shape[0], x.get_device()
+    if torch.is_grad_enabled() and (
+            x.requires_grad or out.requires_grad or (bias is not None and bias.requires_grad)
+            or (adapter is not None and (adapter[0].requires_grad or adapter[1].requires_grad))):
+        raise RuntimeError("the few-row product has no gradient: call it under torch.no_grad(), or use "
+                           "the projection's own forward")
     if out.dtype is not torch.float16 or out.shape != (n, n_rows):
         raise ValueError(f"out must be fp16 [{n}, {n_rows}]")
     ld_y = n_rows
@@ -412,8 +417,8 @@ def launch_matvec(x, packed, absmax8, code, absmax2, offset2, levels, out, row0,
     """x W^T (+ bias) (+ the adapter's branch) for at most 32 rows x [rows, n_cols] fp16 and the
     n_rows x n_cols weight whose packed bytes and coded scales are given (`row0`: the group-wide
     index of its first absmax row, which the second level is indexed by), into `out` [rows, n_rows]
-    fp16. The raw form of `matvec`, as `launch` is of `dequantize_all`; adapter = (lora_A [r,
-    n_cols], lora_B [n_rows, r], scaling), fp32."""
+    fp16. The raw form of `matvec`, as `launch` is of `dequantize_all` (no gradient either); adapter =
+    (lora_A [r, n_cols], lora_B [n_rows, r], scaling), fp32."""
     if qblock < 1 or qblock2 < 1 or row0 < 0 or n_rows < 0:
         raise ValueError("block sizes must be positive, row counts and indices not negative")
     n = n_rows * n_cols
@@ -437,7 +442,8 @@ def matvec(x, group, first, last=None, bias=None, adapter=None):
     alone): x [..., in] fp16 of at most 32 rows -> [..., sum of out]. The weights are read packed
     (a quarter of the fp16 bytes, none written) and not rounded to fp16 before the product; fp32
     sums, one rounding. `adapter` = (lora_A [r, in], lora_B [sum of out, r], scaling) adds its
-    branch before the rounding. No gradient: the serving form of GroupLinear."""
+    branch before the rounding. The serving form of GroupLinear: it has no gradient, and refuses
+    operands that ask for one outside torch.no_grad()."""
     last = first + 1 if last is None else last
     packed, absmax8, row0, rows, cols = _span(group, first, last)
     a = _few_rows(x, cols)

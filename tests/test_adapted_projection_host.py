@@ -7,7 +7,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from talm_b200 import nf4_format, qgroup, qlora
+from talm_b200 import nf4_dequant, nf4_format, qgroup, qlora
 
 
 def _served(rows=1):
@@ -136,3 +136,36 @@ def test_served_projection_runs_the_base_hooks(served, kind):
     assert (got - want).norm() < 1e-2 * want.norm() < branch.norm()
     _call(served, x)
     assert served.calls[-1] is not None
+
+
+# ------------------------------------------------------------------------------------------
+# refusals
+# ------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("which", ["x", "bias", "lora_A", "lora_B", "out"])
+def test_few_row_product_refuses_what_asks_for_a_gradient(which):
+    """A result without a graph would pass the gradient by: refused where one is wanted, for each operand
+    and entry; under no_grad the call goes on (to the next refusal, that of CPU tensors)."""
+    group = SimpleNamespace(
+        shapes=[(8, 64)], pair_bounds=[0, 256], row_bounds=[0, 8], qblock=64, qblock2=256,
+        packed=torch.zeros(256, dtype=torch.uint8), absmax8=torch.zeros(8, dtype=torch.uint8),
+        code=torch.zeros(256), absmax2=torch.zeros(1), offset2=torch.zeros(1),
+        levels=torch.tensor(qgroup.NF4_LEVELS))
+    t = {"x": torch.zeros(2, 64).half(), "bias": torch.zeros(8).half(),
+         "lora_A": torch.zeros(4, 64), "lora_B": torch.zeros(8, 4), "out": torch.zeros(2, 8).half()}
+    t[which].requires_grad_()
+
+    def calls():
+        extra = dict(bias=t["bias"], adapter=(t["lora_A"], t["lora_B"], 1.0))
+        yield lambda: nf4_dequant.nf4_matvec(t["x"], group.packed, torch.zeros(8), 64, out=t["out"],
+                                             **extra)
+        yield lambda: qgroup.launch_matvec(t["x"], group.packed, group.absmax8, group.code,
+                                           group.absmax2, group.offset2, group.levels, t["out"], 0, 8,
+                                           64, 64, 256, **extra)
+        if which != "out":
+            yield lambda: qgroup.matvec(t["x"], group, 0, **extra)
+
+    for call in calls():
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            call()
