@@ -154,7 +154,7 @@ int talm_nf4_linear(const uint16_t* a, int64_t ld_a, int64_t n_rows, const uint8
  *   bias     : fp16 [w_rows] or NULL
  *   lora_a, lora_b : fp32 [rank, w_cols], [w_rows, rank]; rank 0 = no adapter; `down`: a workspace
  *              of n_rows * rank floats (overwritten)
- *   y        : fp16 [n_rows, w_rows], row stride ld_y elements
+ *   y        : fp16 [n_rows, w_rows], row stride ld_y elements, apart from x
  * Preconditions: 0 <= n_rows <= 32, w_cols and blocksize even, 0 <= rank <= 64. Any alignment is
  * accepted. */
 int talm_nf4_matvec(const uint16_t* x, int64_t ld_x, int64_t n_rows, const uint8_t* packed,

@@ -350,6 +350,12 @@ def _few_rows(x, n_cols):
     return x
 
 
+def _share(n, x_ptr, ld_x, n_cols, out_ptr, ld_y, n_rows):
+    """Whether n fp16 rows of n_cols at x_ptr and n of n_rows at out_ptr may share memory."""
+    return (x_ptr < out_ptr + 2 * ((n - 1) * ld_y + n_rows)
+            and out_ptr < x_ptr + 2 * ((n - 1) * ld_x + n_cols))
+
+
 _NO_ADAPTER = (None, None, 0, 0.0, None)
 
 
@@ -370,6 +376,11 @@ def run_matvec(x, packed, absmax8, absmax, code, absmax2, offset2, levels, row0,
         ld_y = out.stride(0) if n > 1 else n_rows
         if (n_rows > 1 and out.stride(1) != 1) or ld_y < n_rows:
             raise ValueError("out must have rows of unit stride that do not overlap")
+    x_ptr, ld_x, out_ptr = x.data_ptr(), x.stride(0) if n > 1 else n_cols, out.data_ptr()
+    if _share(n, x_ptr, ld_x, n_cols, out_ptr, ld_y, n_rows):
+        # CTAs write their outputs while others still read x
+        x = x.clone(memory_format=torch.contiguous_format)
+        x_ptr, ld_x = x.data_ptr(), n_cols
     apart = not packed.get_device() == out.get_device() == device
     if absmax8 is None:
         apart = apart or absmax.get_device() != device
@@ -405,9 +416,8 @@ def run_matvec(x, packed, absmax8, absmax, code, absmax2, offset2, levels, row0,
         raise ValueError("the operands of the few-row product must be on one device")
     with _lib.device_of(x):
         _lib.check(_lib.load().talm_nf4_matvec(
-            x.data_ptr(), x.stride(0) if n > 1 else n_cols, n, packed.data_ptr(), *scales, row0,
-            n_rows, n_cols, blocksize, qblock2, bias_ptr, *extra, out.data_ptr(), ld_y,
-            _lib.raw_stream(x)), "talm_nf4_matvec")
+            x_ptr, ld_x, n, packed.data_ptr(), *scales, row0, n_rows, n_cols, blocksize, qblock2,
+            bias_ptr, *extra, out_ptr, ld_y, _lib.raw_stream(x)), "talm_nf4_matvec")
     RAN["matvec"] += 1
     return out
 
@@ -417,8 +427,8 @@ def launch_matvec(x, packed, absmax8, code, absmax2, offset2, levels, out, row0,
     """x W^T (+ bias) (+ the adapter's branch) for at most 32 rows x [rows, n_cols] fp16 and the
     n_rows x n_cols weight whose packed bytes and coded scales are given (`row0`: the group-wide
     index of its first absmax row, which the second level is indexed by), into `out` [rows, n_rows]
-    fp16. The raw form of `matvec`, as `launch` is of `dequantize_all` (no gradient either); adapter =
-    (lora_A [r, n_cols], lora_B [n_rows, r], scaling), fp32."""
+    fp16 (which may share x's memory). The raw form of `matvec`, as `launch` is of `dequantize_all`
+    (no gradient either); adapter = (lora_A [r, n_cols], lora_B [n_rows, r], scaling), fp32."""
     if qblock < 1 or qblock2 < 1 or row0 < 0 or n_rows < 0:
         raise ValueError("block sizes must be positive, row counts and indices not negative")
     n = n_rows * n_cols

@@ -169,3 +169,40 @@ def test_few_row_product_refuses_what_asks_for_a_gradient(which):
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
             call()
+
+
+# ------------------------------------------------------------------------------------------
+# memory that an output shares with the input
+# ------------------------------------------------------------------------------------------
+def test_outputs_in_the_inputs_memory_are_found():
+    buffer = torch.randn(4, 160).half()
+    x = buffer[:, :64]
+    flat = torch.randn(4 * 64 + 8).half()
+    square = flat[:256].view(4, 64)
+    for rows, out, shared in (
+            (square, square, True), (square, flat[8:264].view(4, 64), True),
+            (square[:1], square[:1], True), (x, buffer[:, 32:96], True),
+            (x, torch.empty(4, 64).half(), False), (square[:2], square[2:], False),
+            (square[2:], square[:2], False), (square[:0], square[:0], False)):
+        assert qgroup._share(rows.shape[0], rows.data_ptr(), rows.stride(0), 64, out.data_ptr(),
+                             out.stride(0), 64) == shared
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 9, 32])
+def test_product_written_over_its_input(rows):
+    """A square projection in place, and beside its input in one buffer: the bits of a separate one."""
+    g = torch.Generator().manual_seed(rows)
+    size = 1536
+    packed = torch.randint(0, 256, (size * size // 2,), generator=g, dtype=torch.uint8).cuda()
+    absmax = (torch.rand(size * size // 64, generator=g) * 0.05).cuda()
+    x = torch.randn(rows, size, generator=g).half().cuda()
+    for extra in (None, ((torch.randn(8, size, generator=g) * 0.02).cuda(),
+                         torch.randn(size, 8, generator=g).cuda(), 1.0)):
+        want = nf4_dequant.nf4_matvec(x, packed, absmax, 64, adapter=extra)
+        buffer = torch.zeros(rows, 2 * size, dtype=torch.float16, device="cuda")
+        for a, b in ((0, 0), (0, 8), (0, size), (size, 0)):
+            buffer[:, a:a + size] = x
+            nf4_dequant.nf4_matvec(buffer[:, a:a + size], packed, absmax, 64,
+                                   out=buffer[:, b:b + size], adapter=extra)
+            assert torch.equal(buffer[:, b:b + size], want), (a, b)
