@@ -257,8 +257,8 @@ def generate(model, input_ids, new_tokens):
     one pass over the prompt, then one token of every row per pass with the decoder's key-value
     cache, under `qgroup.serving`: in passes of at most 32 tokens each 4-bit projection is a few-row
     product with the packed weights, its adapter included. The model is in evaluation mode during
-    the call. Returns [B, S + new_tokens]."""
-    was_training = model.training
+    the call; every module is in its own mode again behind it. Returns [B, S + new_tokens]."""
+    was_training, modes = model.training, [(m, m.training) for m in model.modules()]
     model.eval()
     try:
         ids, step, cache = input_ids, input_ids, None
@@ -272,6 +272,8 @@ def generate(model, input_ids, new_tokens):
         return ids
     finally:
         model.train(was_training)
+        for module, training in modes:  # a part that was in another mode than the whole
+            module.training = training
 
 
 def causal_padding_mask(attention_mask):

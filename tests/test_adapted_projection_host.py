@@ -206,3 +206,40 @@ def test_product_written_over_its_input(rows):
             nf4_dequant.nf4_matvec(buffer[:, a:a + size], packed, absmax, 64,
                                    out=buffer[:, b:b + size], adapter=extra)
             assert torch.equal(buffer[:, b:b + size], want), (a, b)
+
+
+# ------------------------------------------------------------------------------------------
+# decoding
+# ------------------------------------------------------------------------------------------
+class _Counting(torch.nn.Module):
+    """Predicts each token's successor; fails at the token 9."""
+
+    def __init__(self):
+        super().__init__()
+        self.frozen, self.live = torch.nn.Dropout(0.5), torch.nn.Dropout(0.5)
+
+    def forward(self, input_ids, past_key_values, use_cache, logits_to_keep):
+        assert not (self.training or self.frozen.training or self.live.training)
+        assert use_cache and qgroup._SERVING["rows"] == qgroup.MATVEC_MAX_ROWS
+        last = input_ids[:, -1:]
+        if (last == 9).any():
+            raise RuntimeError("nine")
+        logits = torch.nn.functional.one_hot(last + 1, 16).float()
+        return SimpleNamespace(logits=logits, past_key_values=(past_key_values or 0) + 1)
+
+
+def test_generate_leaves_every_module_in_its_own_mode():
+    """A part in evaluation mode inside a model that trains stays there, also behind an error."""
+    model = _Counting().train()
+    model.frozen.eval()
+    ids = torch.tensor([[1, 2], [4, 3]])
+    assert qlora.generate(model, ids, 3).tolist() == [[1, 2, 3, 4, 5], [4, 3, 4, 5, 6]]
+    assert model.training and model.live.training and not model.frozen.training
+    with pytest.raises(RuntimeError, match="nine"):
+        qlora.generate(model, ids, 9)
+    assert model.training and model.live.training and not model.frozen.training
+    assert qgroup._SERVING["rows"] == 0
+    model.eval()
+    model.live.train()
+    assert torch.equal(qlora.generate(model, ids, 0), ids)
+    assert not model.training and model.live.training
