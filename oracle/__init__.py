@@ -10,18 +10,17 @@ library.
   oracle.head  torch CPU restatement of the fused head (solution/test_kernels.py:70-83,
                solution/test_fuzz.py:145-185, solution/fused_head.py:126-182)
 
-Pinning: both are checked against golden vectors that tests/golden/make_golden.py generated by
+  oracle.adapter  float64 restatement of the adapted 4-bit projection
+  oracle.ranks  how the ranks of a CPU test hand their results over
+
+Pinning: the first two are checked against golden vectors that tests/golden/make_golden.py generated by
 importing the reference's own Python functions (`_nf4_manual`, `reference_head`,
 `_head_reference`, `labelled_first`, `LayerGroup` packing) on CPU.
 """
 
 import multiprocessing
-import multiprocessing.util
-import time
 
-if multiprocessing.parent_process() is not None:
-    # A rank of a CPU test puts its tensors on a queue and exits, but the parent fetches them by file
-    # descriptor from the sender: a rank that has already gone leaves it without. The sender stays
-    # for a moment after its queue has been told to finish (10) and before the socket that the parent
-    # connects to is unlinked (0; finalizers of a lower priority run later).
-    multiprocessing.util.Finalize(None, time.sleep, args=(5,), exitpriority=5)
+if multiprocessing.parent_process() is not None:  # a rank of a CPU test
+    from . import ranks
+
+    ranks.send_by_value()
