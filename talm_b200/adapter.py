@@ -18,7 +18,7 @@ replay, and gradient checkpointing, which restores the generator, recomputes the
 
 The reference's adapter node (solution/lora.py:151-231) keeps the dropout's generator state and
 replays it in the backward; its products run in fp16. Here sums are fp32 and each fp16 result is
-rounded once. There is no CPU path.
+rounded once. There is no CPU path, and a failing call raises (no component is turned off by it).
 """
 
 import functools

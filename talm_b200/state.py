@@ -13,11 +13,12 @@ import torch
 
 DISABLED = {}
 
+# What may be recorded there. The opt-in operators beside these paths (qgroup.matvec, adapter.py) only
+# raise: the caller chose them, and nothing else is turned off by their failure.
 COMPONENTS = {
     "fused_head": "fused output head + cross-entropy (fused_head.py)",
     "qgroup": "grouped NF4 dequantisation of a decoder layer (qgroup.py)",
     "nf4_dequant": "per-projection NF4 dequantisation (nf4_dequant.py)",
-    "adapter": "LoRA branch and counter-based dropout (adapter.py)",
 }
 
 

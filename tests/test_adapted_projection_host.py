@@ -1,13 +1,15 @@
 """Host side of the adapted 4-bit projections, on CPU tensors (no kernel launches): who is served, what
 is refused, what a call leaves behind."""
 
+import os
+import re
 import threading
 from types import SimpleNamespace
 
 import pytest
 import torch
 
-from talm_b200 import nf4_dequant, nf4_format, qgroup, qlora
+from talm_b200 import nf4_dequant, nf4_format, qgroup, qlora, state
 
 
 def _served(rows=1):
@@ -243,3 +245,17 @@ def test_generate_leaves_every_module_in_its_own_mode():
     model.live.train()
     assert torch.equal(qlora.generate(model, ids, 0), ids)
     assert not model.training and model.live.training
+
+
+# ------------------------------------------------------------------------------------------
+# bookkeeping
+# ------------------------------------------------------------------------------------------
+def test_every_component_is_one_that_some_call_reports():
+    """The components of state.py are those that a call site records a failure of."""
+    package = os.path.dirname(state.__file__)
+    reported = set()
+    for name in os.listdir(package):
+        if name.endswith(".py"):
+            with open(os.path.join(package, name)) as f:
+                reported |= set(re.findall(r'fallback\("(\w+)"', f.read()))
+    assert reported == set(state.COMPONENTS)
