@@ -118,9 +118,16 @@ def stream_of(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# PyTorch's own short ways to the current stream and device, which its compiled code uses: a microsecond
+# each under the public ones, which serve where a version lacks them.
+_CURRENT_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None)
+
+
 def raw_stream(t):
     """The raw handle of the current stream of a CUDA tensor's device."""
-    return torch._C._cuda_getCurrentRawStream(t.get_device())
+    index = t.get_device()
+    return stream_of(index) if _CURRENT_STREAM is None else _CURRENT_STREAM(index)
 
 
 _HERE = contextlib.nullcontext()
@@ -130,7 +137,8 @@ def device_of(t):
     """A context in which the CUDA tensor's device is the current one (a launch takes the current
     device's kernels); free where it already is."""
     index = t.get_device()
-    return _HERE if index == torch._C._cuda_getDevice() else torch.cuda.device(index)
+    here = torch.cuda.current_device() if _CURRENT_DEVICE is None else _CURRENT_DEVICE()
+    return _HERE if index == here else torch.cuda.device(index)
 
 
 KERNEL_KINDS = ("head_slice", "head_combine", "head_reserved", "head_finalize", "head_merge",

@@ -9,7 +9,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from talm_b200 import nf4_dequant, nf4_format, qgroup, qlora, state
+from talm_b200 import _lib, nf4_dequant, nf4_format, qgroup, qlora, state
 
 
 def _served(rows=1):
@@ -259,3 +259,18 @@ def test_every_component_is_one_that_some_call_reports():
             with open(os.path.join(package, name)) as f:
                 reported |= set(re.findall(r'fallback\("(\w+)"', f.read()))
     assert reported == set(state.COMPONENTS)
+
+
+@pytest.mark.parametrize("short", [True, False])
+def test_stream_and_device_without_the_short_ways(monkeypatch, short):
+    """A PyTorch without the private calls is asked through the public ones."""
+    x = SimpleNamespace(get_device=lambda: 3)
+    entered = []
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d: SimpleNamespace(cuda_stream=100 + d))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: entered.append(d))
+    monkeypatch.setattr(_lib, "_CURRENT_STREAM", (lambda d: 200 + d) if short else None)
+    monkeypatch.setattr(_lib, "_CURRENT_DEVICE", (lambda: 5) if short else None)
+    assert _lib.raw_stream(x) == (203 if short else 103)
+    _lib.device_of(x)
+    assert entered == ([3] if short else [])
