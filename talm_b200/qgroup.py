@@ -290,6 +290,8 @@ class LayerGroup:
 def _span(group, first, last):
     """The packed bytes, coded scales, group-wide first absmax row and [rows, cols] of the
     adjacent projections first .. last - 1 (one weight of sum-of-rows x shared columns)."""
+    if not 0 <= first <= last <= len(group.shapes) or first == len(group.shapes):
+        raise IndexError(f"projections {first}..{last - 1} of a group of {len(group.shapes)}")
     cols = group.shapes[first][1]
     if any(group.shapes[i][1] != cols for i in range(first, last)):
         raise ValueError("projections of a span share their input size")

@@ -173,6 +173,24 @@ def test_few_row_product_refuses_what_asks_for_a_gradient(which):
             call()
 
 
+@pytest.mark.parametrize("first,last", [(-1, None), (-2, -1), (-1, 0), (0, 4), (3, None), (2, 1), (3, 3)])
+def test_spans_outside_the_group_are_refused(first, last):
+    """A negative index reaches a projection's shape but none of its bytes: the kernels would read
+    past the group's buffers."""
+    group = SimpleNamespace(
+        shapes=[(8, 64), (16, 64), (8, 64)], pair_bounds=[0, 256, 768, 1024],
+        row_bounds=[0, 8, 24, 32], qblock=64, qblock2=256, packed=torch.zeros(1024, dtype=torch.uint8),
+        absmax8=torch.zeros(32, dtype=torch.uint8), code=torch.zeros(256), absmax2=torch.zeros(1),
+        offset2=torch.zeros(1), levels=torch.tensor(qgroup.NF4_LEVELS))
+    x = torch.zeros(2, 64).half()
+    for call in (qgroup.matvec, qgroup.fused_linear):
+        with pytest.raises(IndexError, match="of a group of 3"):
+            call(x, group, first, last)
+    packed, absmax8, row0, rows, cols = qgroup._span(group, 1, 3)
+    assert (packed.numel(), absmax8.numel(), row0, rows, cols) == (768, 24, 8, 24, 64)
+    assert qgroup._span(group, 1, 1)[3] == 0
+
+
 # ------------------------------------------------------------------------------------------
 # memory that an output shares with the input
 # ------------------------------------------------------------------------------------------
