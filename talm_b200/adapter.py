@@ -204,7 +204,7 @@ def lora_branch(x, base, lora_A, lora_B, scaling, p=0.0, seed=None):
     if lora_A.shape != (rank, n_in) or lora_B.shape != (n_out, rank):
         raise ValueError(f"adapter {tuple(lora_A.shape)}, {tuple(lora_B.shape)} does not map "
                          f"{n_in} to {n_out}")
-    if not 1 <= rank <= MAX_RANK or n_in % 8 or n_out % 8:
+    if not 1 <= rank <= MAX_RANK or n_in < 8 or n_out < 8 or n_in % 8 or n_out % 8:
         raise ValueError(f"lora_branch needs a rank of 1..{MAX_RANK} and widths of multiples of "
                          f"8, got rank {rank}, {n_in} -> {n_out}")
     drop = drop_threshold(p)

@@ -9,7 +9,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from talm_b200 import _lib, nf4_dequant, nf4_format, qgroup, qlora, state
+from talm_b200 import _lib, adapter, nf4_dequant, nf4_format, qgroup, qlora, state
 
 
 def _served(rows=1):
@@ -189,6 +189,13 @@ def test_spans_outside_the_group_are_refused(first, last):
     packed, absmax8, row0, rows, cols = qgroup._span(group, 1, 3)
     assert (packed.numel(), absmax8.numel(), row0, rows, cols) == (768, 24, 8, 24, 64)
     assert qgroup._span(group, 1, 1)[3] == 0
+
+
+@pytest.mark.parametrize("n_in,n_out", [(0, 8), (8, 0), (0, 0)])
+def test_branch_of_no_columns_is_refused(n_in, n_out):
+    with pytest.raises(ValueError, match="multiples of 8"):
+        adapter.lora_branch(torch.zeros(4, n_in).half(), torch.zeros(4, n_out).half(),
+                            torch.zeros(2, n_in), torch.zeros(n_out, 2), 1.0)
 
 
 # ------------------------------------------------------------------------------------------
