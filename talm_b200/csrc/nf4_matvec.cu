@@ -10,9 +10,9 @@
 // the dequantised copy of a weight is, and its levels keep 22 bits and more of their fp32 values.
 //
 // Measured on one B200, calls replayed in a graph over two sets of inputs (29 MB: L2 holds them):
-// gate + up of the Qwen2.5-1.5B layer (17920 x 1536) for one row 9.6 us (14.2 MB, 1.5 TB/s; the floor
+// gate + up of the Qwen2.5-1.5B layer (17920 x 1536) for one row 9.7 us (14.2 MB, 1.5 TB/s; the floor
 // at the measured copy bandwidth is 2.2 us), k_proj 3.9 us, down_proj for 13 rows 11.5 us, down_proj
-// for 32 rows with an adapter of rank 64 21.1 us. Dequantising the layer and multiplying moves 117 MB
+// for 32 rows with an adapter of rank 64 19.1 us. Dequantising the layer and multiplying moves 117 MB
 // for the same 23 MB of weights.
 #include "common.cuh"
 
@@ -168,8 +168,8 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 }
 
 // ------------------------------------------------------------------------------------------
-// The main kernel: rows of whole 64-column blocks on the tensor cores (mma.sync m16n8k16, the
-// weight as the 16-row operand, up to 8 NT rows of x as the n operand).
+// The main kernel: rows of whole 64-column blocks on the tensor cores (mma.sync m16n8k16, eight
+// weight rows in two parts as the 16-row operand, up to 8 NT rows of x as the n operand).
 //
 // A warp takes tiles of 16 weight rows; lane (g, t) = (lane / 4, lane % 4) reads 8 packed bytes of
 // rows g and g + 8 per block (a quad reads a row's 32 bytes, lane t bytes 4 t .. 4 t + 3 of both
@@ -182,25 +182,29 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 // x, a quad's pieces side by side. A block's 64 columns have one scale per row: its mma's start from
 // zero and their result is added to the fp32 sum with one FMA per value, times the scale.
 //
-// A level has 24 bits and an fp16 operand 11, so a level is two parts (split_levels) and a step two mma's
-// against the same x. With one part, under the best common gain, outputs were 4 to 7 % farther from the exact
-// ones than their own rounding puts them, and a table other than NF4's could be off by 2^-11 of a term
-// or pass fp16's range; the second part costs twice the table's bytes and the mma's (17920 x 1536: one row
-// 7.6 -> 9.6 us, 32 rows 14.8 -> 21.6). The levels take a power of two that brings the largest to [2^14,
-// 2^15), undone by the scales: parts are exact to 2^-22 of a level that is at least 2^-17 of the largest, and
-// to 2^-40 of the largest below.
+// A level has 24 bits and an fp16 operand 11, so a level is two parts (split_levels): an mma takes eight
+// weight rows, the large parts as its upper eight operand rows and the small ones as the lower eight, and
+// the two halves of its result are added. With one part, under the best common gain, outputs were 4 to 7 %
+// farther from the exact ones than their own rounding puts them, and a table other than NF4's could be off
+// by 2^-11 of a term or pass fp16's range; the second part costs twice the table's bytes and the mma's
+// (17920 x 1536: one row 7.6 -> 9.7 us, 32 rows 14.8 -> 19.1; with 16 rows and one part per mma, whose
+// operands have to be gathered from the reads, 9.6 and 21.7). The levels take a power of two that brings the
+// largest to [2^14, 2^15), undone by the scales: parts are exact to 2^-22 of a level that is at least 2^-17
+// of the largest, and to 2^-40 of the largest below.
 //
 // From nine rows on (NT 2 and 4) a warp takes two such tiles, 32 weight rows, against the same x, and
 // a CTA has half as many warps with twice the registers: x is read half as often, and next to nothing
 // spills (17920 x 1536: 16 rows 15.5 us with one tile and 16 warps, 12.4 with two, 32 rows 23.4 and
-// 21.6). The table reads of a step are made before the mma's of the step before it, and each half of x is
-// replaced as soon as the block is done with it (32 rows 22.2 -> 21.6, one row 9.7 -> 9.6).
+// 21.7). The table reads of an mma are made before the mma's ahead of it, and each half of x is replaced as
+// soon as the block is done with it (32 rows 22.2 -> 21.7, one row 9.7 -> 9.6). Prefetching the next blocks
+// of x into L1 was slower (32 rows 19.1 -> 20.9).
 //
 // What bounds it: one row, the latency of dependent shared-memory reads at four warps per scheduler (by
 // count a block of a warp is 40 cycles of the SM's shared memory, 32 of them the table's: 7.3k of gate +
-// up's 18.6k); 32 rows, that and 64 mma's per 32 x 64 weights at two warps per scheduler (128 cycles of the
-// tensor cores: 11.6k of 41k). 32 warps of 64 registers were slower with half the table reads (9.7 us
-// against 7.9, spills), and so were entries 128 bytes apart (two operations per address).
+// up's 18.6k); 32 rows, 64 mma's per 32 x 64 weights (128 cycles of the tensor cores: 11.6k of 36k) and
+// the reads of x, at two warps per scheduler (copies without the small parts' mma's, and without the reads
+// of x, took 15.8 and 16.4 us of 21.7). 32 warps of 64 registers were slower with half the table reads (9.7
+// us against 7.9, spills), and so were entries 128 bytes apart (two operations per address).
 // ------------------------------------------------------------------------------------------
 // 16-row tiles of a warp, and the warps of a CTA
 __host__ __device__ constexpr int tiles_of(int nt) { return nt >= 2 ? 2 : 1; }
@@ -217,7 +221,7 @@ constexpr int mma_smem() {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -226,7 +230,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4],
                                               uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%10, %10, %10, %10};"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -459,51 +463,45 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1)
       const uint8_t* st = my_ring + stage * STAGE_BYTES;
       // block b + i of this step with its x in xv, which then gets that of block `ahead`
       auto block = [&](int i, int ahead) {
-        float c[NT][4];
-        uint2 e[2][4];
-        auto look = [&](int u) {  // the lookups of step u % 4 of row tile u / 4
-          const uint8_t* at = st + (u / 4) * TILE_STAGE_BYTES + (((2 * i + u % 4 / 2) ^ g) << 4);
-          const uint32_t wa = *reinterpret_cast<const uint32_t*>(at);
-          const uint32_t wb = *reinterpret_cast<const uint32_t*>(at + 8 * 128);
-          const int m = 2 * (u & 1);
-          e[u & 1][0] = level_pair(wa, m);
-          e[u & 1][1] = level_pair(wb, m);
-          e[u & 1][2] = level_pair(wa, m + 1);
-          e[u & 1][3] = level_pair(wb, m + 1);
+        // One mma takes eight weight rows: the large parts of their levels as the operand's upper eight
+        // rows, the small parts as the lower eight, so that a read of the table is two operand
+        // registers as it is. Unit u: row tile u / 8, its rows g + 8 (u % 2), step u / 2 % 4.
+        float c[2][NT][4];
+        uint2 e[2][2];
+        auto look = [&](int u) {
+          const int step = u / 2 % 4;
+          const uint32_t word = *reinterpret_cast<const uint32_t*>(
+              st + (u / 8) * TILE_STAGE_BYTES + (u % 2) * (8 * 128) + (((2 * i + step / 2) ^ g) << 4));
+          e[u & 1][0] = level_pair(word, 2 * (step & 1));
+          e[u & 1][1] = level_pair(word, 2 * (step & 1) + 1);
         };
         look(0);
 #pragma unroll
-        for (int u = 0; u < 4 * MT; ++u) {
-          const int mt = u / 4, step = u % 4;
-          if (u + 1 < 4 * MT) look(u + 1);
-          const uint2* f = e[u & 1];
-          const uint32_t hi[4] = {f[0].x, f[1].x, f[2].x, f[3].x};
-          const uint32_t lo[4] = {f[0].y, f[1].y, f[2].y, f[3].y};
+        for (int u = 0; u < 8 * MT; ++u) {
+          const int mt = u / 8, step = u / 2 % 4, h = u % 2;
+          if (u + 1 < 8 * MT) look(u + 1);
+          const uint32_t a[4] = {e[h][0].x, e[h][0].y, e[h][1].x, e[h][1].y};
 #pragma unroll
-          for (int part = 0; part < 2; ++part)
-#pragma unroll
-            for (int q = 0; q < NT; ++q) {
-              const uint4 v = xv[q][step / 2];
-              const uint32_t b0 = step & 1 ? v.z : v.x, b1 = step & 1 ? v.w : v.y;
-              if (step == 0 && part == 0)
-                mma_f16_first(c[q], lo, b0, b1);
-              else
-                mma_f16(c[q], part == 0 ? lo : hi, b0, b1);
-            }
+          for (int q = 0; q < NT; ++q) {
+            const uint4 v = xv[q][step / 2];
+            const uint32_t b0 = step & 1 ? v.z : v.x, b1 = step & 1 ? v.w : v.y;
+            if (step == 0)
+              mma_f16_first(c[h][q], a, b0, b1);
+            else
+              mma_f16(c[h][q], a, b0, b1);
+          }
           // this half of x is done with: that of the next block, which is needed half a block later
-          if (mt == MT - 1 && step % 2 == 1)
+          if (mt == MT - 1 && step % 2 == 1 && h == 1)
 #pragma unroll
             for (int q = 0; q < NT; ++q) xv[q][step / 2] = load_x(xp[q], ahead, step / 2);
           if (step == 3) {
-            const float s0 = __shfl_sync(0xffffffffu, mine[2 * mt], i, 4);
-            const float s1 = __shfl_sync(0xffffffffu, mine[2 * mt + 1], i, 4);
+            const float s = __shfl_sync(0xffffffffu, mine[2 * mt + h], i, 4);
 #pragma unroll
-            for (int q = 0; q < NT; ++q) {
-              acc[mt][q][0] = fmaf(s0, c[q][0], acc[mt][q][0]);
-              acc[mt][q][1] = fmaf(s0, c[q][1], acc[mt][q][1]);
-              acc[mt][q][2] = fmaf(s1, c[q][2], acc[mt][q][2]);
-              acc[mt][q][3] = fmaf(s1, c[q][3], acc[mt][q][3]);
-            }
+            for (int q = 0; q < NT; ++q)
+#pragma unroll
+              for (int k = 0; k < 2; ++k)
+                acc[mt][q][2 * h + k] =
+                    fmaf(s, c[h][q][k] + c[h][q][2 + k], acc[mt][q][2 * h + k]);
           }
         }
       };
@@ -663,11 +661,12 @@ int run_mma(const __half* x, int64_t ld_x, int n_rows, const Weight& w, Split sp
   const int sms = current_sm_count();
   if (sms <= 0) return set_error(TALM_ENODEV, "no CUDA device");
   // How many warps (and CTAs) share a tile's columns: the least time by a model in cycles, fitted to
-  // ten shapes with every choice forced. In each round of tiles a warp works through its blocks
+  // ten shapes with every choice forced (with one part per level; with two its choices are within 1 % of
+  // the best of 66 shapes but for two: 4736 x 64 at one row 3.6 against 3.2 us, 12000 x 2048 11.6 against 11.0). In each round of tiles a warp works through its blocks
   // one after another, finishes the tile (its outputs divided over the warps that share it, whose
   // sums each of them reads) and, in a cluster, meets the other CTAs twice. (17920 x 1536, 32 rows:
-  // W = 2, one round of 12 blocks, 21.6 us; W = 4, two rounds of 6, 23.9. 1536 x 8960, 32 rows:
-  // clusters of 2 18.7 us, none 28.6. 3000 x 4096, 32 rows: none 15.7, clusters of 2 17.3.)
+  // W = 2, one round of 12 blocks, 19.3 us; W = 4, two rounds of 6, 21.4. 1536 x 8960, 32 rows:
+  // clusters of 2 17.2 us, none 26.0. 3000 x 4096, 32 rows: none 14.4, clusters of 2 15.8.)
   // Clusters of 4 find 33 places.
   constexpr int BLOCK = NT == 1 ? 640 : NT == 2 ? 910 : 1490, ROUND = NT == 1 ? 1600 : 2800;
   constexpr int OUTPUTS = 200, JOIN = NT == 1 ? 50 : 150, MEET = NT == 2 ? 2300 : 3200;
