@@ -10,10 +10,11 @@
 // the dequantised copy of a weight is, and its levels keep 22 bits and more of their fp32 values.
 //
 // Measured on one B200, calls replayed in a graph over two sets of inputs (29 MB: L2 holds them):
-// gate + up of the Qwen2.5-1.5B layer (17920 x 1536) for one row 9.7 us (14.2 MB, 1.5 TB/s; the floor
-// at the measured copy bandwidth is 2.2 us), k_proj 3.9 us, down_proj for 13 rows 11.5 us, down_proj
-// for 32 rows with an adapter of rank 64 19.1 us. Dequantising the layer and multiplying moves 117 MB
-// for the same 23 MB of weights.
+// gate + up of the Qwen2.5-1.5B layer (17920 x 1536) for one row 9.3 us (14.2 MB, 1.5 TB/s; the
+// floor at the measured copy bandwidth is 2.2 us), k_proj 3.8 us, down_proj for 13 rows 11.2 us,
+// down_proj for 32 rows with an adapter of rank 64 16.7 us; with the weights from HBM (30 copies
+// and more) 11.7, 4.2, 14.2 and 18.2. Dequantising the layer and multiplying moves 117 MB for the
+// same 23 MB of weights.
 #include "common.cuh"
 
 namespace talm {
@@ -65,8 +66,8 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 // t = x A^T: a cluster takes 16 rows of A, its CTAs (DOWN_PARTS or fewer) a part of the columns
-// each, their warps share those; the CTAs add up their sums in rank order through each other's shared
-// memory. fp16 x is exact in tf32, A is split in two.
+// each, their warps share those; the CTAs add up their sums in rank order through each other's
+// shared memory. fp16 x is exact in tf32, A is split in two.
 constexpr int DOWN_WARPS = 16;
 constexpr int DOWN_PARTS = 8;
 
@@ -173,38 +174,41 @@ __global__ void __launch_bounds__(32 * DOWN_WARPS) adapter_down_kernel(
 //
 // A warp takes tiles of 16 weight rows; lane (g, t) = (lane / 4, lane % 4) reads 8 packed bytes of
 // rows g and g + 8 per block (a quad reads a row's 32 bytes, lane t bytes 4 t .. 4 t + 3 of both
-// halves) and turns each byte into the fp16 pairs of its two levels by one 64-bit shared-memory read: a
-// table of 256 entries, sixteen copies side by side, so that no two lanes of the half warp that such a
-// read takes at a time meet in a bank. Entries lie 256 bytes apart (the second 128 are not used), so that
-// one byte permutation makes the address: the packed byte above the lane's own eight-byte offset. The
-// reduction index may be permuted as long as both operands agree, so a lane's two runs of eight
-// consecutive weights go into four steps as they are and the matching operand is two 16-byte pieces of
-// x, a quad's pieces side by side. A block's 64 columns have one scale per row: its mma's start from
-// zero and their result is added to the fp32 sum with one FMA per value, times the scale.
+// halves) and turns each byte into the fp16 pairs of its two levels by one 64-bit shared-memory
+// read: a table of 256 entries, sixteen copies side by side, so that no two lanes of the half warp
+// that such a read takes at a time meet in a bank. Entries lie 256 bytes apart (the second 128 are
+// not used), so that one byte permutation makes the address: the packed byte above the lane's own
+// eight-byte offset. The reduction index may be permuted as long as both operands agree, so a
+// lane's two runs of eight consecutive weights go into four steps as they are and the matching
+// operand is two 16-byte pieces of x, a quad's pieces side by side. A block's 64 columns have one
+// scale per row: its mma's start from zero and their result is added to the fp32 sum with one FMA
+// per value, times the scale.
 //
-// A level has 24 bits and an fp16 operand 11, so a level is two parts (split_levels): an mma takes eight
-// weight rows, the large parts as its upper eight operand rows and the small ones as the lower eight, and
-// the two halves of its result are added. With one part, under the best common gain, outputs were 4 to 7 %
-// farther from the exact ones than their own rounding puts them, and a table other than NF4's could be off
-// by 2^-11 of a term or pass fp16's range; the second part costs twice the table's bytes and the mma's
-// (17920 x 1536: one row 7.6 -> 9.7 us, 32 rows 14.8 -> 19.1; with 16 rows and one part per mma, whose
-// operands have to be gathered from the reads, 9.6 and 21.7). The levels take a power of two that brings the
-// largest to [2^14, 2^15), undone by the scales: parts are exact to 2^-22 of a level that is at least 2^-17
-// of the largest, and to 2^-40 of the largest below.
+// A level has 24 bits and an fp16 operand 11, so a level is two parts (split_levels): an mma takes
+// eight weight rows, the large parts as its upper eight operand rows and the small ones as the
+// lower eight, and the two halves of its result are added. With one part, under the best common
+// gain, outputs were 4 to 7 % farther from the exact ones than their own rounding puts them, and a
+// table other than NF4's could be off by 2^-11 of a term or pass fp16's range; the second part
+// costs twice the table's bytes and the mma's (17920 x 1536: one row 7.6 -> 9.3 us, 32 rows 14.8 ->
+// 17.0). (16 rows and one part per mma, its operands gathered from the reads by moves: 32 rows 13 %
+// more.) The levels take a power of two that brings the largest to [2^14, 2^15), undone by the
+// scales: parts are exact to 2^-22 of a level that is at least 2^-17 of the largest, and to 2^-40
+// of the largest below.
 //
-// From nine rows on (NT 2 and 4) a warp takes two such tiles, 32 weight rows, against the same x, and
-// a CTA has half as many warps with twice the registers: x is read half as often, and next to nothing
-// spills (17920 x 1536: 16 rows 15.5 us with one tile and 16 warps, 12.4 with two, 32 rows 23.4 and
-// 21.7). The table reads of an mma are made before the mma's ahead of it, and each half of x is replaced as
-// soon as the block is done with it (32 rows 22.2 -> 21.7, one row 9.7 -> 9.6). Prefetching the next blocks
-// of x into L1 was slower (32 rows 19.1 -> 20.9).
+// From nine rows on (NT 2 and 4) a warp takes two such tiles, 32 weight rows, against the same x,
+// and a CTA has half as many warps with twice the registers: x is read half as often (with one tile
+// and 16 warps 17920 x 1536 took a quarter more at 16 rows, 8 % more at 32). The table reads of an
+// mma are made before the mma's ahead of it, and each half of x is replaced as soon as the block is
+// done with it. A step's blocks are a loop: as four copies of a block the kernel spilled and waited
+// for instructions (32 rows 19.1 -> 17.0 us, one row 9.7 -> 9.3). Prefetching the next blocks of x
+// into L1 was slower (32 rows 19.1 -> 20.9).
 //
-// What bounds it: one row, the latency of dependent shared-memory reads at four warps per scheduler (by
-// count a block of a warp is 40 cycles of the SM's shared memory, 32 of them the table's: 7.3k of gate +
-// up's 18.6k); 32 rows, 64 mma's per 32 x 64 weights (128 cycles of the tensor cores: 11.6k of 36k) and
-// the reads of x, at two warps per scheduler (copies without the small parts' mma's, and without the reads
-// of x, took 15.8 and 16.4 us of 21.7). 32 warps of 64 registers were slower with half the table reads (9.7
-// us against 7.9, spills), and so were entries 128 bytes apart (two operations per address).
+// What bounds it: one row, the latency of dependent shared-memory reads at four warps per scheduler
+// (by count a block of a warp is 40 cycles of the SM's shared memory, 32 of them the table's: 7.3k
+// of gate + up's 17.8k); 32 rows, 64 mma's per 32 x 64 weights (128 cycles of the tensor cores:
+// 11.6k of 32k) and the reads of x, at two warps per scheduler. 32 warps of 64 registers were
+// slower with half the table reads (9.7 us against 7.9, spills), and so were entries 128 bytes
+// apart (two operations per address).
 // ------------------------------------------------------------------------------------------
 // 16-row tiles of a warp, and the warps of a CTA
 __host__ __device__ constexpr int tiles_of(int nt) { return nt >= 2 ? 2 : 1; }
@@ -237,10 +241,10 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-// The fp16 parts of two scaled levels: cut towards zero, and the rest (2^-22 of the level and better).
-// The rest of a level that fp16 holds exactly is one step instead of zero, so that both parts have the
-// level's sign: an infinite input then gives an infinity of the right sign, where a rest of zero or of
-// the other sign would make NaN.
+// The fp16 parts of two scaled levels: cut towards zero, and the rest (2^-22 of the level and
+// better). The rest of a level that fp16 holds exactly is one step instead of zero, so that both
+// parts have the level's sign: an infinite input then gives an infinity of the right sign, where a
+// rest of zero or of the other sign would make NaN.
 __device__ __forceinline__ float below_exact(float v) {
   const uint32_t bits = __float_as_uint(v);
   return __uint_as_float((bits & 0x1FFFu) == 0 && v != 0.0f ? bits - 1 : bits);
@@ -287,7 +291,8 @@ __device__ __forceinline__ void load_scales(ScaleIn<H>& in, const Weight& w, con
   }
 }
 
-// x of one row (xp: at lane t's columns), the 8 columns of lane t in a half of block b: 8 t .. 8 t + 7
+// x of one row (xp: at lane t's columns), the 8 columns of lane t in a half of block b: 8 t .. 8 t
+// + 7
 __device__ __forceinline__ uint4 load_x(const __half* xp, int b, int half) {
   return __ldg(reinterpret_cast<const uint4*>(xp + b * 64) + 4 * half);
 }
@@ -463,9 +468,10 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1)
       const uint8_t* st = my_ring + stage * STAGE_BYTES;
       // block b + i of this step with its x in xv, which then gets that of block `ahead`
       auto block = [&](int i, int ahead) {
-        // One mma takes eight weight rows: the large parts of their levels as the operand's upper eight
-        // rows, the small parts as the lower eight, so that a read of the table is two operand
-        // registers as it is. Unit u: row tile u / 8, its rows g + 8 (u % 2), step u / 2 % 4.
+        // One mma takes eight weight rows: the large parts of their levels as the operand's upper
+        // eight rows, the small parts as the lower eight, so that a read of the table is two
+        // operand registers as it is. Unit u: row tile u / 8, its rows g + 8 (u % 2), step u / 2 %
+        // 4.
         float c[2][NT][4];
         uint2 e[2][2];
         auto look = [&](int u) {
@@ -506,15 +512,9 @@ __global__ void __launch_bounds__(32 * warps_of(NT), 1)
         }
       };
       const int behind = more ? n_b : b;  // whose x is loaded behind this step's
-      if (b + STEP_BLOCKS <= b_last) {
-        block(0, b + 1);
-        block(1, b + 2);
-        block(2, b + 3);
-        block(3, behind);
-      } else {  // the share's ragged end
+      const int n_here = min(STEP_BLOCKS, b_last - b);
 #pragma unroll 1
-        for (int i = 0; b + i < b_last; ++i) block(i, b + i + 1 < b_last ? b + i + 1 : behind);
-      }
+      for (int i = 0; i < n_here; ++i) block(i, i + 1 < n_here ? b + i + 1 : behind);
       __syncwarp();  // the stage has been read; the next fetch may fill it
       stage = stage + 1 == STAGES ? 0 : stage + 1;
       cur = next;
@@ -660,14 +660,14 @@ int run_mma(const __half* x, int64_t ld_x, int n_rows, const Weight& w, Split sp
   }
   const int sms = current_sm_count();
   if (sms <= 0) return set_error(TALM_ENODEV, "no CUDA device");
-  // How many warps (and CTAs) share a tile's columns: the least time by a model in cycles, fitted to
-  // ten shapes with every choice forced (with one part per level; with two its choices are within 1 % of
-  // the best of 66 shapes but for two: 4736 x 64 at one row 3.6 against 3.2 us, 12000 x 2048 11.6 against 11.0). In each round of tiles a warp works through its blocks
-  // one after another, finishes the tile (its outputs divided over the warps that share it, whose
-  // sums each of them reads) and, in a cluster, meets the other CTAs twice. (17920 x 1536, 32 rows:
-  // W = 2, one round of 12 blocks, 19.3 us; W = 4, two rounds of 6, 21.4. 1536 x 8960, 32 rows:
-  // clusters of 2 17.2 us, none 26.0. 3000 x 4096, 32 rows: none 14.4, clusters of 2 15.8.)
-  // Clusters of 4 find 33 places.
+  // How many warps (and CTAs) share a tile's columns: the least time by a model in cycles, fitted
+  // to ten shapes with every choice forced (with one part per level; with two its choices are
+  // within 4 % of the best of 66 shapes but for 4736 x 64 at one and eight rows, 3.5 against 3.1
+  // us). In each round of tiles a warp works through its blocks one after another, finishes the
+  // tile (its outputs divided over the warps that share it, whose sums each of them reads) and, in
+  // a cluster, meets the other CTAs twice. (17920 x 1536, 32 rows: W = 2, one round of 12 blocks,
+  // 17.2 us; W = 4, two rounds of 6, 18.6. 1536 x 8960, 32 rows: clusters of 4 15.0 us, none 23.4.
+  // 3000 x 4096, 32 rows: none 13.2, clusters of 2 13.7.) Clusters of 4 find 33 places.
   constexpr int BLOCK = NT == 1 ? 640 : NT == 2 ? 910 : 1490, ROUND = NT == 1 ? 1600 : 2800;
   constexpr int OUTPUTS = 200, JOIN = NT == 1 ? 50 : 150, MEET = NT == 2 ? 2300 : 3200;
   int64_t least = -1;
