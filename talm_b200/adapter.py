@@ -8,8 +8,10 @@
 Both are autograd functions over the kernels of csrc/adapter.cu. The mask of a call is a function of
 its seed and of the element's place in row-major order (Philox4x32 with 7 rounds; element e of `x` is
 kept when the low 15 bits of half e % 8 of counter e / 8 reach round(p * 32768)), so the backward
-pass makes it again instead of reading it: the branch saves its input, the rank-wide product and the
-seed, no dropped copy of the input and no mask. The probability is thereby rounded to a multiple of
+pass makes it again instead of reading it: no dropped copy of the input and no mask are kept. With
+the rank rounded up to R = 16, 32 or 64, the branch saves its input, the seed, the rank-wide product
+(max(128, 4 R) bytes a row and R / 32 for its scales) and the adapter as it was, in the kernels' parts
+(4 R bytes per output and max(128, 4 R) per input column). The probability is thereby rounded to a multiple of
 1 / 32768; the factor 32768 / (32768 - drop) is that of the rounded one, which keeps the expectation.
 
 The seed is a one-element int64 tensor on the device. `draw_seed` fills it from torch's own CUDA
@@ -18,7 +20,8 @@ replay, and gradient checkpointing, which restores the generator, recomputes the
 
 The reference's adapter node (solution/lora.py:151-231) keeps the dropout's generator state and
 replays it in the backward; its products run in fp16. Here sums are fp32 and each fp16 result is
-rounded once. There is no CPU path, and a failing call raises (no component is turned off by it).
+rounded once. There is no CPU path, a failing call raises (no component is turned off by it), and
+like GroupLinear neither function takes part in torch.func's transforms, which refuse it.
 """
 
 import functools

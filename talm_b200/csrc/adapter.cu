@@ -49,9 +49,10 @@ __device__ __forceinline__ uint32_t scale2(uint32_t v, float f, __nv_bfloat16) {
 }
 
 // The flattened tensor on 16-byte boundaries: a thread takes UNROLL groups of eight elements, their
-// loads first. Bound by HBM: 16384 x 8960 bf16, forward and backward, 200 us (1.17 GB, 5.9 TB/s, 0.90 of
-// the measured copy); a group costs 14 multiplications and about 100 operations in all, 46 % of the
-// ALU's rate at that speed (10 rounds, or 32 bits per element, would be the bound themselves).
+// loads first. Bound by HBM: 16384 x 8960 bf16, forward and backward, 200 us (1.17 GB, 5.9 TB/s,
+// 0.90 of the measured copy); a group costs 14 multiplications and about 100 operations in all, 46
+// % of the ALU's rate at that speed (10 rounds, or 32 bits per element, would be the bound
+// themselves).
 template <class T, int UNROLL, bool WIDE>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, int64_t n,
                                                       Dropout d, T* __restrict__ y) {
@@ -106,7 +107,10 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, i
   }
 }
 
-// Any strides and alignment: one thread per group of eight elements in row-major order.
+// Any strides and alignment: one thread per group of eight elements in row-major order, an element
+// at a time (a row may start anywhere in a group and off any boundary). Bound by its scalar loads
+// and stores: rows of a wider tensor, 16384 x 8960, one pass 410 us in 16 bits (flat 100), 686 in
+// fp32 (flat 208); 2048 x 1536 11 us (flat 3.7).
 template <class T>
 __global__ void __launch_bounds__(256) dropout_rows_kernel(const T* __restrict__ x, int64_t ld_x,
                                                            int64_t n_cols, int64_t n, Dropout d,
@@ -169,18 +173,20 @@ int run_dropout(const void* x_, int64_t ld_x, int64_t n_rows, int64_t n_cols, co
 //   outer   dA = dt^T keep x and dB = s g^T t        sums over its rows
 //   up      y = base + s t B^T and dx = keep dt A    sums over the rank
 // and between them small kernels that turn the rank-wide fp32 operands into 16-bit parts for the
-// tensor cores. Where the other operand is an fp16 activation and the result fp32 (inner, outer) they
-// are two fp16 parts of the operand scaled by a power of two that brings its largest element to
-// [2^14, 2^15), one for every rank and 128 elements of the reduction: 2^-22 of an element that is at least
-// 2^-17 of the largest of its 128, 2^-40 of that largest below, at any size of a rank beside the others (one
-// scale for all ranks of 128 rows left a rank of 2^-24 of its neighbour 2^-16 wrong). Where both operands are fp32 and the result is fp16 (up)
-// they are two bf16 parts without scale, and the product of the two small ones is left out: under
-// 2^-16 of each term, a sixteenth of the result's own rounding.
+// tensor cores. Where the other operand is an fp16 activation and the result fp32 (inner, outer)
+// they are two fp16 parts of the operand scaled by a power of two that brings its largest element
+// to [2^14, 2^15), one for every rank and 128 elements of the reduction: 2^-22 of an element that
+// is at least 2^-17 of the largest of its 128, 2^-40 of that largest below, at any size of a rank
+// beside the others (one scale for all ranks of 128 rows left a rank of 2^-24 of its neighbour
+// 2^-16 wrong). Where both operands are fp32 and the result is fp16 (up) they are two bf16 parts
+// without scale, and the product of the two small ones is left out: under 2^-16 of each term, a
+// sixteenth of the result's own rounding.
 //
-// Measured on one B200, forward and backward replayed in a graph: q_proj of 2048 rows, rank 16, 39 us (38
-// MB; nine launches of about 4 us each are the bound), 16384 x 1536 to 8960, rank 64, 304 us (1.04 GB,
-// 3.4 TB/s, 0.52 of the measured copy: g is read twice, once for dt and once for dB, 45 us that the
-// floor does not have, and the masked passes by the generator; the others run at 0.8 to 0.95).
+// Measured on one B200, forward and backward replayed in a graph: q_proj of 2048 rows, rank 16, 39
+// us (38 MB; nine launches of about 4 us each are the bound), 16384 x 1536 to 8960, rank 64, 305 us
+// (1.04 GB, 3.4 TB/s, 0.52 of the measured copy: g is read twice, once for dt and once for dB, 45
+// us that the floor does not have, and the masked passes, 74 us for 23 us of bytes, wait for their
+// masks; y runs at 0.9).
 // ------------------------------------------------------------------------------------------
 struct Shape {
   int64_t n_rows, n_in, n_out;
@@ -228,8 +234,8 @@ struct Matrix {
   int n;
 };
 
-// The operands of one matrix: rows for the sums, cat for the rank-wide product; null where it is not
-// wanted.
+// The operands of one matrix: rows for the sums, cat for the rank-wide product; null where it is
+// not wanted.
 struct Operands {
   Rows rows;
   uint4* cat;
@@ -301,8 +307,8 @@ __global__ void __launch_bounds__(PREP_THREADS) prepare_kernel(Matrix a, Matrix 
 }
 
 // ---- the operands made of t (or dt) ----------------------------------------------------------
-// t[n, j] = factor * (sum of the parts): a CTA per 128 rows, of which each rank has its own scale. The
-// pair is built where it is wanted (out.pair not null).
+// t[n, j] = factor * (sum of the parts): a CTA per 128 rows, of which each rank has its own scale.
+// The pair is built where it is wanted (out.pair not null).
 constexpr int T_THREADS = 1024;
 
 template <int RP>

@@ -1,10 +1,10 @@
 // The adapter's rank-wide product on tcgen05: for an activation of n_rows x n_cols,
 //   ADD:   y  = fp16(base + scale * T M^T)       (the branch's output: T = t, M = B)
 //   MASK:  dx = fp16(keep(...) * scale * T M^T)  (the input's gradient: T = dt, M = A^T)
-// T [n_rows, rank] and M [n_cols, rank] are fp32, each split in two bf16 parts that stand side by side
-// in rows (hi | lo); a 16-rank slice is three tcgen05 steps, lo hi + hi lo + hi hi (the fourth is
-// under 2^-16 of a term). (The 16 x 8 x 16 mma.sync form of the same product needed 96 mma's and 40
-// 16-byte loads per 16 x 64 outputs at rank 64, and took 300 us for 16384 x 8960 outputs.)
+// T [n_rows, rank] and M [n_cols, rank] are fp32, each split in two bf16 parts that stand side by
+// side in rows (hi | lo); a 16-rank slice is three tcgen05 steps, lo hi + hi lo + hi hi (the fourth
+// is under 2^-16 of a term). (The 16 x 8 x 16 mma.sync form of the same product needed 96 mma's and
+// 40 16-byte loads per 16 x 64 outputs at rank 64, and took 300 us for 16384 x 8960 outputs.)
 //
 // Bound by HBM: base is read and y written once (4 bytes per output). A persistent CTA walks 128 x
 // 128 tiles down the rows of a column tile, whose M stays in shared memory:
@@ -17,10 +17,10 @@
 //               mask) -> fp16, in place in the box's slot
 // Every wait is bounded; a wait that gives up ends the CTA's roles and records TALM_ETIMEOUT.
 //
-// Measured: ADD 16384 x 8960 at rank 64 100 us (587 MB, 5.9 TB/s, 0.90 of the measured copy); with T
-// loaded three parts wide and two stages it was 118 us, the MMA issuer waiting for T a third of the
-// time. MASK 16384 x 1536 25 us: 7.7 us of bytes; the generator and the conversions of 128 x 128 outputs
-// per CTA take the rest.
+// Measured: ADD 16384 x 8960 at rank 64 100 us (587 MB, 5.9 TB/s, 0.90 of the measured copy); with
+// T loaded three parts wide and two stages it was 118 us, the MMA issuer waiting for T a third of
+// the time. MASK 16384 x 1536 25 us: 7.7 us of bytes; the generator and the conversions of 128 x
+// 128 outputs per CTA take the rest.
 #pragma once
 
 #include "adapter_common.cuh"
@@ -346,11 +346,11 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
 // The adapter's sums over an activation X [n_rows, n_cols] on tcgen05, X optionally dropped out:
 //   INNER:  part[split][n][j] = sum over the split's columns of X[n, c] W[j, c]
 //   OUTER:  part[split][j][c] = sum over the split's rows of X[n, c] T[n, j]
-// W (an adapter matrix) and T (t or dt) are fp32, scaled by powers of two (a scale for every 128 of the
-// reduction and each rank) and split in two fp16 parts that stand side by side as the n
-// operand (N = 2 RP), so that X passes the tensor core once; the epilogue adds the two halves of the
-// result. X is the 128-row m operand as it lies in memory: rows of it, K-major, for INNER, columns of
-// it, MN-major, for OUTER.
+// W (an adapter matrix) and T (t or dt) are fp32, scaled by powers of two (a scale for every 128 of
+// the reduction and each rank) and split in two fp16 parts that stand side by side as the n operand
+// (N = 2 RP), so that X passes the tensor core once; the epilogue adds the two halves of the
+// result. X is the 128-row m operand as it lies in memory: rows of it, K-major, for INNER, columns
+// of it, MN-major, for OUTER.
 //
 // Bound by HBM: X is read once (2 bytes per element, 4 RP flops). One CTA per 128 rows (INNER) or
 // columns (OUTER) and split, stages of 64 of the reduction:
@@ -361,11 +361,14 @@ int launch(const void* t_op, const void* m_op, const void* base, int64_t ld_base
 //   warps 12-19   (MASK) drop X in shared memory before it is multiplied: a 16-byte piece is one
 //                 group of the generator
 //
-// Measured at rank 64: dB of 16384 x 8960 47 us (294 MB, 6.2 TB/s, 0.95 of the measured copy), dt 55 us
-// (its W, 2.3 MB, is read again by every 128 rows), both in one launch 100 us; with the dropout of 16384
-// x 1536 t 28 us and dA 22 us (7.7 us of bytes; of the 1600 cycles a stage takes a mask warp, 850 are the
-// generator's and 380 the and; 16 mask warps or its products as whole 64-bit ones changed nothing). The
-// mma.sync form of the same sums took 276, 171, 70 and 74 us.
+// Measured at rank 64, captures with cold caches: dt and dB of 16384 x 8960 in one launch 98 to 100
+// us (g is 294 MB and read for each; 493 MB of the 588 come from HBM), dB by itself, where no dt is
+// wanted, 66 us (its splits are those of the pair, so that it has the pair's bits); with the
+// dropout of 16384 x 1536 t 25 to 27 us and dA 22 to 23 (7.7 us of bytes): of the 1600 cycles that
+// a stage takes a mask warp, 850 go into the generator and 380 into the and, at 45 % of the issue
+// slots: latency with eight mask warps per SM, not the generator's own rate (some 9 us in all); 16
+// mask warps or its products as whole 64-bit ones changed nothing. The mma.sync form of t, dt, dB
+// and dA took 70, 171, 276 and 74 us.
 namespace sums {
 
 constexpr int TILE = 128;
@@ -569,9 +572,9 @@ __device__ __forceinline__ void sums_cta(const CUtensorMap& tm_x, const CUtensor
     const uint32_t bias2 = keep_bias2(p.drop.drop);
     constexpr int U = X_BYTES / 16 / (32 * MASK_WARPS);  // pieces of a thread
     constexpr int LINES = 32 * MASK_WARPS / 8;           // between a thread's pieces
-    // A piece is a group of eight columns of line id / 8 + u * LINES of the stage; a line is 128 bytes:
-    // a row of INNER's 64 columns; OUTER: row + 64 * (column group). q[u]: the group's number, which
-    // moves on by a constant from stage to stage.
+    // A piece is a group of eight columns of line id / 8 + u * LINES of the stage; a line is 128
+    // bytes: a row of INNER's 64 columns; OUTER: row + 64 * (column group). q[u]: the group's
+    // number, which moves on by a constant from stage to stage.
     const int64_t row_groups = p.n_cols / 8;
     int64_t q[U];
 #pragma unroll
@@ -624,9 +627,10 @@ __global__ void __launch_bounds__(threads(MASK), MASK ? 1 : 2)
   sums_cta<RP, OUTER, MASK>(tm_x, tm_o, p, blockIdx.x, blockIdx.y);
 }
 
-// dt and dB, which read the same gradient and do not wait for one another, in one launch. dB's CTAs come
-// first, one per SM, and a row tile's splits side by side (16384 x 1536 to 8960, forward and backward:
-// rank 16 269 -> 262 us, rank 64 307 -> 304, against dt first and dB with two CTAs per SM).
+// dt and dB, which read the same gradient and do not wait for one another, in one launch. dB's CTAs
+// come first, one per SM, and a row tile's splits side by side (16384 x 1536 to 8960, forward and
+// backward: rank 16 269 -> 262 us, rank 64 307 -> 304, against dt first and dB with two CTAs per
+// SM).
 template <int RP>
 __global__ void __launch_bounds__(threads(false), 2)
     sums_pair_kernel(const __grid_constant__ CUtensorMap in_x,
@@ -641,8 +645,10 @@ __global__ void __launch_bounds__(threads(false), 2)
     sums_cta<RP, true, false>(out_x, out_o, out_p, id % outer_tiles, id / outer_tiles);
 }
 
-// How the reduction is divided: as many CTAs as 148 SMs hold at a time (two of them, or `one` per SM: with
-// its mask warps, and for dB beside dt), two blocks of 128 (which share a scale) for a CTA at least.
+// How the reduction is divided: as many CTAs as 148 SMs hold at a time (two of them, or `one` per
+// SM: with its mask warps, and for dB beside dt), two blocks of 128 (which share a scale) for a CTA
+// at least. A B200's 148 are a constant: the sizes of workspaces and the order of sums go by it,
+// and neither may depend on which device is current when it is asked.
 struct Plan {
   int tiles = 0, steps = 0, steps_per_split = 0, splits = 0;
   Plan() = default;

@@ -727,8 +727,11 @@ int run_mma_rows(const __half* x, int64_t ld_x, int n_rows, const Weight& w, con
   return run_mma<4, GROUPED>(x, ld_x, n_rows, w, sp, ep, y, ld_y, stream);
 }
 
-// Any even row length and block size: one warp per output, a byte (two weights) per lane and
-// step, eight rows of x at a time.
+// Any even row length, block size and alignment: one warp per output, a byte (two weights) per lane
+// and step, eight rows of x at a time. For correctness beside the kernel above, not for speed:
+// bound by its two 64-bit divisions and its scale per byte (17920 x 1536: one row 97 us, 32 rows
+// 416; 256 x 1536: 16 and 78). Checkpoints as bitsandbytes writes them have blocks of powers of two
+// from 64 on, rows of whole blocks and aligned buffers, and do not come here.
 __global__ void __launch_bounds__(256) nf4_matvec_any_kernel(const __half* __restrict__ x,
                                                              int64_t ld_x, int n_rows, Weight w,
                                                              Epilogue ep, __half* __restrict__ y,
