@@ -58,7 +58,10 @@ def _check_seed(seed, x):
 
 def _rows(t, cols):
     """`t` as [rows, cols] rows of unit stride that do not overlap (a view where its strides
-    allow it, else a copy), and their stride."""
+    allow it, else a copy), and their stride. A lazily negated view (the imaginary part of a conjugate)
+    is written out."""
+    if t.is_neg():
+        t = t.resolve_neg()
     if t.is_contiguous():
         return t, cols
     t = t.reshape(-1, cols)

@@ -235,6 +235,47 @@ def test_product_written_over_its_input(rows):
             assert torch.equal(buffer[:, b:b + size], want), (a, b)
 
 
+@pytest.mark.parametrize("cols", [1, 2, 40])
+def test_negated_views_are_written_out(cols):
+    """The data of a lazily negated view (the imaginary part of a conjugate) has the other sign: what the
+    kernels are given holds the view's values. One column is not copied for its stride."""
+    real = torch.randn(30, cols, 2, generator=torch.Generator().manual_seed(1))
+    view = torch.view_as_complex(real).conj().imag
+    assert view.is_neg()
+    rows, ld = adapter._rows(view, cols)
+    assert not rows.is_neg() and ld >= cols and torch.equal(rows, -real[..., 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [1, 40])
+def test_dropout_of_a_negated_view(cols):
+    seed = torch.zeros(1, dtype=torch.int64, device="cuda")
+    z = torch.randn(30, cols, dtype=torch.complex64, device="cuda")
+    x = z.conj().imag
+    assert x.is_neg()
+    assert torch.equal(adapter.dropout(x, 0.3, seed), adapter.dropout((-z.imag).contiguous(), 0.3, seed))
+
+
+@pytest.mark.gpu
+def test_function_transforms_are_refused():
+    """torch.func's transforms of the two training operators and of the few-row product end in an error,
+    before any launch."""
+    seed = torch.zeros(1, dtype=torch.int64, device="cuda")
+    x = torch.randn(3, 4, 64, device="cuda").half()
+    base = torch.zeros(3, 4, 16, device="cuda").half()
+    a, b = torch.randn(4, 64, device="cuda"), torch.randn(16, 4, device="cuda")
+    packed = torch.zeros(16 * 32, dtype=torch.uint8, device="cuda")
+    absmax = torch.ones(16, device="cuda")
+    calls = (lambda v: adapter.dropout(v, 0.1, seed).float().sum(),
+             lambda v: adapter.lora_branch(v, base[0], a, b, 1.0).float().sum(),
+             lambda v: nf4_dequant.nf4_matvec(v, packed, absmax, 64).float().sum())
+    for call in calls:
+        with pytest.raises(RuntimeError):
+            torch.func.grad(call)(x[0])
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x)
+
+
 # ------------------------------------------------------------------------------------------
 # decoding
 # ------------------------------------------------------------------------------------------
