@@ -10,9 +10,10 @@ its seed and of the element's place in row-major order (Philox4x32 with 7 rounds
 kept when the low 15 bits of half e % 8 of counter e / 8 reach round(p * 32768)), so the backward
 pass makes it again instead of reading it: no dropped copy of the input and no mask are kept. With
 the rank rounded up to R = 16, 32 or 64, the branch saves its input, the seed, the rank-wide product
-(max(128, 4 R) bytes a row and R / 32 for its scales) and the adapter as it was, in the kernels' parts
-(4 R bytes per output and max(128, 4 R) per input column). The probability is thereby rounded to a multiple of
-1 / 32768; the factor 32768 / (32768 - drop) is that of the rounded one, which keeps the expectation.
+(max(128, 4 R) bytes a row and R / 32 for its scales) and the adapter as it was, in the kernels'
+parts (4 R bytes per output and max(128, 4 R) per input column). The probability is thereby rounded
+to a multiple of 1 / 32768; the factor 32768 / (32768 - drop) is that of the rounded one, which
+keeps the expectation.
 
 The seed is a one-element int64 tensor on the device. `draw_seed` fills it from torch's own CUDA
 generator: torch.manual_seed makes a run repeatable, a captured graph draws a new seed on every
